@@ -331,6 +331,82 @@ int mgq_gptq_affine(float* W, const float* U, int64_t B, int64_t R, int64_t C, i
                     double max_shrink, uint8_t* q_out, void* s_store, void* b_store, float* Err,
                     int64_t err_cols, void* stream);
 
+/* ======================================================================== *
+ * Matrix products with the weights -- mlx_gptq/linear.py                    *
+ *                                                                           *
+ * Not in the reference: the products a calibration forward, a fine-tuning   *
+ * step or a serving program makes with dense, MXFP or int8 weights.         *
+ *                                                                           *
+ * Group g owns the list entries [offsets[g], offsets[g + 1]) (offsets:      *
+ * device int32 [n_groups + 1], or NULL for one group of all entries). Entry *
+ * t reads row row_index[t] of X (device int32 [n_entries], or NULL: row t). *
+ * Entries before offsets[0] or from offsets[n_groups] on belong to no group *
+ * and give zero rows. Offsets are clamped to [0, n_entries] and row indexes *
+ * to [0, n_rows): whatever they hold, nothing outside the tensors is        *
+ * touched. Offsets that decrease leave rows of the result unwritten.        *
+ * X and weights have any row pitch (ldx, ldw: elements, at least a row) and *
+ * any alignment of their elements; w_group is the distance of two groups'   *
+ * weights in elements. Results are contiguous.                              *
+ * ======================================================================== */
+
+/* Y[t, n] = sum_k X[row(t), k] W[g, n, k], fp32 sums, rounded once to dtype
+ * (bf16 or f16, the type of X and W). Y: [n_entries, N]. */
+int mgq_grouped_linear(const void* X, int dtype, int64_t n_rows, int64_t ldx,
+                       const int32_t* row_index, int64_t n_entries, const void* W,
+                       int64_t n_groups, int64_t N, int64_t K, int64_t ldw, int64_t w_group,
+                       const int32_t* offsets, void* Y, void* stream);
+
+/* dX[t, k] = sum_n dY[t, n] W[g, n, k] for every list entry; out_dtype is
+ * dtype or f32. dX: [n_entries, K] (a gathered product sums its entries per
+ * row with mgq_rows_sum). */
+int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy, const void* W,
+                      int64_t n_groups, int64_t N, int64_t K, int64_t ldw, int64_t w_group,
+                      const int32_t* offsets, void* dX, int out_dtype, void* stream);
+
+/* dW[g, n, k] = sum over the entries t of group g of dY[t, n] X[row(t), k];
+ * zeros for a group without entries. out_dtype is dtype or f32. */
+int64_t mgq_grouped_wgrad_workspace_size(int64_t n_entries, int64_t n_groups, int64_t N,
+                                         int64_t K);
+int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy, const void* X,
+                      int64_t n_rows, int64_t ldx, const int32_t* row_index, int64_t n_groups,
+                      int64_t N, int64_t K, const int32_t* offsets, void* dW, int out_dtype,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* out[r, :] = sum of src[t, :] over the entries t with row_index[t] = r, in
+ * fp32 and in the order of t, rounded once to out_dtype (zeros for a row that
+ * no entry reads). src: f32 [n_entries, cols]; out: [n_rows, cols]. */
+int64_t mgq_rows_sum_workspace_size(int64_t n_rows);
+int mgq_rows_sum(const float* src, const int32_t* row_index, int64_t n_entries, int64_t n_rows,
+                 int64_t cols, void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
+                 void* stream);
+
+/* Y[t, n] = sum_k X[row(t), k] v(code[g, n, k]) 2^(scales[g, n, k / 32] - 127),
+ * X and Y bf16. words: [n_groups, N, K * bits / 32] as mgq_pack_q writes them
+ * (bits 4 for MGQ_MODE_MXFP4, 8 for _MXFP8), scales: u8 [n_groups, N, K / 32],
+ * both contiguous; K % 32 == 0. A weight's value is exact in bf16 (below
+ * 2^-126 rounded to its subnormal step 2^-133); scale byte 255 is not a
+ * number, as E8M0 has it. */
+int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const int32_t* row_index,
+                    int64_t n_entries, const uint32_t* words, const uint8_t* scales, int mode,
+                    int64_t n_groups, int64_t N, int64_t K, const int32_t* offsets, void* Y,
+                    void* stream);
+
+/* q = rne(x / s), s = max |x| of the row / 127 (fp32 quotients). A zero row
+ * has s = 0, q = 0; a row holding a NaN or an infinity s = NaN, q = 0.
+ * X: [rows, cols] of dtype (f32/bf16/f16) -> q i8 [rows, cols], scales f32. */
+int mgq_quantize_rows_int8(const void* X, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                           int8_t* q, float* scales, void* stream);
+
+/* Y[t, n] = float(sum_k X[row(t), k] W[g, n, k]) * x_scale[row(t)] *
+ * w_scale[g, n] (+ bias[g, n]), the sum in int32 (K <= 131071 keeps it from
+ * overflowing), the rest in fp32, rounded once to out_dtype (f32/bf16/f16).
+ * x_scale f32 [n_rows], w_scale and bias f32 [n_groups, N] (bias or NULL). */
+int mgq_int8_linear(const int8_t* X, const float* x_scale, int64_t n_rows, int64_t ldx,
+                    const int32_t* row_index, int64_t n_entries, const int8_t* W,
+                    const float* w_scale, const float* bias, int64_t n_groups, int64_t N,
+                    int64_t K, int64_t ldw, int64_t w_group, const int32_t* offsets, void* Y,
+                    int out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

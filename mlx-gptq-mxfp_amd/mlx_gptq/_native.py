@@ -86,9 +86,26 @@ SIGNATURES: dict[str, list] = {
                               _INT, _F64, _VP, _VP, _VP, _VP, _VP],
     "mgq_gptq_affine": [_VP, _VP, _I64, _I64, _I64, _I64, _INT, _INT, _INT, _INT, _INT, _F64,
                         _VP, _VP, _VP, _VP, _I64, _VP],
+    # linear.py
+    "mgq_grouped_linear": [_VP, _INT, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _I64,
+                           _VP, _VP, _VP],
+    "mgq_grouped_dgrad": [_VP, _INT, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64, _VP, _VP,
+                          _INT, _VP],
+    "mgq_grouped_wgrad_workspace_size": [_I64, _I64, _I64, _I64],
+    "mgq_grouped_wgrad": [_VP, _INT, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _VP, _VP,
+                          _INT, _VP, _I64, _VP],
+    "mgq_rows_sum_workspace_size": [_I64],
+    "mgq_rows_sum": [_VP, _VP, _I64, _I64, _I64, _VP, _INT, _VP, _I64, _VP],
+    "mgq_mxfp_linear": [_VP, _I64, _I64, _VP, _I64, _VP, _VP, _INT, _I64, _I64, _I64, _VP, _VP,
+                        _VP],
+    "mgq_quantize_rows_int8": [_VP, _INT, _I64, _I64, _I64, _VP, _VP, _VP],
+    "mgq_int8_linear": [_VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _I64,
+                        _I64, _VP, _VP, _INT, _VP],
 }
 
 _RESTYPES = {
+    "mgq_grouped_wgrad_workspace_size": ctypes.c_int64,
+    "mgq_rows_sum_workspace_size": ctypes.c_int64,
     "mgq_last_error": ctypes.c_char_p,
     "mgq_gptq_mxfp_workspace_size": ctypes.c_int64,
     "mgq_noalloc_scratch_bytes": ctypes.c_int64,

@@ -1,0 +1,343 @@
+"""Matrix products with dense, MXFP and int8 weights on MI355X.
+
+What the solver's codes are multiplied with: the products of a calibration
+forward, a fine-tuning step or a serving program, for one weight or for every
+expert of a routed layer at once. The reference leaves these to torch and MLX;
+the kernels are csrc/linear*.hip.
+
+* ``grouped_linear`` (bf16 or f16 weights, differentiable) with its two
+  gradients ``grouped_linear_dgrad`` and ``grouped_linear_wgrad``;
+* ``mxfp_linear``: the same product with packed MXFP4 / MXFP8 weights, decoded
+  inside the kernel;
+* ``quantize_rows_int8`` and ``int8_linear``: rows quantized to 8-bit integers
+  with a scale each, and their product with 8-bit weights that have a scale for
+  each output channel.
+
+Groups. The rows are a list of entries in the experts' order: expert g owns
+entries ``offsets[g]:offsets[g + 1]``, as ``capture.RoutedStash.plan`` lays
+them out. With ``row_index`` entry t reads row ``row_index[t]`` of ``x`` (the
+gather is part of the product; nothing is copied), without it row t. Entries
+that belong to no group give zero rows. ``offsets=None`` is one dense weight
+(without its leading dimension). Offsets on the device stay there: with
+``validate=False`` no call waits for the device, so a decoding loop can be
+captured in a graph. Offsets and indexes outside their ranges are clamped by the
+kernels, never followed; ``validate`` raises for them.
+
+Work is enqueued on the current stream of the tensors' device. Host tensors are
+staged through the current HIP device, as in the other modules.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import _native as nat
+
+_MX_BITS = {"mxfp4": 4, "mxfp8": 8}
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _pitched(t: torch.Tensor) -> torch.Tensor:
+    """`t` with contiguous rows that do not overlap (a copy if need be)."""
+    if t.stride(-1) != 1 or (t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row pitch in elements (a single row's stride says nothing)."""
+    return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], 1)
+
+
+def _weight3(fn: str, weight: torch.Tensor, offsets) -> torch.Tensor:
+    """The weight as [G, N, K]; dense weights are [N, K]."""
+    if offsets is None:
+        if weight.dim() != 2:
+            raise ValueError(f"{fn}: without offsets the weight is [N, K] (got {tuple(weight.shape)})")
+        return weight.unsqueeze(0)
+    if weight.dim() != 3:
+        raise ValueError(f"{fn}: with offsets the weight is [G, N, K] (got {tuple(weight.shape)})")
+    return weight
+
+
+def _rows2(fn: str, name: str, x: torch.Tensor) -> None:
+    if x.dim() != 2:
+        raise ValueError(f"{fn}: {name} must be a matrix (got {tuple(x.shape)})")
+
+
+def _list(fn: str, offsets, row_index, groups: int, n_rows: int, dev: torch.device, validate: bool):
+    """(offsets int32 on dev | None, row_index int32 on dev | None, entries)."""
+    if row_index is not None:
+        if row_index.dim() != 1 or row_index.dtype.is_floating_point:
+            raise ValueError(f"{fn}: row_index must be a list of integers")
+        if validate and row_index.numel():
+            lo, hi = torch.aminmax(row_index)
+            if int(lo) < 0 or int(hi) >= n_rows:
+                raise IndexError(f"{fn}: row_index outside [0, {n_rows})")
+        row_index = nat.on_device(row_index.to(torch.int32), dev)
+    entries = n_rows if row_index is None else row_index.numel()
+    if offsets is None:
+        return None, row_index, entries
+    if not isinstance(offsets, torch.Tensor):
+        offsets = torch.from_numpy(np.array(offsets, dtype=np.int64))
+    if offsets.dim() != 1 or offsets.numel() != groups + 1 or offsets.dtype.is_floating_point:
+        raise ValueError(f"{fn}: offsets must hold {groups + 1} integers for {groups} groups")
+    if validate or not offsets.is_cuda:
+        o = offsets.detach().cpu().numpy()
+        if np.any(np.diff(o) < 0) or o[0] < 0:
+            raise ValueError(f"{fn}: offsets must be non-negative and non-decreasing")
+        if o[-1] > entries:
+            raise ValueError(f"{fn}: offsets exceed the {entries} list entries")
+    return nat.on_device(offsets.to(torch.int32), dev), row_index, entries
+
+
+def _check_half(fn: str, *tensors: torch.Tensor) -> None:
+    dt = tensors[0].dtype
+    if dt not in _HALF or any(t.dtype != dt for t in tensors):
+        raise TypeError(f"{fn}: expects bfloat16 or float16 tensors of one type "
+                        f"(got {', '.join(str(t.dtype) for t in tensors)})")
+
+
+def _forward(x, weight, offsets, row_index, validate):
+    fn = "grouped_linear"
+    _check_half(fn, x, weight)
+    _rows2(fn, "x", x)
+    w = _weight3(fn, weight, offsets)
+    G, N, K = w.shape
+    if x.shape[1] != K:
+        raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the weight {K}")
+    dev = nat.device_for(x, weight)
+    xd, wd = _pitched(x.to(dev)), _pitched(w.to(dev))
+    off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    if M and N:
+        nat.call("mgq_grouped_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0], _ld(xd),
+                 nat.ptr(idx), M, wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off),
+                 y.data_ptr(), nat.stream_of(dev))
+    return y.to(x.device)
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets, row_index, validate):
+        ctx.save_for_backward(x, weight)
+        ctx.lists = (offsets, row_index)
+        return _forward(x, weight, offsets, row_index, validate)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        offsets, row_index = ctx.lists
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = grouped_linear_dgrad(dy, weight, offsets, row_index, x.shape[0], validate=False)
+        if ctx.needs_input_grad[1]:
+            dw = grouped_linear_wgrad(dy, x, offsets, row_index, validate=False)
+        return dx, dw, None, None, None
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets=None,
+                   row_index: torch.Tensor | None = None, validate: bool = True) -> torch.Tensor:
+    """y[t] = x[row_index[t]] @ weight[g].T for the entries t of every group g.
+
+    x: [T, K] bf16 or f16, weight: [G, N, K] of the same type (any row pitch),
+    offsets: G + 1 integers (a device tensor or any host sequence) ->
+    [entries, N]. fp32 sums, rounded once. Differentiable in x and weight: the
+    gradients are ``grouped_linear_dgrad`` and ``grouped_linear_wgrad``.
+    """
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _GroupedLinear.apply(x, weight, offsets, row_index, validate)
+    return _forward(x, weight, offsets, row_index, validate)
+
+
+@torch.no_grad()
+def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
+                         row_index: torch.Tensor | None = None, n_rows: int | None = None,
+                         validate: bool = True) -> torch.Tensor:
+    """Gradient of ``grouped_linear`` with respect to x: [n_rows, K].
+
+    dy: [entries, N]. With ``row_index``, row r is the sum over the entries that
+    read it, in fp32 and in the entries' order, rounded once (``n_rows`` is
+    required; rows that no entry reads are zero).
+    """
+    fn = "grouped_linear_dgrad"
+    _check_half(fn, dy, weight)
+    _rows2(fn, "dy", dy)
+    w = _weight3(fn, weight, offsets)
+    G, N, K = w.shape
+    if dy.shape[1] != N:
+        raise AssertionError(f"{fn}: dy has {dy.shape[1]} columns, the weight {N} rows")
+    if row_index is not None and n_rows is None:
+        raise ValueError(f"{fn}: n_rows is required with row_index")
+    dev = nat.device_for(dy, weight)
+    dyd, wd = _pitched(dy.to(dev)), _pitched(w.to(dev))
+    M = int(dy.shape[0])
+    off, idx, entries = _list(fn, offsets, row_index, G, M if row_index is None else int(n_rows),
+                              dev, validate)
+    if entries != M:
+        raise ValueError(f"{fn}: dy has {M} rows, row_index {entries} entries")
+    gathered = idx is not None
+    out_type = torch.float32 if gathered else dy.dtype
+    dx = torch.empty(M, K, dtype=out_type, device=dev)
+    stream = nat.stream_of(dev)
+    if M and K and N:
+        nat.call("mgq_grouped_dgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
+                 wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off), dx.data_ptr(),
+                 nat.dtype_code(out_type), stream)
+    elif N == 0:
+        dx.zero_()
+    if gathered:
+        out = torch.empty(int(n_rows), K, dtype=dy.dtype, device=dev)
+        if out.numel():
+            ws = torch.empty(nat.load().mgq_rows_sum_workspace_size(int(n_rows)), dtype=torch.uint8,
+                             device=dev)
+            nat.call("mgq_rows_sum", dx.data_ptr(), idx.data_ptr(), M, int(n_rows), K,
+                     out.data_ptr(), nat.dtype_code(out.dtype), ws.data_ptr(), ws.numel(), stream)
+        dx = out
+    return dx.to(dy.device)
+
+
+@torch.no_grad()
+def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
+                         row_index: torch.Tensor | None = None, validate: bool = True,
+                         out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Gradient of ``grouped_linear`` with respect to the weight: [G, N, K]
+    ([N, K] without offsets), of dy's type or ``out_dtype=torch.float32``.
+
+    dy: [entries, N], x: [T, K]. fp32 sums over a group's entries, rounded
+    once; zeros for a group without entries.
+    """
+    fn = "grouped_linear_wgrad"
+    _check_half(fn, dy, x)
+    _rows2(fn, "dy", dy)
+    _rows2(fn, "x", x)
+    out_dtype = dy.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (dy.dtype, torch.float32):
+        raise TypeError(f"{fn}: the result is {dy.dtype} or float32 (got {out_dtype})")
+    dev = nat.device_for(dy, x)
+    dyd, xd = _pitched(dy.to(dev)), _pitched(x.to(dev))
+    G = 1 if offsets is None else len(offsets) - 1
+    if G < 1:
+        raise ValueError(f"{fn}: offsets must hold at least two integers")
+    off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
+    if dy.shape[0] != M:
+        raise ValueError(f"{fn}: dy has {dy.shape[0]} rows, the list {M} entries")
+    N, K = int(dy.shape[1]), int(x.shape[1])
+    dw = torch.empty(G, N, K, dtype=out_dtype, device=dev)
+    if N and K:
+        size = nat.load().mgq_grouped_wgrad_workspace_size(M, G, N, K)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        nat.call("mgq_grouped_wgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
+                 xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), G, N, K, nat.ptr(off),
+                 dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size, nat.stream_of(dev))
+    if offsets is None:
+        dw = dw[0]
+    return dw.to(dy.device)
+
+
+@torch.no_grad()
+def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mode: str,
+                offsets=None, row_index: torch.Tensor | None = None,
+                validate: bool = True) -> torch.Tensor:
+    """``grouped_linear`` with MXFP4 or MXFP8 weights.
+
+    x: [T, K] bf16, packed: [G, N, K * bits / 32] words as ``packing.pack_q``
+    (or the solver's ``packed_out``) lays them out, scales: uint8
+    [G, N, K / 32] E8M0 bytes; without offsets both lack the leading G.
+    -> bf16 [entries, N]. The decoded weights are exact in bf16, the sums fp32.
+    """
+    fn = "mxfp_linear"
+    if mode not in _MX_BITS:
+        raise ValueError(f"not a microscaling mode: {mode}")
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"{fn}: expects bfloat16 rows (got {x.dtype})")
+    if packed.dtype not in (torch.int32, torch.uint32) or scales.dtype != torch.uint8:
+        raise TypeError(f"{fn}: expects 32-bit words and uint8 scales "
+                        f"(got {packed.dtype} and {scales.dtype})")
+    _rows2(fn, "x", x)
+    w, s = _weight3(fn, packed, offsets), _weight3(fn, scales, offsets)
+    G, N, words = w.shape
+    K = words * 32 // _MX_BITS[mode]
+    if x.shape[1] != K or K % 32:
+        raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the words hold {K} "
+                             "(a multiple of 32)")
+    if tuple(s.shape) != (G, N, K // 32):
+        raise AssertionError(f"{fn}: scales must be {(G, N, K // 32)} (got {tuple(s.shape)})")
+    dev = nat.device_for(x, packed, scales)
+    xd = _pitched(x.to(dev))
+    wd, sd = nat.on_device(w, dev), nat.on_device(s, dev)
+    off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    if M and N:
+        nat.call("mgq_mxfp_linear", xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), M,
+                 wd.data_ptr(), sd.data_ptr(), nat.mode_code(mode), G, N, K, nat.ptr(off),
+                 y.data_ptr(), nat.stream_of(dev))
+    return y.to(x.device)
+
+
+@torch.no_grad()
+def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows as 8-bit integers with a scale each: (q int8 [..., K], scales f32
+    [...]), scale = max|row| / 127, q = round-half-even(row / scale).
+
+    A zero row has scale 0 and zero codes. A row that holds a NaN or an infinity
+    has scale NaN and zero codes, so products with it are NaN.
+    """
+    if x.dtype not in (torch.float32, *_HALF):
+        raise TypeError(f"quantize_rows_int8: expects float32, bfloat16 or float16 (got {x.dtype})")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"quantize_rows_int8: rows of no elements ({tuple(x.shape)})")
+    dev = nat.device_for(x)
+    rows = _pitched(x.to(dev).reshape(-1, x.shape[-1]))
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    s = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    if rows.shape[0]:
+        nat.call("mgq_quantize_rows_int8", rows.data_ptr(), nat.dtype_code(x.dtype), rows.shape[0],
+                 rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr(), nat.stream_of(dev))
+    return q.to(x.device), s.to(x.device)
+
+
+@torch.no_grad()
+def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
+                w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.bfloat16, offsets=None,
+                row_index: torch.Tensor | None = None, validate: bool = True) -> torch.Tensor:
+    """y[t, n] = (x[r] . weight[g, n]) * x_scale[r] * w_scale[g, n] (+ bias[g, n]).
+
+    x: int8 [T, K] with x_scale f32 [T] (``quantize_rows_int8``), weight: int8
+    [G, N, K] with w_scale f32 [G, N], bias f32 [G, N]; without offsets the
+    weight's tensors lack the leading G. -> ``out_dtype`` [entries, N]. The sum
+    is exact (int32, K <= 131071), the scaling fp32, rounded once. Entries of no
+    group are zero, without bias.
+    """
+    fn = "int8_linear"
+    if x.dtype != torch.int8 or weight.dtype != torch.int8:
+        raise TypeError(f"{fn}: expects int8 rows and weights (got {x.dtype} and {weight.dtype})")
+    for name, t in (("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias)):
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"{fn}: {name} must be float32 (got {t.dtype})")
+    if out_dtype not in (torch.float32, *_HALF):
+        raise TypeError(f"{fn}: the result is float32, bfloat16 or float16 (got {out_dtype})")
+    _rows2(fn, "x", x)
+    w = _weight3(fn, weight, offsets)
+    G, N, K = w.shape
+    if x.shape[1] != K:
+        raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the weight {K}")
+    per_channel = (N,) if offsets is None else (G, N)
+    if tuple(x_scale.shape) != (x.shape[0],) or tuple(w_scale.shape) != per_channel or (
+            bias is not None and tuple(bias.shape) != per_channel):
+        raise AssertionError(f"{fn}: x_scale must be {(int(x.shape[0]),)}, w_scale and bias "
+                             f"{per_channel}")
+    dev = nat.device_for(x, weight)
+    xd, wd = _pitched(x.to(dev)), _pitched(w.to(dev))
+    xs, ws = nat.on_device(x_scale, dev), nat.on_device(w_scale, dev)
+    b = None if bias is None else nat.on_device(bias, dev)
+    off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
+    y = torch.empty(M, N, dtype=out_dtype, device=dev)
+    if M and N:
+        nat.call("mgq_int8_linear", xd.data_ptr(), xs.data_ptr(), xd.shape[0], _ld(xd),
+                 nat.ptr(idx), M, wd.data_ptr(), ws.data_ptr(), nat.ptr(b), G, N, K, _ld(wd),
+                 wd.stride(0), nat.ptr(off), y.data_ptr(), nat.dtype_code(out_dtype),
+                 nat.stream_of(dev))
+    return y.to(x.device)
