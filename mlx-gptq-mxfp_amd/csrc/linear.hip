@@ -5,7 +5,7 @@
 // linear_any_kernel takes every size, pitch and alignment: operands go
 // through registers into LDS, piecewise where a row ends inside a 16-byte
 // piece.
-#include "linear_common.h"
+#include "linear_tile.h"
 
 namespace mgq {
 namespace {
@@ -211,11 +211,6 @@ __global__ void __launch_bounds__(256) linear_any_kernel(const LinArgs a) {
   }
 }
 
-int64_t row_tiles(const LinArgs& a, int bm) {
-  const int64_t segs = a.offsets ? a.G + 2 : 1;
-  return a.offsets ? a.M / bm + (segs < a.M ? segs : a.M) : ceil_div(a.M, bm);
-}
-
 template <int OP, bool PT, bool QT, bool RC>
 int launch_any(const LinArgs& a, int64_t grid, hipStream_t s, const char* what) {
   MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
@@ -223,9 +218,16 @@ int launch_any(const LinArgs& a, int64_t grid, hipStream_t s, const char* what) 
   return check_launch(what);
 }
 
-int rows_grid_any(const LinArgs& a, int64_t* grid) {
-  *grid = row_tiles(a, kAnyT) * ceil_div(a.np, kAnyT);
-  return MGQ_OK;
+// Forward and dgrad. The large tiles take operands of whole 16-byte pieces; how
+// many rows a tile has goes by the average group's.
+template <int OP, int KIND>
+int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
+  if (lin_tile_takes(a, OP, KIND)) {
+    const int64_t avg = a.M / a.G;
+    return lin_tile_rows(a, OP, KIND, avg > 192 ? 4 : avg > 64 ? 2 : 1, s, what);
+  }
+  const int64_t grid = lin_row_tiles(a, kAnyT) * ceil_div(a.np, kAnyT);
+  return launch_any<OP, KIND == kLinDgrad, false, false>(a, grid, s, what);
 }
 
 int check_list(const char* what, const int32_t* offsets, const int32_t* row_index,
@@ -249,8 +251,11 @@ int check_dims(const char* what, int64_t N, int64_t K) {
   return MGQ_OK;
 }
 
+// 2: 16-byte stores, 1: four results at once, 0: one by one.
 int vec_ok(const void* out, int64_t ldo, int out_type) {
-  return ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (out_type == kF32 ? 15 : 7)) == 0;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(out);
+  if (ldo % 8 == 0 && (at & 15) == 0) return 2;
+  return ldo % 4 == 0 && (at & (out_type == kF32 ? 15 : 7)) == 0;
 }
 
 }  // namespace
@@ -286,11 +291,9 @@ extern "C" int mgq_grouped_linear(const void* X, int dtype, int64_t n_rows, int6
   a.ldo = N;
   a.out_type = dtype;
   a.vec_out = vec_ok(Y, N, dtype);
-  int64_t grid;
-  rows_grid_any(a, &grid);
   hipStream_t s = as_stream(stream);
-  return dtype == kF16 ? launch_any<kOpF16, false, false, false>(a, grid, s, what)
-                       : launch_any<kOpBF16, false, false, false>(a, grid, s, what);
+  return dtype == kF16 ? run_rows<kOpF16, kLinForward>(a, s, what)
+                       : run_rows<kOpBF16, kLinForward>(a, s, what);
 }
 
 extern "C" int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy,
@@ -322,20 +325,15 @@ extern "C" int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, i
   a.ldo = K;
   a.out_type = out_dtype;
   a.vec_out = vec_ok(dX, K, out_dtype);
-  int64_t grid;
-  rows_grid_any(a, &grid);
   hipStream_t s = as_stream(stream);
-  return dtype == kF16 ? launch_any<kOpF16, true, false, false>(a, grid, s, what)
-                       : launch_any<kOpBF16, true, false, false>(a, grid, s, what);
+  return dtype == kF16 ? run_rows<kOpF16, kLinDgrad>(a, s, what)
+                       : run_rows<kOpBF16, kLinDgrad>(a, s, what);
 }
 
 extern "C" int64_t mgq_grouped_wgrad_workspace_size(int64_t n_entries, int64_t n_groups, int64_t N,
                                                     int64_t K) {
-  (void)n_entries;
-  (void)n_groups;
-  (void)N;
-  (void)K;
-  return 0;
+  if (n_entries < 0 || n_groups < 1 || n_groups > kLinPlanGroups || N < 1 || K < 1) return 0;
+  return lin_plan_sizes(n_entries, n_groups, N, K).bytes;
 }
 
 extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy,
@@ -371,9 +369,11 @@ extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, i
   a.ldo = K;
   a.o_group = N * K;
   a.out_type = out_dtype;
-  a.vec_out = vec_ok(dW, K, out_dtype) && (N * K) % 4 == 0;
-  const int64_t grid = n_groups * ceil_div(N, kAnyT) * ceil_div(K, kAnyT);
+  a.vec_out = vec_ok(dW, K, out_dtype);
   hipStream_t s = as_stream(stream);
+  if (lin_tile_takes(a, dtype == kF16 ? kOpF16 : kOpBF16, kLinWgrad))
+    return lin_tile_wgrad(a, dtype == kF16 ? kOpF16 : kOpBF16, workspace, s, what);
+  const int64_t grid = n_groups * ceil_div(N, kAnyT) * ceil_div(K, kAnyT);
   return dtype == kF16 ? launch_any<kOpF16, true, true, true>(a, grid, s, what)
                        : launch_any<kOpBF16, true, true, true>(a, grid, s, what);
 }
@@ -410,11 +410,9 @@ extern "C" int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const
   a.ldo = N;
   a.out_type = kBF16;
   a.vec_out = vec_ok(Y, N, kBF16);
-  int64_t grid;
-  rows_grid_any(a, &grid);
   hipStream_t s = as_stream(stream);
-  return mode == kMxfp4 ? launch_any<kOpMx4, false, false, false>(a, grid, s, what)
-                        : launch_any<kOpMx8, false, false, false>(a, grid, s, what);
+  return mode == kMxfp4 ? run_rows<kOpMx4, kLinForward>(a, s, what)
+                        : run_rows<kOpMx8, kLinForward>(a, s, what);
 }
 
 extern "C" int mgq_int8_linear(const int8_t* X, const float* x_scale, int64_t n_rows, int64_t ldx,
@@ -453,7 +451,5 @@ extern "C" int mgq_int8_linear(const int8_t* X, const float* x_scale, int64_t n_
   a.sx = x_scale;
   a.sw = w_scale;
   a.bias = bias;
-  int64_t grid;
-  rows_grid_any(a, &grid);
-  return launch_any<kOpI8, false, false, false>(a, grid, as_stream(stream), what);
+  return run_rows<kOpI8, kLinForward>(a, as_stream(stream), what);
 }

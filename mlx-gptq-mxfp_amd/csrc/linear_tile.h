@@ -1,0 +1,73 @@
+// The large-tile kernels' host side (linear_tile.hip) and wgrad's work list.
+#pragma once
+
+#include "linear_common.h"
+
+namespace mgq {
+
+enum LinKind : int { kLinForward = 0, kLinDgrad = 1, kLinWgrad = 2 };
+
+// wgrad: group g's entries [t0, t1). slot >= 0: the group is cut and the unit's
+// tile `i` goes to partial tile slot * tiles + i.
+struct LinUnit {
+  int32_t g, t0, t1, slot;
+};
+// A cut group: its units' slots are slot0 .. slot0 + n - 1.
+struct LinSplit {
+  int32_t g, slot0, n;
+};
+struct LinPlanArgs {
+  int32_t* counts;  // units, cut groups
+  LinUnit* units;
+  LinSplit* splits;
+  float* partials;
+  int npt, nqt;
+  int cap;
+  int max_units, max_splits, max_slots;
+  int deal;  // whole units per XCD
+};
+struct LinPlanSizes {
+  int64_t tiles, cap, max_units, max_splits, max_slots;
+  int64_t units_off, splits_off, partials_off, bytes;
+};
+constexpr int kLinPlanGroups = 4096;
+
+// wgrad: which unit and tile a workgroup takes. With many units an XCD takes
+// every eighth of them whole (in snake order: they are sorted by length), so that
+// its L2 holds the unit's rows; with few, a unit's tiles go round the XCDs.
+__device__ __forceinline__ bool lin_find_unit(const LinArgs& a, const LinPlanArgs& pl, LinUnit* u,
+                                              int* tile) {
+  const int tiles = pl.npt * pl.nqt;
+  const int n = pl.counts[0];
+  int i;
+  if (pl.deal) {
+    const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const int round = j / tiles;
+    *tile = j % tiles;
+    i = round * 8 + (round & 1 ? 7 - x : x);
+  } else {
+    i = blockIdx.x / tiles;
+    *tile = blockIdx.x % tiles;
+  }
+  if (i >= n) return false;
+  const LinUnit v = pl.units[i];
+  u->g = __builtin_amdgcn_readfirstlane(v.g);
+  u->t0 = __builtin_amdgcn_readfirstlane(v.t0);
+  u->t1 = __builtin_amdgcn_readfirstlane(v.t1);
+  u->slot = __builtin_amdgcn_readfirstlane(v.slot);
+  if (u->slot >= 0) u->slot = u->slot * tiles + *tile;
+  return true;
+}
+
+// The host's bound on the row tiles of a launch.
+inline int64_t lin_row_tiles(const LinArgs& a, int bm) {
+  const int64_t segs = a.G + 2;
+  return a.offsets ? a.M / bm + (segs < a.M ? segs : a.M) : ceil_div(a.M, bm);
+}
+
+bool lin_tile_takes(const LinArgs& a, int op, int kind);
+int lin_tile_rows(const LinArgs& a, int op, int kind, int fq, hipStream_t s, const char* what);
+LinPlanSizes lin_plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K);
+int lin_tile_wgrad(const LinArgs& a, int op, void* workspace, hipStream_t s, const char* what);
+
+}  // namespace mgq

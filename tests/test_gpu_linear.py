@@ -61,6 +61,11 @@ LISTS = {
     "many_groups": ([i % 4 for i in range(300)], 40, 64, 50, 0, 0),
     "big": ([700, 0, 300, 513], 520, 776, 400, 0, 0),
     "wide": ([600], 1100, 264, 0, 0, 0),
+    # groups long enough to be cut along their entries, few and many of them
+    "heavy": ([3000, 10, 0, 1500], 136, 328, 700, 0, 0),
+    "heavy_of_many": ([2500] + [i % 3 for i in range(70)] + [4100, 64, 65], 72, 264, 0, 3, 0),
+    "mid": ([90, 0, 150, 111, 64], 320, 200, 300, 0, 0),
+    "deep": ([300, 260, 1], 264, 1160, 0, 0, 5),
 }
 
 
@@ -166,7 +171,7 @@ def test_a_row_read_by_many_entries_sums_in_order():
 
 
 MX_LISTS = ["one_token", "token_of_eight", "empty_ends", "nothing", "no_group", "tile_edges",
-            "few_each", "many_groups"]
+            "few_each", "many_groups", "big", "mid", "deep"]
 
 
 def mx_case(name, mode, K=None):
@@ -188,6 +193,8 @@ def mx_case(name, mode, K=None):
 @pytest.mark.parametrize("mode", ["mxfp4", "mxfp8"])
 @pytest.mark.parametrize("K", [None, 32, 352])
 def test_mxfp(name, mode, K):
+    if K is None and LISTS[name][2] % 32:
+        K = LISTS[name][2] // 32 * 32
     x, q, s, off, idx = mx_case(name, mode, K)
     packed = packing.pack_q(q.to(DEV), 4 if mode == "mxfp4" else 8)
     y = linear.mxfp_linear(dev(x), packed, dev(s), mode, off, dev(idx))
@@ -335,7 +342,8 @@ def test_int8_dense(M, N, K):
     close_int8(y, want, prod, bm, "dense f16")
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 200, 512), (5, 64, 96), (300, 260, 320), (700, 96, 1000)])
+@pytest.mark.parametrize("M,N,K", [(1, 200, 512), (5, 64, 96), (300, 260, 320), (700, 96, 1000),
+                                   (4000, 264, 136)])
 def test_dense_forms(M, N, K):
     g = gen(M * N)
     x, w = randn(g, M, K, dtype=torch.bfloat16), randn(g, N, K, dtype=torch.bfloat16, scale=0.1)
