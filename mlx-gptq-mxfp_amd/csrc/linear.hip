@@ -2,232 +2,30 @@
 // weights; both gradients of the dense form. Group g owns the list entries
 // [offsets[g], offsets[g + 1]); entry t reads row row_index[t] of X (or row t).
 //
-// linear_any_kernel takes every size, pitch and alignment: operands go
-// through registers into LDS, piecewise where a row ends inside a 16-byte
-// piece.
-#include "linear_tile.h"
+// Here are the entry points: their checks, and which kernel takes a call.
+#include "linear_few.h"
 
 namespace mgq {
 namespace {
 
-constexpr int kAnyT = 128;     // output tile 128 x 128
-constexpr int kAnyB = 64;      // bytes of a row per stage: 32 16-bit or 64 int8 elements
-constexpr int kAnyPitch = 80;  // LDS row pitch, 16-byte aligned
-
-// 16 bytes of a row: `n` of its elements exist, the rest are zeros.
-template <int ES>
-__device__ __forceinline__ lin_u32x4_t load_piece(const char* p, int n) {
-  lin_u32x4_t r = {0, 0, 0, 0};
-  if (n >= 16 / ES) {
-    const lin_u128_u_t u = *reinterpret_cast<const lin_u128_u_t*>(p);
-    r = lin_u32x4_t{u.v[0], u.v[1], u.v[2], u.v[3]};
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16 / ES; ++i) {
-      if (i < n) {
-        const uint32_t v = ES == 2 ? *reinterpret_cast<const uint16_t*>(p + 2 * i)
-                                   : *reinterpret_cast<const uint8_t*>(p + i);
-        r[i * ES / 4] |= v << (8 * ((i * ES) & 3));
-      }
-    }
-  }
-  return r;
-}
-
-// Piece c (16 bytes of bf16, i.e. 8 elements) of an MX weight row.
-template <int OP>
-__device__ __forceinline__ lin_u32x4_t load_mx_piece(const char* row, const uint8_t* srow, int c0,
-                                                     int nc) {
-  lin_u32x4_t r = {0, 0, 0, 0};
-  if (c0 < nc) {  // nc is a multiple of 32
-    const uint32_t s = srow[c0 >> 5];
-    if constexpr (OP == kOpMx4) {
-      r = lin_decode_mx4(*reinterpret_cast<const uint32_t*>(row + (c0 >> 1)), s);
-    } else {
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(row + c0);
-      r = lin_decode_mx8(q[0], q[1], s);
-    }
-  }
-  return r;
-}
-
-// PT / QT: the operand's contraction dimension is its row dimension
-// (transposed reads, 16-bit types only). RAGGED_C: wgrad, whose contraction
-// runs over a group's entries.
-template <int OP, bool PT, bool QT, bool RAGGED_C>
-__global__ void __launch_bounds__(256) linear_any_kernel(const LinArgs a) {
-  constexpr int ES = lin_esize<OP>();
-  constexpr int EP = 16 / ES;         // elements per piece
-  constexpr int EK = kAnyB / ES;      // contraction elements per stage
-  typedef typename LinAcc<OP>::t32 acc_t;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kAnyT * kAnyPitch];
-  char* lq = lds;
-  char* lp = lds + kAnyT * kAnyPitch;
-
-  int g, p0, q0, nq;
-  int64_t c_begin = 0, c_end = a.nc;  // contraction range
-  int64_t e0 = 0;                     // forward, dgrad: list entry of q = 0
-  if constexpr (RAGGED_C) {
-    const int npt = (a.np + kAnyT - 1) / kAnyT, nqt = (a.nq + kAnyT - 1) / kAnyT;
-    const uint32_t per = static_cast<uint32_t>(npt) * nqt;
-    g = blockIdx.x / per;
-    const uint32_t in = blockIdx.x % per;
-    p0 = (in % npt) * kAnyT;
-    q0 = (in / npt) * kAnyT;
-    nq = a.nq;
-    c_end = a.M;
-    if (a.offsets) lin_segment(a, g, &c_begin, &c_end);
-    if (c_end < c_begin) c_end = c_begin;
-  } else {
-    LinTile t;
-    if (!lin_find_tile<kAnyT>(a, (a.np + kAnyT - 1) / kAnyT, &t)) return;
-    g = t.g;
-    p0 = t.pt * kAnyT;
-    q0 = 0;
-    e0 = t.q0;
-    nq = static_cast<int>(t.q_end - t.q0 < kAnyT ? t.q_end - t.q0 : kAnyT);
-    if (g >= a.G) c_end = 0;  // entries of no group: zeros
-  }
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wq = (wave >> 1) * 64, wp = (wave & 1) * 64;
-  const int gw = RAGGED_C || g >= a.G ? 0 : g;
-  const char* Pg = a.P + gw * a.p_group;
-  const uint8_t* Psg =
-      lin_is_mx<OP>() ? a.Ps + static_cast<int64_t>(gw) * a.np * (a.nc / 32) : nullptr;
-
-  lin_u32x4_t rq[2], rp[2];
-  // thread's pieces: plain operands by (row, piece of 4), transposed ones by
-  // (contraction row of 32, 8 columns of 128)
-  auto fetch = [&](int64_t c0) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int id = tid + 256 * j;
-      rq[j] = lin_u32x4_t{0, 0, 0, 0};
-      rp[j] = lin_u32x4_t{0, 0, 0, 0};
-      if constexpr (QT) {
-        const int64_t c = c0 + (id >> 4);
-        const int col = q0 + 8 * (id & 15);
-        if (c < c_end && col < a.nq) rq[j] = load_piece<ES>(a.Q + c * a.ldq + 2 * col, a.nq - col);
-      } else {
-        const int r = id >> 2;
-        const int64_t c = c0 + (id & 3) * EP;
-        if (r < nq && c < c_end) {
-          const int64_t row = PT ? e0 + r : lin_row(a, e0 + r);
-          rq[j] = load_piece<ES>(a.Q + row * a.ldq + c * ES,
-                                 static_cast<int>(c_end - c < EP ? c_end - c : EP));
-        }
-      }
-      if constexpr (PT) {
-        const int64_t c = c0 + (id >> 4);
-        const int col = p0 + 8 * (id & 15);
-        if (c < c_end && col < a.np) {
-          const int64_t row = RAGGED_C ? lin_row(a, c) : c;
-          rp[j] = load_piece<ES>(Pg + row * a.ldp + 2 * col, a.np - col);
-        }
-      } else {
-        const int p = p0 + (id >> 2);
-        const int64_t c = c0 + (id & 3) * EP;
-        if (p < a.np && c < c_end) {
-          if constexpr (lin_is_mx<OP>())
-            rp[j] = load_mx_piece<OP>(Pg + p * a.ldp, Psg + static_cast<int64_t>(p) * (a.nc / 32),
-                                      static_cast<int>(c), a.nc);
-          else
-            rp[j] = load_piece<ES>(Pg + p * a.ldp + c * ES,
-                                   static_cast<int>(c_end - c < EP ? c_end - c : EP));
-        }
-      }
-    }
-  };
-  auto put = [&](char* l, bool transposed, lin_u32x4_t v, int id) {
-    if (transposed) {
-      const int c = id >> 4, r = 8 * (id & 15);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<uint16_t*>(l + (r + i) * kAnyPitch + 2 * c) =
-            static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
-    } else {
-      *reinterpret_cast<lin_u32x4_t*>(l + (id >> 2) * kAnyPitch + 16 * (id & 3)) = v;
-    }
-  };
-
-  acc_t acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-
-  if (c_begin < c_end) fetch(c_begin);
-  for (int64_t c = c_begin; c < c_end; c += EK) {
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      put(lq, QT, rq[j], tid + 256 * j);
-      put(lp, PT, rp[j], tid + 256 * j);
-    }
-    __syncthreads();
-    if (c + EK < c_end) fetch(c + EK);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int off = (2 * ks + (lane >> 5)) * 16;
-      lin_u32x4_t fp[2], fq[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fp[i] = *reinterpret_cast<const lin_u32x4_t*>(
-            lp + (wp + 32 * i + (lane & 31)) * kAnyPitch + off);
-        fq[i] = *reinterpret_cast<const lin_u32x4_t*>(
-            lq + (wq + 32 * i + (lane & 31)) * kAnyPitch + off);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = lin_mfma32<OP>(fp[i], fq[j], acc[i][j]);
-    }
-  }
-
-  const int osize = a.out_type == kF32 ? 4 : 2;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int q = q0 + wq + 32 * j + (lane & 31);
-    if (q >= nq) continue;
-    const int64_t orow = RAGGED_C ? q : e0 + q;
-    char* row = a.out + (orow * a.ldo + (RAGGED_C ? g * a.o_group : 0)) * osize;
-    float sx = 0.0f;
-    if constexpr (OP == kOpI8) sx = g < a.G ? a.sx[lin_row(a, e0 + q)] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int p = p0 + wp + 32 * i + 8 * r + 4 * (lane >> 5);
-        if (p >= a.np) continue;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(acc[i][j][4 * r + e]);
-        if (g < a.G) lin_scale4<OP>(a, g, p, sx, v);
-        lin_store4(a, row, p, v);
-      }
-  }
-}
-
-template <int OP, bool PT, bool QT, bool RC>
-int launch_any(const LinArgs& a, int64_t grid, hipStream_t s, const char* what) {
-  MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  linear_any_kernel<OP, PT, QT, RC><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
-  return check_launch(what);
-}
-
-// Forward and dgrad. The large tiles take operands of whole 16-byte pieces; how
-// many rows a tile has goes by the average group's.
+// Forward and dgrad: which kernel and tile.
 template <int OP, int KIND>
 int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
-  if (lin_tile_takes(a, OP, KIND)) {
-    const int64_t avg = a.M / a.G;
-    return lin_tile_rows(a, OP, KIND, avg > 192 ? 4 : avg > 64 ? 2 : 1, s, what);
+  const bool direct = lin_tile_direct(a, OP, KIND);
+  const char* ev = getenv("LIN_V");
+  if (ev) {
+    const int v = atoi(ev);
+    if (v < 10 && KIND == kLinForward) return lin_few_rows(a, OP, v, s, what);
+    if (v > 10 && v < 1000)
+      return lin_tile_rows(a, OP, KIND, LinTileShape{v == 65 ? 64 : v, v == 64 ? 128 : 256, !direct}, s, what);
+    if (v > 1000)
+      return lin_tile_rows(a, OP, KIND, LinTileShape{v == 1065 ? 64 : v - 1000, v == 1064 ? 128 : 256, true}, s, what);
   }
-  const int64_t grid = lin_row_tiles(a, kAnyT) * ceil_div(a.np, kAnyT);
-  return launch_any<OP, KIND == kLinDgrad, false, false>(a, grid, s, what);
+  if (KIND == kLinForward && a.M <= 16 * static_cast<int64_t>(a.G))
+    return lin_few_rows(a, OP, 1, s, what);
+  const int64_t avg = a.M / a.G;
+  return lin_tile_rows(a, OP, KIND,
+                       LinTileShape{avg > 192 ? 256 : avg > 64 ? 128 : 64, 256, !direct}, s, what);
 }
 
 int check_list(const char* what, const int32_t* offsets, const int32_t* row_index,
@@ -332,8 +130,8 @@ extern "C" int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, i
 
 extern "C" int64_t mgq_grouped_wgrad_workspace_size(int64_t n_entries, int64_t n_groups, int64_t N,
                                                     int64_t K) {
-  if (n_entries < 0 || n_groups < 1 || n_groups > kLinPlanGroups || N < 1 || K < 1) return 0;
-  return lin_plan_sizes(n_entries, n_groups, N, K).bytes;
+  if (n_entries < 0 || n_groups < 1 || N < 1 || K < 1) return 0;
+  return lin_tile_wgrad_bytes(n_entries, n_groups, N, K);
 }
 
 extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy,
@@ -352,6 +150,8 @@ extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, i
   const int64_t need = mgq_grouped_wgrad_workspace_size(n_entries, n_groups, N, K);
   MGQ_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), MGQ_ERR_WORKSPACE,
               "%s: workspace %lld < %lld bytes", what, (long long)workspace_bytes, (long long)need);
+  MGQ_REQUIRE(n_groups <= kLinPlanGroups, MGQ_ERR_SHAPE, "%s: %lld groups (at most %d)", what,
+              (long long)n_groups, kLinPlanGroups);
   if (K == 0) return MGQ_OK;
   LinArgs a = {};
   a.P = static_cast<const char*>(X);
@@ -371,11 +171,7 @@ extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, i
   a.out_type = out_dtype;
   a.vec_out = vec_ok(dW, K, out_dtype);
   hipStream_t s = as_stream(stream);
-  if (lin_tile_takes(a, dtype == kF16 ? kOpF16 : kOpBF16, kLinWgrad))
-    return lin_tile_wgrad(a, dtype == kF16 ? kOpF16 : kOpBF16, workspace, s, what);
-  const int64_t grid = n_groups * ceil_div(N, kAnyT) * ceil_div(K, kAnyT);
-  return dtype == kF16 ? launch_any<kOpF16, true, true, true>(a, grid, s, what)
-                       : launch_any<kOpBF16, true, true, true>(a, grid, s, what);
+  return lin_tile_wgrad(a, dtype == kF16 ? kOpF16 : kOpBF16, workspace, s, what);
 }
 
 extern "C" int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const int32_t* row_index,

@@ -154,63 +154,125 @@ __device__ __forceinline__ void lin_segment(const LinArgs& a, int seg, int64_t* 
   }
 }
 
+// Sum of v over this lane and the lanes below it: four DPP shifts inside the
+// rows of 16 lanes, then the rows' last lanes broadcast to the rows above.
+__device__ __forceinline__ uint32_t lin_wave_scan(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // Every wave of the workgroup calls this with the same arguments. BM list
 // entries per tile, n_pt tiles along p. Workgroups are dealt to the eight XCDs
 // round robin, so workgroup b takes tile (b % 8) * (total / 8) + b / 8 of the
 // list: an XCD's concurrent tiles are neighbours and share rows in its L2.
 // Inside a group the tiles go in strips of kStrip tiles along q, p outer.
+//
+// A lane holds the bounds of up to kSegRegs segments, all loaded at once: a
+// single token's product takes a few microseconds, of which every dependent load
+// here would be a tenth. More segments than 64 kSegRegs are read in a loop, twice.
+constexpr int kSegRegs = 4;
 template <int BM, int kStrip = 8>
 __device__ inline bool lin_find_tile(const LinArgs& a, uint32_t n_pt, LinTile* t) {
   const uint32_t lane = threadIdx.x & 63;
-  const int n_seg = a.offsets ? a.G + 2 : 1;
-  const int per = (n_seg + 63) >> 6;
-  uint32_t own = 0;
-  if (a.offsets) {
-    for (int i = 0; i < per; ++i) {
-      const int seg = static_cast<int>(lane) * per + i;
-      int64_t b = 0, e = 0;
-      if (seg < n_seg) lin_segment(a, seg, &b, &e);
-      if (e > b) own += static_cast<uint32_t>((e - b + BM - 1) / BM);
-    }
-  } else if (lane == 0) {
-    own = static_cast<uint32_t>((a.M + BM - 1) / BM);
-  }
-  uint32_t incl = own;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t up = __shfl_up(incl, d);
-    if (lane >= static_cast<uint32_t>(d)) incl += up;
-  }
-  const uint32_t total = __builtin_amdgcn_readlane(incl, 63) * n_pt;
   const uint32_t bid = blockIdx.x;
-  if (bid >= total) return false;
-  const uint32_t x = bid & 7, rem = total & 7;
-  const uint32_t id = x * (total >> 3) + (x < rem ? x : rem) + (bid >> 3);
-  const uint32_t mt_all = id / n_pt;
-  const uint64_t hit = __ballot(mt_all >= incl - own && mt_all < incl);
-  if (hit == 0) return false;  // offsets that overlap may wrap the sums
-  const int src = __builtin_ctzll(hit);
-  uint32_t base = __builtin_amdgcn_readlane(incl - own, src);
-  int64_t b = 0, e = a.M;
+  auto tiles_of = [](int64_t b, int64_t e) -> uint32_t {
+    return e > b ? static_cast<uint32_t>(static_cast<uint64_t>(e - b + BM - 1) / BM) : 0u;
+  };
+  auto remap = [&](uint32_t total) -> uint32_t {
+    const uint32_t x = bid & 7, rem = total & 7;
+    return x * (total >> 3) + (x < rem ? x : rem) + (bid >> 3);
+  };
+  uint32_t id, base = 0, tiles = 0;
+  int32_t b = 0, e = static_cast<int32_t>(a.M);
   int g = 0;
-  uint32_t tiles = __builtin_amdgcn_readlane(own, src);
-  if (a.offsets) {
-    for (int i = 0; i < per; ++i) {
-      g = src * per + i;
-      lin_segment(a, g, &b, &e);
-      tiles = e > b ? static_cast<uint32_t>((e - b + BM - 1) / BM) : 0;
-      if (mt_all < base + tiles) break;
-      base += tiles;
+  if (!a.offsets) {
+    tiles = tiles_of(0, a.M);
+    if (bid >= tiles * n_pt) return false;
+    id = remap(tiles * n_pt);
+  } else if (a.G + 2 <= 64 * kSegRegs) {
+    int32_t sb[kSegRegs], se[kSegRegs];
+    uint32_t own[kSegRegs], incl[kSegRegs];
+#pragma unroll
+    for (int k = 0; k < kSegRegs; ++k) {
+      const int s = 64 * k + static_cast<int>(lane);
+      sb[k] = a.offsets[s <= a.G ? s : a.G];
+      se[k] = a.offsets[s < a.G ? s + 1 : 0];
     }
+    uint32_t total = 0;
+#pragma unroll
+    for (int k = 0; k < kSegRegs; ++k) {
+      // segment s: offsets[s] to offsets[s + 1], with M after the last one; then
+      // the entries before the first
+      const int s = 64 * k + static_cast<int>(lane);
+      sb[k] = s <= a.G ? sb[k] : 0;
+      se[k] = s == a.G ? e : (s <= a.G + 1 ? se[k] : 0);
+      sb[k] = sb[k] < 0 ? 0 : (sb[k] > e ? e : sb[k]);
+      se[k] = se[k] < 0 ? 0 : (se[k] > e ? e : se[k]);
+      own[k] = se[k] > sb[k] ? static_cast<uint32_t>(se[k] - sb[k] + BM - 1) / BM : 0u;
+      incl[k] = total + lin_wave_scan(own[k]);
+      total = __builtin_amdgcn_readlane(incl[k], 63);
+    }
+    if (bid >= total * n_pt) return false;
+    id = remap(total * n_pt);
+    const uint32_t mt = id / n_pt;
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < kSegRegs; ++k) {
+      const uint64_t hit = __ballot(mt >= incl[k] - own[k] && mt < incl[k]);
+      if (!found && hit) {
+        const int src = __builtin_ctzll(hit);
+        found = true;
+        g = 64 * k + src;
+        tiles = __builtin_amdgcn_readlane(own[k], src);
+        base = __builtin_amdgcn_readlane(incl[k], src) - tiles;
+        b = __builtin_amdgcn_readlane(sb[k], src);
+        e = __builtin_amdgcn_readlane(se[k], src);
+      }
+    }
+    if (!found) return false;  // offsets that overlap may wrap the sums
+  } else {
+    uint32_t total = 0;
+    for (int s0 = 0; s0 < a.G + 2; s0 += 64) {
+      int64_t lo = 0, hi = 0;
+      if (s0 + static_cast<int>(lane) < a.G + 2) lin_segment(a, s0 + lane, &lo, &hi);
+      total += __builtin_amdgcn_readlane(lin_wave_scan(tiles_of(lo, hi)), 63);
+    }
+    if (bid >= total * n_pt) return false;
+    id = remap(total * n_pt);
+    const uint32_t mt = id / n_pt;
+    bool found = false;
+    for (int s0 = 0; s0 < a.G + 2 && !found; s0 += 64) {
+      int64_t lo = 0, hi = 0;
+      if (s0 + static_cast<int>(lane) < a.G + 2) lin_segment(a, s0 + lane, &lo, &hi);
+      const uint32_t own = tiles_of(lo, hi), incl = base + lin_wave_scan(own);
+      const uint64_t hit = __ballot(mt >= incl - own && mt < incl);
+      if (hit) {
+        const int src = __builtin_ctzll(hit);
+        found = true;
+        g = s0 + src;
+        tiles = __builtin_amdgcn_readlane(own, src);
+        base = __builtin_amdgcn_readlane(incl, src) - tiles;
+        b = __builtin_amdgcn_readlane(static_cast<int32_t>(lo), src);
+        e = __builtin_amdgcn_readlane(static_cast<int32_t>(hi), src);
+      } else {
+        base = __builtin_amdgcn_readlane(incl, 63);
+      }
+    }
+    if (!found) return false;
   }
   const uint32_t local = id - base * n_pt;
   const uint32_t strip = local / (kStrip * n_pt);
   const uint32_t in = local - strip * kStrip * n_pt;
   const uint32_t left = tiles - strip * kStrip;
   const uint32_t sm = left < kStrip ? left : kStrip;
-  t->g = __builtin_amdgcn_readfirstlane(g);
-  t->pt = __builtin_amdgcn_readfirstlane(static_cast<int>(in / sm));
-  t->q0 = b + static_cast<int64_t>(__builtin_amdgcn_readfirstlane(strip * kStrip + in % sm)) * BM;
+  t->g = g;
+  t->pt = static_cast<int>(in / sm);
+  t->q0 = b + static_cast<int64_t>(strip * kStrip + in % sm) * BM;
   t->q_end = e;
   return true;
 }
@@ -218,8 +280,8 @@ __device__ inline bool lin_find_tile(const LinArgs& a, uint32_t n_pt, LinTile* t
 // Row of the gathered operand that list entry t reads (indexes are clamped,
 // never followed out of the matrix).
 __device__ __forceinline__ int64_t lin_row(const LinArgs& a, int64_t t) {
-  if (!a.row_index) return t;
-  int64_t r = a.row_index[t];
+  int64_t r = t;
+  if (a.row_index) r = a.row_index[t];
   r = r < 0 ? 0 : r;
   return r < a.n_rows ? r : a.n_rows - 1;
 }
@@ -245,6 +307,17 @@ __device__ __forceinline__ void lin_scale4(const LinArgs& a, int g, int p, float
   }
 }
 
+// Two results rounded half-even to 16 bits (one conversion each pair on bf16).
+template <int TYPE>
+__device__ __forceinline__ uint32_t lin_pack2(float x, float y) {
+  if constexpr (TYPE == kF16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
+  } else {
+    return __builtin_bit_cast(uint32_t,
+                              lin_bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+  }
+}
 __device__ __forceinline__ uint16_t lin_round16(float v, int type) {
   return type == kF16 ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);
 }

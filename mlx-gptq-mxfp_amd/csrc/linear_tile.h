@@ -21,7 +21,7 @@ struct LinPlanArgs {
   LinUnit* units;
   LinSplit* splits;
   float* partials;
-  int npt, nqt;
+  int npt, nqt, bq;
   int cap;
   int max_units, max_splits, max_slots;
   int deal;  // whole units per XCD
@@ -65,9 +65,18 @@ inline int64_t lin_row_tiles(const LinArgs& a, int bm) {
   return a.offsets ? a.M / bm + (segs < a.M ? segs : a.M) : ceil_div(a.M, bm);
 }
 
-bool lin_tile_takes(const LinArgs& a, int op, int kind);
-int lin_tile_rows(const LinArgs& a, int op, int kind, int fq, hipStream_t s, const char* what);
-LinPlanSizes lin_plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K);
+// Output tile of a product over rows: 64, 128 or 256 entries by 256 columns, or
+// 64 by 128. staged: through registers (up to 128 entries).
+struct LinTileShape {
+  int rows, cols;
+  bool staged;
+};
+
+// Whether the operands' rows start and end on 16-byte boundaries.
+bool lin_tile_direct(const LinArgs& a, int op, int kind);
+int lin_tile_rows(const LinArgs& a, int op, int kind, LinTileShape t, hipStream_t s,
+                  const char* what);
+int64_t lin_tile_wgrad_bytes(int64_t M, int64_t G, int64_t N, int64_t K);
 int lin_tile_wgrad(const LinArgs& a, int op, void* workspace, hipStream_t s, const char* what);
 
 }  // namespace mgq

@@ -1,15 +1,19 @@
-// Large tiles of the matrix products, for operands whose rows start and end on
-// 16-byte boundaries (linear_common.h has the products and their operands).
+// Large tiles of the matrix products (linear_common.h has the products and their
+// operands).
 //
 // Tile kernel: 512 threads = 8 waves, 2 along q and 4 along p, one workgroup
-// per CU. A wave owns 32 FQ x 64 outputs as FQ x 2 blocks of a 32x32 MFMA (at
-// FQ = 4 a 256 x 256 tile, 128 fp32 accumulators per lane).
+// per CU. A wave owns 32 FQ x 32 FP outputs as blocks of a 32x32 MFMA (FQ = 4,
+// FP = 2: a 256 x 256 tile, 128 fp32 accumulators per lane).
 //
 //   - A stage is 128 bytes of every row: 64 16-bit or 128 int8 elements of the
-//     contraction, four K-steps of one MFMA depth each. The rows go from memory
-//     straight into LDS (global_load_lds_dwordx4, 16 bytes a lane), NB stages
-//     deep. What lies past the contraction's end reads a page of zeros; rows past
-//     the operand's end repeat its last row and their results are not stored.
+//     contraction, four K-steps of one MFMA depth each. Rows that start and end on
+//     16-byte boundaries go from memory straight into LDS
+//     (global_load_lds_dwordx4, 16 bytes a lane), NB stages deep. Other rows
+//     (STAGED) go through registers, loaded a stage ahead of their way into LDS,
+//     with 16-byte loads at any address; a piece that a row ends in is masked, and
+//     read element by element only where the 16 bytes would leave the tensor.
+//     What lies past the contraction's end is zeros; rows past the operand's end
+//     repeat its last row and their results are not stored.
 //   - Plain operands keep 128-byte rows in LDS. The 16-byte chunk c of row r
 //     sits at c ^ (r / 2 % 8): the lanes of an MFMA operand read the same chunk of
 //     32 consecutive rows, and any 16 of them cover all 64 banks once.
@@ -22,17 +26,17 @@
 //     a stage and its codes in one or two 16-byte reads; they are decoded to bf16
 //     in registers, two a conversion, 8 conversions beside 8 MFMAs.
 //   - K-step schedule: each MFMA is followed by its share of the next K-step's
-//     LDS reads, and in the first K-step after a stage's barrier by the loads of
-//     the stage that takes the buffer just released. The last K-step of a stage
-//     runs after the barrier, over the first reads of the next stage.
+//     LDS reads and of the loads of the stage that takes the buffer released by
+//     the last barrier. The last K-step of a stage runs after the barrier, over the
+//     first reads of the next stage.
 #include "linear_tile.h"
 
 namespace mgq {
 namespace {
 
-constexpr int kBP = 256;
-constexpr int kRowB = 128;  // bytes of a plain row per stage
 constexpr int kLdsMax = 160 * 1024;
+constexpr int kSteps = 4;    // K-steps per stage
+constexpr int kRowB = 128;   // bytes of a plain row per stage
 
 __device__ uint32_t g_lin_zeros[64];  // never written: what lies past an operand's end
 
@@ -42,22 +46,28 @@ typedef short lin_s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) lin_s16x4_t lds_s16x4;
 typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
 
-// Wait until at most VM of this wave's loads are in flight and its LDS reads are
-// done, then for the other waves. The memory clobber orders the LDS accesses for
-// the compiler as __syncthreads would, without its wait for every load.
+// Wait until at most VM of this wave's loads are in flight (VM < 0: whatever is)
+// and its LDS accesses are done, then for the other waves. The memory clobber
+// orders the LDS accesses for the compiler as __syncthreads would, without its
+// wait for every load.
 template <int VM>
 __device__ __forceinline__ void stage_barrier() {
   static_assert(VM <= 63, "vmcnt range");
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(VM) : "memory");
+  if constexpr (VM >= 0)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(VM) : "memory");
+  else
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // 16 bytes (1 byte, widened to a dword) per lane from `src` to LDS at
-// dst + 16 (4) * lane.
+// dst + 16 (4) * lane. (One wait state between the write of m0 and its use.)
 __device__ __forceinline__ void dma16(uint32_t dst, uint64_t src) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src)
+               : "memory");
 }
 __device__ __forceinline__ void dma1(uint32_t dst, uint64_t src) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(dst), "v"(src) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(dst), "v"(src)
+               : "memory");
 }
 
 __device__ __forceinline__ lin_u32x4_t read16(uint32_t at) {
@@ -72,34 +82,60 @@ __device__ __forceinline__ lin_u32x4_t read_tr(uint32_t at, int pitch) {
   return lin_u32x4_t{l.x, l.y, h.x, h.y};
 }
 
-template <int OP>
-constexpr int p_stage_bytes() {
-  return OP == kOpMx4 ? kBP * 32 + kBP * 8 : OP == kOpMx8 ? kBP * 64 + kBP * 8 : kBP * kRowB;
+__device__ __forceinline__ lin_u32x4_t load16(uint64_t src) {
+  const lin_u128_u_t u = *reinterpret_cast<const lin_u128_u_t*>(src);
+  return lin_u32x4_t{u.v[0], u.v[1], u.v[2], u.v[3]};
 }
-template <int OP, int FQ>
-constexpr int n_buffers() {
-  const int n = kLdsMax / (64 * FQ * kRowB + p_stage_bytes<OP>());
-  return n > 4 ? 4 : n;
+// The first n bytes at `src` (n <= 0: none, n >= 16: all), zeros after them. 16
+// bytes are read where they lie before `end`, single elements otherwise.
+template <int ES>
+__device__ __forceinline__ lin_u32x4_t load_cut(uint64_t src, int64_t n, uint64_t end) {
+  lin_u32x4_t r = {0, 0, 0, 0};
+  if (n <= 0) return r;
+  if (src + 16 <= end) {
+    r = load16(src);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t left = n - 4 * i;
+      r[i] &= left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1u : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16 / ES; ++i)
+      if (i * ES < n) {
+        const uint32_t v = ES == 2 ? *reinterpret_cast<const uint16_t*>(src + 2 * i)
+                                   : *reinterpret_cast<const uint8_t*>(src + i);
+        r[i * ES / 4] |= v << (8 * ((i * ES) & 3));
+      }
+  }
+  return r;
 }
 
-template <int OP, int KIND, int FQ>
+template <int OP>
+constexpr int mx_stage_bytes(int bp) {
+  return OP == kOpMx4 ? bp * 32 + bp * 8 : bp * 64 + bp * 8;
+}
+
+template <int OP, int KIND, int FQ, int FP, bool STAGED>
 __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const LinPlanArgs pl) {
   constexpr bool PT = KIND != kLinForward;
   constexpr bool QT = KIND == kLinWgrad;
   constexpr bool MX = lin_is_mx<OP>();
   constexpr int ES = lin_esize<OP>();
-  constexpr int BQ = 64 * FQ;
+  constexpr int BQ = 64 * FQ, BP = 128 * FP;
   constexpr int QB = BQ * kRowB;                 // Q bytes per stage
-  constexpr int SB = QB + p_stage_bytes<OP>();   // stage bytes
-  constexpr int NB = n_buffers<OP, FQ>();
-  constexpr int EPI = BQ * kBP * 2;              // 16-bit results on their way out
-  constexpr int VQ = FQ;                         // loads per wave and stage
-  constexpr int VP = OP == kOpMx4 ? 2 : OP == kOpMx8 ? 3 : 4;
+  constexpr int SB = QB + (MX ? mx_stage_bytes<OP>(BP) : BP * kRowB);  // stage bytes
+  constexpr int NB = STAGED ? 2 : kLdsMax / SB < 4 ? kLdsMax / SB : 4;
+  constexpr int EPI = BQ * BP * 2;               // 16-bit results on their way out
+  constexpr int VQ = FQ;                         // 16-byte loads per lane and stage: Q,
+  constexpr int per = OP == kOpMx4 ? 2 : 4;      // (MX: 16-byte pieces of a row's codes)
+  constexpr int VC = OP == kOpMx8 ? FP : 1;      // codes, and one of a scale byte,
+  constexpr int VP = MX ? VC + 1 : 2 * FP;       // or a dense P
   constexpr int V = VQ + VP;
-  constexpr int NM = 2 * FQ;                     // MFMAs per K-step
+  constexpr int NM = FP * FQ;                    // MFMAs per K-step
   constexpr int EK = kRowB / ES;                 // contraction elements per stage
   static_assert(NB >= 2 && (NB - 2) * V <= 63, "stages");
-  static_assert(!QT || FQ == 4, "transposed Q tiles are 256 wide");
+  static_assert(!QT || FQ >= 2, "transposed Q tiles are 128 or 256 wide");
   __shared__ __attribute__((aligned(1024))) char lds[NB * SB > EPI ? NB * SB : EPI];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -120,13 +156,13 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     c_begin = u.t0;
     c_len = u.t1 - u.t0;
     q0 = static_cast<int64_t>(tile % pl.nqt) * BQ;
-    p0 = tile / pl.nqt * kBP;
+    p0 = tile / pl.nqt * BP;
     q_end = a.nq;
   } else {
     LinTile t;
-    if (!lin_find_tile<BQ>(a, (a.np + kBP - 1) / kBP, &t)) return;
+    if (!lin_find_tile<BQ>(a, (a.np + BP - 1) / BP, &t)) return;
     g = t.g;
-    p0 = t.pt * kBP;
+    p0 = t.pt * BP;
     q0 = t.q0;
     q_end = t.q_end;
     if (g >= a.G) c_len = 0;  // entries of no group: zeros
@@ -138,20 +174,26 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   // ---- loads ------------------------------------------------------------
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char*)lds));
   const uint64_t zeros = reinterpret_cast<uint64_t>(g_lin_zeros);
-  // plain rows: instruction i of a wave takes rows 8 (n wave + i) .. + 7, lane l
-  // the chunk l % 8 of row l / 8, which holds the row's chunk ^ its swizzle
-  // (that depends on i's parity only)
+  // plain rows: load i of a wave takes rows 8 (n wave + i) .. + 7, lane l the place
+  // l % 8 of row l / 8, which holds the row's chunk ^ its swizzle (that depends on
+  // i's parity only)
   const int ch0 = (lane & 7) ^ ((lane >> 4) & 7), ch1 = ch0 ^ 4;
-  // transposed rows: instruction i takes contraction rows 8 wave + 2 i, + 1
-  const int tr_row = 8 * wave + half;
-  const int tc0 = (lane & 31) ^ (4 * half), tc1 = tc0 ^ 8;
-  uint64_t qp[VQ], pp[MX ? VP : 4];
+  // transposed rows, W columns: a load takes 512 / W of the stage's 64 contraction
+  // rows, a wave eight of them; lane l the place l % (W / 8) of its row, which holds
+  // the row's chunk ^ 4 (row % 4)
+  auto tr_row = [&](int W, int i) { return 8 * wave + (512 / W) * i + lane / (W / 8); };
+  auto tr_col = [&](int W, int i) { return 8 * ((lane % (W / 8)) ^ (4 * (tr_row(W, i) & 3))); };
+  // MX: mxfp4 codes and the scales of 128 rows are four loads, which waves 4..7
+  // repeat so that every wave has the same loads to wait for
+  const int mx_wave = FP == 2 ? wave : wave & 3;
+  uint64_t qp[VQ], pp[VP];
   if constexpr (QT) {
 #pragma unroll
     for (int i = 0; i < VQ; ++i) {
-      int64_t col = q0 + 8 * (i & 1 ? tc1 : tc0);
-      col = col + 8 <= a.nq ? col : a.nq - 8;
-      qp[i] = reinterpret_cast<uint64_t>(a.Q) + (c_begin + tr_row + 2 * i) * a.ldq + 2 * col;
+      int64_t col = q0 + tr_col(BQ, i);
+      if (!STAGED) col = col + 8 <= a.nq ? col : a.nq - 8;
+      if (STAGED) col = col < a.nq ? col : a.nq - 1;
+      qp[i] = reinterpret_cast<uint64_t>(a.Q) + (c_begin + tr_row(BQ, i)) * a.ldq + 2 * col;
     }
   } else {
 #pragma unroll
@@ -159,47 +201,55 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       int64_t q = q0 + 8 * (VQ * wave + i) + (lane >> 3);
       q = q < q_end ? q : q_end - 1;
       const int64_t row = KIND == kLinForward ? lin_row(a, q) : q;
-      const int sw = ((VQ * wave + i) & 1) ? ch1 : ch0;
-      qp[i] = reinterpret_cast<uint64_t>(a.Q) + row * a.ldq + 16 * sw;
+      qp[i] = reinterpret_cast<uint64_t>(a.Q) + row * a.ldq + 16 * (((VQ * wave + i) & 1) ? ch1 : ch0);
     }
   }
-  const uint8_t* Psg = nullptr;
   if constexpr (MX) {
-    Psg = a.Ps + static_cast<int64_t>(gw) * a.np * (a.nc / 32);
-    constexpr int per = OP == kOpMx4 ? 2 : 4;  // 16-byte pieces of a row's codes
+    const uint8_t* Psg = a.Ps + static_cast<int64_t>(gw) * a.np * (a.nc / 32);
 #pragma unroll
-    for (int i = 0; i < VP - 1; ++i) {
-      const int r = 32 * wave + (64 / per) * i + lane / per;
+    for (int i = 0; i < VC; ++i) {
+      const int r = (64 / per) * (VC * (per == 2 ? mx_wave : wave) + i) + lane / per;
       const int pos = lane % per;
       const int c = per == 2 ? pos ^ ((r >> 3) & 1) : pos ^ ((r >> 2) & 3);
       const int p = p0 + r < a.np ? p0 + r : a.np - 1;
       pp[i] = reinterpret_cast<uint64_t>(Pg) + p * a.ldp + 16 * c;
     }
-    const int r = 32 * wave + (lane >> 1);
+    const int r = 32 * mx_wave + (lane >> 1);
     const int p = p0 + r < a.np ? p0 + r : a.np - 1;
-    pp[VP - 1] = reinterpret_cast<uint64_t>(Psg) + static_cast<int64_t>(p) * (a.nc / 32) + (lane & 1);
+    pp[VC] = reinterpret_cast<uint64_t>(Psg) + static_cast<int64_t>(p) * (a.nc / 32) + (lane & 1);
   } else if constexpr (PT) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      int64_t col = p0 + 8 * (i & 1 ? tc1 : tc0);
-      col = col + 8 <= a.np ? col : a.np - 8;
+    for (int i = 0; i < VP; ++i) {
+      int64_t col = p0 + tr_col(BP, i);
+      if (!STAGED) col = col + 8 <= a.np ? col : a.np - 8;
+      if (STAGED) col = col < a.np ? col : a.np - 1;
       // wgrad: the row is added when it is known
       pp[i] = reinterpret_cast<uint64_t>(Pg) + 2 * col +
-              (KIND == kLinWgrad ? 0 : (tr_row + 2 * i) * a.ldp);
+              (KIND == kLinWgrad ? 0 : tr_row(BP, i) * a.ldp);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * (4 * wave + i) + (lane >> 3);
+    for (int i = 0; i < VP; ++i) {
+      const int r = 8 * (VP * wave + i) + (lane >> 3);
       const int p = p0 + r < a.np ? p0 + r : a.np - 1;
       pp[i] = reinterpret_cast<uint64_t>(Pg) + p * a.ldp + 16 * (i & 1 ? ch1 : ch0);
     }
   }
+  // STAGED: where the operands end
+  uint64_t q_stop = 0, p_stop = 0;
+  if constexpr (STAGED) {
+    const int64_t q_rows = KIND == kLinForward ? a.n_rows : a.M;
+    const int64_t q_cols = QT ? a.nq : a.nc;
+    q_stop = reinterpret_cast<uint64_t>(a.Q) + (q_rows - 1) * a.ldq + q_cols * ES;
+    const int64_t p_rows = KIND == kLinWgrad ? a.n_rows : KIND == kLinDgrad ? a.nc : a.np;
+    const int64_t p_cols = PT ? a.np : a.nc;
+    p_stop = reinterpret_cast<uint64_t>(Pg) + (p_rows - 1) * a.ldp + p_cols * ES;
+  }
 
-  // wgrad: the rows of X that this wave loads in the next stage, two per
-  // instruction, read through the scalar cache (a vector load's wait would also
-  // wait for the loads into LDS before it)
-  uint32_t rows[8];
+  // wgrad: the rows of X that this wave loads in the next stage, read through the
+  // scalar cache (a vector load's wait would also wait for the loads into LDS
+  // before it)
+  uint32_t rows[8], rows_next[8];
   auto load_rows = [&](int st) {
     if constexpr (KIND == kLinWgrad) {
       const int64_t t0 = c_begin + static_cast<int64_t>(st) * EK + 8 * wave;
@@ -213,61 +263,123 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
           r = r < 0 ? 0 : r;
           r = r < a.n_rows ? r : static_cast<int32_t>(a.n_rows - 1);
         }
-        rows[i] = static_cast<uint32_t>(r);
+        rows_next[i] = static_cast<uint32_t>(r);
       }
     }
   };
+  auto take_rows = [&]() {
+    if constexpr (KIND == kLinWgrad) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rows[i] = rows_next[i];
+    }
+  };
 
-  // load i of stage st into buffer at LDS address `buf`
-  auto load = [&](int i, int st, uint32_t buf) {
+  // load i of stage st: where it comes from (advancing the pointer), how many bytes
+  // of it exist, and its place in the stage
+  auto source = [&](int i, int st, uint64_t* src, int64_t* n, uint32_t* dst) __attribute__((
+                    always_inline)) {
+    const int64_t left = c_len - static_cast<int64_t>(st) * EK;  // contraction elements
     if (i < VQ) {
-      bool ok;
+      *dst = (VQ * wave + i) * 1024;
+      *src = qp[i];
       if constexpr (QT) {
-        ok = tr_row + 2 * i < c_len - static_cast<int64_t>(st) * EK;
+        *n = tr_row(BQ, i) < left ? 16 : 0;
+        qp[i] += EK * a.ldq;
       } else {
-        const int64_t rem = (c_len - static_cast<int64_t>(st) * EK) * ES;
-        ok = 16 * (((VQ * wave + i) & 1) ? ch1 : ch0) < rem;
+        *n = left * ES - 16 * (((VQ * wave + i) & 1) ? ch1 : ch0);
+        qp[i] += kRowB;
       }
-      dma16(buf + (VQ * wave + i) * 1024, ok ? qp[i] : zeros);
-      qp[i] += QT ? EK * a.ldq : kRowB;
       return;
     }
     const int k = i - VQ;
+    *src = pp[k];
     if constexpr (MX) {
-      const int64_t rem = c_len / 32 - 2 * static_cast<int64_t>(st);  // MX groups left
-      constexpr int per = OP == kOpMx4 ? 2 : 4;
-      if (k < VP - 1) {
-        const int r = 32 * wave + (64 / per) * k + lane / per;
+      if (k < VC) {
+        const int at = VC * (per == 2 ? mx_wave : wave) + k;
+        const int r = (64 / per) * at + lane / per;
         const int pos = lane % per;
         const int c = per == 2 ? pos ^ ((r >> 3) & 1) : pos ^ ((r >> 2) & 3);
-        dma16(buf + QB + ((VP - 1) * wave + k) * 1024, (c * 2 / per) < rem ? pp[k] : zeros);
+        *dst = QB + at * 1024;
+        *n = 32 * (c * 2 / per) < left ? 16 : 0;  // whole MX groups
         pp[k] += 16 * per;
       } else {
-        dma1(buf + QB + kBP * 16 * per + wave * 256, (lane & 1) < rem ? pp[k] : zeros);
+        *dst = QB + BP * 16 * per + mx_wave * 256;
+        *n = 32 * (lane & 1) < left ? 1 : 0;
         pp[k] += 2;
       }
     } else if constexpr (PT) {
-      const bool ok = tr_row + 2 * k < c_len - static_cast<int64_t>(st) * EK;
-      uint64_t src = pp[k];
+      *dst = QB + (VP * wave + k) * 1024;
+      *n = tr_row(BP, k) < left ? 16 : 0;
       if constexpr (KIND == kLinWgrad) {
-        const uint32_t r = half ? rows[2 * k + 1] : rows[2 * k];
-        src += static_cast<uint64_t>(r) * static_cast<uint32_t>(a.ldp);
+        constexpr int RP = 512 / BP;  // rows per load
+        uint32_t r = rows[RP * k];
+#pragma unroll
+        for (int j = 1; j < RP; ++j) r = lane / (BP / 8) == j ? rows[RP * k + j] : r;
+        *src += static_cast<uint64_t>(r) * static_cast<uint64_t>(a.ldp);
       } else {
         pp[k] += EK * a.ldp;
       }
-      dma16(buf + QB + (4 * wave + k) * 1024, ok ? src : zeros);
     } else {
-      const int64_t rem = (c_len - static_cast<int64_t>(st) * EK) * ES;
-      dma16(buf + QB + (4 * wave + k) * 1024, 16 * (k & 1 ? ch1 : ch0) < rem ? pp[k] : zeros);
+      *dst = QB + (VP * wave + k) * 1024;
+      *n = left * ES - 16 * (k & 1 ? ch1 : ch0);
       pp[k] += kRowB;
     }
+  };
+  auto is_scale = [&](int i) { return MX && i == V - 1; };
+  // straight into LDS (rows are whole pieces: n is 16 or more, or nothing is left)
+  auto load = [&](int i, int st, uint32_t buf) __attribute__((always_inline)) {
+    uint64_t src;
+    int64_t n;
+    uint32_t dst;
+    source(i, st, &src, &n, &dst);
+    if (is_scale(i))
+      dma1(buf + dst, n > 0 ? src : zeros);
+    else
+      dma16(buf + dst, n > 0 ? src : zeros);
+  };
+  // through registers
+  lin_u32x4_t hold[STAGED ? V : 1];
+  auto fetch = [&](int i, int st) __attribute__((always_inline)) {
+    uint64_t src;
+    int64_t n;
+    uint32_t dst;
+    source(i, st, &src, &n, &dst);
+    const bool tr = i < VQ ? QT : PT;
+    if (is_scale(i)) {
+      const uint32_t v = *reinterpret_cast<const uint8_t*>(n > 0 ? src : zeros);
+      hold[i] = lin_u32x4_t{v, 0, 0, 0};
+    } else if (tr || (MX && i >= VQ)) {
+      // a transposed row may end inside the piece: the columns past its end are not
+      // stored, but nothing is read past the tensor's end
+      const uint64_t stop = i < VQ ? q_stop : p_stop;
+      if (n > 0 && src + 16 > stop)
+        hold[i] = load_cut<ES>(src, static_cast<int64_t>(stop - src), stop);
+      else
+        hold[i] = load16(n > 0 ? src : zeros);
+    } else if (__builtin_amdgcn_readfirstlane((st + 1) * static_cast<int64_t>(EK) <= c_len)) {
+      hold[i] = load16(src);
+    } else {
+      hold[i] = load_cut<ES>(src, n, i < VQ ? q_stop : p_stop);
+    }
+  };
+  auto put = [&](int i, uint32_t buf) __attribute__((always_inline)) {
+    const int k = i - VQ;
+    uint32_t dst;
+    if (i < VQ) dst = (VQ * wave + i) * 1024;
+    else if (is_scale(i)) dst = QB + BP * 16 * per + mx_wave * 256;
+    else if (MX) dst = QB + (VC * (per == 2 ? mx_wave : wave) + k) * 1024;
+    else dst = QB + (VP * wave + k) * 1024;
+    if (is_scale(i))
+      *reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(buf + dst + 4 * lane) = hold[i][0];
+    else
+      *reinterpret_cast<lds_u32x4*>(buf + dst + 16 * lane) = hold[i];
   };
 
   // ---- LDS reads of a K-step's operands -----------------------------------
   // plain: chunk 2 ks + half of the row (MX: 4 half + ks, so that a half-wave
   // keeps to its MX group)
   const int sw = (lane >> 1) & 7;
-  uint32_t qa[4], pa[4];  // plain: by ks; transposed: by block
+  uint32_t qa[4], pa[4];  // plain: by K-step; transposed: by block
   const int j4 = (lane >> 2) & 3;
   const uint32_t tr_lane = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
 #pragma unroll
@@ -275,24 +387,23 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     const uint32_t c = 16 * ((MX ? 4 * half + k : 2 * k + half) ^ sw);
     qa[k] = QT ? (8 * half + j4) * (2 * BQ) + (((FQ * wq + k) ^ j4) * 64) + tr_lane
                : (32 * FQ * wq + (lane & 31)) * kRowB + c;
-    pa[k] = PT ? QB + (8 * half + j4) * (2 * kBP) + (((2 * wp + (k & 1)) ^ j4) * 64) + tr_lane
-               : QB + (64 * wp + (lane & 31)) * kRowB + c;
+    pa[k] = PT ? QB + (8 * half + j4) * (2 * BP) + (((FP * wp + (k & (FP - 1))) ^ j4) * 64) + tr_lane
+               : QB + (32 * FP * wp + (lane & 31)) * kRowB + c;
   }
   uint32_t code_at[2], scale_at = 0;
   if constexpr (MX) {
-    constexpr int per = OP == kOpMx4 ? 2 : 4;
-    const int r = 64 * wp + (lane & 31);
+    const int r = 32 * FP * wp + (lane & 31);
 #pragma unroll
     for (int k = 0; k < per / 2; ++k) {
       const int c = per == 2 ? half : 2 * half + k;
       const int pos = per == 2 ? c ^ ((r >> 3) & 1) : c ^ ((r >> 2) & 3);
       code_at[k] = QB + r * 16 * per + 16 * pos;
     }
-    scale_at = QB + kBP * 16 * per + (2 * r + half) * 4;
+    scale_at = QB + BP * 16 * per + (2 * r + half) * 4;
   }
-  lin_u32x4_t fq[2][FQ], fp[2][2];
-  lin_u32x4_t codes[2][2];
-  uint32_t scale[2];
+  lin_u32x4_t fq[2][FQ], fp[2][FP];
+  lin_u32x4_t codes[FP][2];
+  uint32_t scale[FP];
   auto read_q = [&](int b, int f, int ks, uint32_t buf) {
     if constexpr (QT)
       fq[b][f] = read_tr(buf + qa[f] + 16 * ks * (2 * BQ), 2 * BQ);
@@ -301,12 +412,11 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   };
   auto read_p = [&](int b, int f, int ks, uint32_t buf) {
     if constexpr (PT)
-      fp[b][f] = read_tr(buf + pa[f] + 16 * ks * (2 * kBP), 2 * kBP);
+      fp[b][f] = read_tr(buf + pa[f] + 16 * ks * (2 * BP), 2 * BP);
     else
       fp[b][f] = read16(buf + pa[ks] + f * 32 * kRowB);
   };
   auto read_codes = [&](int f, uint32_t buf) {
-    constexpr int per = OP == kOpMx4 ? 2 : 4;
 #pragma unroll
     for (int k = 0; k < per / 2; ++k) codes[f][k] = read16(buf + code_at[k] + f * 32 * 16 * per);
     scale[f] = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(
@@ -319,67 +429,112 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       fp[b][f] = lin_decode_mx8(codes[f][ks >> 1][2 * (ks & 1)], codes[f][ks >> 1][2 * (ks & 1) + 1],
                                 scale[f]);
   };
-  // read r of a K-step (dense: p0 q0 p1 q1 q2 q3; MX: the q only)
-  constexpr int NR = MX ? FQ : FQ + 2;
+  // read r of a K-step (dense: p0 q0 p1 .. q1 ..; MX: the q only)
+  constexpr int NR = MX ? FQ : FQ + FP;
   auto read = [&](int r, int b, int ks, uint32_t buf) {
     if constexpr (MX) {
       read_q(b, r, ks, buf);
-    } else if constexpr (FQ == 1) {
-      if (r == 1) read_q(b, 0, ks, buf);
-      else read_p(b, r >> 1, ks, buf);
     } else {
       if (r == 0) read_p(b, 0, ks, buf);
-      else if (r == 2) read_p(b, 1, ks, buf);
-      else read_q(b, r == 1 ? 0 : r - 2, ks, buf);
+      else if (r == 1) read_q(b, 0, ks, buf);
+      else if (r <= FP) read_p(b, r - 1, ks, buf);
+      else read_q(b, r - FP, ks, buf);
     }
   };
 
   typedef typename LinAcc<OP>::t32 acc_t;
-  acc_t acc[FQ][2];
+  acc_t acc[FQ][FP];
 #pragma unroll
   for (int i = 0; i < FQ; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < FP; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  auto mfma = [&](int b, int j) {
+    acc[j / FP][j % FP] = lin_mfma32<OP>(fp[b][j % FP], fq[b][j / FP], acc[j / FP][j % FP]);
+  };
+  auto decode_all = [&](int b, int ks) {
+#pragma unroll
+    for (int f = 0; f < FP; ++f) decode(b, f, ks);
+  };
 
+  // Slot t of a stage's period (four K-steps of NM MFMAs; the first K-step's MFMAs
+  // are the previous stage's last): the reads of the next K-step come first, so
+  // that none is young at the barrier; the loads of stage s + NB - 1, into the
+  // buffer that the barrier released, are spread over the period, because a load
+  // instruction occupies the address unit of the CU for 16 cycles and all eight
+  // waves issue theirs in the same slots; with two buffers over its first half,
+  // because the next barrier waits for them. STAGED: what was loaded in the last
+  // period goes into LDS, and the next stage's loads take its registers.
+  constexpr int SPREAD = NB == 2 ? kSteps / 2 : kSteps;
+  constexpr int RPS = (NR + NM - 1) / NM;
+  constexpr int WAIT = STAGED ? -1 : (NB - 2) * V;
+  auto slot_reads = [&](int j, int b, int ks, uint32_t buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = j * RPS; r < (j + 1) * RPS && r < NR; ++r) read(r, b, ks, buf);
+  };
+  auto slot_loads = [&](int t, int st, uint32_t buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = t * V / (NM * SPREAD); i < (t + 1) * V / (NM * SPREAD) && i < V; ++i) {
+      if constexpr (STAGED) {
+        put(i, buf);
+        fetch(i, st + 1);
+      } else {
+        load(i, st, buf);
+      }
+    }
+  };
   if (n_stages > 0) {
+    if constexpr (STAGED) {
+      load_rows(0);
+      take_rows();
 #pragma unroll
-    for (int st = 0; st < NB - 1; ++st) {
-      load_rows(st);
+      for (int i = 0; i < V; ++i) fetch(i, 0);
+      load_rows(1);
+      take_rows();
 #pragma unroll
-      for (int i = 0; i < V; ++i) load(i, st, lds0 + st * SB);
+      for (int i = 0; i < V; ++i) {
+        put(i, lds0);
+        fetch(i, 1);
+      }
+      load_rows(2);
+    } else {
+#pragma unroll
+      for (int st = 0; st < NB - 1; ++st) {
+        load_rows(st);
+        take_rows();
+#pragma unroll
+        for (int i = 0; i < V; ++i) load(i, st, lds0 + st * SB);
+      }
+      load_rows(NB - 1);
     }
-    load_rows(NB - 1);
-    stage_barrier<(NB - 2) * V>();
+    stage_barrier<WAIT>();
+    take_rows();
     if constexpr (MX) {
-      read_codes(0, lds0);
-      read_codes(1, lds0);
+#pragma unroll
+      for (int f = 0; f < FP; ++f) read_codes(f, lds0);
     }
+    uint32_t wbuf = lds0 + (NB - 1) * SB;
 #pragma unroll
     for (int r = 0; r < NR; ++r) read(r, 0, 0, lds0);
 #pragma unroll
-    for (int i = 0; i < V; ++i) load(i, NB - 1, lds0 + (NB - 1) * SB);
-    load_rows(NB);
-    if constexpr (MX) {
-      decode(0, 0, 0);
-      decode(0, 1, 0);
-    }
+    for (int j = 0; j < NM; ++j) slot_loads(j, NB - 1, wbuf);
+    if constexpr (MX) decode_all(0, 0);
     __builtin_amdgcn_sched_barrier(0);
     int rb = 0;
     for (int s = 0; s < n_stages; ++s) {
       const uint32_t buf = lds0 + rb * SB;
+      load_rows(s + NB + (STAGED ? 1 : 0));
 #pragma unroll
-      for (int ks = 1; ks < 4; ++ks) {
+      for (int ks = 1; ks < kSteps; ++ks) {
         const int b = (ks - 1) & 1;
 #pragma unroll
         for (int j = 0; j < NM; ++j) {
-          acc[j >> 1][j & 1] = lin_mfma32<OP>(fp[b][j & 1], fq[b][j >> 1], acc[j >> 1][j & 1]);
-#pragma unroll
-          for (int r = j * NR / NM; r < (j + 1) * NR / NM; ++r) read(r, b ^ 1, ks, buf);
+          mfma(b, j);
+          slot_reads(j, b ^ 1, ks, buf);
+          slot_loads(ks * NM + j, s + NB - 1, wbuf);
           if constexpr (MX) {
-            if (j == 0) decode(b ^ 1, 0, ks);
-            if (j == NM / 2) decode(b ^ 1, 1, ks);
+            if (j % FQ == 0) decode(b ^ 1, j / FQ, ks);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -387,45 +542,40 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       if (s + 1 == n_stages) break;
       rb = rb + 1 == NB ? 0 : rb + 1;
       const uint32_t next = lds0 + rb * SB;
-      stage_barrier<(NB - 2) * V>();
+      wbuf = buf;
+      stage_barrier<WAIT>();
+      take_rows();
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (MX) {
-        read_codes(0, next);
-        read_codes(1, next);
+#pragma unroll
+        for (int f = 0; f < FP; ++f) read_codes(f, next);
       }
 #pragma unroll
       for (int j = 0; j < NM; ++j) {
-        acc[j >> 1][j & 1] = lin_mfma32<OP>(fp[1][j & 1], fq[1][j >> 1], acc[j >> 1][j & 1]);
-#pragma unroll
-        for (int r = j * NR / NM; r < (j + 1) * NR / NM; ++r) read(r, 0, 0, next);
-#pragma unroll
-        for (int i = j * V / NM; i < (j + 1) * V / NM; ++i) load(i, s + NB, buf);
+        mfma(1, j);
+        slot_reads(j, 0, 0, next);
+        slot_loads(j, s + NB, wbuf);
         __builtin_amdgcn_sched_barrier(0);
       }
-      load_rows(s + NB + 1);
-      if constexpr (MX) {
-        decode(0, 0, 0);
-        decode(0, 1, 0);
-      }
+      if constexpr (MX) decode_all(0, 0);
     }
 #pragma unroll
-    for (int j = 0; j < NM; ++j)
-      acc[j >> 1][j & 1] = lin_mfma32<OP>(fp[1][j & 1], fq[1][j >> 1], acc[j >> 1][j & 1]);
+    for (int j = 0; j < NM; ++j) mfma(1, j);
   }
 
   // ---- results ------------------------------------------------------------
   if (KIND == kLinWgrad && slot >= 0) {
-    // a partial tile: fp32, [256][256]
-    float* o = pl.partials + static_cast<int64_t>(slot) * BQ * kBP;
+    // a partial tile: fp32, [BQ][BP]
+    float* o = pl.partials + static_cast<int64_t>(slot) * BQ * BP;
 #pragma unroll
     for (int f = 0; f < FQ; ++f)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < FP; ++k)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int q = 32 * (FQ * wq + f) + (lane & 31);
-          const int p = 64 * wp + 32 * k + 8 * r + 4 * half;
-          *reinterpret_cast<float4*>(o + q * kBP + p) =
+          const int p = 32 * FP * wp + 32 * k + 8 * r + 4 * half;
+          *reinterpret_cast<float4*>(o + q * BP + p) =
               float4{static_cast<float>(acc[f][k][4 * r]), static_cast<float>(acc[f][k][4 * r + 1]),
                      static_cast<float>(acc[f][k][4 * r + 2]),
                      static_cast<float>(acc[f][k][4 * r + 3])};
@@ -444,149 +594,183 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   }
   char* out = a.out + (KIND == kLinWgrad ? g * a.o_group : 0) * (a.out_type == kF32 ? 4 : 2);
   lds_handover();  // every wave is done with the last stage's buffer
-  // 16-bit results go through LDS (a wave's own part of it) to leave as 128-byte
-  // pieces of a row; the chunk swizzle is the operands'
-  char* part = lds + wave * (32 * FQ * kRowB);
+  // Results go through LDS (a wave's own part of it) to leave as whole pieces of a
+  // row: 64 columns of 16-bit results or 32 of fp32 at a time, rows of 128 bytes
+  // (64 at FP = 1) with the operands' chunk swizzle.
+  auto store_out = [&](auto type) __attribute__((always_inline)) {
+    constexpr int T = decltype(type)::value;
+    constexpr int OS = T == kF32 ? 4 : 2;
+    constexpr int KP = T == kF32 || FP == 1 ? 1 : 2;  // 32-column blocks per pass
+    constexpr int RB = 32 * KP * OS, CH = RB / 16;    // bytes and 16-byte chunks of a row
+    constexpr int EC = 16 / OS;                       // results per chunk
+    auto swizzle = [](int row) { return CH == 8 ? (row >> 1) & 7 : (row >> 2) & 3; };
+    char* part = lds + wave * (32 * FQ * RB);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+    for (int k0 = 0; k0 < FP; k0 += KP) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int p = p0 + 64 * wp + 32 * k + 8 * r + 4 * half;
-      float sw4[4] = {0, 0, 0, 0}, b4[4] = {0, 0, 0, 0};
-      if constexpr (OP == kOpI8) {
-        const int64_t c = static_cast<int64_t>(gw) * a.np;
+      for (int k = k0; k < k0 + KP; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t ce = c + (p + e < a.np ? p + e : a.np - 1);
-          sw4[e] = a.sw[ce];
-          if (a.bias) b4[e] = a.bias[ce];
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < FQ; ++f) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = static_cast<float>(acc[f][k][4 * r + e]);
+        for (int r = 0; r < 4; ++r) {
+          const int p = p0 + 32 * (FP * wp + k) + 8 * r + 4 * half;
+          float sw4[4] = {0, 0, 0, 0}, b4[4] = {0, 0, 0, 0};
           if constexpr (OP == kOpI8) {
-            v[e] = v[e] * sx[f] * sw4[e];
-            if (a.bias) v[e] = v[e] + b4[e];
-            if (g >= a.G) v[e] = 0.0f;
+            const int64_t c = static_cast<int64_t>(gw) * a.np;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int64_t ce = c + (p + e < a.np ? p + e : a.np - 1);
+              sw4[e] = a.sw[ce];
+              if (a.bias) b4[e] = a.bias[ce];
+            }
+          }
+#pragma unroll
+          for (int f = 0; f < FQ; ++f) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[e] = static_cast<float>(acc[f][k][4 * r + e]);
+              if constexpr (OP == kOpI8) {
+                v[e] = v[e] * sx[f] * sw4[e];
+                if (a.bias) v[e] = v[e] + b4[e];
+                if (g >= a.G) v[e] = 0.0f;
+              }
+            }
+            const int row = 32 * f + (lane & 31);
+            if constexpr (T == kF32) {
+              *reinterpret_cast<float4*>(part + row * RB + 16 * ((2 * r + half) ^ swizzle(row))) =
+                  float4{v[0], v[1], v[2], v[3]};
+            } else {
+              uint2 h;
+              h.x = lin_pack2<T>(v[0], v[1]);
+              h.y = lin_pack2<T>(v[2], v[3]);
+              *reinterpret_cast<uint2*>(part + row * RB +
+                                        16 * ((4 * (k - k0) + r) ^ swizzle(row)) + 8 * half) = h;
+            }
           }
         }
-        const int row = 32 * f + (lane & 31);
-        if (a.out_type == kF32) {
-          const int64_t q = q0 + 32 * FQ * wq + row;
-          if (q < q_end && p < a.np)
-            lin_store4(a, out + q * a.ldo * 4, p, v);
+      __builtin_amdgcn_wave_barrier();
+      // the loop stays small: it is most of what a short contraction runs
+#pragma unroll 4
+      for (int i = 0; i < 32 * FQ * CH / 64; ++i) {
+        const int row = (64 / CH) * i + lane / CH;
+        const int c = (lane % CH) ^ swizzle(row);
+        const int64_t q = q0 + 32 * FQ * wq + row;
+        const int p = p0 + 32 * (FP * wp + k0) + EC * c;
+        const lin_u32x4_t v =
+            *reinterpret_cast<const lin_u32x4_t*>(part + row * RB + 16 * (lane % CH));
+        if (q >= q_end) continue;
+        char* o = out + (q * a.ldo + p) * OS;
+        if (a.vec_out == 2 && p + EC <= a.np) {
+          *reinterpret_cast<lin_u32x4_t*>(o) = v;
         } else {
-          uint2 h;
-          h.x = lin_round16(v[0], a.out_type) |
-                (static_cast<uint32_t>(lin_round16(v[1], a.out_type)) << 16);
-          h.y = lin_round16(v[2], a.out_type) |
-                (static_cast<uint32_t>(lin_round16(v[3], a.out_type)) << 16);
-          *reinterpret_cast<uint2*>(part + row * kRowB + 16 * ((4 * k + r) ^ ((row >> 1) & 7)) +
-                                    8 * half) = h;
+          for (int e = 0; e < EC && p + e < a.np; ++e) {
+            if constexpr (T == kF32)
+              reinterpret_cast<uint32_t*>(o)[e] = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
+            else
+              reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(
+                  (e < 2 ? v[0] : e < 4 ? v[1] : e < 6 ? v[2] : v[3]) >> (16 * (e & 1)));
+          }
         }
       }
+      if (k0 + KP < FP) __builtin_amdgcn_wave_barrier();
     }
-  if (a.out_type == kF32) return;
-  __builtin_amdgcn_wave_barrier();
-#pragma unroll
-  for (int i = 0; i < 4 * FQ; ++i) {
-    const int row = 8 * i + (lane >> 3);
-    const int c = (lane & 7) ^ ((row >> 1) & 7);
-    const int64_t q = q0 + 32 * FQ * wq + row;
-    const int p = p0 + 64 * wp + 8 * c;
-    const lin_u32x4_t v = *reinterpret_cast<const lin_u32x4_t*>(part + row * kRowB + 16 * (lane & 7));
-    if (q >= q_end) continue;
-    uint16_t* o = reinterpret_cast<uint16_t*>(out) + q * a.ldo + p;
-    if (a.vec_out == 2 && p + 8 <= a.np) {
-      *reinterpret_cast<lin_u32x4_t*>(o) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (p + e < a.np) o[e] = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
-    }
+  };
+  if (a.out_type == kF32) {
+    if constexpr (OP == kOpI8 || KIND != kLinForward) store_out(std::integral_constant<int, kF32>{});
+  } else if (a.out_type == kF16) {
+    if constexpr (OP == kOpI8 || OP == kOpF16) store_out(std::integral_constant<int, kF16>{});
+  } else {
+    if constexpr (OP != kOpF16) store_out(std::integral_constant<int, kBF16>{});
   }
 }
 
 // ---------------------------------------------------------------------------
-// wgrad's units: a group's entries, cut into chunks of at most `cap`, heaviest
-// first so that the last tiles to start are the shortest. One workgroup plans.
+// wgrad's units: a group's entries, cut into chunks of at most `cap`, longest
+// first so that the last tiles to start are the shortest. One workgroup plans, a
+// wave per group at a time: each place in the order is a sum over all groups.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(1024) lin_plan_kernel(const LinArgs a, const LinPlanArgs pl) {
-  __shared__ int32_t size[kLinPlanGroups], parts[kLinPlanGroups];
+  __shared__ int32_t size[kLinPlanGroups], parts[kLinPlanGroups], chunk[kLinPlanGroups];
   for (int g = threadIdx.x; g < a.G; g += 1024) {
     int64_t b = 0, e = a.M;
     if (a.offsets) lin_segment(a, g, &b, &e);
     const int n = e > b ? static_cast<int>(e - b) : 0;
+    const int k = n > pl.cap ? (n + pl.cap - 1) / pl.cap : 1;
     size[g] = n;
-    parts[g] = n > pl.cap ? (n + pl.cap - 1) / pl.cap : 1;
+    parts[g] = k;
+    chunk[g] = ((n + k - 1) / k + 63) & ~63;  // whole stages
   }
   __syncthreads();
-  for (int g = threadIdx.x; g < a.G; g += 1024) {
-    const int n = size[g], k = parts[g];
-    const int len = ((n + k - 1) / k + 63) & ~63;
-    int first = 0, slots = 0, splits = 0, units = 0, all_splits = 0;
-    for (int o = 0; o < a.G; ++o) {
-      const int no = size[o], ko = parts[o];
-      const int lo = (no + ko - 1) / ko;
-      const int lg = (n + k - 1) / k;
-      if (lo > lg || (lo == lg && o < g)) first += ko;
-      if (ko > 1) {
-        ++all_splits;
-        if (o < g) {
-          slots += ko;
-          ++splits;
+  const int lane = threadIdx.x & 63;
+  for (int g = threadIdx.x >> 6; g < a.G; g += 16) {
+    const int n = size[g], k = parts[g], len = chunk[g];
+    uint32_t first = 0, slots = 0, splits = 0, units = 0, all_splits = 0;
+    for (int o0 = 0; o0 < a.G; o0 += 64) {
+      const int o = o0 + lane;
+      uint32_t f = 0, sl = 0, sp = 0, un = 0, al = 0;
+      if (o < a.G) {
+        const int lo = chunk[o];
+        un = parts[o];
+        if (lo > len || (lo == len && o < g)) f = un;
+        al = un > 1;
+        if (o < g && un > 1) {
+          sl = un;
+          sp = 1;
         }
       }
-      units += ko;
+      first += __builtin_amdgcn_readlane(lin_wave_scan(f), 63);
+      slots += __builtin_amdgcn_readlane(lin_wave_scan(sl), 63);
+      splits += __builtin_amdgcn_readlane(lin_wave_scan(sp), 63);
+      units += __builtin_amdgcn_readlane(lin_wave_scan(un), 63);
+      all_splits += __builtin_amdgcn_readlane(lin_wave_scan(al), 63);
     }
     int64_t b = 0, e = a.M;
     if (a.offsets) lin_segment(a, g, &b, &e);
-    for (int i = 0; i < k; ++i) {
-      if (first + i >= pl.max_units) break;
+    // (a list whose offsets decrease may have more units than there is room for)
+    const bool room = slots + k <= static_cast<uint32_t>(pl.max_slots);
+    for (int i = lane; i < k; i += 64) {
+      if (first + i >= static_cast<uint32_t>(pl.max_units)) break;
+      const int64_t t0 = static_cast<int64_t>(i) * len, t1 = t0 + len;
       LinUnit u;
       u.g = g;
-      const int64_t t0 = static_cast<int64_t>(i) * len, t1 = t0 + len;
       u.t0 = static_cast<int32_t>(b + (t0 < n ? t0 : n));
       u.t1 = static_cast<int32_t>(b + (t1 < n ? t1 : n));
-      u.slot = k > 1 && slots + i < pl.max_slots ? slots + i : -1;
+      u.slot = k > 1 && room ? static_cast<int32_t>(slots) + i : -1;
       pl.units[first + i] = u;
     }
-    if (k > 1 && splits < pl.max_splits) {
-      pl.splits[splits].g = g;
-      pl.splits[splits].slot0 = slots;
-      pl.splits[splits].n = slots + k <= pl.max_slots ? k : 0;
-    }
-    if (g == 0) {
-      pl.counts[0] = units < pl.max_units ? units : pl.max_units;
-      pl.counts[1] = all_splits < pl.max_splits ? all_splits : pl.max_splits;
+    if (lane == 0) {
+      if (k > 1 && splits < static_cast<uint32_t>(pl.max_splits)) {
+        pl.splits[splits].g = g;
+        pl.splits[splits].slot0 = static_cast<int32_t>(slots);
+        pl.splits[splits].n = room ? k : 0;
+      }
+      if (g == 0) {
+        pl.counts[0] = min(static_cast<int>(units), pl.max_units);
+        pl.counts[1] = min(static_cast<int>(all_splits), pl.max_splits);
+      }
     }
   }
 }
 
-// Partial tiles summed in chunk order: grid (tiles * 16, splits), 256 threads,
-// 16 rows of a tile each.
+// Partial tiles summed in chunk order: grid (tiles * bq / 16, splits), 256
+// threads, 16 rows of a tile each.
 __global__ void __launch_bounds__(256) lin_reduce_kernel(const LinArgs a, const LinPlanArgs pl) {
   if (static_cast<int>(blockIdx.y) >= pl.counts[1]) return;
   const LinSplit sp = pl.splits[blockIdx.y];
-  const int tiles = pl.npt * pl.nqt;
-  const int tile = blockIdx.x >> 4, sub = blockIdx.x & 15;
-  const int q0 = tile % pl.nqt * 256 + sub * 16, p0 = tile / pl.nqt * 256;
+  const int tiles = pl.npt * pl.nqt, subs = pl.bq / 16;
+  const int tile = blockIdx.x / subs, sub = blockIdx.x % subs;
+  const int q0 = tile % pl.nqt * pl.bq + sub * 16, p0 = tile / pl.nqt * 256;
   const int p = p0 + 4 * (threadIdx.x & 63);
-  if (p >= a.np) return;
+  if (p >= a.np || sp.n == 0) return;
   const int osize = a.out_type == kF32 ? 4 : 2;
+  const int64_t tile_size = static_cast<int64_t>(pl.bq) * 256;
   for (int r = threadIdx.x >> 6; r < 16; r += 4) {
     const int q = q0 + r;
     if (q >= a.nq) return;
     float v[4] = {0, 0, 0, 0};
     for (int i = 0; i < sp.n; ++i) {
-      const float* src = pl.partials +
-                         (static_cast<int64_t>(sp.slot0 + i) * tiles + tile) * 65536 +
-                         (sub * 16 + r) * 256 + (p - p0);
-      const float4 f = *reinterpret_cast<const float4*>(src);
+      const float4 f = *reinterpret_cast<const float4*>(
+          pl.partials + (static_cast<int64_t>(sp.slot0 + i) * tiles + tile) * tile_size +
+          (sub * 16 + r) * 256 + (p - p0));
       v[0] += f.x;
       v[1] += f.y;
       v[2] += f.z;
@@ -596,63 +780,46 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(const LinArgs a, const 
   }
 }
 
-template <int OP, int KIND, int FQ>
+template <int OP, int KIND, int FQ, int FP, bool STAGED>
 int launch(const LinArgs& a, const LinPlanArgs& pl, int64_t grid, hipStream_t s, const char* what) {
   MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  lin_tile_kernel<OP, KIND, FQ><<<static_cast<unsigned>(grid), 512, 0, s>>>(a, pl);
+  lin_tile_kernel<OP, KIND, FQ, FP, STAGED><<<static_cast<unsigned>(grid), 512, 0, s>>>(a, pl);
   return check_launch(what);
 }
 
+template <int OP, int KIND, int FQ, int FP, bool STAGED>
+int launch_rows(const LinArgs& a, hipStream_t s, const char* what) {
+  const int64_t grid = lin_row_tiles(a, 64 * FQ) * ceil_div(a.np, 128 * FP);
+  return launch<OP, KIND, FQ, FP, STAGED>(a, LinPlanArgs{}, grid, s, what);
+}
+
 template <int OP, int KIND>
-int launch_rows(const LinArgs& a, int fq, hipStream_t s, const char* what) {
-  const LinPlanArgs none = {};
-  const int64_t grid = lin_row_tiles(a, 64 * fq) * ceil_div(a.np, kBP);
-  if (fq == 1) return launch<OP, KIND, 1>(a, none, grid, s, what);
-  if (fq == 2) return launch<OP, KIND, 2>(a, none, grid, s, what);
-  return launch<OP, KIND, 4>(a, none, grid, s, what);
+int pick_rows(const LinArgs& a, LinTileShape t, hipStream_t s, const char* what) {
+  if (t.staged) {
+    if (t.rows >= 128) return launch_rows<OP, KIND, 2, 2, true>(a, s, what);
+    return t.cols == 256 ? launch_rows<OP, KIND, 1, 2, true>(a, s, what)
+                         : launch_rows<OP, KIND, 1, 1, true>(a, s, what);
+  }
+  if (t.rows == 256) return launch_rows<OP, KIND, 4, 2, false>(a, s, what);
+  if (t.rows == 128) return launch_rows<OP, KIND, 2, 2, false>(a, s, what);
+  return t.cols == 256 ? launch_rows<OP, KIND, 1, 2, false>(a, s, what)
+                       : launch_rows<OP, KIND, 1, 1, false>(a, s, what);
 }
 
 inline bool aligned16(const void* p, int64_t pitch) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (pitch & 15) == 0;
 }
 
-}  // namespace
-
-bool lin_tile_takes(const LinArgs& a, int op, int kind) {
-  const int es = op == kOpI8 ? 1 : 2;
-  if (!aligned16(a.Q, a.ldq) || !aligned16(a.P, a.ldp) || (a.p_group & 15)) return false;
-  if (kind == kLinForward) return a.nc * es % 16 == 0;
-  if (kind == kLinDgrad) return a.nc % 8 == 0 && a.np % 8 == 0;
-  return a.nq % 8 == 0 && a.np % 8 == 0 && a.G <= kLinPlanGroups && a.ldp < (int64_t(1) << 32);
-}
-
-int lin_tile_rows(const LinArgs& a, int op, int kind, int fq, hipStream_t s, const char* what) {
-  if (kind == kLinDgrad)
-    return op == kOpF16 ? launch_rows<kOpF16, kLinDgrad>(a, fq, s, what)
-                        : launch_rows<kOpBF16, kLinDgrad>(a, fq, s, what);
-  switch (op) {
-    case kOpBF16: return launch_rows<kOpBF16, kLinForward>(a, fq, s, what);
-    case kOpF16: return launch_rows<kOpF16, kLinForward>(a, fq, s, what);
-    case kOpI8: return launch_rows<kOpI8, kLinForward>(a, fq, s, what);
-    case kOpMx4: return launch_rows<kOpMx4, kLinForward>(a, fq, s, what);
-    default: return launch_rows<kOpMx8, kLinForward>(a, fq, s, what);
-  }
-}
-
-// Entries per unit at most. With several groups half the average load of a CU
-// (entries x tiles / CUs): a heavier group is cut, so that its tiles do not run
-// on when the others are done. One group alone is cut so that its tiles fill
-// whole rounds of the 256 CUs.
-LinPlanSizes lin_plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K) {
+LinPlanSizes plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K, int bq) {
   LinPlanSizes z;
-  z.tiles = ceil_div(N, 256) * ceil_div(K, kBP);
+  z.tiles = ceil_div(N, bq) * ceil_div(K, 256);
   int64_t cap = M * z.tiles / 512;
   if (G == 1) {
     double best = 1e300;
     int64_t chunks = 1;
     for (int64_t c = 1; c <= 64 && (c == 1 || M / c >= 256); ++c) {
-      // 40 ns an entry of a 256 x 256 tile, 150 ns a partial tile written and read
-      const double cost = static_cast<double>(ceil_div(z.tiles * c, 256)) * ceil_div(M, c) * 40e-9 +
+      // 20 ns an entry of a 256 x 256 tile, 150 ns a partial tile written and read
+      const double cost = static_cast<double>(ceil_div(z.tiles * c, 256)) * ceil_div(M, c) * 20e-9 +
                           (c > 1 ? z.tiles * c * 150e-9 : 0.0);
       if (cost < 0.98 * best) {
         best = cost;
@@ -661,8 +828,8 @@ LinPlanSizes lin_plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K) {
     }
     cap = ceil_div(M, chunks);
   }
-  z.cap = (cap < 1024 && G > 1 ? 1024 : (cap < 64 ? 64 : cap) + 63) & ~int64_t(63);
-  const int64_t over = M / z.cap + 1;  // groups longer than cap, and whole chunks
+  z.cap = ((G > 1 && cap < 1024 ? 1024 : cap < 64 ? 64 : cap) + 63) & ~int64_t(63);
+  const int64_t over = M / z.cap + 1;  // whole chunks, and groups longer than cap
   z.max_splits = M > z.cap ? (over < G ? over : G) : 0;
   z.max_slots = z.max_splits ? over + z.max_splits : 0;
   z.max_units = G + (z.max_splits ? over : 0);
@@ -670,20 +837,55 @@ LinPlanSizes lin_plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K) {
   z.splits_off = z.units_off + ceil_div(z.max_units * static_cast<int64_t>(sizeof(LinUnit)), 256) * 256;
   z.partials_off =
       z.splits_off + ceil_div(z.max_splits * static_cast<int64_t>(sizeof(LinSplit)), 256) * 256;
-  z.bytes = z.partials_off + z.max_slots * z.tiles * 65536 * 4;
+  z.bytes = z.partials_off + z.max_slots * z.tiles * bq * 256 * 4;
   return z;
 }
 
+}  // namespace
+
+bool lin_tile_direct(const LinArgs& a, int op, int kind) {
+  const int es = op == kOpI8 ? 1 : 2;
+  if (!aligned16(a.Q, a.ldq) || !aligned16(a.P, a.ldp) || (a.p_group & 15)) return false;
+  if (kind == kLinForward) return a.nc * es % 16 == 0;
+  return (kind == kLinDgrad ? a.nc : a.nq) % 8 == 0 && a.np % 8 == 0;
+}
+
+int lin_tile_rows(const LinArgs& a, int op, int kind, LinTileShape t, hipStream_t s,
+                  const char* what) {
+  if (kind == kLinDgrad)
+    return op == kOpF16 ? pick_rows<kOpF16, kLinDgrad>(a, t, s, what)
+                        : pick_rows<kOpBF16, kLinDgrad>(a, t, s, what);
+  switch (op) {
+    case kOpBF16: return pick_rows<kOpBF16, kLinForward>(a, t, s, what);
+    case kOpF16: return pick_rows<kOpF16, kLinForward>(a, t, s, what);
+    case kOpI8: return pick_rows<kOpI8, kLinForward>(a, t, s, what);
+    case kOpMx4: return pick_rows<kOpMx4, kLinForward>(a, t, s, what);
+    default: return pick_rows<kOpMx8, kLinForward>(a, t, s, what);
+  }
+}
+
+// Entries per unit at most. With several groups half the average load of a CU
+// (entries x tiles / CUs): a heavier group is cut, so that its tiles do not run
+// on when the others are done. One group alone is cut so that its tiles fill
+// whole rounds of the 256 CUs.
+int64_t lin_tile_wgrad_bytes(int64_t M, int64_t G, int64_t N, int64_t K) {
+  const int64_t a = plan_sizes(M, G, N, K, 128).bytes, b = plan_sizes(M, G, N, K, 256).bytes;
+  return a > b ? a : b;
+}
+
 int lin_tile_wgrad(const LinArgs& a, int op, void* workspace, hipStream_t s, const char* what) {
-  const LinPlanSizes z = lin_plan_sizes(a.M, a.G, a.nq, a.np);
+  const bool staged = !lin_tile_direct(a, op, kLinWgrad);
+  const int bq = staged ? 128 : 256;
+  const LinPlanSizes z = plan_sizes(a.M, a.G, a.nq, a.np, bq);
   char* ws = static_cast<char*>(workspace);
   LinPlanArgs pl = {};
   pl.counts = reinterpret_cast<int32_t*>(ws);
   pl.units = reinterpret_cast<LinUnit*>(ws + z.units_off);
   pl.splits = reinterpret_cast<LinSplit*>(ws + z.splits_off);
   pl.partials = reinterpret_cast<float*>(ws + z.partials_off);
-  pl.npt = static_cast<int>(ceil_div(a.np, kBP));
-  pl.nqt = static_cast<int>(ceil_div(a.nq, 256));
+  pl.npt = static_cast<int>(ceil_div(a.np, 256));
+  pl.nqt = static_cast<int>(ceil_div(a.nq, bq));
+  pl.bq = bq;
   pl.cap = static_cast<int>(z.cap);
   pl.max_units = static_cast<int>(z.max_units);
   pl.max_splits = static_cast<int>(z.max_splits);
@@ -692,10 +894,15 @@ int lin_tile_wgrad(const LinArgs& a, int op, void* workspace, hipStream_t s, con
   lin_plan_kernel<<<1, 1024, 0, s>>>(a, pl);
   if (int rc = check_launch(what)) return rc;
   const int64_t grid = (pl.deal ? ceil_div(z.max_units, 8) * 8 : z.max_units) * z.tiles;
-  const int rc = op == kOpF16 ? launch<kOpF16, kLinWgrad, 4>(a, pl, grid, s, what)
-                              : launch<kOpBF16, kLinWgrad, 4>(a, pl, grid, s, what);
+  int rc;
+  if (staged)
+    rc = op == kOpF16 ? launch<kOpF16, kLinWgrad, 2, 2, true>(a, pl, grid, s, what)
+                      : launch<kOpBF16, kLinWgrad, 2, 2, true>(a, pl, grid, s, what);
+  else
+    rc = op == kOpF16 ? launch<kOpF16, kLinWgrad, 4, 2, false>(a, pl, grid, s, what)
+                      : launch<kOpBF16, kLinWgrad, 4, 2, false>(a, pl, grid, s, what);
   if (rc || z.max_splits == 0) return rc;
-  const dim3 rg(static_cast<unsigned>(z.tiles * 16), static_cast<unsigned>(z.max_splits));
+  const dim3 rg(static_cast<unsigned>(z.tiles * (bq / 16)), static_cast<unsigned>(z.max_splits));
   lin_reduce_kernel<<<rg, 256, 0, s>>>(a, pl);
   return check_launch(what);
 }
