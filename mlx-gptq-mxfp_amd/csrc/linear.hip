@@ -3,29 +3,79 @@
 // [offsets[g], offsets[g + 1]); entry t reads row row_index[t] of X (or row t).
 //
 // Here are the entry points: their checks, and which kernel takes a call.
+#include <math.h>
+
 #include "linear_few.h"
 
 namespace mgq {
 namespace {
 
-// Forward and dgrad: which kernel and tile.
+// Which kernel and tile a product over rows takes: the one whose time by the
+// model below is least. The model was fitted to 539 measurements (all types,
+// 1 .. 16384 entries, 0 .. 128 groups, K 256 .. 7168, aligned and not; 2 to 7
+// choices each): the choice costs 1.3 % over the best of each, at most 45 %, where
+// always taking the largest tile that the average group fills costs 60 %.
+//
+//   large tiles: rounds of the 256 CUs x (stages x time of a stage + a fixed time
+//     for the tile's first loads and its results), or the weight's bytes at the
+//     rate the tile's loads reach;
+//   few rows: a wave's batches of loads one after the other, or the bytes that all
+//     workgroups read through L2, or the weight's bytes from memory.
+//
+// How the entries fall into groups is not known here: each active group is taken
+// to leave 0.6 tiles partly filled.
+struct TileTime {
+  int rows, cols;
+  bool staged;
+  double stage, fixed;  // us
+};
+constexpr TileTime kTileTimes[] = {
+    {64, 128, false, 0.33, 3.2}, {64, 256, false, 0.58, 2.9},  {128, 256, false, 0.87, 3.2},
+    {256, 256, false, 1.47, 5.0}, {64, 128, true, 0.81, 3.2}, {64, 256, true, 0.89, 2.9},
+    {128, 256, true, 1.14, 3.2},
+};
+
 template <int OP, int KIND>
 int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
   const bool direct = lin_tile_direct(a, OP, KIND);
-  const char* ev = getenv("LIN_V");
-  if (ev) {
-    const int v = atoi(ev);
-    if (v < 10 && KIND == kLinForward) return lin_few_rows(a, OP, v, s, what);
-    if (v > 10 && v < 1000)
-      return lin_tile_rows(a, OP, KIND, LinTileShape{v == 65 ? 64 : v, v == 64 ? 128 : 256, !direct}, s, what);
-    if (v > 1000)
-      return lin_tile_rows(a, OP, KIND, LinTileShape{v == 1065 ? 64 : v - 1000, v == 1064 ? 128 : 256, true}, s, what);
+  const int es = lin_esize<OP>();
+  const double wb = OP == kOpMx4 ? 0.53 : OP == kOpMx8 ? 1.03 : es;  // bytes of a weight
+  const double M = static_cast<double>(a.M), np = a.np, nc = a.nc;
+  const double active = a.offsets ? (a.G < a.M ? a.G : M) : 1;
+  const double weight_bytes = active * np * nc * wb;
+  auto row_tiles = [&](int rows) {
+    return a.offsets ? fmax(1.0, M / rows + 0.6 * active) : ceil(M / rows);
+  };
+  double best = 1e300;
+  LinTileShape shape = {};
+  for (const TileTime& t : kTileTimes) {
+    if (t.staged == direct) continue;
+    double rounds = row_tiles(t.rows) * ceil(np / t.cols) / 256;
+    rounds = rounds < 1 ? 1 : rounds + 0.76 * (ceil(rounds) - rounds);
+    const double stage = t.stage * (wb < 1 ? 1.25 : 1.0);
+    const double us = 2 + fmax(rounds * (ceil(nc * es / 128) * stage + t.fixed),
+                               weight_bytes / (direct ? 14.0e6 : 3.4e6));
+    if (us < best) {
+      best = us;
+      shape = LinTileShape{t.rows, t.cols, t.staged};
+    }
   }
-  if (KIND == kLinForward && a.M <= 16 * static_cast<int64_t>(a.G))
-    return lin_few_rows(a, OP, 1, s, what);
-  const int64_t avg = a.M / a.G;
-  return lin_tile_rows(a, OP, KIND,
-                       LinTileShape{avg > 192 ? 256 : avg > 64 ? 128 : 64, 256, !direct}, s, what);
+  if (KIND == kLinForward) {
+    int few = 0;
+    for (const int nq : {1, 2, 4}) {
+      const int rows = 16 * nq, cols = nq == 4 ? 32 : 16, batch = nq == 4 ? 4 : 8;
+      const double cost = direct ? 1.0 : 2.9;  // of a load that crosses its pieces
+      const double l2 = row_tiles(rows) * ceil(np / cols) * (cols * wb + rows * es) * nc * cost;
+      const double chain = ceil(ceil(nc * es / 256) / batch) * batch * (nq + cols / 16) * 0.12 * cost;
+      const double us = 5.8 + fmax(chain, fmax(l2 / 7.2e6, weight_bytes / 4.2e6));
+      if (us < best) {
+        best = us;
+        few = nq;
+      }
+    }
+    if (few) return lin_few_rows(a, OP, few, s, what);
+  }
+  return lin_tile_rows(a, OP, KIND, shape, s, what);
 }
 
 int check_list(const char* what, const int32_t* offsets, const int32_t* row_index,

@@ -1,8 +1,6 @@
 // Products of few rows (linear_few.hip): forward only, any alignment.
 #pragma once
 
-#include <stdlib.h>
-
 #include "linear_tile.h"
 
 namespace mgq {

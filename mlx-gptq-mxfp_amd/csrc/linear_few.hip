@@ -59,10 +59,12 @@ __device__ __forceinline__ typename LinAcc<OP>::t16 mfma16(lin_u32x4_t a, lin_u3
                                                    __builtin_bit_cast(lin_bf16x8_t, b), c, 0, 0, 0);
 }
 
-constexpr int kMaxWaves = 8;
+// Waves that share the contraction. Two and eight measured the same within 10 % for
+// 16-bit weights, eight up to twice slower for MXFP4 (too few codes a wave).
+constexpr int kWaves = 4;
 
 template <int OP, int NP, int NQ, bool AL>
-__global__ void __launch_bounds__(64 * kMaxWaves) lin_few_kernel(const LinArgs a) {
+__global__ void __launch_bounds__(64 * kWaves) lin_few_kernel(const LinArgs a) {
   constexpr int ES = lin_esize<OP>();
   constexpr bool MX = lin_is_mx<OP>();
   constexpr int STEP = MX ? 256 : 64;        // bytes of an X row per step
@@ -72,13 +74,13 @@ __global__ void __launch_bounds__(64 * kMaxWaves) lin_few_kernel(const LinArgs a
   constexpr int CB = OP == kOpMx4 ? 16 : 32;                      // MX: bytes of a group's codes
   constexpr int WV = MX ? CB / 16 : 1, XV = MX ? 4 : 1;           // 16-byte loads per step
   typedef typename LinAcc<OP>::t16 acc_t;
-  __shared__ acc_t part[kMaxWaves * NP * NQ * 64];
+  __shared__ acc_t part[kWaves * NP * NQ * 64];
 
   LinTile t;
   if (!lin_find_tile<16 * NQ>(a, (a.np + 16 * NP - 1) / (16 * NP), &t)) return;
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = blockDim.x >> 6;
+  constexpr int waves = kWaves;
   const int g = t.g, gw = g < a.G ? g : 0;
   const int p0 = t.pt * 16 * NP;
   const int64_t row_bytes = static_cast<int64_t>(a.nc) * ES;
@@ -259,25 +261,24 @@ __global__ void __launch_bounds__(64 * kMaxWaves) lin_few_kernel(const LinArgs a
 }
 
 template <int OP, int NP, int NQ>
-int launch(const LinArgs& a, int waves, hipStream_t s, const char* what) {
+int launch(const LinArgs& a, hipStream_t s, const char* what) {
   const int64_t grid = lin_row_tiles(a, 16 * NQ) * ceil_div(a.np, 16 * NP);
   MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.P) | reinterpret_cast<uintptr_t>(a.Q) |
                        static_cast<uintptr_t>(a.ldp | a.ldq | a.p_group) |
                        static_cast<uintptr_t>(static_cast<int64_t>(a.nc) * lin_esize<OP>());
   if ((at & 15) == 0)
-    lin_few_kernel<OP, NP, NQ, true><<<static_cast<unsigned>(grid), 64 * waves, 0, s>>>(a);
+    lin_few_kernel<OP, NP, NQ, true><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
   else
-    lin_few_kernel<OP, NP, NQ, false><<<static_cast<unsigned>(grid), 64 * waves, 0, s>>>(a);
+    lin_few_kernel<OP, NP, NQ, false><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
   return check_launch(what);
 }
 
 template <int OP>
 int run(const LinArgs& a, int nq, hipStream_t s, const char* what) {
-  const int waves = getenv("LIN_WV") ? atoi(getenv("LIN_WV")) : 4;
-  if (nq == 1) return launch<OP, 1, 1>(a, waves, s, what);
-  if (nq == 2) return launch<OP, 1, 2>(a, waves, s, what);
-  return launch<OP, 2, 4>(a, waves, s, what);
+  if (nq == 1) return launch<OP, 1, 1>(a, s, what);
+  if (nq == 2) return launch<OP, 1, 2>(a, s, what);
+  return launch<OP, 2, 4>(a, s, what);
 }
 
 }  // namespace

@@ -38,11 +38,33 @@ _MX_BITS = {"mxfp4": 4, "mxfp8": 8}
 _HALF = (torch.bfloat16, torch.float16)
 
 
-def _pitched(t: torch.Tensor) -> torch.Tensor:
-    """`t` with contiguous rows that do not overlap (a copy if need be)."""
-    if t.stride(-1) != 1 or (t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]):
+# A single token's product takes a few microseconds, which the calls below reach
+# only if the host side of one takes no longer: contiguous device tensors pass with
+# one comparison each.
+
+
+def _pitched(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """`t` on `dev` with contiguous rows that do not overlap (a copy if need be)."""
+    if t.device != dev:
+        t = t.to(dev)
+    if not t.is_contiguous() and (
+            t.stride(-1) != 1 or (t.shape[-2] > 1 and t.stride(-2) < t.shape[-1])):
         t = t.contiguous()
     return t
+
+
+def _dense(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """`t` on `dev`, contiguous."""
+    return t if t.device == dev and t.is_contiguous() else nat.on_device(t, dev)
+
+
+def _home(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    """The result on the caller's device."""
+    return t if like.is_cuda else t.to(like.device)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -75,7 +97,9 @@ def _list(fn: str, offsets, row_index, groups: int, n_rows: int, dev: torch.devi
             lo, hi = torch.aminmax(row_index)
             if int(lo) < 0 or int(hi) >= n_rows:
                 raise IndexError(f"{fn}: row_index outside [0, {n_rows})")
-        row_index = nat.on_device(row_index.to(torch.int32), dev)
+        if row_index.dtype != torch.int32:
+            row_index = row_index.to(torch.int32)
+        row_index = _dense(row_index, dev)
     entries = n_rows if row_index is None else row_index.numel()
     if offsets is None:
         return None, row_index, entries
@@ -89,7 +113,9 @@ def _list(fn: str, offsets, row_index, groups: int, n_rows: int, dev: torch.devi
             raise ValueError(f"{fn}: offsets must be non-negative and non-decreasing")
         if o[-1] > entries:
             raise ValueError(f"{fn}: offsets exceed the {entries} list entries")
-    return nat.on_device(offsets.to(torch.int32), dev), row_index, entries
+    if offsets.dtype != torch.int32:
+        offsets = offsets.to(torch.int32)
+    return _dense(offsets, dev), row_index, entries
 
 
 def _check_half(fn: str, *tensors: torch.Tensor) -> None:
@@ -108,14 +134,14 @@ def _forward(x, weight, offsets, row_index, validate):
     if x.shape[1] != K:
         raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the weight {K}")
     dev = nat.device_for(x, weight)
-    xd, wd = _pitched(x.to(dev)), _pitched(w.to(dev))
+    xd, wd = _pitched(x, dev), _pitched(w, dev)
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
     if M and N:
         nat.call("mgq_grouped_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0], _ld(xd),
                  nat.ptr(idx), M, wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off),
-                 y.data_ptr(), nat.stream_of(dev))
-    return y.to(x.device)
+                 y.data_ptr(), _stream(dev))
+    return _home(y, x)
 
 
 class _GroupedLinear(torch.autograd.Function):
@@ -151,7 +177,6 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets=None,
     return _forward(x, weight, offsets, row_index, validate)
 
 
-@torch.no_grad()
 def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
                          row_index: torch.Tensor | None = None, n_rows: int | None = None,
                          validate: bool = True) -> torch.Tensor:
@@ -171,7 +196,7 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
     if row_index is not None and n_rows is None:
         raise ValueError(f"{fn}: n_rows is required with row_index")
     dev = nat.device_for(dy, weight)
-    dyd, wd = _pitched(dy.to(dev)), _pitched(w.to(dev))
+    dyd, wd = _pitched(dy, dev), _pitched(w, dev)
     M = int(dy.shape[0])
     off, idx, entries = _list(fn, offsets, row_index, G, M if row_index is None else int(n_rows),
                               dev, validate)
@@ -180,7 +205,7 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
     gathered = idx is not None
     out_type = torch.float32 if gathered else dy.dtype
     dx = torch.empty(M, K, dtype=out_type, device=dev)
-    stream = nat.stream_of(dev)
+    stream = _stream(dev)
     if M and K and N:
         nat.call("mgq_grouped_dgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
                  wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off), dx.data_ptr(),
@@ -195,10 +220,9 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
             nat.call("mgq_rows_sum", dx.data_ptr(), idx.data_ptr(), M, int(n_rows), K,
                      out.data_ptr(), nat.dtype_code(out.dtype), ws.data_ptr(), ws.numel(), stream)
         dx = out
-    return dx.to(dy.device)
+    return _home(dx, dy)
 
 
-@torch.no_grad()
 def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
                          row_index: torch.Tensor | None = None, validate: bool = True,
                          out_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -216,7 +240,7 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     if out_dtype not in (dy.dtype, torch.float32):
         raise TypeError(f"{fn}: the result is {dy.dtype} or float32 (got {out_dtype})")
     dev = nat.device_for(dy, x)
-    dyd, xd = _pitched(dy.to(dev)), _pitched(x.to(dev))
+    dyd, xd = _pitched(dy, dev), _pitched(x, dev)
     G = 1 if offsets is None else len(offsets) - 1
     if G < 1:
         raise ValueError(f"{fn}: offsets must hold at least two integers")
@@ -230,13 +254,12 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         nat.call("mgq_grouped_wgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
                  xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), G, N, K, nat.ptr(off),
-                 dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size, nat.stream_of(dev))
+                 dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size, _stream(dev))
     if offsets is None:
         dw = dw[0]
-    return dw.to(dy.device)
+    return _home(dw, dy)
 
 
-@torch.no_grad()
 def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mode: str,
                 offsets=None, row_index: torch.Tensor | None = None,
                 validate: bool = True) -> torch.Tensor:
@@ -265,18 +288,17 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
     if tuple(s.shape) != (G, N, K // 32):
         raise AssertionError(f"{fn}: scales must be {(G, N, K // 32)} (got {tuple(s.shape)})")
     dev = nat.device_for(x, packed, scales)
-    xd = _pitched(x.to(dev))
-    wd, sd = nat.on_device(w, dev), nat.on_device(s, dev)
+    xd = _pitched(x, dev)
+    wd, sd = _dense(w, dev), _dense(s, dev)
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
     if M and N:
         nat.call("mgq_mxfp_linear", xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), M,
                  wd.data_ptr(), sd.data_ptr(), nat.mode_code(mode), G, N, K, nat.ptr(off),
-                 y.data_ptr(), nat.stream_of(dev))
-    return y.to(x.device)
+                 y.data_ptr(), _stream(dev))
+    return _home(y, x)
 
 
-@torch.no_grad()
 def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows as 8-bit integers with a scale each: (q int8 [..., K], scales f32
     [...]), scale = max|row| / 127, q = round-half-even(row / scale).
@@ -289,16 +311,15 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"quantize_rows_int8: rows of no elements ({tuple(x.shape)})")
     dev = nat.device_for(x)
-    rows = _pitched(x.to(dev).reshape(-1, x.shape[-1]))
+    rows = _pitched(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), dev)
     q = torch.empty(x.shape, dtype=torch.int8, device=dev)
     s = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     if rows.shape[0]:
         nat.call("mgq_quantize_rows_int8", rows.data_ptr(), nat.dtype_code(x.dtype), rows.shape[0],
-                 rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr(), nat.stream_of(dev))
-    return q.to(x.device), s.to(x.device)
+                 rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr(), _stream(dev))
+    return _home(q, x), _home(s, x)
 
 
-@torch.no_grad()
 def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
                 w_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.bfloat16, offsets=None,
@@ -330,14 +351,14 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
         raise AssertionError(f"{fn}: x_scale must be {(int(x.shape[0]),)}, w_scale and bias "
                              f"{per_channel}")
     dev = nat.device_for(x, weight)
-    xd, wd = _pitched(x.to(dev)), _pitched(w.to(dev))
-    xs, ws = nat.on_device(x_scale, dev), nat.on_device(w_scale, dev)
-    b = None if bias is None else nat.on_device(bias, dev)
+    xd, wd = _pitched(x, dev), _pitched(w, dev)
+    xs, ws = _dense(x_scale, dev), _dense(w_scale, dev)
+    b = None if bias is None else _dense(bias, dev)
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
     if M and N:
         nat.call("mgq_int8_linear", xd.data_ptr(), xs.data_ptr(), xd.shape[0], _ld(xd),
                  nat.ptr(idx), M, wd.data_ptr(), ws.data_ptr(), nat.ptr(b), G, N, K, _ld(wd),
                  wd.stride(0), nat.ptr(off), y.data_ptr(), nat.dtype_code(out_dtype),
-                 nat.stream_of(dev))
-    return y.to(x.device)
+                 _stream(dev))
+    return _home(y, x)
