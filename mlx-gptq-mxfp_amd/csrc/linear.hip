@@ -99,13 +99,6 @@ int check_dims(const char* what, int64_t N, int64_t K) {
   return MGQ_OK;
 }
 
-// 2: 16-byte stores, 1: four results at once, 0: one by one.
-int vec_ok(const void* out, int64_t ldo, int out_type) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(out);
-  if (ldo % 8 == 0 && (at & 15) == 0) return 2;
-  return ldo % 4 == 0 && (at & (out_type == kF32 ? 15 : 7)) == 0;
-}
-
 }  // namespace
 }  // namespace mgq
 
@@ -138,7 +131,6 @@ extern "C" int mgq_grouped_linear(const void* X, int dtype, int64_t n_rows, int6
   a.out = static_cast<char*>(Y);
   a.ldo = N;
   a.out_type = dtype;
-  a.vec_out = vec_ok(Y, N, dtype);
   hipStream_t s = as_stream(stream);
   return dtype == kF16 ? run_rows<kOpF16, kLinForward>(a, s, what)
                        : run_rows<kOpBF16, kLinForward>(a, s, what);
@@ -172,7 +164,6 @@ extern "C" int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, i
   a.out = static_cast<char*>(dX);
   a.ldo = K;
   a.out_type = out_dtype;
-  a.vec_out = vec_ok(dX, K, out_dtype);
   hipStream_t s = as_stream(stream);
   return dtype == kF16 ? run_rows<kOpF16, kLinDgrad>(a, s, what)
                        : run_rows<kOpBF16, kLinDgrad>(a, s, what);
@@ -219,7 +210,6 @@ extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, i
   a.ldo = K;
   a.o_group = N * K;
   a.out_type = out_dtype;
-  a.vec_out = vec_ok(dW, K, out_dtype);
   hipStream_t s = as_stream(stream);
   return lin_tile_wgrad(a, dtype == kF16 ? kOpF16 : kOpBF16, workspace, s, what);
 }
@@ -255,7 +245,6 @@ extern "C" int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const
   a.out = static_cast<char*>(Y);
   a.ldo = N;
   a.out_type = kBF16;
-  a.vec_out = vec_ok(Y, N, kBF16);
   hipStream_t s = as_stream(stream);
   return mode == kMxfp4 ? run_rows<kOpMx4, kLinForward>(a, s, what)
                         : run_rows<kOpMx8, kLinForward>(a, s, what);
@@ -293,7 +282,6 @@ extern "C" int mgq_int8_linear(const int8_t* X, const float* x_scale, int64_t n_
   a.out = static_cast<char*>(Y);
   a.ldo = N;
   a.out_type = out_dtype;
-  a.vec_out = vec_ok(Y, N, out_dtype);
   a.sx = x_scale;
   a.sw = w_scale;
   a.bias = bias;

@@ -37,7 +37,6 @@ struct LinArgs {
   int64_t ldo;           // elements
   int64_t o_group;       // wgrad: elements from one group's output to the next
   int out_type;          // DType
-  int vec_out;           // four consecutive outputs may be stored at once
   const float* sx;       // int8: scale of each X row
   const float* sw;       // int8: scale of each weight row [G, np]
   const float* bias;     // int8: [G, np] or null
@@ -322,12 +321,16 @@ __device__ __forceinline__ uint16_t lin_round16(float v, int type) {
   return type == kF16 ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);
 }
 
-// row: the output row's first element; p: first column.
+// row: the output row's first element; p: first column. Four results leave in one
+// store at any address (a row of odd length starts anywhere).
+struct __attribute__((packed, aligned(2))) lin_u64_u_t {
+  uint32_t v[2];
+};
 __device__ __forceinline__ void lin_store4(const LinArgs& a, char* row, int p, const float (&v)[4]) {
   if (a.out_type == kF32) {
     float* o = reinterpret_cast<float*>(row) + p;
-    if (a.vec_out && p + 4 <= a.np) {
-      *reinterpret_cast<float4*>(o) = float4{v[0], v[1], v[2], v[3]};
+    if (p + 4 <= a.np) {
+      *reinterpret_cast<f32x4_u_t*>(o) = f32x4_u_t{v[0], v[1], v[2], v[3]};
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -339,9 +342,11 @@ __device__ __forceinline__ void lin_store4(const LinArgs& a, char* row, int p, c
   uint16_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = lin_round16(v[i], a.out_type);
-  if (a.vec_out && p + 4 <= a.np) {
-    *reinterpret_cast<uint2*>(o) =
-        uint2{h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16)};
+  if (p + 4 <= a.np) {
+    lin_u64_u_t u;
+    u.v[0] = h[0] | (static_cast<uint32_t>(h[1]) << 16);
+    u.v[1] = h[2] | (static_cast<uint32_t>(h[3]) << 16);
+    *reinterpret_cast<lin_u64_u_t*>(o) = u;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)

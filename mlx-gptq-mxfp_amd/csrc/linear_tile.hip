@@ -659,8 +659,11 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
             *reinterpret_cast<const lin_u32x4_t*>(part + row * RB + 16 * (lane % CH));
         if (q >= q_end) continue;
         char* o = out + (q * a.ldo + p) * OS;
-        if (a.vec_out == 2 && p + EC <= a.np) {
-          *reinterpret_cast<lin_u32x4_t*>(o) = v;
+        if (p + EC <= a.np) {  // (at any address)
+          lin_u128_u_t u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u.v[e] = v[e];
+          *reinterpret_cast<lin_u128_u_t*>(o) = u;
         } else {
           for (int e = 0; e < EC && p + e < a.np; ++e) {
             if constexpr (T == kF32)
@@ -703,26 +706,24 @@ __global__ void __launch_bounds__(1024) lin_plan_kernel(const LinArgs a, const L
   const int lane = threadIdx.x & 63;
   for (int g = threadIdx.x >> 6; g < a.G; g += 16) {
     const int n = size[g], k = parts[g], len = chunk[g];
-    uint32_t first = 0, slots = 0, splits = 0, units = 0, all_splits = 0;
+    // units before this group's, and its first slot, 16 bits each (a valid list has
+    // at most a few thousand)
+    uint32_t sums = 0, splits = 0, units = 0, all_splits = 0;
     for (int o0 = 0; o0 < a.G; o0 += 64) {
       const int o = o0 + lane;
-      uint32_t f = 0, sl = 0, sp = 0, un = 0, al = 0;
-      if (o < a.G) {
-        const int lo = chunk[o];
-        un = parts[o];
-        if (lo > len || (lo == len && o < g)) f = un;
-        al = un > 1;
-        if (o < g && un > 1) {
-          sl = un;
-          sp = 1;
-        }
+      const int lo = o < a.G ? chunk[o] : -1;
+      const uint32_t un = o < a.G ? parts[o] : 0;
+      const bool before = o < g;
+      const uint32_t own = (lo > len || (lo == len && before) ? un << 16 : 0) +
+                           (before && un > 1 ? un : 0);
+      sums += __builtin_amdgcn_readlane(lin_wave_scan(own), 63);
+      splits += __popcll(__ballot(before && un > 1));
+      if (g == 0) {
+        units += __builtin_amdgcn_readlane(lin_wave_scan(un), 63);
+        all_splits += __popcll(__ballot(un > 1));
       }
-      first += __builtin_amdgcn_readlane(lin_wave_scan(f), 63);
-      slots += __builtin_amdgcn_readlane(lin_wave_scan(sl), 63);
-      splits += __builtin_amdgcn_readlane(lin_wave_scan(sp), 63);
-      units += __builtin_amdgcn_readlane(lin_wave_scan(un), 63);
-      all_splits += __builtin_amdgcn_readlane(lin_wave_scan(al), 63);
     }
+    const uint32_t first = sums >> 16, slots = sums & 0xffffu;
     int64_t b = 0, e = a.M;
     if (a.offsets) lin_segment(a, g, &b, &e);
     // (a list whose offsets decrease may have more units than there is room for)
