@@ -288,20 +288,30 @@ __device__ __forceinline__ int64_t lin_row(const LinArgs& a, int64_t t) {
 // ---------------------------------------------------------------------------
 // Epilogue: four consecutive p of one q, rounded once to the output type.
 // ---------------------------------------------------------------------------
-template <typename A>
-__device__ __forceinline__ float lin_acc_f32(A v) {
-  return static_cast<float>(v);
+// Elements p .. p + 3 of an fp32 row of np (the last one again past its end).
+__device__ __forceinline__ void lin_load4(const float* row, int p, int np, float (&v)[4]) {
+  if (p + 4 <= np) {
+    const f32x4_u_t f = load_f32x4(row + p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = row[p + i < np ? p + i : np - 1];
+  }
 }
 
 // int8: (acc * sx) * sw + b, in fp32; the int32 sum is rounded to fp32 first.
 template <int OP>
 __device__ __forceinline__ void lin_scale4(const LinArgs& a, int g, int p, float sx, float (&v)[4]) {
   if constexpr (OP == kOpI8) {
+    const int64_t c = static_cast<int64_t>(g) * a.np;
+    float w[4], b[4] = {0, 0, 0, 0};
+    lin_load4(a.sw + c, p, a.np, w);
+    if (a.bias) lin_load4(a.bias + c, p, a.np, b);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t c = static_cast<int64_t>(g) * a.np + (p + i < a.np ? p + i : a.np - 1);
-      v[i] = v[i] * sx * a.sw[c];
-      if (a.bias) v[i] = v[i] + a.bias[c];
+      v[i] = v[i] * sx * w[i];
+      if (a.bias) v[i] = v[i] + b[i];
     }
   }
 }

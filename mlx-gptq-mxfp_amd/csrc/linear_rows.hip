@@ -301,7 +301,6 @@ extern "C" int mgq_rows_sum(const float* src, const int32_t* row_index, int64_t 
   int32_t* count = static_cast<int32_t*>(workspace);
   int32_t* slots = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + slots_off(n_rows));
   rows_clear_kernel<<<elementwise_blocks(n_rows, 256), 256, 0, s>>>(count, n_rows);
-  if (n_entries > 0)
     rows_fill_kernel<<<elementwise_blocks(n_entries, 256), 256, 0, s>>>(row_index, n_entries, n_rows,
                                                                         count, slots);
   rows_sum_kernel<<<static_cast<unsigned>(ceil_div(n_rows, 4)), 256, 0, s>>>(

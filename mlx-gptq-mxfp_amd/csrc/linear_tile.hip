@@ -564,25 +564,6 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   }
 
   // ---- results ------------------------------------------------------------
-  if (KIND == kLinWgrad && slot >= 0) {
-    // a partial tile: fp32, [BQ][BP]
-    float* o = pl.partials + static_cast<int64_t>(slot) * BQ * BP;
-#pragma unroll
-    for (int f = 0; f < FQ; ++f)
-#pragma unroll
-      for (int k = 0; k < FP; ++k)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int q = 32 * (FQ * wq + f) + (lane & 31);
-          const int p = 32 * FP * wp + 32 * k + 8 * r + 4 * half;
-          *reinterpret_cast<float4*>(o + q * BP + p) =
-              float4{static_cast<float>(acc[f][k][4 * r]), static_cast<float>(acc[f][k][4 * r + 1]),
-                     static_cast<float>(acc[f][k][4 * r + 2]),
-                     static_cast<float>(acc[f][k][4 * r + 3])};
-        }
-    __builtin_amdgcn_s_waitcnt(0);  // loads into LDS of stages past the end
-    return;
-  }
   float sx[FQ];
   if constexpr (OP == kOpI8) {
 #pragma unroll
@@ -593,6 +574,12 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     }
   }
   char* out = a.out + (KIND == kLinWgrad ? g * a.o_group : 0) * (a.out_type == kF32 ? 4 : 2);
+  int64_t ldo = a.ldo;
+  const bool partial = KIND == kLinWgrad && slot >= 0;
+  if (partial) {  // fp32, [BQ][BP]
+    ldo = BP;
+    out = reinterpret_cast<char*>(pl.partials + static_cast<int64_t>(slot) * BQ * BP - q0 * BP - p0);
+  }
   lds_handover();  // every wave is done with the last stage's buffer
   // Results go through LDS (a wave's own part of it) to leave as whole pieces of a
   // row: 64 columns of 16-bit results or 32 of fp32 at a time, rows of 128 bytes
@@ -615,12 +602,8 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
           float sw4[4] = {0, 0, 0, 0}, b4[4] = {0, 0, 0, 0};
           if constexpr (OP == kOpI8) {
             const int64_t c = static_cast<int64_t>(gw) * a.np;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int64_t ce = c + (p + e < a.np ? p + e : a.np - 1);
-              sw4[e] = a.sw[ce];
-              if (a.bias) b4[e] = a.bias[ce];
-            }
+            lin_load4(a.sw + c, p, a.np, sw4);
+            if (a.bias) lin_load4(a.bias + c, p, a.np, b4);
           }
 #pragma unroll
           for (int f = 0; f < FQ; ++f) {
@@ -658,7 +641,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
         const lin_u32x4_t v =
             *reinterpret_cast<const lin_u32x4_t*>(part + row * RB + 16 * (lane % CH));
         if (q >= q_end) continue;
-        char* o = out + (q * a.ldo + p) * OS;
+        char* o = out + (q * ldo + p) * OS;
         if (p + EC <= a.np) {  // (at any address)
           lin_u128_u_t u;
 #pragma unroll
@@ -677,7 +660,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       if (k0 + KP < FP) __builtin_amdgcn_wave_barrier();
     }
   };
-  if (a.out_type == kF32) {
+  if (a.out_type == kF32 || partial) {
     if constexpr (OP == kOpI8 || KIND != kLinForward) store_out(std::integral_constant<int, kF32>{});
   } else if (a.out_type == kF16) {
     if constexpr (OP == kOpI8 || OP == kOpF16) store_out(std::integral_constant<int, kF16>{});
@@ -688,23 +671,66 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
 
 // ---------------------------------------------------------------------------
 // wgrad's units: a group's entries, cut into chunks of at most `cap`, longest
-// first so that the last tiles to start are the shortest. One workgroup plans, a
-// wave per group at a time: each place in the order is a sum over all groups.
+// first so that the last tiles to start are the shortest. One workgroup plans. Each
+// of its 16 waves prices one cap, cap_min 2^(k / 2): a CU takes about 1.5 us for 64
+// entries of a tile and 5 us beside them, a cut tile's partial results cost the chip
+// 0.11 us of memory traffic; the tiles of one round end with the longest, those of
+// several about half the longest after the average load. Then a wave per group
+// at a time: each place in the order is a sum over all groups.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(1024) lin_plan_kernel(const LinArgs a, const LinPlanArgs pl) {
   __shared__ int32_t size[kLinPlanGroups], parts[kLinPlanGroups], chunk[kLinPlanGroups];
+  __shared__ float price[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int g = threadIdx.x; g < a.G; g += 1024) {
     int64_t b = 0, e = a.M;
     if (a.offsets) lin_segment(a, g, &b, &e);
-    const int n = e > b ? static_cast<int>(e - b) : 0;
-    const int k = n > pl.cap ? (n + pl.cap - 1) / pl.cap : 1;
-    size[g] = n;
+    size[g] = e > b ? static_cast<int>(e - b) : 0;
+  }
+  __syncthreads();
+  auto cap_of = [&](int k) {  // a multiple of 64
+    const int64_t c = (static_cast<int64_t>(pl.cap) << (k >> 1)) * (k & 1 ? 181 : 128) / 128;
+    return static_cast<int>((c < 0x3fffffff ? c : 0x3fffffff) & ~int64_t(63));
+  };
+  {
+    const int cap = cap_of(wave), tiles = pl.npt * pl.nqt;
+    float load = 0, longest = 0;
+    uint32_t units = 0, cut = 0;
+    for (int o0 = 0; o0 < a.G; o0 += 64) {
+      const int n = o0 + lane < a.G ? size[o0 + lane] : 0;
+      const int k = n > cap ? (n + cap - 1) / cap : 1;
+      const float us = 5.0f + 1.5f / 64 * ((n + k - 1) / k);
+      if (o0 + lane < a.G) {
+        load += k * us;
+        longest = fmaxf(longest, us);
+        units += k;
+        cut += k > 1 ? k : 0;
+      }
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      load += __shfl_xor(load, d);
+      longest = fmaxf(longest, __shfl_xor(longest, d));
+      units += __shfl_xor(units, d);
+      cut += __shfl_xor(cut, d);
+    }
+    const float items = static_cast<float>(units) * tiles;
+    const float us = (items <= 256 ? longest : load * tiles / 256 + 0.5f * longest) +
+                     0.11f * cut * tiles;
+    if (lane == 0) price[wave] = us;
+  }
+  __syncthreads();
+  int pick = 15;  // the longest cap among the cheapest
+  for (int k = 14; k >= 0; --k) pick = price[k] < 0.97f * price[pick] ? k : pick;
+  const int cap = cap_of(pick);
+  for (int g = threadIdx.x; g < a.G; g += 1024) {
+    const int n = size[g];
+    const int k = n > cap ? (n + cap - 1) / cap : 1;
     parts[g] = k;
     chunk[g] = ((n + k - 1) / k + 63) & ~63;  // whole stages
   }
   __syncthreads();
-  const int lane = threadIdx.x & 63;
-  for (int g = threadIdx.x >> 6; g < a.G; g += 16) {
+  for (int g = wave; g < a.G; g += 16) {
     const int n = size[g], k = parts[g], len = chunk[g];
     // units before this group's, and its first slot, 16 bits each (a valid list has
     // at most a few thousand)
@@ -814,22 +840,8 @@ inline bool aligned16(const void* p, int64_t pitch) {
 LinPlanSizes plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K, int bq) {
   LinPlanSizes z;
   z.tiles = ceil_div(N, bq) * ceil_div(K, 256);
-  int64_t cap = M * z.tiles / 512;
-  if (G == 1) {
-    double best = 1e300;
-    int64_t chunks = 1;
-    for (int64_t c = 1; c <= 64 && (c == 1 || M / c >= 256); ++c) {
-      // 20 ns an entry of a 256 x 256 tile, 150 ns a partial tile written and read
-      const double cost = static_cast<double>(ceil_div(z.tiles * c, 256)) * ceil_div(M, c) * 20e-9 +
-                          (c > 1 ? z.tiles * c * 150e-9 : 0.0);
-      if (cost < 0.98 * best) {
-        best = cost;
-        chunks = c;
-      }
-    }
-    cap = ceil_div(M, chunks);
-  }
-  z.cap = ((G > 1 && cap < 1024 ? 1024 : cap < 64 ? 64 : cap) + 63) & ~int64_t(63);
+  const int64_t cap = M * z.tiles / 1024;  // at most 2048 partial tiles
+  z.cap = (cap < 256 ? 256 : cap + 63) & ~int64_t(63);
   const int64_t over = M / z.cap + 1;  // whole chunks, and groups longer than cap
   z.max_splits = M > z.cap ? (over < G ? over : G) : 0;
   z.max_slots = z.max_splits ? over + z.max_splits : 0;
@@ -865,10 +877,6 @@ int lin_tile_rows(const LinArgs& a, int op, int kind, LinTileShape t, hipStream_
   }
 }
 
-// Entries per unit at most. With several groups half the average load of a CU
-// (entries x tiles / CUs): a heavier group is cut, so that its tiles do not run
-// on when the others are done. One group alone is cut so that its tiles fill
-// whole rounds of the 256 CUs.
 int64_t lin_tile_wgrad_bytes(int64_t M, int64_t G, int64_t N, int64_t K) {
   const int64_t a = plan_sizes(M, G, N, K, 128).bytes, b = plan_sizes(M, G, N, K, 256).bytes;
   return a > b ? a : b;
