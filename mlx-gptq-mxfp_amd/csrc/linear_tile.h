@@ -32,31 +32,33 @@ struct LinPlanSizes {
 };
 constexpr int kLinPlanGroups = 4096;
 
-// wgrad: which unit and tile a workgroup takes. With many units an XCD takes
-// every eighth of them whole (in snake order: they are sorted by length), so that
-// its L2 holds the unit's rows; with few, a unit's tiles go round the XCDs.
-__device__ __forceinline__ bool lin_find_unit(const LinArgs& a, const LinPlanArgs& pl, LinUnit* u,
-                                              int* tile) {
-  const int tiles = pl.npt * pl.nqt;
+// wgrad: which unit and tile an item is: 1 if there is one, 0 past the last, -1 for a
+// hole in the order. With many units an XCD takes every eighth of them whole (in
+// snake order: they are sorted by length), so that its L2 holds the unit's rows;
+// with few, a unit's tiles go round the XCDs.
+__device__ __forceinline__ int lin_find_unit(const LinArgs& a, const LinPlanArgs& pl, uint32_t item,
+                                             LinUnit* u, int* tile) {
+  const uint32_t tiles = static_cast<uint32_t>(pl.npt) * pl.nqt;
   const int n = pl.counts[0];
   int i;
   if (pl.deal) {
-    const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
-    const int round = j / tiles;
-    *tile = j % tiles;
-    i = round * 8 + (round & 1 ? 7 - x : x);
+    const uint32_t x = item & 7, j = item >> 3;
+    const uint32_t round = j / tiles;
+    *tile = static_cast<int>(j % tiles);
+    i = static_cast<int>(round * 8 + (round & 1 ? 7 - x : x));
+    if (i >= n) return static_cast<int>(round * 8) >= n ? 0 : -1;
   } else {
-    i = blockIdx.x / tiles;
-    *tile = blockIdx.x % tiles;
+    i = static_cast<int>(item / tiles);
+    *tile = static_cast<int>(item % tiles);
+    if (i >= n) return 0;
   }
-  if (i >= n) return false;
   const LinUnit v = pl.units[i];
   u->g = __builtin_amdgcn_readfirstlane(v.g);
   u->t0 = __builtin_amdgcn_readfirstlane(v.t0);
   u->t1 = __builtin_amdgcn_readfirstlane(v.t1);
   u->slot = __builtin_amdgcn_readfirstlane(v.slot);
-  if (u->slot >= 0) u->slot = u->slot * tiles + *tile;
-  return true;
+  if (u->slot >= 0) u->slot = u->slot * static_cast<int>(tiles) + *tile;
+  return 1;
 }
 
 // The host's bound on the row tiles of a launch.

@@ -35,6 +35,7 @@ namespace mgq {
 namespace {
 
 constexpr int kLdsMax = 160 * 1024;
+constexpr int kCUs = 256;
 constexpr int kSteps = 4;    // K-steps per stage
 constexpr int kRowB = 128;   // bytes of a plain row per stage
 
@@ -144,13 +145,21 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   const int half = lane >> 5;
 
   // ---- which tile -------------------------------------------------------
+  // wgrad: the host's bound on the work list is loose (it does not know the groups'
+  // lengths), so that a workgroup takes every gridDim.x'th item instead of leaving
+  // the holes to workgroups of their own. The products over rows have few holes,
+  // and one tile a workgroup: taking several, with the next one's first loads before
+  // the results of the last, measured 2 to 4 % slower in long contractions.
+  for (uint32_t item = blockIdx.x;; item += gridDim.x) {
   int g, p0, slot = -1;
   int64_t q0, q_end;                 // rows of Q (forward, dgrad) or of the output (wgrad)
   int64_t c_begin = 0, c_len = a.nc;  // contraction range
   if constexpr (KIND == kLinWgrad) {
     LinUnit u;
     int tile;
-    if (!lin_find_unit(a, pl, &u, &tile)) return;
+    const int found = lin_find_unit(a, pl, item, &u, &tile);
+    if (found == 0) return;
+    if (found < 0) continue;
     g = u.g;
     slot = u.slot;
     c_begin = u.t0;
@@ -667,6 +676,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   } else {
     if constexpr (OP != kOpF16) store_out(std::integral_constant<int, kBF16>{});
   }
+  if constexpr (KIND != kLinWgrad) return;
+  lds_handover();  // every wave has its results out of LDS
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -810,7 +822,9 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(const LinArgs a, const 
 template <int OP, int KIND, int FQ, int FP, bool STAGED>
 int launch(const LinArgs& a, const LinPlanArgs& pl, int64_t grid, hipStream_t s, const char* what) {
   MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  lin_tile_kernel<OP, KIND, FQ, FP, STAGED><<<static_cast<unsigned>(grid), 512, 0, s>>>(a, pl);
+  const int64_t most = KIND == kLinWgrad ? 2 * kCUs : grid;
+  const unsigned blocks = static_cast<unsigned>(grid < most ? grid : most);
+  lin_tile_kernel<OP, KIND, FQ, FP, STAGED><<<blocks, 512, 0, s>>>(a, pl);
   return check_launch(what);
 }
 
