@@ -169,13 +169,15 @@ __device__ __forceinline__ uint32_t lin_wave_scan(uint32_t v) {
 // entries per tile, n_pt tiles along p. Workgroups are dealt to the eight XCDs
 // round robin, so workgroup b takes tile (b % 8) * (total / 8) + b / 8 of the
 // list: an XCD's concurrent tiles are neighbours and share rows in its L2.
-// Inside a group the tiles go in strips of kStrip tiles along q, p outer.
+// Inside a group the tiles go in strips along q, p outer: the 32 tiles that an XCD
+// runs at a time are then 8 along q and 4 along p, or all of p and 32 / n_pt along q
+// where that is less, so that a row of Q is fetched once.
 //
 // A lane holds the bounds of up to kSegRegs segments, all loaded at once: a
 // single token's product takes a few microseconds, of which every dependent load
 // here would be a tenth. More segments than 64 kSegRegs are read in a loop, twice.
 constexpr int kSegRegs = 4;
-template <int BM, int kStrip = 8>
+template <int BM>
 __device__ inline bool lin_find_tile(const LinArgs& a, uint32_t n_pt, LinTile* t) {
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t bid = blockIdx.x;
@@ -265,13 +267,14 @@ __device__ inline bool lin_find_tile(const LinArgs& a, uint32_t n_pt, LinTile* t
     if (!found) return false;
   }
   const uint32_t local = id - base * n_pt;
-  const uint32_t strip = local / (kStrip * n_pt);
-  const uint32_t in = local - strip * kStrip * n_pt;
-  const uint32_t left = tiles - strip * kStrip;
-  const uint32_t sm = left < kStrip ? left : kStrip;
+  const uint32_t wide = n_pt > 8 || n_pt < 4 ? 8 : 32 / n_pt;
+  const uint32_t strip = local / (wide * n_pt);
+  const uint32_t in = local - strip * wide * n_pt;
+  const uint32_t left = tiles - strip * wide;
+  const uint32_t sm = left < wide ? left : wide;
   t->g = g;
   t->pt = static_cast<int>(in / sm);
-  t->q0 = b + static_cast<int64_t>(strip * kStrip + in % sm) * BM;
+  t->q0 = b + static_cast<int64_t>(strip * wide + in % sm) * BM;
   t->q_end = e;
   return true;
 }

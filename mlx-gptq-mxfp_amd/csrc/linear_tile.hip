@@ -8,7 +8,7 @@
 //   - A stage is 128 bytes of every row: 64 16-bit or 128 int8 elements of the
 //     contraction, four K-steps of one MFMA depth each. Rows that start and end on
 //     16-byte boundaries go from memory straight into LDS
-//     (global_load_lds_dwordx4, 16 bytes a lane), NB stages deep. Other rows
+//     (global_load_lds_dwordx4, 16 bytes a lane), two to four stages deep. Other rows
 //     (STAGED) go through registers, loaded a stage ahead of their way into LDS,
 //     with 16-byte loads at any address; a piece that a row ends in is masked, and
 //     read element by element only where the 16 bytes would leave the tensor.
@@ -125,8 +125,12 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   constexpr int ES = lin_esize<OP>();
   constexpr int BQ = 64 * FQ, BP = 128 * FP;
   constexpr int QB = BQ * kRowB;                 // Q bytes per stage
-  constexpr int SB = QB + (MX ? mx_stage_bytes<OP>(BP) : BP * kRowB);  // stage bytes
-  constexpr int NB = STAGED ? 2 : kLdsMax / SB < 4 ? kLdsMax / SB : 4;
+  constexpr int PB = MX ? mx_stage_bytes<OP>(BP) : BP * kRowB;  // and P bytes
+  // buffers of stages: where two whole ones leave room, Q has a third, so that only
+  // P's loads have to come within the period they are issued in
+  constexpr int NBP = STAGED ? 2 : kLdsMax / (QB + PB) < 4 ? kLdsMax / (QB + PB) : 4;
+  constexpr int NBQ = !STAGED && NBP == 2 && 3 * QB + 2 * PB <= kLdsMax ? 3 : NBP;
+  constexpr int LDS = NBQ * QB + NBP * PB;
   constexpr int EPI = BQ * BP * 2;               // 16-bit results on their way out
   constexpr int VQ = FQ;                         // 16-byte loads per lane and stage: Q,
   constexpr int per = OP == kOpMx4 ? 2 : 4;      // (MX: 16-byte pieces of a row's codes)
@@ -135,9 +139,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   constexpr int V = VQ + VP;
   constexpr int NM = FP * FQ;                    // MFMAs per K-step
   constexpr int EK = kRowB / ES;                 // contraction elements per stage
-  static_assert(NB >= 2 && (NB - 2) * V <= 63, "stages");
+  static_assert(NBP >= 2 && (NBP - 2) * V <= 63, "stages");
   static_assert(!QT || FQ >= 2, "transposed Q tiles are 128 or 256 wide");
-  __shared__ __attribute__((aligned(1024))) char lds[NB * SB > EPI ? NB * SB : EPI];
+  __shared__ __attribute__((aligned(1024))) char lds[LDS > EPI ? LDS : EPI];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -308,16 +312,16 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
         const int r = (64 / per) * at + lane / per;
         const int pos = lane % per;
         const int c = per == 2 ? pos ^ ((r >> 3) & 1) : pos ^ ((r >> 2) & 3);
-        *dst = QB + at * 1024;
+        *dst = at * 1024;
         *n = 32 * (c * 2 / per) < left ? 16 : 0;  // whole MX groups
         pp[k] += 16 * per;
       } else {
-        *dst = QB + BP * 16 * per + mx_wave * 256;
+        *dst = BP * 16 * per + mx_wave * 256;
         *n = 32 * (lane & 1) < left ? 1 : 0;
         pp[k] += 2;
       }
     } else if constexpr (PT) {
-      *dst = QB + (VP * wave + k) * 1024;
+      *dst = (VP * wave + k) * 1024;
       *n = tr_row(BP, k) < left ? 16 : 0;
       if constexpr (KIND == kLinWgrad) {
         constexpr int RP = 512 / BP;  // rows per load
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
         pp[k] += EK * a.ldp;
       }
     } else {
-      *dst = QB + (VP * wave + k) * 1024;
+      *dst = (VP * wave + k) * 1024;
       *n = left * ES - 16 * (k & 1 ? ch1 : ch0);
       pp[k] += kRowB;
     }
@@ -375,9 +379,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     const int k = i - VQ;
     uint32_t dst;
     if (i < VQ) dst = (VQ * wave + i) * 1024;
-    else if (is_scale(i)) dst = QB + BP * 16 * per + mx_wave * 256;
-    else if (MX) dst = QB + (VC * (per == 2 ? mx_wave : wave) + k) * 1024;
-    else dst = QB + (VP * wave + k) * 1024;
+    else if (is_scale(i)) dst = BP * 16 * per + mx_wave * 256;
+    else if (MX) dst = (VC * (per == 2 ? mx_wave : wave) + k) * 1024;
+    else dst = (VP * wave + k) * 1024;
     if (is_scale(i))
       *reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(buf + dst + 4 * lane) = hold[i][0];
     else
@@ -396,8 +400,8 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     const uint32_t c = 16 * ((MX ? 4 * half + k : 2 * k + half) ^ sw);
     qa[k] = QT ? (8 * half + j4) * (2 * BQ) + (((FQ * wq + k) ^ j4) * 64) + tr_lane
                : (32 * FQ * wq + (lane & 31)) * kRowB + c;
-    pa[k] = PT ? QB + (8 * half + j4) * (2 * BP) + (((FP * wp + (k & (FP - 1))) ^ j4) * 64) + tr_lane
-               : QB + (32 * FP * wp + (lane & 31)) * kRowB + c;
+    pa[k] = PT ? (8 * half + j4) * (2 * BP) + (((FP * wp + (k & (FP - 1))) ^ j4) * 64) + tr_lane
+               : (32 * FP * wp + (lane & 31)) * kRowB + c;
   }
   uint32_t code_at[2], scale_at = 0;
   if constexpr (MX) {
@@ -406,9 +410,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     for (int k = 0; k < per / 2; ++k) {
       const int c = per == 2 ? half : 2 * half + k;
       const int pos = per == 2 ? c ^ ((r >> 3) & 1) : c ^ ((r >> 2) & 3);
-      code_at[k] = QB + r * 16 * per + 16 * pos;
+      code_at[k] = r * 16 * per + 16 * pos;
     }
-    scale_at = QB + BP * 16 * per + (2 * r + half) * 4;
+    scale_at = BP * 16 * per + (2 * r + half) * 4;
   }
   lin_u32x4_t fq[2][FQ], fp[2][FP];
   lin_u32x4_t codes[FP][2];
@@ -440,14 +444,14 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   };
   // read r of a K-step (dense: p0 q0 p1 .. q1 ..; MX: the q only)
   constexpr int NR = MX ? FQ : FQ + FP;
-  auto read = [&](int r, int b, int ks, uint32_t buf) {
+  auto read = [&](int r, int b, int ks, uint32_t qbuf, uint32_t pbuf) {
     if constexpr (MX) {
-      read_q(b, r, ks, buf);
+      read_q(b, r, ks, qbuf);
     } else {
-      if (r == 0) read_p(b, 0, ks, buf);
-      else if (r == 1) read_q(b, 0, ks, buf);
-      else if (r <= FP) read_p(b, r - 1, ks, buf);
-      else read_q(b, r - FP, ks, buf);
+      if (r == 0) read_p(b, 0, ks, pbuf);
+      else if (r == 1) read_q(b, 0, ks, qbuf);
+      else if (r <= FP) read_p(b, r - 1, ks, pbuf);
+      else read_q(b, r - FP, ks, qbuf);
     }
   };
 
@@ -469,22 +473,29 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
 
   // Slot t of a stage's period (four K-steps of NM MFMAs; the first K-step's MFMAs
   // are the previous stage's last): the reads of the next K-step come first, so
-  // that none is young at the barrier; the loads of stage s + NB - 1, into the
-  // buffer that the barrier released, are spread over the period, because a load
-  // instruction occupies the address unit of the CU for 16 cycles and all eight
-  // waves issue theirs in the same slots; with two buffers over its first half,
-  // because the next barrier waits for them. STAGED: what was loaded in the last
-  // period goes into LDS, and the next stage's loads take its registers.
-  constexpr int SPREAD = NB == 2 ? kSteps / 2 : kSteps;
+  // that none is young at the barrier. The loads into the buffers that the barrier
+  // released (P of stage s + NBP - 1, then Q of stage s + NBQ - 1) are spread over
+  // the period, because a load instruction occupies the address unit of the CU for
+  // 16 cycles and all eight waves issue theirs in the same slots; with two buffers
+  // over its first half, because the next barrier waits for them. STAGED: what was
+  // loaded in the last period goes into LDS, and the next stage's loads take its
+  // registers.
+  constexpr int SPREAD = NBP == 2 ? kSteps / 2 : kSteps;
   constexpr int RPS = (NR + NM - 1) / NM;
-  constexpr int WAIT = STAGED ? -1 : (NB - 2) * V;
-  auto slot_reads = [&](int j, int b, int ks, uint32_t buf) __attribute__((always_inline)) {
+  constexpr int WAIT = STAGED ? -1 : (NBQ - 2) * VQ + (NBP - 2) * VP;
+  auto q_at = [&](int i) { return lds0 + i * QB; };
+  auto p_at = [&](int i) { return lds0 + NBQ * QB + i * PB; };
+  auto slot_reads = [&](int j, int b, int ks, uint32_t qbuf, uint32_t pbuf) __attribute__((
+                        always_inline)) {
 #pragma unroll
-    for (int r = j * RPS; r < (j + 1) * RPS && r < NR; ++r) read(r, b, ks, buf);
+    for (int r = j * RPS; r < (j + 1) * RPS && r < NR; ++r) read(r, b, ks, qbuf, pbuf);
   };
-  auto slot_loads = [&](int t, int st, uint32_t buf) __attribute__((always_inline)) {
+  auto slot_loads = [&](int t, int s, uint32_t qbuf, uint32_t pbuf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = t * V / (NM * SPREAD); i < (t + 1) * V / (NM * SPREAD) && i < V; ++i) {
+    for (int k = t * V / (NM * SPREAD); k < (t + 1) * V / (NM * SPREAD) && k < V; ++k) {
+      const int i = k < VP ? VQ + k : k - VP;
+      const uint32_t buf = k < VP ? pbuf : qbuf;
+      const int st = s + (k < VP ? NBP : NBQ) - 1;
       if constexpr (STAGED) {
         put(i, buf);
         fetch(i, st + 1);
@@ -503,68 +514,74 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       take_rows();
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        put(i, lds0);
+        put(i, i < VQ ? q_at(0) : p_at(0));
         fetch(i, 1);
       }
       load_rows(2);
     } else {
 #pragma unroll
-      for (int st = 0; st < NB - 1; ++st) {
-        load_rows(st);
-        take_rows();
+      for (int st = 0; st < NBQ - 1; ++st) {
+        if (st < NBP - 1) {
+          load_rows(st);
+          take_rows();
 #pragma unroll
-        for (int i = 0; i < V; ++i) load(i, st, lds0 + st * SB);
+          for (int i = VQ; i < V; ++i) load(i, st, p_at(st));
+        }
+#pragma unroll
+        for (int i = 0; i < VQ; ++i) load(i, st, q_at(st));
       }
-      load_rows(NB - 1);
+      load_rows(NBP - 1);
     }
     stage_barrier<WAIT>();
     take_rows();
     if constexpr (MX) {
 #pragma unroll
-      for (int f = 0; f < FP; ++f) read_codes(f, lds0);
+      for (int f = 0; f < FP; ++f) read_codes(f, p_at(0));
     }
-    uint32_t wbuf = lds0 + (NB - 1) * SB;
+    uint32_t wqb = q_at(NBQ - 1), wpb = p_at(NBP - 1);
 #pragma unroll
-    for (int r = 0; r < NR; ++r) read(r, 0, 0, lds0);
+    for (int r = 0; r < NR; ++r) read(r, 0, 0, q_at(0), p_at(0));
 #pragma unroll
-    for (int j = 0; j < NM; ++j) slot_loads(j, NB - 1, wbuf);
+    for (int j = 0; j < NM; ++j) slot_loads(j, 0, wqb, wpb);
     if constexpr (MX) decode_all(0, 0);
     __builtin_amdgcn_sched_barrier(0);
-    int rb = 0;
+    int rq = 0, rp = 0;
     for (int s = 0; s < n_stages; ++s) {
-      const uint32_t buf = lds0 + rb * SB;
-      load_rows(s + NB + (STAGED ? 1 : 0));
+      const uint32_t qbuf = q_at(rq), pbuf = p_at(rp);
+      load_rows(s + NBP + (STAGED ? 1 : 0));
 #pragma unroll
       for (int ks = 1; ks < kSteps; ++ks) {
         const int b = (ks - 1) & 1;
 #pragma unroll
         for (int j = 0; j < NM; ++j) {
           mfma(b, j);
-          slot_reads(j, b ^ 1, ks, buf);
-          slot_loads(ks * NM + j, s + NB - 1, wbuf);
+          slot_reads(j, b ^ 1, ks, qbuf, pbuf);
+          slot_loads(ks * NM + j, s, wqb, wpb);
           if constexpr (MX) {
             if (j % FQ == 0) decode(b ^ 1, j / FQ, ks);
           }
-          __builtin_amdgcn_sched_barrier(0);
+          if (j & 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (s + 1 == n_stages) break;
-      rb = rb + 1 == NB ? 0 : rb + 1;
-      const uint32_t next = lds0 + rb * SB;
-      wbuf = buf;
+      rq = rq + 1 == NBQ ? 0 : rq + 1;
+      rp = rp + 1 == NBP ? 0 : rp + 1;
+      const uint32_t next_q = q_at(rq), next_p = p_at(rp);
+      wqb = qbuf;
+      wpb = pbuf;
       stage_barrier<WAIT>();
       take_rows();
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (MX) {
 #pragma unroll
-        for (int f = 0; f < FP; ++f) read_codes(f, next);
+        for (int f = 0; f < FP; ++f) read_codes(f, next_p);
       }
 #pragma unroll
       for (int j = 0; j < NM; ++j) {
         mfma(1, j);
-        slot_reads(j, 0, 0, next);
-        slot_loads(j, s + NB, wbuf);
-        __builtin_amdgcn_sched_barrier(0);
+        slot_reads(j, 0, 0, next_q, next_p);
+        slot_loads(j, s + 1, wqb, wpb);
+        if (j & 1) __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (MX) decode_all(0, 0);
     }
