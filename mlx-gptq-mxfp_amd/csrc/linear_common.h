@@ -131,8 +131,8 @@ __device__ __forceinline__ lin_u32x4_t lin_decode_mx8(uint32_t lo, uint32_t hi,
 struct LinTile {
   int g;          // group; >= G: entries of no group
   int pt;         // tile along p
-  int64_t q0;     // first list entry
-  int64_t q_end;  // end of the segment
+  int q0;         // first list entry
+  int q_end;      // end of the segment
 };
 
 __device__ __forceinline__ int64_t lin_offset(const LinArgs& a, int i) {
@@ -272,10 +272,10 @@ __device__ inline bool lin_find_tile(const LinArgs& a, uint32_t n_pt, LinTile* t
   const uint32_t in = local - strip * wide * n_pt;
   const uint32_t left = tiles - strip * wide;
   const uint32_t sm = left < wide ? left : wide;
-  t->g = g;
-  t->pt = static_cast<int>(in / sm);
-  t->q0 = b + static_cast<int64_t>(strip * wide + in % sm) * BM;
-  t->q_end = e;
+  t->g = __builtin_amdgcn_readfirstlane(g);
+  t->pt = __builtin_amdgcn_readfirstlane(static_cast<int>(in / sm));
+  t->q0 = __builtin_amdgcn_readfirstlane(b + static_cast<int>((strip * wide + in % sm) * BM));
+  t->q_end = __builtin_amdgcn_readfirstlane(e);
   return true;
 }
 

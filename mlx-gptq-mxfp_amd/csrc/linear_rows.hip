@@ -231,14 +231,24 @@ __global__ void __launch_bounds__(256)
     mine = __builtin_amdgcn_ds_permute(4 * rank, v);
   }
   for (int64_t c0 = 0; c0 < cols; c0 += kSumCols) {
-    float acc[kSumCols / 64];
+    // four consecutive columns a lane and piece
+    constexpr int kPieces = kSumCols / 256;
+    f32x4_u_t acc[kPieces];
 #pragma unroll
-    for (int i = 0; i < kSumCols / 64; ++i) acc[i] = 0.0f;
+    for (int i = 0; i < kPieces; ++i) acc[i] = f32x4_u_t{0, 0, 0, 0};
     auto add = [&](int64_t t) {
-      const float* p = src + t * cols + c0;
+      const float* p = src + t * cols + c0 + 4 * lane;
 #pragma unroll
-      for (int i = 0; i < kSumCols / 64; ++i)
-        if (c0 + 64 * i + lane < cols) acc[i] += p[64 * i + lane];
+      for (int i = 0; i < kPieces; ++i) {
+        const int64_t c = c0 + 256 * i + 4 * lane;
+        if (c + 4 <= cols) {
+          acc[i] += load_f32x4(p + 256 * i);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < cols) acc[i][e] += p[256 * i + e];
+        }
+      }
     };
     if (n <= kSlots) {
       for (int j = 0; j < n; ++j) add(__builtin_amdgcn_readlane(mine, j));
@@ -248,9 +258,16 @@ __global__ void __launch_bounds__(256)
         for (uint64_t b = __ballot(hit); b; b &= b - 1) add(t0 + __builtin_ctzll(b));
       }
     }
+    LinArgs a = {};  // lin_store4's row length and type
+    a.np = static_cast<int>(cols);
+    a.out_type = out_type;
+    char* row = static_cast<char*>(out) + r * cols * (out_type == kF32 ? 4 : 2);
 #pragma unroll
-    for (int i = 0; i < kSumCols / 64; ++i)
-      if (c0 + 64 * i + lane < cols) store_storage(out, r * cols + c0 + 64 * i + lane, acc[i], out_type);
+    for (int i = 0; i < kPieces; ++i) {
+      const int64_t c = c0 + 256 * i + 4 * lane;
+      const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+      if (c < cols) lin_store4(a, row, static_cast<int>(c), v);
+    }
   }
 }
 
@@ -291,7 +308,7 @@ extern "C" int mgq_rows_sum(const float* src, const int32_t* row_index, int64_t 
   MGQ_REQUIRE(out_dtype == kF32 || out_dtype == kBF16 || out_dtype == kF16, MGQ_ERR_VALUE,
               "rows_sum: the result is float32, bfloat16 or float16");
   MGQ_REQUIRE(n_entries >= 0 && n_entries < (int64_t(1) << 31) && n_rows >= 0 &&
-                  n_rows < (int64_t(1) << 31) && cols >= 0,
+                  n_rows < (int64_t(1) << 31) && cols >= 0 && cols < (int64_t(1) << 30),
               MGQ_ERR_SHAPE, "rows_sum: bad shape");
   const int64_t need = mgq_rows_sum_workspace_size(n_rows);
   MGQ_REQUIRE(workspace != nullptr && workspace_bytes >= need, MGQ_ERR_WORKSPACE,

@@ -5,7 +5,7 @@
 
 namespace mgq {
 
-enum LinKind : int { kLinForward = 0, kLinDgrad = 1, kLinWgrad = 2 };
+enum LinKind : int { kLinForward = 0, kLinDgrad = 1, kLinWgrad = 2, kLinWgradGather = 3 };
 
 // wgrad: group g's entries [t0, t1). slot >= 0: the group is cut and the unit's
 // tile `i` goes to partial tile slot * tiles + i.

@@ -90,14 +90,14 @@ __device__ __forceinline__ lin_u32x4_t load16(uint64_t src) {
 // The first n bytes at `src` (n <= 0: none, n >= 16: all), zeros after them. 16
 // bytes are read where they lie before `end`, single elements otherwise.
 template <int ES>
-__device__ __forceinline__ lin_u32x4_t load_cut(uint64_t src, int64_t n, uint64_t end) {
+__device__ __forceinline__ lin_u32x4_t load_cut(uint64_t src, int n, uint64_t end) {
   lin_u32x4_t r = {0, 0, 0, 0};
   if (n <= 0) return r;
   if (src + 16 <= end) {
     r = load16(src);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t left = n - 4 * i;
+      const int left = n - 4 * i;
       r[i] &= left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1u : 0u;
     }
   } else {
@@ -120,7 +120,9 @@ constexpr int mx_stage_bytes(int bp) {
 template <int OP, int KIND, int FQ, int FP, bool STAGED>
 __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const LinPlanArgs pl) {
   constexpr bool PT = KIND != kLinForward;
-  constexpr bool QT = KIND == kLinWgrad;
+  constexpr bool WGRAD = KIND == kLinWgrad || KIND == kLinWgradGather;
+  constexpr bool GATHER = KIND == kLinWgradGather;
+  constexpr bool QT = WGRAD;
   constexpr bool MX = lin_is_mx<OP>();
   constexpr int ES = lin_esize<OP>();
   constexpr int BQ = 64 * FQ, BP = 128 * FP;
@@ -156,9 +158,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   // the results of the last, measured 2 to 4 % slower in long contractions.
   for (uint32_t item = blockIdx.x;; item += gridDim.x) {
   int g, p0, slot = -1;
-  int64_t q0, q_end;                 // rows of Q (forward, dgrad) or of the output (wgrad)
-  int64_t c_begin = 0, c_len = a.nc;  // contraction range
-  if constexpr (KIND == kLinWgrad) {
+  int q0, q_end;                 // rows of Q (forward, dgrad) or of the output (wgrad)
+  int c_begin = 0, c_len = a.nc;  // contraction range
+  if constexpr (WGRAD) {
     LinUnit u;
     int tile;
     const int found = lin_find_unit(a, pl, item, &u, &tile);
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     slot = u.slot;
     c_begin = u.t0;
     c_len = u.t1 - u.t0;
-    q0 = static_cast<int64_t>(tile % pl.nqt) * BQ;
+    q0 = tile % pl.nqt * BQ;
     p0 = tile / pl.nqt * BP;
     q_end = a.nq;
   } else {
@@ -180,9 +182,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     q_end = t.q_end;
     if (g >= a.G) c_len = 0;  // entries of no group: zeros
   }
-  const int gw = KIND == kLinWgrad || g >= a.G ? 0 : g;
+  const int gw = WGRAD || g >= a.G ? 0 : g;
   const char* Pg = a.P + gw * a.p_group;
-  const int n_stages = static_cast<int>((c_len + EK - 1) / EK);
+  const int n_stages = (c_len + EK - 1) / EK;
 
   // ---- loads ------------------------------------------------------------
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char*)lds));
@@ -203,15 +205,15 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   if constexpr (QT) {
 #pragma unroll
     for (int i = 0; i < VQ; ++i) {
-      int64_t col = q0 + tr_col(BQ, i);
+      int col = q0 + tr_col(BQ, i);
       if (!STAGED) col = col + 8 <= a.nq ? col : a.nq - 8;
       if (STAGED) col = col < a.nq ? col : a.nq - 1;
-      qp[i] = reinterpret_cast<uint64_t>(a.Q) + (c_begin + tr_row(BQ, i)) * a.ldq + 2 * col;
+      qp[i] = reinterpret_cast<uint64_t>(a.Q) + (c_begin + tr_row(BQ, i)) * a.ldq + 2 * static_cast<int64_t>(col);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < VQ; ++i) {
-      int64_t q = q0 + 8 * (VQ * wave + i) + (lane >> 3);
+      int q = q0 + 8 * (VQ * wave + i) + (lane >> 3);
       q = q < q_end ? q : q_end - 1;
       const int64_t row = KIND == kLinForward ? lin_row(a, q) : q;
       qp[i] = reinterpret_cast<uint64_t>(a.Q) + row * a.ldq + 16 * (((VQ * wave + i) & 1) ? ch1 : ch0);
@@ -233,12 +235,12 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   } else if constexpr (PT) {
 #pragma unroll
     for (int i = 0; i < VP; ++i) {
-      int64_t col = p0 + tr_col(BP, i);
+      int col = p0 + tr_col(BP, i);
       if (!STAGED) col = col + 8 <= a.np ? col : a.np - 8;
       if (STAGED) col = col < a.np ? col : a.np - 1;
-      // wgrad: the row is added when it is known
-      pp[i] = reinterpret_cast<uint64_t>(Pg) + 2 * col +
-              (KIND == kLinWgrad ? 0 : tr_row(BP, i) * a.ldp);
+      // (gathered: the row is added when it is known)
+      pp[i] = reinterpret_cast<uint64_t>(Pg) + 2 * static_cast<int64_t>(col) +
+              (GATHER ? 0 : (c_begin + tr_row(BP, i)) * a.ldp);
     }
   } else {
 #pragma unroll
@@ -254,44 +256,41 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     const int64_t q_rows = KIND == kLinForward ? a.n_rows : a.M;
     const int64_t q_cols = QT ? a.nq : a.nc;
     q_stop = reinterpret_cast<uint64_t>(a.Q) + (q_rows - 1) * a.ldq + q_cols * ES;
-    const int64_t p_rows = KIND == kLinWgrad ? a.n_rows : KIND == kLinDgrad ? a.nc : a.np;
+    const int64_t p_rows = WGRAD ? a.n_rows : KIND == kLinDgrad ? a.nc : a.np;
     const int64_t p_cols = PT ? a.np : a.nc;
     p_stop = reinterpret_cast<uint64_t>(Pg) + (p_rows - 1) * a.ldp + p_cols * ES;
   }
 
-  // wgrad: the rows of X that this wave loads in the next stage, read through the
+  // gathered wgrad: the rows of X that this wave loads in the next stage, read through the
   // scalar cache (a vector load's wait would also wait for the loads into LDS
   // before it)
-  uint32_t rows[8], rows_next[8];
+  int rows[8], rows_next[8];
   auto load_rows = [&](int st) {
-    if constexpr (KIND == kLinWgrad) {
-      const int64_t t0 = c_begin + static_cast<int64_t>(st) * EK + 8 * wave;
-      const int64_t last = c_begin + c_len - 1;
+    if constexpr (GATHER) {
+      const int t0 = c_begin + st * EK + 8 * wave;  // (below 2^31: see the entry points)
+      const int last = c_begin + c_len - 1;
+      const const_i32_ptr index =
+          reinterpret_cast<const_i32_ptr>(reinterpret_cast<uint64_t>(a.row_index));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t t = t0 + i < last ? t0 + i : last;
-        int32_t r = static_cast<int32_t>(t);
-        if (a.row_index) {
-          r = reinterpret_cast<const_i32_ptr>(reinterpret_cast<uint64_t>(a.row_index))[t];
-          r = r < 0 ? 0 : r;
-          r = r < a.n_rows ? r : static_cast<int32_t>(a.n_rows - 1);
-        }
-        rows_next[i] = static_cast<uint32_t>(r);
-      }
+      for (int i = 0; i < 8; ++i) rows_next[i] = index[t0 + i < last ? t0 + i : last];
     }
   };
-  auto take_rows = [&]() {
-    if constexpr (KIND == kLinWgrad) {
+  auto take_rows = [&]() {  // (clamped here, so that no load is waited for above)
+    if constexpr (GATHER) {
+      const int top = static_cast<int>(a.n_rows - 1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) rows[i] = rows_next[i];
+      for (int i = 0; i < 8; ++i) {
+        const int r = rows_next[i] < 0 ? 0 : rows_next[i];
+        rows[i] = r < top ? r : top;
+      }
     }
   };
 
   // load i of stage st: where it comes from (advancing the pointer), how many bytes
   // of it exist, and its place in the stage
-  auto source = [&](int i, int st, uint64_t* src, int64_t* n, uint32_t* dst) __attribute__((
+  auto source = [&](int i, int st, uint64_t* src, int* n, uint32_t* dst) __attribute__((
                     always_inline)) {
-    const int64_t left = c_len - static_cast<int64_t>(st) * EK;  // contraction elements
+    const int left = c_len - st * EK;  // contraction elements
     if (i < VQ) {
       *dst = (VQ * wave + i) * 1024;
       *src = qp[i];
@@ -323,12 +322,12 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     } else if constexpr (PT) {
       *dst = (VP * wave + k) * 1024;
       *n = tr_row(BP, k) < left ? 16 : 0;
-      if constexpr (KIND == kLinWgrad) {
+      if constexpr (GATHER) {
         constexpr int RP = 512 / BP;  // rows per load
-        uint32_t r = rows[RP * k];
+        int64_t at = rows[RP * k] * a.ldp;
 #pragma unroll
-        for (int j = 1; j < RP; ++j) r = lane / (BP / 8) == j ? rows[RP * k + j] : r;
-        *src += static_cast<uint64_t>(r) * static_cast<uint64_t>(a.ldp);
+        for (int j = 1; j < RP; ++j) at = lane / (BP / 8) == j ? rows[RP * k + j] * a.ldp : at;
+        *src += at;
       } else {
         pp[k] += EK * a.ldp;
       }
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   // straight into LDS (rows are whole pieces: n is 16 or more, or nothing is left)
   auto load = [&](int i, int st, uint32_t buf) __attribute__((always_inline)) {
     uint64_t src;
-    int64_t n;
+    int n;
     uint32_t dst;
     source(i, st, &src, &n, &dst);
     if (is_scale(i))
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   lin_u32x4_t hold[STAGED ? V : 1];
   auto fetch = [&](int i, int st) __attribute__((always_inline)) {
     uint64_t src;
-    int64_t n;
+    int n;
     uint32_t dst;
     source(i, st, &src, &n, &dst);
     const bool tr = i < VQ ? QT : PT;
@@ -366,10 +365,10 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       // stored, but nothing is read past the tensor's end
       const uint64_t stop = i < VQ ? q_stop : p_stop;
       if (n > 0 && src + 16 > stop)
-        hold[i] = load_cut<ES>(src, static_cast<int64_t>(stop - src), stop);
+        hold[i] = load_cut<ES>(src, static_cast<int>(stop - src), stop);
       else
         hold[i] = load16(n > 0 ? src : zeros);
-    } else if (__builtin_amdgcn_readfirstlane((st + 1) * static_cast<int64_t>(EK) <= c_len)) {
+    } else if ((st + 1) * EK <= c_len) {
       hold[i] = load16(src);
     } else {
       hold[i] = load_cut<ES>(src, n, i < VQ ? q_stop : p_stop);
@@ -594,17 +593,18 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   if constexpr (OP == kOpI8) {
 #pragma unroll
     for (int f = 0; f < FQ; ++f) {
-      int64_t q = q0 + 32 * (FQ * wq + f) + (lane & 31);
+      int q = q0 + 32 * (FQ * wq + f) + (lane & 31);
       q = q < q_end ? q : q_end - 1;
       sx[f] = g < a.G ? a.sx[lin_row(a, q)] : 0.0f;
     }
   }
-  char* out = a.out + (KIND == kLinWgrad ? g * a.o_group : 0) * (a.out_type == kF32 ? 4 : 2);
+  char* out = a.out + (WGRAD ? g * a.o_group : 0) * (a.out_type == kF32 ? 4 : 2);
   int64_t ldo = a.ldo;
-  const bool partial = KIND == kLinWgrad && slot >= 0;
+  const bool partial = WGRAD && slot >= 0;
   if (partial) {  // fp32, [BQ][BP]
     ldo = BP;
-    out = reinterpret_cast<char*>(pl.partials + static_cast<int64_t>(slot) * BQ * BP - q0 * BP - p0);
+    out = reinterpret_cast<char*>(pl.partials + static_cast<int64_t>(slot) * BQ * BP -
+                                  static_cast<int64_t>(q0) * BP - p0);
   }
   lds_handover();  // every wave is done with the last stage's buffer
   // Results go through LDS (a wave's own part of it) to leave as whole pieces of a
@@ -662,12 +662,12 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       for (int i = 0; i < 32 * FQ * CH / 64; ++i) {
         const int row = (64 / CH) * i + lane / CH;
         const int c = (lane % CH) ^ swizzle(row);
-        const int64_t q = q0 + 32 * FQ * wq + row;
+        const int q = q0 + 32 * FQ * wq + row;
         const int p = p0 + 32 * (FP * wp + k0) + EC * c;
         const lin_u32x4_t v =
             *reinterpret_cast<const lin_u32x4_t*>(part + row * RB + 16 * (lane % CH));
         if (q >= q_end) continue;
-        char* o = out + (q * ldo + p) * OS;
+        char* o = out + (static_cast<int64_t>(q) * ldo + p) * OS;
         if (p + EC <= a.np) {  // (at any address)
           lin_u128_u_t u;
 #pragma unroll
@@ -693,8 +693,8 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   } else {
     if constexpr (OP != kOpF16) store_out(std::integral_constant<int, kBF16>{});
   }
-  if constexpr (KIND != kLinWgrad) return;
-  lds_handover();  // every wave has its results out of LDS
+  if constexpr (!WGRAD) return;
+  stage_barrier<-1>();  // every wave has its results out of LDS (they need not be stored yet)
   }
 }
 
@@ -839,7 +839,7 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(const LinArgs a, const 
 template <int OP, int KIND, int FQ, int FP, bool STAGED>
 int launch(const LinArgs& a, const LinPlanArgs& pl, int64_t grid, hipStream_t s, const char* what) {
   MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  const int64_t most = KIND == kLinWgrad ? 2 * kCUs : grid;
+  const int64_t most = KIND == kLinWgrad || KIND == kLinWgradGather ? 2 * kCUs : grid;
   const unsigned blocks = static_cast<unsigned>(grid < most ? grid : most);
   lin_tile_kernel<OP, KIND, FQ, FP, STAGED><<<blocks, 512, 0, s>>>(a, pl);
   return check_launch(what);
@@ -862,6 +862,16 @@ int pick_rows(const LinArgs& a, LinTileShape t, hipStream_t s, const char* what)
   if (t.rows == 128) return launch_rows<OP, KIND, 2, 2, false>(a, s, what);
   return t.cols == 256 ? launch_rows<OP, KIND, 1, 2, false>(a, s, what)
                        : launch_rows<OP, KIND, 1, 1, false>(a, s, what);
+}
+
+template <int OP>
+int launch_wgrad(const LinArgs& a, const LinPlanArgs& pl, bool staged, int64_t grid, hipStream_t s,
+                 const char* what) {
+  if (a.row_index)
+    return staged ? launch<OP, kLinWgradGather, 2, 2, true>(a, pl, grid, s, what)
+                  : launch<OP, kLinWgradGather, 4, 2, false>(a, pl, grid, s, what);
+  return staged ? launch<OP, kLinWgrad, 2, 2, true>(a, pl, grid, s, what)
+                : launch<OP, kLinWgrad, 4, 2, false>(a, pl, grid, s, what);
 }
 
 inline bool aligned16(const void* p, int64_t pitch) {
@@ -934,13 +944,8 @@ int lin_tile_wgrad(const LinArgs& a, int op, void* workspace, hipStream_t s, con
   lin_plan_kernel<<<1, 1024, 0, s>>>(a, pl);
   if (int rc = check_launch(what)) return rc;
   const int64_t grid = (pl.deal ? ceil_div(z.max_units, 8) * 8 : z.max_units) * z.tiles;
-  int rc;
-  if (staged)
-    rc = op == kOpF16 ? launch<kOpF16, kLinWgrad, 2, 2, true>(a, pl, grid, s, what)
-                      : launch<kOpBF16, kLinWgrad, 2, 2, true>(a, pl, grid, s, what);
-  else
-    rc = op == kOpF16 ? launch<kOpF16, kLinWgrad, 4, 2, false>(a, pl, grid, s, what)
-                      : launch<kOpBF16, kLinWgrad, 4, 2, false>(a, pl, grid, s, what);
+  const int rc = op == kOpF16 ? launch_wgrad<kOpF16>(a, pl, staged, grid, s, what)
+                              : launch_wgrad<kOpBF16>(a, pl, staged, grid, s, what);
   if (rc || z.max_splits == 0) return rc;
   const dim3 rg(static_cast<unsigned>(z.tiles * (bq / 16)), static_cast<unsigned>(z.max_splits));
   lin_reduce_kernel<<<rg, 256, 0, s>>>(a, pl);

@@ -58,6 +58,10 @@ def _dense(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     return t if t.device == dev and t.is_contiguous() else nat.on_device(t, dev)
 
 
+def _device(*tensors: torch.Tensor) -> torch.device:
+    return tensors[0].device if tensors[0].is_cuda else nat.device_for(*tensors)
+
+
 def _home(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     """The result on the caller's device."""
     return t if like.is_cuda else t.to(like.device)
@@ -133,7 +137,7 @@ def _forward(x, weight, offsets, row_index, validate):
     G, N, K = w.shape
     if x.shape[1] != K:
         raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the weight {K}")
-    dev = nat.device_for(x, weight)
+    dev = _device(x, weight)
     xd, wd = _pitched(x, dev), _pitched(w, dev)
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
@@ -195,7 +199,7 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
         raise AssertionError(f"{fn}: dy has {dy.shape[1]} columns, the weight {N} rows")
     if row_index is not None and n_rows is None:
         raise ValueError(f"{fn}: n_rows is required with row_index")
-    dev = nat.device_for(dy, weight)
+    dev = _device(dy, weight)
     dyd, wd = _pitched(dy, dev), _pitched(w, dev)
     M = int(dy.shape[0])
     off, idx, entries = _list(fn, offsets, row_index, G, M if row_index is None else int(n_rows),
@@ -239,7 +243,7 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     out_dtype = dy.dtype if out_dtype is None else out_dtype
     if out_dtype not in (dy.dtype, torch.float32):
         raise TypeError(f"{fn}: the result is {dy.dtype} or float32 (got {out_dtype})")
-    dev = nat.device_for(dy, x)
+    dev = _device(dy, x)
     dyd, xd = _pitched(dy, dev), _pitched(x, dev)
     G = 1 if offsets is None else len(offsets) - 1
     if G < 1:
@@ -287,7 +291,7 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
                              "(a multiple of 32)")
     if tuple(s.shape) != (G, N, K // 32):
         raise AssertionError(f"{fn}: scales must be {(G, N, K // 32)} (got {tuple(s.shape)})")
-    dev = nat.device_for(x, packed, scales)
+    dev = _device(x, packed, scales)
     xd = _pitched(x, dev)
     wd, sd = _dense(w, dev), _dense(s, dev)
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
@@ -310,7 +314,7 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise TypeError(f"quantize_rows_int8: expects float32, bfloat16 or float16 (got {x.dtype})")
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"quantize_rows_int8: rows of no elements ({tuple(x.shape)})")
-    dev = nat.device_for(x)
+    dev = _device(x)
     rows = _pitched(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), dev)
     q = torch.empty(x.shape, dtype=torch.int8, device=dev)
     s = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
@@ -350,7 +354,7 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
             bias is not None and tuple(bias.shape) != per_channel):
         raise AssertionError(f"{fn}: x_scale must be {(int(x.shape[0]),)}, w_scale and bias "
                              f"{per_channel}")
-    dev = nat.device_for(x, weight)
+    dev = _device(x, weight)
     xd, wd = _pitched(x, dev), _pitched(w, dev)
     xs, ws = _dense(x_scale, dev), _dense(w_scale, dev)
     b = None if bias is None else _dense(bias, dev)
