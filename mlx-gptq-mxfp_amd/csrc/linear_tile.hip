@@ -60,10 +60,14 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// 16 bytes (1 byte, widened to a dword) per lane from `src` to LDS at
-// dst + 16 (4) * lane. (One wait state between the write of m0 and its use.)
+// 16 bytes (4; 1, widened to a dword) per lane from `src` to LDS at
+// dst + 16 (4; 4) * lane. (One wait state between the write of m0 and its use.)
 __device__ __forceinline__ void dma16(uint32_t dst, uint64_t src) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src)
+               : "memory");
+}
+__device__ __forceinline__ void dma4(uint32_t dst, uint64_t src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src)
                : "memory");
 }
 __device__ __forceinline__ void dma1(uint32_t dst, uint64_t src) {
@@ -131,8 +135,10 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   // buffers of stages: where two whole ones leave room, Q has a third, so that only
   // P's loads have to come within the period they are issued in
   constexpr int NBP = STAGED ? 2 : kLdsMax / (QB + PB) < 4 ? kLdsMax / (QB + PB) : 4;
-  constexpr int NBQ = !STAGED && NBP == 2 && 3 * QB + 2 * PB <= kLdsMax ? 3 : NBP;
-  constexpr int LDS = NBQ * QB + NBP * PB;
+  constexpr bool RING = GATHER && !STAGED;       // the gathered rows' indexes come through LDS
+  constexpr int NBQ = !STAGED && !RING && NBP == 2 && 3 * QB + 2 * PB <= kLdsMax ? 3 : NBP;
+  constexpr int RING_AT = NBQ * QB + NBP * PB;
+  constexpr int LDS = RING_AT + (RING ? 8 * 512 : 0);
   constexpr int EPI = BQ * BP * 2;               // 16-bit results on their way out
   constexpr int VQ = FQ;                         // 16-byte loads per lane and stage: Q,
   constexpr int per = OP == kOpMx4 ? 2 : 4;      // (MX: 16-byte pieces of a row's codes)
@@ -261,12 +267,27 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     p_stop = reinterpret_cast<uint64_t>(Pg) + (p_rows - 1) * a.ldp + p_cols * ES;
   }
 
-  // gathered wgrad: the rows of X that this wave loads in the next stage, read through the
-  // scalar cache (a vector load's wait would also wait for the loads into LDS
-  // before it)
+  // gathered wgrad: the rows of X that this wave loads in the next stage, 8 a stage.
+  // RING: their indexes come into LDS 64 at a time (8 stages), at least six stages
+  // before their use, into the wave's ring of two such blocks, and from there a stage
+  // ahead: a load into registers would be waited for with every load into LDS issued
+  // before it, and scalar loads return out of order with the LDS reads, which then
+  // wait for all of them (2.6 us a stage against 1.5).
   int rows[8], rows_next[8];
+  const uint32_t ring = lds0 + RING_AT + wave * 512;
+  auto ring_fetch = [&](int block) {
+    if constexpr (RING) {
+      const int t0 = c_begin + (8 * block + (lane >> 3)) * EK + 8 * wave + (lane & 7);
+      const int last = c_begin + c_len - 1;
+      dma4(ring + (block & 1) * 256,
+           reinterpret_cast<uint64_t>(a.row_index) + 4 * static_cast<int64_t>(t0 < last ? t0 : last));
+    }
+  };
   auto load_rows = [&](int st) {
-    if constexpr (GATHER) {
+    if constexpr (RING) {
+      rows_next[0] = *reinterpret_cast<const __attribute__((address_space(3))) int32_t*>(
+          ring + ((st >> 3) & 1) * 256 + ((st & 7) * 8 + (lane & 7)) * 4);
+    } else if constexpr (GATHER) {
       const int t0 = c_begin + st * EK + 8 * wave;  // (below 2^31: see the entry points)
       const int last = c_begin + c_len - 1;
       const const_i32_ptr index =
@@ -280,7 +301,8 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       const int top = static_cast<int>(a.n_rows - 1);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int r = rows_next[i] < 0 ? 0 : rows_next[i];
+        const int v = RING ? __builtin_amdgcn_readlane(rows_next[0], i) : rows_next[i];
+        const int r = v < 0 ? 0 : v;
         rows[i] = r < top ? r : top;
       }
     }
@@ -518,6 +540,10 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       }
       load_rows(2);
     } else {
+      if constexpr (RING) {
+        ring_fetch(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
 #pragma unroll
       for (int st = 0; st < NBQ - 1; ++st) {
         if (st < NBP - 1) {
@@ -547,6 +573,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     int rq = 0, rp = 0;
     for (int s = 0; s < n_stages; ++s) {
       const uint32_t qbuf = q_at(rq), pbuf = p_at(rp);
+      if (RING && (s & 7) == 0) ring_fetch((s >> 3) + 1);
       load_rows(s + NBP + (STAGED ? 1 : 0));
 #pragma unroll
       for (int ks = 1; ks < kSteps; ++ks) {
