@@ -116,6 +116,28 @@ __device__ __forceinline__ lin_u32x4_t load_cut(uint64_t src, int n, uint64_t en
   return r;
 }
 
+// The low cut >> 8 bytes shifted out, then all but the low (cut & 255) cleared.
+__device__ __forceinline__ lin_u32x4_t cut16(lin_u32x4_t v, int cut) {
+  const int d = cut >> 8, m = cut & 255;
+  if (__any(d != 0)) {
+    // whole dwords, then bytes
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+      const bool go = (d >> 2) > w;
+      v = lin_u32x4_t{go ? v[1] : v[0], go ? v[2] : v[1], go ? v[3] : v[2], go ? 0u : v[3]};
+    }
+    const uint32_t s = 8 * (d & 3);
+    v = lin_u32x4_t{__builtin_amdgcn_alignbit(v[1], v[0], s), __builtin_amdgcn_alignbit(v[2], v[1], s),
+                    __builtin_amdgcn_alignbit(v[3], v[2], s), v[3] >> s};
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int left = m - 4 * i;
+    v[i] &= left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1u : 0u;
+  }
+  return v;
+}
+
 template <int OP>
 constexpr int mx_stage_bytes(int bp) {
   return OP == kOpMx4 ? bp * 32 + bp * 8 : bp * 64 + bp * 8;
@@ -373,6 +395,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   };
   // through registers
   lin_u32x4_t hold[STAGED ? V : 1];
+  int cut[STAGED ? V : 1];  // bytes kept | bytes shifted out << 8
+  const bool tiny = STAGED && (q_stop - reinterpret_cast<uint64_t>(a.Q) < 16 ||
+                               p_stop - reinterpret_cast<uint64_t>(Pg) < 16);
   auto fetch = [&](int i, int st) __attribute__((always_inline)) {
     uint64_t src;
     int n;
@@ -393,11 +418,25 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     } else if ((st + 1) * EK <= c_len) {
       hold[i] = load16(src);
     } else {
-      hold[i] = load_cut<ES>(src, n, i < VQ ? q_stop : p_stop);
+      // the stage in which the rows end: n of the 16 bytes exist. They are loaded
+      // whole (from 16 bytes before the operand's end if they would pass it) and cut on
+      // the way into LDS, so that no load is waited for here.
+      const uint64_t stop = i < VQ ? q_stop : p_stop;
+      const int m = n < 0 ? 0 : n > 16 ? 16 : n;
+      if (tiny) {
+        hold[i] = load_cut<ES>(src, m, stop);
+        cut[i] = 16;
+      } else {
+        const bool past = m > 0 && src + 16 > stop;
+        hold[i] = load16(m == 0 ? zeros : past ? stop - 16 : src);
+        cut[i] = m | (past ? static_cast<int>(src + 16 - stop) << 8 : 0);
+      }
     }
   };
-  auto put = [&](int i, uint32_t buf) __attribute__((always_inline)) {
+  auto put = [&](int i, int st, uint32_t buf) __attribute__((always_inline)) {
     const int k = i - VQ;
+    const bool plain = i < VQ ? !QT : !PT && !MX;
+    if (plain && (st + 1) * EK > c_len) hold[i] = cut16(hold[i], cut[i]);
     uint32_t dst;
     if (i < VQ) dst = (VQ * wave + i) * 1024;
     else if (is_scale(i)) dst = BP * 16 * per + mx_wave * 256;
@@ -518,7 +557,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       const uint32_t buf = k < VP ? pbuf : qbuf;
       const int st = s + (k < VP ? NBP : NBQ) - 1;
       if constexpr (STAGED) {
-        put(i, buf);
+        put(i, st, buf);
         fetch(i, st + 1);
       } else {
         load(i, st, buf);
@@ -535,7 +574,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
       take_rows();
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        put(i, i < VQ ? q_at(0) : p_at(0));
+        put(i, 0, i < VQ ? q_at(0) : p_at(0));
         fetch(i, 1);
       }
       load_rows(2);
