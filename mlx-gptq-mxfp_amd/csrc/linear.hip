@@ -11,10 +11,11 @@ namespace mgq {
 namespace {
 
 // Which kernel and tile a product over rows takes: the one whose time by the
-// model below is least. The model was fitted to 539 measurements (all types,
-// 1 .. 16384 entries, 0 .. 128 groups, K 256 .. 7168, aligned and not; 2 to 7
-// choices each): the choice costs 1.3 % over the best of each, at most 45 %, where
-// always taking the largest tile that the average group fills costs 60 %.
+// model below is least. The model was fitted to 741 products (all types, 1 .. 16384
+// entries, 0 .. 128 groups, K 256 .. 7168, aligned and not) that were timed with each
+// of their 3 to 7 choices: the model's choice costs 1.9 % over the best one on
+// average and 59 % at worst, where the largest tile that the average group fills
+// costs 37 % on average and tenfold at worst.
 //
 //   large tiles: rounds of the 256 CUs x (stages x time of a stage + a fixed time
 //     for the tile's first loads and its results), or the weight's bytes at the
@@ -23,16 +24,16 @@ namespace {
 //     workgroups read through L2, or the weight's bytes from memory.
 //
 // How the entries fall into groups is not known here: each active group is taken
-// to leave 0.6 tiles partly filled.
+// to leave half a tile unfilled.
 struct TileTime {
   int rows, cols;
   bool staged;
   double stage, fixed;  // us
 };
 constexpr TileTime kTileTimes[] = {
-    {64, 128, false, 0.33, 3.2}, {64, 256, false, 0.58, 2.9},  {128, 256, false, 0.87, 3.2},
-    {256, 256, false, 1.47, 5.0}, {64, 128, true, 0.81, 3.2}, {64, 256, true, 0.89, 2.9},
-    {128, 256, true, 1.14, 3.2},
+    {64, 128, false, 0.38, 3.0}, {64, 256, false, 0.58, 2.9},  {128, 256, false, 0.87, 2.9},
+    {256, 256, false, 1.27, 4.1}, {64, 128, true, 0.70, 3.5}, {64, 256, true, 0.89, 2.9},
+    {128, 256, true, 1.47, 3.2},
 };
 
 template <int OP, int KIND>
@@ -44,14 +45,14 @@ int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
   const double active = a.offsets ? (a.G < a.M ? a.G : M) : 1;
   const double weight_bytes = active * np * nc * wb;
   auto row_tiles = [&](int rows) {
-    return a.offsets ? fmax(1.0, M / rows + 0.6 * active) : ceil(M / rows);
+    return a.offsets ? fmax(1.0, M / rows + 0.51 * active) : ceil(M / rows);
   };
   double best = 1e300;
   LinTileShape shape = {};
   for (const TileTime& t : kTileTimes) {
     if (t.staged == direct) continue;
     double rounds = row_tiles(t.rows) * ceil(np / t.cols) / 256;
-    rounds = rounds < 1 ? 1 : rounds + 0.76 * (ceil(rounds) - rounds);
+    rounds = rounds < 1 ? 1 : rounds + 0.65 * (ceil(rounds) - rounds);
     const double stage = t.stage * (wb < 1 ? 1.25 : 1.0);
     const double us = 2 + fmax(rounds * (ceil(nc * es / 128) * stage + t.fixed),
                                weight_bytes / (direct ? 14.0e6 : 3.4e6));
@@ -64,10 +65,10 @@ int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
     int few = 0;
     for (const int nq : {1, 2, 4}) {
       const int rows = 16 * nq, cols = nq == 4 ? 32 : 16, batch = nq == 4 ? 4 : 8;
-      const double cost = direct ? 1.0 : 2.9;  // of a load that crosses its pieces
+      const double cost = direct ? 1.0 : 2.7;  // of a load that crosses its pieces
       const double l2 = row_tiles(rows) * ceil(np / cols) * (cols * wb + rows * es) * nc * cost;
       const double chain = ceil(ceil(nc * es / 256) / batch) * batch * (nq + cols / 16) * 0.12 * cost;
-      const double us = 5.8 + fmax(chain, fmax(l2 / 7.2e6, weight_bytes / 4.2e6));
+      const double us = 5.4 + fmax(chain, fmax(l2 / 5.55e6, weight_bytes / 4.35e6));
       if (us < best) {
         best = us;
         few = nq;
