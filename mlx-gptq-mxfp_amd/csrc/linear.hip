@@ -189,11 +189,11 @@ extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, i
   if (int rc = check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
   if (int rc = check_dims(what, N, K)) return rc;
   MGQ_REQUIRE(lddy >= N && ldx >= K, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
+  MGQ_REQUIRE(n_groups <= kLinPlanGroups, MGQ_ERR_SHAPE, "%s: %lld groups (at most %d)", what,
+              (long long)n_groups, kLinPlanGroups);
   const int64_t need = mgq_grouped_wgrad_workspace_size(n_entries, n_groups, N, K);
   MGQ_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), MGQ_ERR_WORKSPACE,
               "%s: workspace %lld < %lld bytes", what, (long long)workspace_bytes, (long long)need);
-  MGQ_REQUIRE(n_groups <= kLinPlanGroups, MGQ_ERR_SHAPE, "%s: %lld groups (at most %d)", what,
-              (long long)n_groups, kLinPlanGroups);
   if (K == 0) return MGQ_OK;
   LinArgs a = {};
   a.P = static_cast<const char*>(X);

@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(64 * kWaves) lin_few_kernel(const LinArgs a) {
 template <int OP, int NP, int NQ>
 int launch(const LinArgs& a, hipStream_t s, const char* what) {
   const int64_t grid = lin_row_tiles(a, 16 * NQ) * ceil_div(a.np, 16 * NP);
-  MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  MGQ_REQUIRE(grid < (int64_t(1) << 24), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.P) | reinterpret_cast<uintptr_t>(a.Q) |
                        static_cast<uintptr_t>(a.ldp | a.ldq | a.p_group) |
                        static_cast<uintptr_t>(static_cast<int64_t>(a.nc) * lin_esize<OP>());

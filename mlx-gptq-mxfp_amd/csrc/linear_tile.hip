@@ -764,6 +764,9 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
   }
 }
 
+// A cap that no group is longer than.
+constexpr int kLinNoCap = 0x7fffffc0;
+
 // ---------------------------------------------------------------------------
 // wgrad's units: a group's entries, cut into chunks of at most `cap`, longest
 // first so that the last tiles to start are the shortest. One workgroup plans. Each
@@ -776,6 +779,7 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
 __global__ void __launch_bounds__(1024) lin_plan_kernel(const LinArgs a, const LinPlanArgs pl) {
   __shared__ int32_t size[kLinPlanGroups], parts[kLinPlanGroups], chunk[kLinPlanGroups];
   __shared__ float price[16];
+  __shared__ bool fits[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int g = threadIdx.x; g < a.G; g += 1024) {
     int64_t b = 0, e = a.M;
@@ -785,21 +789,22 @@ __global__ void __launch_bounds__(1024) lin_plan_kernel(const LinArgs a, const L
   __syncthreads();
   auto cap_of = [&](int k) {  // a multiple of 64
     const int64_t c = (static_cast<int64_t>(pl.cap) << (k >> 1)) * (k & 1 ? 181 : 128) / 128;
-    return static_cast<int>((c < 0x3fffffff ? c : 0x3fffffff) & ~int64_t(63));
+    return static_cast<int>(c < kLinNoCap ? c & ~int64_t(63) : kLinNoCap);
   };
   {
     const int cap = cap_of(wave), tiles = pl.npt * pl.nqt;
     float load = 0, longest = 0;
-    uint32_t units = 0, cut = 0;
+    uint32_t units = 0, cut = 0, splits = 0;
     for (int o0 = 0; o0 < a.G; o0 += 64) {
       const int n = o0 + lane < a.G ? size[o0 + lane] : 0;
-      const int k = n > cap ? (n + cap - 1) / cap : 1;
+      const int k = n > cap ? (n - 1) / cap + 1 : 1;
       const float us = 5.0f + 1.5f / 64 * ((n + k - 1) / k);
       if (o0 + lane < a.G) {
         load += k * us;
         longest = fmaxf(longest, us);
         units += k;
         cut += k > 1 ? k : 0;
+        splits += k > 1;
       }
     }
 #pragma unroll
@@ -808,27 +813,35 @@ __global__ void __launch_bounds__(1024) lin_plan_kernel(const LinArgs a, const L
       longest = fmaxf(longest, __shfl_xor(longest, d));
       units += __shfl_xor(units, d);
       cut += __shfl_xor(cut, d);
+      splits += __shfl_xor(splits, d);
     }
     const float items = static_cast<float>(units) * tiles;
     const float us = (items <= 256 ? longest : load * tiles / 256 + 0.5f * longest) +
                      0.11f * cut * tiles;
-    if (lane == 0) price[wave] = us;
+    if (lane == 0) {
+      price[wave] = us;
+      fits[wave] = units <= static_cast<uint32_t>(pl.max_units) &&
+                   cut <= static_cast<uint32_t>(pl.max_slots) &&
+                   splits <= static_cast<uint32_t>(pl.max_splits);
+    }
   }
   __syncthreads();
   int pick = 15;  // the longest cap among the cheapest
   for (int k = 14; k >= 0; --k) pick = price[k] < 0.97f * price[pick] ? k : pick;
-  const int cap = cap_of(pick);
+  // (the workspace has room for the cuts of any list; groups whose offsets decrease may
+  // overlap and add up to more: they stay whole)
+  const int cap = fits[pick] ? cap_of(pick) : kLinNoCap;
   for (int g = threadIdx.x; g < a.G; g += 1024) {
     const int n = size[g];
-    const int k = n > cap ? (n + cap - 1) / cap : 1;
+    const int k = n > cap ? (n - 1) / cap + 1 : 1;
     parts[g] = k;
     chunk[g] = ((n + k - 1) / k + 63) & ~63;  // whole stages
   }
   __syncthreads();
   for (int g = wave; g < a.G; g += 16) {
     const int n = size[g], k = parts[g], len = chunk[g];
-    // units before this group's, and its first slot, 16 bits each (a valid list has
-    // at most a few thousand)
+    // units before this group's, and its first slot, 16 bits each (there are at
+    // most 4096 groups and 1025 cuts)
     uint32_t sums = 0, splits = 0, units = 0, all_splits = 0;
     for (int o0 = 0; o0 < a.G; o0 += 64) {
       const int o = o0 + lane;
@@ -847,27 +860,24 @@ __global__ void __launch_bounds__(1024) lin_plan_kernel(const LinArgs a, const L
     const uint32_t first = sums >> 16, slots = sums & 0xffffu;
     int64_t b = 0, e = a.M;
     if (a.offsets) lin_segment(a, g, &b, &e);
-    // (a list whose offsets decrease may have more units than there is room for)
-    const bool room = slots + k <= static_cast<uint32_t>(pl.max_slots);
     for (int i = lane; i < k; i += 64) {
-      if (first + i >= static_cast<uint32_t>(pl.max_units)) break;
       const int64_t t0 = static_cast<int64_t>(i) * len, t1 = t0 + len;
       LinUnit u;
       u.g = g;
       u.t0 = static_cast<int32_t>(b + (t0 < n ? t0 : n));
       u.t1 = static_cast<int32_t>(b + (t1 < n ? t1 : n));
-      u.slot = k > 1 && room ? static_cast<int32_t>(slots) + i : -1;
+      u.slot = k > 1 ? static_cast<int32_t>(slots) + i : -1;
       pl.units[first + i] = u;
     }
     if (lane == 0) {
-      if (k > 1 && splits < static_cast<uint32_t>(pl.max_splits)) {
+      if (k > 1) {
         pl.splits[splits].g = g;
         pl.splits[splits].slot0 = static_cast<int32_t>(slots);
-        pl.splits[splits].n = room ? k : 0;
+        pl.splits[splits].n = k;
       }
       if (g == 0) {
-        pl.counts[0] = min(static_cast<int>(units), pl.max_units);
-        pl.counts[1] = min(static_cast<int>(all_splits), pl.max_splits);
+        pl.counts[0] = static_cast<int>(units);
+        pl.counts[1] = static_cast<int>(all_splits);
       }
     }
   }
@@ -882,7 +892,7 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(const LinArgs a, const 
   const int tile = blockIdx.x / subs, sub = blockIdx.x % subs;
   const int q0 = tile % pl.nqt * pl.bq + sub * 16, p0 = tile / pl.nqt * 256;
   const int p = p0 + 4 * (threadIdx.x & 63);
-  if (p >= a.np || sp.n == 0) return;
+  if (p >= a.np) return;
   const int osize = a.out_type == kF32 ? 4 : 2;
   const int64_t tile_size = static_cast<int64_t>(pl.bq) * 256;
   for (int r = threadIdx.x >> 6; r < 16; r += 4) {
@@ -904,8 +914,10 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(const LinArgs a, const 
 
 template <int OP, int KIND, int FQ, int FP, bool STAGED>
 int launch(const LinArgs& a, const LinPlanArgs& pl, int64_t grid, hipStream_t s, const char* what) {
-  MGQ_REQUIRE(grid < (int64_t(1) << 31), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
   const int64_t most = KIND == kLinWgrad || KIND == kLinWgradGather ? 2 * kCUs : grid;
+  // (a launch has less than 2^32 threads)
+  MGQ_REQUIRE(most < (int64_t(1) << 23) && grid < (int64_t(1) << 31), MGQ_ERR_SHAPE,
+              "%s: too many output tiles", what);
   const unsigned blocks = static_cast<unsigned>(grid < most ? grid : most);
   lin_tile_kernel<OP, KIND, FQ, FP, STAGED><<<blocks, 512, 0, s>>>(a, pl);
   return check_launch(what);
@@ -948,7 +960,7 @@ LinPlanSizes plan_sizes(int64_t M, int64_t G, int64_t N, int64_t K, int bq) {
   LinPlanSizes z;
   z.tiles = ceil_div(N, bq) * ceil_div(K, 256);
   const int64_t cap = M * z.tiles / 1024;  // at most 2048 partial tiles
-  z.cap = (cap < 256 ? 256 : cap + 63) & ~int64_t(63);
+  z.cap = cap < 256 ? 256 : cap < kLinNoCap ? (cap + 63) & ~int64_t(63) : kLinNoCap;
   const int64_t over = M / z.cap + 1;  // whole chunks, and groups longer than cap
   z.max_splits = M > z.cap ? (over < G ? over : G) : 0;
   z.max_slots = z.max_splits ? over + z.max_splits : 0;

@@ -107,3 +107,13 @@ def test_entry_points_return_a_status():
     assert _rc("mgq_grouped_dgrad", *dg) == nat.ERR_VALUE
     wg = [1, nat.DTYPE_BF16, 4, 2, 1, 4, 8, None, 1, 3, 8, None, 1, nat.DTYPE_BF16, None, 0, None]
     assert _rc("mgq_grouped_wgrad", *wg) == nat.ERR_SHAPE  # lddy < N
+
+
+def test_weight_gradient_takes_4096_groups():
+    wg = [1, nat.DTYPE_BF16, 4, 8, 1, 4, 8, None, 4097, 8, 8, 1, 1, nat.DTYPE_BF16, 1, 1 << 40, None]
+    assert _rc("mgq_grouped_wgrad", *wg) == nat.ERR_SHAPE and "4096" in nat.last_error()
+
+
+def test_more_tiles_than_a_launch_holds_are_refused():
+    gl = [16, nat.DTYPE_BF16, 1 << 30, 8, None, 1 << 30, 16, 1, 1 << 29, 8, 8, 0, None, 16, None]
+    assert _rc("mgq_grouped_linear", *gl) == nat.ERR_SHAPE and "tiles" in nat.last_error()
