@@ -53,6 +53,11 @@ SIZES = [
     (8, 1536, 1024, 64, True), (64, 768, 1024, 32, True), (512, 768, 1024, 32, True),
     (4096, 512, 1024, 60, True), (6000, 1408, 264, 8, False), (2048, 256, 128, 300, True),
     (64, 767, 1001, 32, True), (3000, 511, 999, 32, True), (5000, 1407, 129, 8, False),
+    (256, 256, 1024, 0, False), (384, 512, 2048, 0, True), (384, 512, 4096, 0, False),
+    (384, 512, 512, 0, False), (256, 255, 1023, 0, False), (128, 32767, 15, 8, False),
+    (200, 32767, 17, 8, False), (8192, 128, 64, 256, False), (16384, 128, 64, 256, True),
+    (16384, 64, 128, 256, False), (8192, 60, 100, 256, True), (384, 255, 1407, 0, False),
+    (3000, 1536, 2048, 0, False), (6000, 2048, 1024, 0, True),
 ]
 
 
@@ -88,10 +93,11 @@ def test_forward(M, N, K, G, gathered, dtype):
 
 
 @pytest.mark.parametrize("M,N,K,G,gathered", SIZES)
-def test_dgrad(M, N, K, G, gathered):
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_dgrad(M, N, K, G, gathered, dtype):
     g, off, T, idx = case(M, N, K, G, gathered)
-    dy = randn(g, M, N)
-    w = randn(g, *([G] if G else []), N, K, scale=0.1)
+    dy = randn(g, M, N, dtype=dtype)
+    w = randn(g, *([G] if G else []), N, K, dtype=dtype, scale=0.1)
     dx = linear.grouped_linear_dgrad(dy, w, off, idx, T)
     want, mag = forward64(dy, w.transpose(-1, -2).contiguous(), off, None)
     most = 1
@@ -104,10 +110,11 @@ def test_dgrad(M, N, K, G, gathered):
 
 
 @pytest.mark.parametrize("M,N,K,G,gathered", SIZES)
-@pytest.mark.parametrize("out", [None, torch.float32])
-def test_wgrad(M, N, K, G, gathered, out):
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, None), (torch.bfloat16, torch.float32),
+                                       (torch.float16, None)])
+def test_wgrad(M, N, K, G, gathered, dtype, out):
     g, off, T, idx = case(M, N, K, G, gathered)
-    dy, x = randn(g, M, N, scale=0.1), randn(g, T, K)
+    dy, x = randn(g, M, N, dtype=dtype, scale=0.1), randn(g, T, K, dtype=dtype)
     dw = linear.grouped_linear_wgrad(dy, x, off, idx, out_dtype=out)
     xs = x.double() if idx is None else x.double()[idx.long()]
     spans = [(0, M)] if off is None else list(zip(off[:-1], off[1:]))
