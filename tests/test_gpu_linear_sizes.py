@@ -212,3 +212,24 @@ def test_no_entries(off):
     assert q.shape == (0, 64) and s.shape == (0,)
     y = linear.int8_linear(q, s, w.to(torch.int8), torch.ones(*gs, 40, device=DEV), offsets=off)
     assert y.shape == (0, 40)
+
+
+@pytest.mark.parametrize("mode", ["mxfp4", "mxfp8"])
+@pytest.mark.parametrize("M,N,K,G", [(3, 129, 544, 0), (70, 1000, 96, 0), (900, 515, 1056, 0),
+                                     (3000, 1030, 288, 0), (500, 260, 160, 9)])
+def test_mxfp_rows_and_words_off_every_boundary(M, N, K, G, mode):
+    """Rows that start two bytes past a boundary, words that start four past one."""
+    g, off, _, _ = case(M, N, K, G, False)
+    gs = [G] if G else []
+    bits = 4 if mode == "mxfp4" else 8
+    x = randn(g, M, K + 3)[:, 1 : K + 1]
+    codes = torch.randint(0, 127, (*gs, N, K), generator=g, dtype=torch.uint8, device=DEV) % (1 << bits)
+    packed = packing.pack_q(codes, bits)
+    words = torch.empty(packed.numel() + 1, dtype=packed.dtype, device=DEV)[1:].view(packed.shape)
+    words.copy_(packed)
+    flat = torch.randint(115, 131, (codes.numel() // 32 + 1,), generator=g, dtype=torch.uint8,
+                         device=DEV)
+    scales = flat[1:].view(*gs, N, K // 32)
+    y = linear.mxfp_linear(x, words, scales, mode, off)
+    w = ref.decode(codes.cpu(), scales.cpu(), mode).to(DEV)
+    close(y, *forward64(x, w, off, None), K, (M, N, K, G, mode))
