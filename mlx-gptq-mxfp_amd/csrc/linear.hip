@@ -11,64 +11,66 @@ namespace mgq {
 namespace {
 
 // Which kernel and tile a product over rows takes: the one whose time by the
-// model below is least. The model was fitted to 741 products (all types, 1 .. 16384
-// entries, 0 .. 128 groups, K 256 .. 7168, aligned and not) that were timed with each
-// of their 3 to 7 choices: the model's choice costs 1.9 % over the best one on
-// average and 59 % at worst, where the largest tile that the average group fills
-// costs 37 % on average and tenfold at worst.
+// model below is least. The model was fitted to 980 products (all types, 1 .. 16384
+// entries, 0 .. 128 groups, K 256 .. 14336, aligned and not) that were timed with each
+// of their 3 to 7 choices: the model's choice costs 1.7 % over the best one on
+// average and 46 % at worst, where the largest tile that the average group fills
+// costs 33 % on average and tenfold at worst.
 //
 //   large tiles: rounds of the 256 CUs x (stages x time of a stage + a fixed time
 //     for the tile's first loads and its results), or the weight's bytes at the
 //     rate the tile's loads reach;
 //   few rows: a wave's batches of loads one after the other, or the bytes that all
-//     workgroups read through L2, or the weight's bytes from memory.
+//     workgroups read through L2 (rows that a tile repeats are read once), or the
+//     weight's bytes from memory. Loads of pieces that are not even on 4-byte
+//     boundaries cost 2.4 times as much.
 //
 // How the entries fall into groups is not known here: each active group is taken
-// to leave half a tile unfilled.
+// to leave 0.7 tiles unfilled.
 struct TileTime {
   int rows, cols;
   bool staged;
   double stage, fixed;  // us
 };
 constexpr TileTime kTileTimes[] = {
-    {64, 128, false, 0.38, 3.0}, {64, 256, false, 0.58, 2.9},  {128, 256, false, 0.87, 2.9},
-    {256, 256, false, 1.27, 4.1}, {64, 128, true, 0.70, 3.5}, {64, 256, true, 0.89, 2.9},
-    {128, 256, true, 1.47, 3.2},
+    {64, 128, false, 0.40, 2.5}, {64, 256, false, 0.52, 2.5}, {128, 256, false, 0.81, 2.4},
+    {256, 256, false, 1.18, 3.8}, {64, 128, true, 0.60, 3.3}, {64, 256, true, 1.00, 3.1},
+    {128, 256, true, 1.27, 2.7},
 };
 
 template <int OP, int KIND>
 int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
   const bool direct = lin_tile_direct(a, OP, KIND);
-  const int es = lin_esize<OP>();
+  const int64_t es = lin_esize<OP>();
   const double wb = OP == kOpMx4 ? 0.53 : OP == kOpMx8 ? 1.03 : es;  // bytes of a weight
   const double M = static_cast<double>(a.M), np = a.np, nc = a.nc;
   const double active = a.offsets ? (a.G < a.M ? a.G : M) : 1;
   const double weight_bytes = active * np * nc * wb;
   auto row_tiles = [&](int rows) {
-    return a.offsets ? fmax(1.0, M / rows + 0.51 * active) : ceil(M / rows);
+    return a.offsets ? fmax(1.0, M / rows + 0.7 * active) : ceil(M / rows);
   };
   double best = 1e300;
   LinTileShape shape = {};
   for (const TileTime& t : kTileTimes) {
     if (t.staged == direct) continue;
     double rounds = row_tiles(t.rows) * ceil(np / t.cols) / 256;
-    rounds = rounds < 1 ? 1 : rounds + 0.65 * (ceil(rounds) - rounds);
-    const double stage = t.stage * (wb < 1 ? 1.25 : 1.0);
-    const double us = 2 + fmax(rounds * (ceil(nc * es / 128) * stage + t.fixed),
-                               weight_bytes / (direct ? 14.0e6 : 3.4e6));
+    rounds = rounds < 1 ? 1 : rounds + 0.54 * (ceil(rounds) - rounds);
+    const double us = 2 + fmax(rounds * (ceil(nc * es / 128) * t.stage + t.fixed),
+                               weight_bytes / (direct ? 14.0e6 : 3.7e6));
     if (us < best) {
       best = us;
       shape = LinTileShape{t.rows, t.cols, t.staged};
     }
   }
   if (KIND == kLinForward) {
+    const double cost = (lin_row_bounds(a, a.nc * es) & 3) ? 2.4 : 1.0;
     int few = 0;
     for (const int nq : {1, 2, 4}) {
       const int rows = 16 * nq, cols = nq == 4 ? 32 : 16, batch = nq == 4 ? 4 : 8;
-      const double cost = direct ? 1.0 : 2.7;  // of a load that crosses its pieces
-      const double l2 = row_tiles(rows) * ceil(np / cols) * (cols * wb + rows * es) * nc * cost;
+      const double read = fmin(rows, ceil(M / active));
+      const double l2 = row_tiles(rows) * ceil(np / cols) * (cols * wb + read * es) * nc * cost;
       const double chain = ceil(ceil(nc * es / 256) / batch) * batch * (nq + cols / 16) * 0.12 * cost;
-      const double us = 5.4 + fmax(chain, fmax(l2 / 5.55e6, weight_bytes / 4.35e6));
+      const double us = 4.9 + fmax(chain, fmax(l2 / 6.7e6, weight_bytes / 2.86e6));
       if (us < best) {
         best = us;
         few = nq;

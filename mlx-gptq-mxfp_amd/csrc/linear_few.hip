@@ -264,10 +264,7 @@ template <int OP, int NP, int NQ>
 int launch(const LinArgs& a, hipStream_t s, const char* what) {
   const int64_t grid = lin_row_tiles(a, 16 * NQ) * ceil_div(a.np, 16 * NP);
   MGQ_REQUIRE(grid < (int64_t(1) << 24), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(a.P) | reinterpret_cast<uintptr_t>(a.Q) |
-                       static_cast<uintptr_t>(a.ldp | a.ldq | a.p_group) |
-                       static_cast<uintptr_t>(static_cast<int64_t>(a.nc) * lin_esize<OP>());
-  if ((at & 15) == 0)
+  if ((lin_row_bounds(a, static_cast<int64_t>(a.nc) * lin_esize<OP>()) & 15) == 0)
     lin_few_kernel<OP, NP, NQ, true><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
   else
     lin_few_kernel<OP, NP, NQ, false><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
