@@ -364,7 +364,8 @@ int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy
                       const int32_t* offsets, void* dX, int out_dtype, void* stream);
 
 /* dW[g, n, k] = sum over the entries t of group g of dY[t, n] X[row(t), k];
- * zeros for a group without entries. out_dtype is dtype or f32. */
+ * zeros for a group without entries. out_dtype is dtype or f32. At most 4096
+ * groups; the workspace is 256-byte aligned. */
 int64_t mgq_grouped_wgrad_workspace_size(int64_t n_entries, int64_t n_groups, int64_t N,
                                          int64_t K);
 int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy, const void* X,
@@ -391,7 +392,8 @@ int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const int32_t* r
                     int64_t n_groups, int64_t N, int64_t K, const int32_t* offsets, void* Y,
                     void* stream);
 
-/* q = rne(x / s), s = max |x| of the row / 127 (fp32 quotients). A zero row
+/* q = rne(x / s) within +-127, s = max |x| of the row / 127 (fp32 quotients; a
+ * subnormal s may be too small for its row, whose codes stop at 127). A zero row
  * has s = 0, q = 0; a row holding a NaN or an infinity s = NaN, q = 0.
  * X: [rows, cols] of dtype (f32/bf16/f16) -> q i8 [rows, cols], scales f32. */
 int mgq_quantize_rows_int8(const void* X, int dtype, int64_t rows, int64_t cols, int64_t ldx,

@@ -10,7 +10,7 @@ namespace {
 // 127. A zero row has s = 0 and q = 0; a row that holds a NaN or an infinity has
 // s = NaN and q = 0, so that every product with it is NaN.
 //
-// Bound by memory (65537 x 5120 bf16 in 0.2 ms, 4.7 TB/s read and written): a row
+// Bound by memory (65537 x 5120 bf16 in 0.17 ms, 5.8 TB/s read and written): a row
 // is read once and stays in registers, PIECES of 16 bytes a lane, between its
 // maximum and its codes; WAVES waves share it. Longer rows (PIECES = 0) are read
 // twice. Rows have any pitch and alignment: a 16-byte load takes any address, and
@@ -191,7 +191,9 @@ void quantize_rows(const char* X, int64_t rows, int64_t cols, int64_t ldx, int8_
 // out[r] = sum of src[t] over the list entries t with row_index[t] = r, in the
 // order of t, in fp32. Each row has kSlots slots that the entries fill in any
 // order; the sum sorts them, so it does not depend on the atomics' order. A row
-// with more entries than slots finds them by scanning the list.
+// with more entries than slots finds them by scanning the list. Bound by memory:
+// 8198 entries into 4099 rows of 1024 take 8.2 us (50 MB, mostly from the caches), and
+// clearing and filling the slots 3 us each; both in one workgroup took 16.
 // ---------------------------------------------------------------------------
 constexpr int kSlots = 16;
 constexpr int kSumCols = 1024;  // columns a wave sums at once

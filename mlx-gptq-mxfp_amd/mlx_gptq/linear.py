@@ -21,7 +21,9 @@ that belong to no group give zero rows. ``offsets=None`` is one dense weight
 (without its leading dimension). Offsets on the device stay there: with
 ``validate=False`` no call waits for the device, so a decoding loop can be
 captured in a graph. Offsets and indexes outside their ranges are clamped by the
-kernels, never followed; ``validate`` raises for them.
+kernels, never followed; ``validate`` raises for them. Only ``grouped_linear``
+is differentiable: codes and int8 rows have no gradient, and their products
+return none for ``x``.
 
 Work is enqueued on the current stream of the tensors' device. Host tensors are
 staged through the current HIP device, as in the other modules.
@@ -234,7 +236,7 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     ([N, K] without offsets), of dy's type or ``out_dtype=torch.float32``.
 
     dy: [entries, N], x: [T, K]. fp32 sums over a group's entries, rounded
-    once; zeros for a group without entries.
+    once; zeros for a group without entries. At most 4096 groups.
     """
     fn = "grouped_linear_wgrad"
     _check_half(fn, dy, x)
