@@ -14,7 +14,7 @@ namespace {
 // model below is least. The model was fitted to 980 products (all types, 1 .. 16384
 // entries, 0 .. 128 groups, K 256 .. 14336, aligned and not) that were timed with each
 // of their 3 to 7 choices: the model's choice costs 1.7 % over the best one on
-// average and 46 % at worst, where the largest tile that the average group fills
+// average and 64 % at worst, where the largest tile that the average group fills
 // costs 33 % on average and tenfold at worst.
 //
 //   large tiles: rounds of the 256 CUs x (stages x time of a stage + a fixed time
@@ -22,20 +22,21 @@ namespace {
 //     rate the tile's loads reach;
 //   few rows: a wave's batches of loads one after the other, or the bytes that all
 //     workgroups read through L2 (rows that a tile repeats are read once), or the
-//     weight's bytes from memory. Loads of pieces that are not even on 4-byte
-//     boundaries cost 2.4 times as much.
+//     weight's bytes from memory at 4.35 TB/s. Loads off 16-byte boundaries cost 1.14
+//     times as much, off 4-byte boundaries 2.7 times.
 //
 // How the entries fall into groups is not known here: each active group is taken
-// to leave 0.7 tiles unfilled.
+// to leave 0.58 tiles unfilled, and a tile of several entries to belong to a group
+// 2.4 times as long as the average.
 struct TileTime {
   int rows, cols;
   bool staged;
   double stage, fixed;  // us
 };
 constexpr TileTime kTileTimes[] = {
-    {64, 128, false, 0.40, 2.5}, {64, 256, false, 0.52, 2.5}, {128, 256, false, 0.81, 2.4},
-    {256, 256, false, 1.18, 3.8}, {64, 128, true, 0.60, 3.3}, {64, 256, true, 1.00, 3.1},
-    {128, 256, true, 1.27, 2.7},
+    {64, 128, false, 0.451, 2.2}, {64, 256, false, 0.483, 2.3}, {128, 256, false, 0.806, 2.6},
+    {256, 256, false, 1.18, 3.2}, {64, 128, true, 0.581, 3.0}, {64, 256, true, 1.19, 3.2},
+    {128, 256, true, 1.75, 3.2},
 };
 
 template <int OP, int KIND>
@@ -47,30 +48,32 @@ int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
   const double active = a.offsets ? (a.G < a.M ? a.G : M) : 1;
   const double weight_bytes = active * np * nc * wb;
   auto row_tiles = [&](int rows) {
-    return a.offsets ? fmax(1.0, M / rows + 0.7 * active) : ceil(M / rows);
+    return a.offsets ? fmax(1.0, M / rows + 0.575 * active) : ceil(M / rows);
   };
   double best = 1e300;
   LinTileShape shape = {};
   for (const TileTime& t : kTileTimes) {
     if (t.staged == direct) continue;
     double rounds = row_tiles(t.rows) * ceil(np / t.cols) / 256;
-    rounds = rounds < 1 ? 1 : rounds + 0.54 * (ceil(rounds) - rounds);
-    const double us = 2 + fmax(rounds * (ceil(nc * es / 128) * t.stage + t.fixed),
-                               weight_bytes / (direct ? 14.0e6 : 3.7e6));
+    rounds = rounds < 1 ? 1 : rounds + 0.617 * (ceil(rounds) - rounds);
+    const double stage = t.stage * (wb < 1 ? 0.92 : 1.0);
+    const double us = 2 + fmax(rounds * (ceil(nc * es / 128) * stage + t.fixed),
+                               weight_bytes / (direct ? 12.5e6 : 8.1e6));
     if (us < best) {
       best = us;
       shape = LinTileShape{t.rows, t.cols, t.staged};
     }
   }
   if (KIND == kLinForward) {
-    const double cost = (lin_row_bounds(a, a.nc * es) & 3) ? 2.4 : 1.0;
+    const uintptr_t bounds = lin_row_bounds(a, a.nc * es);
+    const double cost = (bounds & 3) ? 2.72 : (bounds & 15) ? 1.14 : 1.0;
     int few = 0;
     for (const int nq : {1, 2, 4}) {
       const int rows = 16 * nq, cols = nq == 4 ? 32 : 16, batch = nq == 4 ? 4 : 8;
-      const double read = fmin(rows, ceil(M / active));
+      const double read = fmin(rows, ceil(M / active * (a.offsets && M > active ? 2.44 : 1.0)));
       const double l2 = row_tiles(rows) * ceil(np / cols) * (cols * wb + read * es) * nc * cost;
-      const double chain = ceil(ceil(nc * es / 256) / batch) * batch * (nq + cols / 16) * 0.12 * cost;
-      const double us = 4.9 + fmax(chain, fmax(l2 / 6.7e6, weight_bytes / 2.86e6));
+      const double chain = ceil(ceil(nc * es / 256) / batch) * batch * (nq + cols / 16) * 0.125 * cost;
+      const double us = 5.45 + fmax(chain, fmax(l2 / 6.25e6, weight_bytes / 4.35e6));
       if (us < best) {
         best = us;
         few = nq;
