@@ -14,8 +14,8 @@
 // four quarters of a wave take four consecutive groups, so MFMA i of four
 // multiplies codes 8 i .. 8 i + 7 of each.
 //
-// Measured: one token through 8 of 128 experts [1536, 2048], bf16 10.6 us (4.7 TB/s of
-// weight), MXFP4 codes 8 us, of which a launch with its two dependent loads (offsets,
+// Measured: one token through 8 of 128 experts [1536, 2048], bf16 11 us (4.6 TB/s of
+// weight, half of it from the memory-side cache), MXFP4 codes 8 us, of which a launch with its two dependent loads (offsets,
 // row index) takes 5; one row of int8 [14336, 4096] 13.5 us. A group's second 16
 // entries repeat its weight from L2; 64 entries in one workgroup (NQ = 4) load it once.
 #include "linear_few.h"
