@@ -132,6 +132,7 @@ def _check_half(fn: str, *tensors: torch.Tensor) -> None:
 
 
 def _forward(x, weight, offsets, row_index, validate):
+    """(y, offsets, row_index), the lists as the product ran on them."""
     fn = "grouped_linear"
     _check_half(fn, x, weight)
     _rows2(fn, "x", x)
@@ -147,20 +148,23 @@ def _forward(x, weight, offsets, row_index, validate):
         nat.call("mgq_grouped_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0], _ld(xd),
                  nat.ptr(idx), M, wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off),
                  y.data_ptr(), _stream(dev))
-    return _home(y, x)
+    return _home(y, x), off, idx
 
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets, row_index, validate):
-        ctx.save_for_backward(x, weight)
-        ctx.lists = (offsets, row_index)
-        return _forward(x, weight, offsets, row_index, validate)
+        y, offsets, row_index = _forward(x, weight, offsets, row_index, validate)
+        # the lists are saved like the operands, so that a routing buffer that is
+        # written again before the backward is an error there (routing made in
+        # inference mode has no version to check: a copy is saved)
+        lists = (t.clone() if t is not None and t.is_inference() else t for t in (offsets, row_index))
+        ctx.save_for_backward(x, weight, *lists)
+        return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, weight = ctx.saved_tensors
-        offsets, row_index = ctx.lists
+        x, weight, offsets, row_index = ctx.saved_tensors
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = grouped_linear_dgrad(dy, weight, offsets, row_index, x.shape[0], validate=False)
@@ -176,11 +180,13 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets=None,
     x: [T, K] bf16 or f16, weight: [G, N, K] of the same type (any row pitch),
     offsets: G + 1 integers (a device tensor or any host sequence) ->
     [entries, N]. fp32 sums, rounded once. Differentiable in x and weight: the
-    gradients are ``grouped_linear_dgrad`` and ``grouped_linear_wgrad``.
+    gradients are ``grouped_linear_dgrad`` and ``grouped_linear_wgrad`` on the
+    lists of the forward (autograd refuses a backward after int32 lists on the
+    device were written again).
     """
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedLinear.apply(x, weight, offsets, row_index, validate)
-    return _forward(x, weight, offsets, row_index, validate)
+    return _forward(x, weight, offsets, row_index, validate)[0]
 
 
 def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
