@@ -33,6 +33,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -163,6 +164,7 @@ class _GroupedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, offsets, row_index = ctx.saved_tensors
         dx = dw = None
@@ -182,7 +184,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets=None,
     [entries, N]. fp32 sums, rounded once. Differentiable in x and weight: the
     gradients are ``grouped_linear_dgrad`` and ``grouped_linear_wgrad`` on the
     lists of the forward (autograd refuses a backward after int32 lists on the
-    device were written again).
+    device were written again). The gradients have none themselves: a second
+    derivative raises.
     """
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedLinear.apply(x, weight, offsets, row_index, validate)

@@ -78,3 +78,13 @@ def test_lists_made_in_inference_mode(calls):
         off, idx = offsets.clone(), index.clone()
     linear.grouped_linear(x, w, off, idx).backward(dy)
     assert_gradients(x, w, reference(x, w, dy, offsets, index))
+
+
+def test_a_second_derivative_is_refused(calls):
+    """A penalty on a gradient would lose the product's part: the gradients come
+    from kernels that autograd does not see."""
+    x, w, dy, offsets, index = inputs()
+    y = linear.grouped_linear(x, w, offsets, index)
+    (gx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (y.float().sum() + gx.float().square().sum()).backward()
