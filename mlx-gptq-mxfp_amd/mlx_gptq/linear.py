@@ -33,7 +33,6 @@ from __future__ import annotations
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -132,6 +131,28 @@ def _check_half(fn: str, *tensors: torch.Tensor) -> None:
                         f"(got {', '.join(str(t.dtype) for t in tensors)})")
 
 
+class _NoGradient(torch.autograd.Function):
+    """A result that has no gradient, handed on with a backward that says so."""
+
+    @staticmethod
+    def forward(ctx, fn, out, *inputs):
+        ctx.fn = fn
+        return out.detach()
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise NotImplementedError(f"{ctx.fn} has no gradient: detach its inputs, or call it under "
+                                  "torch.no_grad()")
+
+
+def _without_gradient(fn: str, out: torch.Tensor, *inputs: torch.Tensor) -> torch.Tensor:
+    """`out`, computed from `inputs`: a backward that reaches it raises, where a
+    plain result would read as a constant."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
+        return _NoGradient.apply(fn, out, *inputs)
+    return out
+
+
 def _forward(x, weight, offsets, row_index, validate):
     """(y, offsets, row_index), the lists as the product ran on them."""
     fn = "grouped_linear"
@@ -164,7 +185,6 @@ class _GroupedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         x, weight, offsets, row_index = ctx.saved_tensors
         dx = dw = None
@@ -235,7 +255,7 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
             nat.call("mgq_rows_sum", dx.data_ptr(), idx.data_ptr(), M, int(n_rows), K,
                      out.data_ptr(), nat.dtype_code(out.dtype), ws.data_ptr(), ws.numel(), stream)
         dx = out
-    return _home(dx, dy)
+    return _without_gradient(fn, _home(dx, dy), dy, weight)
 
 
 def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
@@ -272,7 +292,7 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
                  dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size, _stream(dev))
     if offsets is None:
         dw = dw[0]
-    return _home(dw, dy)
+    return _without_gradient(fn, _home(dw, dy), dy, x)
 
 
 def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mode: str,

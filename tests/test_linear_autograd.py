@@ -80,11 +80,24 @@ def test_lists_made_in_inference_mode(calls):
     assert_gradients(x, w, reference(x, w, dy, offsets, index))
 
 
-def test_a_second_derivative_is_refused(calls):
+@pytest.mark.parametrize("operand", ["x", "w", "dy"])
+def test_a_second_derivative_is_refused(calls, operand):
     """A penalty on a gradient would lose the product's part: the gradients come
-    from kernels that autograd does not see."""
+    from kernels that autograd does not see. dx depends on w and dy, dw on x and dy."""
+    x, w, dy, offsets, index = inputs()
+    if operand == "dy":
+        dy.requires_grad_()
+    y = linear.grouped_linear(x, w, offsets, index)
+    (grad,) = torch.autograd.grad(y, w if operand == "x" else x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="has no gradient"):
+        (y.float().sum() + grad.float().square().sum()).backward()
+
+
+def test_a_first_derivative_may_keep_its_graph(calls):
+    """create_graph for another term of the loss leaves the product's gradients usable."""
     x, w, dy, offsets, index = inputs()
     y = linear.grouped_linear(x, w, offsets, index)
-    (gx,) = torch.autograd.grad(y, x, dy, create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
-        (y.float().sum() + gx.float().square().sum()).backward()
+    got = torch.autograd.grad(y, (x, w), dy, create_graph=True)
+    x.grad, w.grad = (g.detach() for g in got)
+    assert_gradients(x, w, reference(x, w, dy, offsets, index))
+    (y.float().square().sum() + got[0].detach().float().sum()).backward()
