@@ -13,6 +13,9 @@ with weights that are
 * ``"int8"``: 8-bit weights with a scale for each output channel, rows quantized
   to 8 bits on the way into each product.
 
+Only dense experts are differentiable; in the other formats a backward that reaches
+the rows raises.
+
 No call waits for the device: the routing stays there.
 """
 
@@ -94,7 +97,7 @@ class ExpertMLP:
     @staticmethod
     def _nearest(w: torch.Tensor, mode: str):
         if mode == "int8":
-            return linear.quantize_rows_int8(w)
+            return linear.quantize_rows_int8(w.detach())
         q, s, _, _ = grid.rtn_quantize_mxfp(w, mode)
         return packing.pack_q(q, grid.mode_defaults(mode)[1]), s
 

@@ -22,8 +22,8 @@ that belong to no group give zero rows. ``offsets=None`` is one dense weight
 ``validate=False`` no call waits for the device, so a decoding loop can be
 captured in a graph. Offsets and indexes outside their ranges are clamped by the
 kernels, never followed; ``validate`` raises for them. Only ``grouped_linear``
-is differentiable: codes and int8 rows have no gradient, and their products
-return none for ``x``.
+is differentiable. The other calls run on tensors that require a gradient, but a
+backward that reaches their results raises.
 
 Work is enqueued on the current stream of the tensors' device. Host tensors are
 staged through the current HIP device, as in the other modules.
@@ -331,7 +331,7 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
         nat.call("mgq_mxfp_linear", xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), M,
                  wd.data_ptr(), sd.data_ptr(), nat.mode_code(mode), G, N, K, nat.ptr(off),
                  y.data_ptr(), _stream(dev))
-    return _home(y, x)
+    return _without_gradient(fn, _home(y, x), x)
 
 
 def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -352,7 +352,7 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if rows.shape[0]:
         nat.call("mgq_quantize_rows_int8", rows.data_ptr(), nat.dtype_code(x.dtype), rows.shape[0],
                  rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr(), _stream(dev))
-    return _home(q, x), _home(s, x)
+    return _home(q, x), _without_gradient("quantize_rows_int8", _home(s, x), x)
 
 
 def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
@@ -396,4 +396,4 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
                  nat.ptr(idx), M, wd.data_ptr(), ws.data_ptr(), nat.ptr(b), G, N, K, _ld(wd),
                  wd.stride(0), nat.ptr(off), y.data_ptr(), nat.dtype_code(out_dtype),
                  _stream(dev))
-    return _home(y, x)
+    return _without_gradient(fn, _home(y, x), x_scale, w_scale, *(() if bias is None else (bias,)))

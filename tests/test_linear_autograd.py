@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from mlx_gptq import linear
+from mlx_gptq.experts import ExpertMLP
 from tests import host_products
 
 
@@ -101,3 +102,51 @@ def test_a_first_derivative_may_keep_its_graph(calls):
     x.grad, w.grad = (g.detach() for g in got)
     assert_gradients(x, w, reference(x, w, dy, offsets, index))
     (y.float().square().sum() + got[0].detach().float().sum()).backward()
+
+
+def mx_inputs():
+    return torch.zeros(3, 4, dtype=torch.int32), torch.full((3, 1), 127, dtype=torch.uint8)
+
+
+def int8_inputs():
+    return torch.ones(3, 32, dtype=torch.int8), torch.ones(3)
+
+
+def products(x):
+    """Every product whose weight has no gradient, of rows x [4, 32]."""
+    words, scales = mx_inputs()
+    w8, ws = int8_inputs()
+    yield linear.mxfp_linear(x, words, scales, "mxfp4")
+    yield linear.int8_linear(*linear.quantize_rows_int8(x), w8, ws)
+
+
+def test_rows_of_quantized_products_do_not_lose_their_gradient_silently(calls):
+    x = torch.ones(4, 32, dtype=torch.bfloat16, requires_grad=True)
+    for y in products(x):  # the forward runs
+        assert y.requires_grad
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            y.float().sum().backward()
+    for y in products(x.detach()):
+        assert not y.requires_grad
+    with torch.no_grad():
+        for y in products(x):
+            assert not y.requires_grad
+
+
+@pytest.mark.parametrize("name", ["x_scale", "w_scale", "bias"])
+def test_int8_scales_and_bias_do_not_lose_their_gradient_silently(calls, name):
+    w8, ws = int8_inputs()
+    args = {"x_scale": torch.ones(4), "w_scale": ws, "bias": torch.zeros(3)}
+    args[name].requires_grad_()
+    y = linear.int8_linear(torch.ones(4, 32, dtype=torch.int8), args["x_scale"], w8, args["w_scale"],
+                           args["bias"])
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        y.float().sum().backward()
+
+
+def test_int8_weights_rounded_from_parameters_are_constants(calls):
+    """ExpertMLP.from_weights takes a module's parameters; a training program's loss
+    may reach other tensors past them."""
+    w = torch.ones(2, 64, 32, dtype=torch.bfloat16, requires_grad=True)
+    mlp = ExpertMLP.from_weights(w, torch.ones(2, 32, 32, dtype=torch.bfloat16), "int8")
+    assert not any(t.requires_grad for t in (*mlp.gate_up, *mlp.down))
