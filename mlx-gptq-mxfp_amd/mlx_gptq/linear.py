@@ -23,7 +23,7 @@ that belong to no group give zero rows. ``offsets=None`` is one dense weight
 captured in a graph. Offsets and indexes outside their ranges are clamped by the
 kernels, never followed; ``validate`` raises for them. Only ``grouped_linear``
 is differentiable. The other calls run on tensors that require a gradient, but a
-backward that reaches their results raises.
+backward that reaches their results raises, as forward-mode tangents do in every call.
 
 Work is enqueued on the current stream of the tensors' device. Host tensors are
 staged through the current HIP device, as in the other modules.
@@ -33,6 +33,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -131,6 +132,14 @@ def _check_half(fn: str, *tensors: torch.Tensor) -> None:
                         f"(got {', '.join(str(t.dtype) for t in tensors)})")
 
 
+def _check_tangents(fn: str, *tensors: torch.Tensor) -> None:
+    """No operand carries a forward-mode tangent (one comparison outside such a level)."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{fn} has no forward-mode derivative")
+
+
 class _NoGradient(torch.autograd.Function):
     """A result that has no gradient, handed on with a backward that says so."""
 
@@ -207,6 +216,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets=None,
     device were written again). The gradients have none themselves: a second
     derivative raises.
     """
+    _check_tangents("grouped_linear", x, weight)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedLinear.apply(x, weight, offsets, row_index, validate)
     return _forward(x, weight, offsets, row_index, validate)[0]
@@ -222,6 +232,7 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
     required; rows that no entry reads are zero).
     """
     fn = "grouped_linear_dgrad"
+    _check_tangents(fn, dy, weight)
     _check_half(fn, dy, weight)
     _rows2(fn, "dy", dy)
     w = _weight3(fn, weight, offsets)
@@ -268,6 +279,7 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     once; zeros for a group without entries. At most 4096 groups.
     """
     fn = "grouped_linear_wgrad"
+    _check_tangents(fn, dy, x)
     _check_half(fn, dy, x)
     _rows2(fn, "dy", dy)
     _rows2(fn, "x", x)
@@ -306,6 +318,7 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
     -> bf16 [entries, N]. The decoded weights are exact in bf16, the sums fp32.
     """
     fn = "mxfp_linear"
+    _check_tangents(fn, x)
     if mode not in _MX_BITS:
         raise ValueError(f"not a microscaling mode: {mode}")
     if x.dtype != torch.bfloat16:
@@ -341,6 +354,7 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     A zero row has scale 0 and zero codes. A row that holds a NaN or an infinity
     has scale NaN and zero codes, so products with it are NaN.
     """
+    _check_tangents("quantize_rows_int8", x)
     if x.dtype not in (torch.float32, *_HALF):
         raise TypeError(f"quantize_rows_int8: expects float32, bfloat16 or float16 (got {x.dtype})")
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -368,6 +382,8 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     group are zero, without bias.
     """
     fn = "int8_linear"
+    scaling = (x_scale, w_scale) if bias is None else (x_scale, w_scale, bias)
+    _check_tangents(fn, *scaling)
     if x.dtype != torch.int8 or weight.dtype != torch.int8:
         raise TypeError(f"{fn}: expects int8 rows and weights (got {x.dtype} and {weight.dtype})")
     for name, t in (("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias)):
@@ -396,4 +412,4 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
                  nat.ptr(idx), M, wd.data_ptr(), ws.data_ptr(), nat.ptr(b), G, N, K, _ld(wd),
                  wd.stride(0), nat.ptr(off), y.data_ptr(), nat.dtype_code(out_dtype),
                  _stream(dev))
-    return _without_gradient(fn, _home(y, x), x_scale, w_scale, *(() if bias is None else (bias,)))
+    return _without_gradient(fn, _home(y, x), *scaling)

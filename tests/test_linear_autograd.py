@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from mlx_gptq import linear
 from mlx_gptq.experts import ExpertMLP
@@ -150,3 +151,26 @@ def test_int8_weights_rounded_from_parameters_are_constants(calls):
     w = torch.ones(2, 64, 32, dtype=torch.bfloat16, requires_grad=True)
     mlp = ExpertMLP.from_weights(w, torch.ones(2, 32, 32, dtype=torch.bfloat16), "int8")
     assert not any(t.requires_grad for t in (*mlp.gate_up, *mlp.down))
+
+
+def test_a_tangent_is_refused(calls):
+    """Forward-mode derivatives: a result without a tangent would read as a constant."""
+    x, w, dy, offsets, index = (t.detach() for t in inputs())
+    rows = torch.ones(4, 32, dtype=torch.bfloat16)
+    w8, ws = int8_inputs()
+    q = torch.ones(4, 32, dtype=torch.int8)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: linear.grouped_linear(dual(x), w, offsets, index),
+                     lambda: linear.grouped_linear(x, dual(w), offsets, index),
+                     lambda: linear.grouped_linear(x.requires_grad_(), dual(w), offsets, index),
+                     lambda: linear.grouped_linear_dgrad(dual(dy), w, offsets, index, 4),
+                     lambda: linear.grouped_linear_wgrad(dy, dual(x.detach()), offsets, index),
+                     lambda: linear.mxfp_linear(dual(rows), *mx_inputs(), "mxfp4"),
+                     lambda: linear.quantize_rows_int8(dual(rows)),
+                     lambda: linear.int8_linear(q, torch.ones(4), w8, dual(ws))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        linear.grouped_linear(x.detach(), w, offsets, index)  # no tangent: runs
