@@ -153,9 +153,26 @@ def check(rc: int, what: str) -> None:
     raise RuntimeError(f"{what}: {msg} (status {rc})")
 
 
+class Stream(int):
+    """A HIP stream's handle with the index of its device: the default stream's
+    handle is 0 on every device, and a launch goes to the current one."""
+
+    device: int
+
+
+_streams: dict[tuple[int, int], Stream] = {}  # torch has a few dozen for each device
+
+
 def call(name: str, *args) -> None:
+    """The entry point `name`, with the device of the stream that ends its
+    arguments current."""
     fn = getattr(load(), name)
-    check(fn(*args), name)
+    device = getattr(args[-1], "device", None)
+    if device is None or device == torch._C._cuda_getDevice():
+        check(fn(*args), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args), name)
 
 
 # --------------------------------------------------------------------------
@@ -203,8 +220,17 @@ def on_device(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     return t.contiguous()
 
 
-def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def stream_of(device: torch.device) -> Stream:
+    """The device's current stream, for the last argument of ``call``."""
+    index = device.index if isinstance(device, torch.device) else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
+    handle = torch._C._cuda_getCurrentRawStream(index)
+    stream = _streams.get((index, handle))
+    if stream is None:
+        stream = _streams[index, handle] = Stream(handle)
+        stream.device = index
+    return stream
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

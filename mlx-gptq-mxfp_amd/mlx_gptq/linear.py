@@ -70,10 +70,6 @@ def _home(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     return t if like.is_cuda else t.to(like.device)
 
 
-def _stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
-
-
 def _ld(t: torch.Tensor) -> int:
     """Row pitch in elements (a single row's stride says nothing)."""
     return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], 1)
@@ -178,7 +174,7 @@ def _forward(x, weight, offsets, row_index, validate):
     if M and N:
         nat.call("mgq_grouped_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0], _ld(xd),
                  nat.ptr(idx), M, wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off),
-                 y.data_ptr(), _stream(dev))
+                 y.data_ptr(), nat.stream_of(dev))
     return _home(y, x), off, idx
 
 
@@ -251,7 +247,7 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
     gathered = idx is not None
     out_type = torch.float32 if gathered else dy.dtype
     dx = torch.empty(M, K, dtype=out_type, device=dev)
-    stream = _stream(dev)
+    stream = nat.stream_of(dev)
     if M and K and N:
         nat.call("mgq_grouped_dgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
                  wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off), dx.data_ptr(),
@@ -301,7 +297,7 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         nat.call("mgq_grouped_wgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
                  xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), G, N, K, nat.ptr(off),
-                 dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size, _stream(dev))
+                 dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size, nat.stream_of(dev))
     if offsets is None:
         dw = dw[0]
     return _without_gradient(fn, _home(dw, dy), dy, x)
@@ -343,7 +339,7 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
     if M and N:
         nat.call("mgq_mxfp_linear", xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), M,
                  wd.data_ptr(), sd.data_ptr(), nat.mode_code(mode), G, N, K, nat.ptr(off),
-                 y.data_ptr(), _stream(dev))
+                 y.data_ptr(), nat.stream_of(dev))
     return _without_gradient(fn, _home(y, x), x)
 
 
@@ -365,7 +361,7 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     s = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     if rows.shape[0]:
         nat.call("mgq_quantize_rows_int8", rows.data_ptr(), nat.dtype_code(x.dtype), rows.shape[0],
-                 rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr(), _stream(dev))
+                 rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr(), nat.stream_of(dev))
     return _home(q, x), _without_gradient("quantize_rows_int8", _home(s, x), x)
 
 
@@ -411,5 +407,5 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
         nat.call("mgq_int8_linear", xd.data_ptr(), xs.data_ptr(), xd.shape[0], _ld(xd),
                  nat.ptr(idx), M, wd.data_ptr(), ws.data_ptr(), nat.ptr(b), G, N, K, _ld(wd),
                  wd.stride(0), nat.ptr(off), y.data_ptr(), nat.dtype_code(out_dtype),
-                 _stream(dev))
+                 nat.stream_of(dev))
     return _without_gradient(fn, _home(y, x), *scaling)

@@ -99,6 +99,6 @@ def install(monkeypatch, device=torch.device("cpu")):
         globals()[name.removeprefix("mgq_")](*args)
 
     monkeypatch.setattr(linear, "_device", lambda *tensors: device)
-    monkeypatch.setattr(linear, "_stream", lambda dev: 0)
+    monkeypatch.setattr(nat, "stream_of", lambda dev: 0)
     monkeypatch.setattr(nat, "call", call)
     return calls
