@@ -186,7 +186,10 @@ class _GroupedLinear(torch.autograd.Function):
         # written again before the backward is an error there (routing made in
         # inference mode has no version to check: a copy is saved)
         lists = (t.clone() if t is not None and t.is_inference() else t for t in (offsets, row_index))
-        ctx.save_for_backward(x, weight, *lists)
+        # (each operand only for the other one's gradient)
+        needs_x, needs_weight = ctx.needs_input_grad[:2]
+        ctx.n_rows = x.shape[0]
+        ctx.save_for_backward(x if needs_weight else None, weight if needs_x else None, *lists)
         return y
 
     @staticmethod
@@ -194,7 +197,7 @@ class _GroupedLinear(torch.autograd.Function):
         x, weight, offsets, row_index = ctx.saved_tensors
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            dx = grouped_linear_dgrad(dy, weight, offsets, row_index, x.shape[0], validate=False)
+            dx = grouped_linear_dgrad(dy, weight, offsets, row_index, ctx.n_rows, validate=False)
         if ctx.needs_input_grad[1]:
             dw = grouped_linear_wgrad(dy, x, offsets, row_index, validate=False)
         return dx, dw, None, None, None

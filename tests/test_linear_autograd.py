@@ -174,3 +174,18 @@ def test_a_tangent_is_refused(calls):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
         linear.grouped_linear(x.detach(), w, offsets, index)  # no tangent: runs
+
+
+@pytest.mark.parametrize("which", ["x", "w"])
+def test_only_what_the_gradient_reads_is_saved(calls, which):
+    """Frozen experts keep no rows alive, frozen rows no weight."""
+    x, w, dy, offsets, index = inputs()
+    want = reference(x, w, dy, offsets, index)
+    (w if which == "x" else x).requires_grad_(False)
+    y = linear.grouped_linear(x, w, offsets, index)
+    saved = [t for t in y.grad_fn.saved_tensors if t is not None and t.is_floating_point()]
+    assert len(saved) == 1 and saved[0].shape == (w if which == "x" else x).shape
+    y.backward(dy)
+    got, ref = (x.grad, want[0]) if which == "x" else (w.grad, want[1])
+    assert bool(((got.float() - ref).abs() <= 2.0**-11 * ref.abs() + 2.0**-16).all())
+    assert (w if which == "x" else x).grad is None
