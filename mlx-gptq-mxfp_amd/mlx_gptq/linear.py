@@ -91,24 +91,38 @@ def _rows2(fn: str, name: str, x: torch.Tensor) -> None:
         raise ValueError(f"{fn}: {name} must be a matrix (got {tuple(x.shape)})")
 
 
+def _integers(t: torch.Tensor) -> bool:
+    return not (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool)
+
+
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    """`t` in 32 bits. What lies past them stays out of range, as the kernels' clamps
+    expect it."""
+    if t.dtype == torch.int32:
+        return t
+    if t.dtype == torch.int64:
+        t = t.clamp(-(2**31), 2**31 - 1)
+    return t.to(torch.int32)
+
+
 def _list(fn: str, offsets, row_index, groups: int, n_rows: int, dev: torch.device, validate: bool):
     """(offsets int32 on dev | None, row_index int32 on dev | None, entries)."""
     if row_index is not None:
-        if row_index.dim() != 1 or row_index.dtype.is_floating_point:
+        if row_index.dim() != 1 or not _integers(row_index):
             raise ValueError(f"{fn}: row_index must be a list of integers")
         if validate and row_index.numel():
             lo, hi = torch.aminmax(row_index)
             if int(lo) < 0 or int(hi) >= n_rows:
                 raise IndexError(f"{fn}: row_index outside [0, {n_rows})")
-        if row_index.dtype != torch.int32:
-            row_index = row_index.to(torch.int32)
-        row_index = _dense(row_index, dev)
+        row_index = _dense(_int32(row_index), dev)
     entries = n_rows if row_index is None else row_index.numel()
     if offsets is None:
         return None, row_index, entries
     if not isinstance(offsets, torch.Tensor):
-        offsets = torch.from_numpy(np.array(offsets, dtype=np.int64))
-    if offsets.dim() != 1 or offsets.numel() != groups + 1 or offsets.dtype.is_floating_point:
+        host = np.asarray(offsets)
+        whole = host.dtype.kind != "f" or bool(np.all(host == np.floor(host)))
+        offsets = torch.from_numpy(host.astype(np.int64) if whole else np.array(host, dtype=np.float64))
+    if offsets.dim() != 1 or offsets.numel() != groups + 1 or not _integers(offsets):
         raise ValueError(f"{fn}: offsets must hold {groups + 1} integers for {groups} groups")
     if validate or not offsets.is_cuda:
         o = offsets.detach().cpu().numpy()
@@ -116,9 +130,7 @@ def _list(fn: str, offsets, row_index, groups: int, n_rows: int, dev: torch.devi
             raise ValueError(f"{fn}: offsets must be non-negative and non-decreasing")
         if o[-1] > entries:
             raise ValueError(f"{fn}: offsets exceed the {entries} list entries")
-    if offsets.dtype != torch.int32:
-        offsets = offsets.to(torch.int32)
-    return _dense(offsets, dev), row_index, entries
+    return _dense(_int32(offsets), dev), row_index, entries
 
 
 def _check_half(fn: str, *tensors: torch.Tensor) -> None:
