@@ -200,7 +200,7 @@ class _GroupedLinear(torch.autograd.Function):
         lists = (t.clone() if t is not None and t.is_inference() else t for t in (offsets, row_index))
         # (each operand only for the other one's gradient)
         needs_x, needs_weight = ctx.needs_input_grad[:2]
-        ctx.n_rows = x.shape[0]
+        ctx.n_rows, ctx.weight_device = x.shape[0], weight.device
         ctx.save_for_backward(x if needs_weight else None, weight if needs_x else None, *lists)
         return y
 
@@ -211,7 +211,7 @@ class _GroupedLinear(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = grouped_linear_dgrad(dy, weight, offsets, row_index, ctx.n_rows, validate=False)
         if ctx.needs_input_grad[1]:
-            dw = grouped_linear_wgrad(dy, x, offsets, row_index, validate=False)
+            dw = grouped_linear_wgrad(dy, x, offsets, row_index, validate=False).to(ctx.weight_device)
         return dx, dw, None, None, None
 
 
