@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(512, 1) lin_tile_kernel(const LinArgs a, const
     };
     auto take_rows = [&]() {  // (clamped here, so that no load is waited for above)
       if constexpr (GATHER) {
-        const int top = static_cast<int>(a.n_rows - 1);
+        // (X may have more rows than an index can name)
+        const int top = a.n_rows < 0x7fffffff ? static_cast<int>(a.n_rows) - 1 : 0x7fffffff;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int v = RING ? __builtin_amdgcn_readlane(rows_next[0], i) : rows_next[i];
