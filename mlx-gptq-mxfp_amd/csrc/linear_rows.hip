@@ -163,28 +163,37 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Rows of one launch: a workgroup a row has 256 threads, a launch less than 2^32.
+constexpr int64_t kLaunchRows = int64_t(1) << 23;
+
 // A wave per row while four pieces a lane hold it, then a workgroup.
 template <int DT>
-void quantize_rows(const char* X, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, float* scales,
-                   hipStream_t s) {
+void quantize_rows(const char* X, int64_t n_rows, int64_t cols, int64_t ldx, int8_t* q,
+                   float* scales, hipStream_t s) {
   const int64_t pieces = ceil_div(cols, RowPiece<DT>::N);
-  const unsigned quads = static_cast<unsigned>(ceil_div(rows, 4)), wg = static_cast<unsigned>(rows);
-  if (pieces <= 64)
-    quantize_rows_kernel<DT, 1, 1><<<quads, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
-  else if (pieces <= 128)
-    quantize_rows_kernel<DT, 1, 2><<<quads, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
-  else if (pieces <= 256)
-    quantize_rows_kernel<DT, 1, 4><<<quads, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
-  else if (pieces <= 512)
-    quantize_rows_kernel<DT, 4, 2><<<wg, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
-  else if (pieces <= 768)
-    quantize_rows_kernel<DT, 4, 3><<<wg, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
-  else if (pieces <= 1024)
-    quantize_rows_kernel<DT, 4, 4><<<wg, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
-  else if (pieces <= 2048)
-    quantize_rows_kernel<DT, 4, 8><<<wg, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
-  else
-    quantize_rows_kernel<DT, 4, 0><<<wg, 256, 0, s>>>(X, rows, cols, ldx, q, scales);
+  for (int64_t r0 = 0; r0 < n_rows; r0 += kLaunchRows) {
+    const int64_t rows = n_rows - r0 < kLaunchRows ? n_rows - r0 : kLaunchRows;
+    const unsigned quads = static_cast<unsigned>(ceil_div(rows, 4)), wg = static_cast<unsigned>(rows);
+    const char* x = X + r0 * ldx * (16 / RowPiece<DT>::N);
+    int8_t* qr = q + r0 * cols;
+    float* sr = scales + r0;
+    if (pieces <= 64)
+      quantize_rows_kernel<DT, 1, 1><<<quads, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+    else if (pieces <= 128)
+      quantize_rows_kernel<DT, 1, 2><<<quads, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+    else if (pieces <= 256)
+      quantize_rows_kernel<DT, 1, 4><<<quads, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+    else if (pieces <= 512)
+      quantize_rows_kernel<DT, 4, 2><<<wg, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+    else if (pieces <= 768)
+      quantize_rows_kernel<DT, 4, 3><<<wg, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+    else if (pieces <= 1024)
+      quantize_rows_kernel<DT, 4, 4><<<wg, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+    else if (pieces <= 2048)
+      quantize_rows_kernel<DT, 4, 8><<<wg, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+    else
+      quantize_rows_kernel<DT, 4, 0><<<wg, 256, 0, s>>>(x, rows, cols, ldx, qr, sr);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -219,10 +228,10 @@ __global__ void __launch_bounds__(256)
 
 __global__ void __launch_bounds__(256)
     rows_sum_kernel(const float* __restrict__ src, const int32_t* __restrict__ row_index, int64_t M,
-                    int64_t n_rows, int64_t cols, const int32_t* __restrict__ count,
+                    int64_t first, int64_t n_rows, int64_t cols, const int32_t* __restrict__ count,
                     const int32_t* __restrict__ slots, void* __restrict__ out, int out_type) {
   const int lane = threadIdx.x & 63;
-  const int64_t r = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  const int64_t r = first + blockIdx.x * 4ll + (threadIdx.x >> 6);
   if (r >= n_rows) return;
   const int n = __builtin_amdgcn_readfirstlane(count[r]);
   int32_t mine = 0;
@@ -322,7 +331,10 @@ extern "C" int mgq_rows_sum(const float* src, const int32_t* row_index, int64_t 
   rows_clear_kernel<<<elementwise_blocks(n_rows, 256), 256, 0, s>>>(count, n_rows);
     rows_fill_kernel<<<elementwise_blocks(n_entries, 256), 256, 0, s>>>(row_index, n_entries, n_rows,
                                                                         count, slots);
-  rows_sum_kernel<<<static_cast<unsigned>(ceil_div(n_rows, 4)), 256, 0, s>>>(
-      src, row_index, n_entries, n_rows, cols, count, slots, out, out_dtype);
+  for (int64_t r0 = 0; r0 < n_rows; r0 += kLaunchRows) {
+    const int64_t rows = n_rows - r0 < kLaunchRows ? n_rows - r0 : kLaunchRows;
+    rows_sum_kernel<<<static_cast<unsigned>(ceil_div(rows, 4)), 256, 0, s>>>(
+        src, row_index, n_entries, r0, n_rows, cols, count, slots, out, out_dtype);
+  }
   return check_launch("rows_sum");
 }

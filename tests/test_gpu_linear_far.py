@@ -35,3 +35,32 @@ def test_more_rows_than_an_index_can_name(K):
     y = linear.grouped_linear(x, w.to(DEV), off, index.to(DEV))
     want, _ = ref.forward(picked, w, off)
     assert bool(((y.cpu().double() - want).abs() <= ULP * want.abs()).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(2**26 + 5, 3), (2**24 + 3, 1030)])
+def test_quantizing_more_rows_than_one_launch_holds(rows, cols):
+    """Past 2^26 rows of a wave and 2^24 of a workgroup (fp32 rows of 1030): the first
+    and last rows, and those around 2^23 and its multiples, against the oracle."""
+    x = torch.ones(rows, cols, device=DEV)
+    at = sorted({r for k in range(0, rows + 2**23, 2**23) for r in (k - 1, k, k + 1)} | {rows - 1})
+    at = torch.tensor([r for r in at if 0 <= r < rows])
+    sample = torch.randn(len(at), cols, generator=torch.Generator().manual_seed(cols))
+    x[at.to(DEV)] = sample.to(DEV)
+    q, s = linear.quantize_rows_int8(x)
+    del x
+    wq, ws = ref.quantize_rows(sample)
+    assert torch.equal(q[at.to(DEV)].cpu(), wq) and torch.equal(s[at.to(DEV)].cpu(), ws)
+    # all the others are ones: scale 1 / 127, codes 127
+    assert int((s != torch.tensor(1.0) / 127).sum()) <= len(at)
+    assert int((q != 127).sum()) <= sample.numel()
+
+
+def test_more_summed_rows_than_one_launch_holds():
+    """dX of 2^26 + 7 rows of one column, of which seven are read."""
+    rows = 2**26 + 7
+    at = torch.tensor([0, 2**23 - 1, 2**23, 2**25 + 1, rows - 1, 3, 0], dtype=torch.int32)
+    dy = torch.arange(1, 8, dtype=torch.bfloat16).view(7, 1)
+    w = torch.full((1, 1), 2.0, dtype=torch.bfloat16)
+    dx = linear.grouped_linear_dgrad(dy.to(DEV), w.to(DEV), row_index=at.to(DEV), n_rows=rows)
+    want = torch.zeros(rows, dtype=torch.float64).index_add_(0, at.long(), 2.0 * dy.double()[:, 0])
+    assert torch.equal(dx[:, 0].cpu().double(), want)
