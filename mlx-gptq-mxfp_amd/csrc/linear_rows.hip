@@ -198,17 +198,28 @@ void quantize_rows(const char* X, int64_t n_rows, int64_t cols, int64_t ldx, int
 
 // ---------------------------------------------------------------------------
 // out[r] = sum of src[t] over the list entries t with row_index[t] = r, in the
-// order of t, in fp32. Each row has kSlots slots that the entries fill in any
-// order; the sum sorts them, so it does not depend on the atomics' order. A row
-// with more entries than slots finds them by scanning the list. Bound by memory:
-// 8198 entries into 4099 rows of 1024 take 8.2 us (50 MB, mostly from the caches), and
-// clearing and filling the slots 3 us each; both in one workgroup took 16.
+// order of t, in fp32. The entries of a row arrive in any order: the first kSlots
+// take its slots, the others chain up behind its head, and the sum sorts them, so
+// that it does not depend on the atomics' order. A row of n entries past its slots
+// walks its chain once for every 64 of them, keeping the next 64 in order over the
+// lanes, or reads the whole list, 64 indexes at a time, where that is less: the
+// loads that wait for each other are at most n^2 / 64 and M / 64, together M^1.5 / 64
+// for any list. Bound by memory: 8198 entries into 4099 rows of 1024 take 8.2 us (50 MB,
+// mostly from the caches), and clearing and filling the slots 3 us each; both in one
+// workgroup took 16. 16384 rows of 64 read 24 times each take 0.18 ms with the product
+// in front, read 16 times each 0.12.
 // ---------------------------------------------------------------------------
 constexpr int kSlots = 16;
 constexpr int kSumCols = 1024;  // columns a wave sums at once
 
-__global__ void __launch_bounds__(256) rows_clear_kernel(int32_t* __restrict__ count, int64_t n) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) count[i] = 0;
+struct RowState {
+  int32_t count;  // entries
+  int32_t head;   // the last one that found no slot, -1 if all did
+};
+
+__global__ void __launch_bounds__(256) rows_clear_kernel(RowState* __restrict__ state, int64_t n) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll)
+    state[i] = RowState{0, -1};
 }
 
 __device__ inline int64_t clamp_row(int64_t r, int64_t n_rows) {
@@ -218,29 +229,55 @@ __device__ inline int64_t clamp_row(int64_t r, int64_t n_rows) {
 
 __global__ void __launch_bounds__(256)
     rows_fill_kernel(const int32_t* __restrict__ row_index, int64_t M, int64_t n_rows,
-                     int32_t* __restrict__ count, int32_t* __restrict__ slots) {
+                     RowState* __restrict__ state, int32_t* __restrict__ slots,
+                     int32_t* __restrict__ next) {
   for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < M; t += gridDim.x * 256ll) {
     const int64_t r = clamp_row(row_index[t], n_rows);
-    const int32_t i = atomicAdd(&count[r], 1);
-    if (i < kSlots) slots[r * kSlots + i] = static_cast<int32_t>(t);
+    const int32_t i = atomicAdd(&state[r].count, 1);
+    if (i < kSlots)
+      slots[r * kSlots + i] = static_cast<int32_t>(t);
+    else
+      next[t] = atomicExch(&state[r].head, static_cast<int32_t>(t));
   }
 }
 
 __global__ void __launch_bounds__(256)
     rows_sum_kernel(const float* __restrict__ src, const int32_t* __restrict__ row_index, int64_t M,
-                    int64_t first, int64_t n_rows, int64_t cols, const int32_t* __restrict__ count,
-                    const int32_t* __restrict__ slots, void* __restrict__ out, int out_type) {
+                    int64_t first, int64_t n_rows, int64_t cols,
+                    const RowState* __restrict__ state, const int32_t* __restrict__ slots,
+                    const int32_t* __restrict__ next, void* __restrict__ out, int out_type) {
   const int lane = threadIdx.x & 63;
   const int64_t r = first + blockIdx.x * 4ll + (threadIdx.x >> 6);
   if (r >= n_rows) return;
-  const int n = __builtin_amdgcn_readfirstlane(count[r]);
+  const int n = __builtin_amdgcn_readfirstlane(state[r].count);
+  const int head = __builtin_amdgcn_readfirstlane(state[r].head);
+  const bool chained = n > kSlots && (n + 63ll) / 64 * n <= M / 64;
+  // lane k: entry k in the list's order (up to kSlots), or slot k
+  const int32_t slot = lane < (n < kSlots ? n : kSlots) ? slots[r * kSlots + lane] : 0;
   int32_t mine = 0;
   if (n <= kSlots) {
-    const int32_t v = lane < n ? slots[r * kSlots + lane] : 0;
     int rank = lane < n ? 0 : lane;
-    for (int j = 0; j < n; ++j) rank += (lane < n && __builtin_amdgcn_readlane(v, j) < v) ? 1 : 0;
-    mine = __builtin_amdgcn_ds_permute(4 * rank, v);
+    for (int j = 0; j < n; ++j) rank += (lane < n && __builtin_amdgcn_readlane(slot, j) < slot) ? 1 : 0;
+    mine = __builtin_amdgcn_ds_permute(4 * rank, slot);
   }
+  // the 64 smallest entries above `last` (a chain has n - kSlots entries)
+  auto next_batch = [&](int32_t last) {
+    int32_t best = 0x7fffffff;
+    auto insert = [&](int32_t t) {
+      if (t <= last) return;
+      const int at = static_cast<int>(__popcll(__ballot(best < t)));
+      const int32_t below = __shfl_up(best, 1);
+      best = lane > at ? below : lane == at ? t : best;
+    };
+    for (int j = 0; j < kSlots; ++j) insert(__builtin_amdgcn_readlane(slot, j));
+    int32_t t = head;
+    for (int k = kSlots; k < n && t >= 0; ++k) {
+      const int32_t after = __builtin_amdgcn_readfirstlane(next[t]);
+      insert(t);
+      t = after;
+    }
+    return best;
+  };
   for (int64_t c0 = 0; c0 < cols; c0 += kSumCols) {
     // four consecutive columns a lane and piece
     constexpr int kPieces = kSumCols / 256;
@@ -263,6 +300,14 @@ __global__ void __launch_bounds__(256)
     };
     if (n <= kSlots) {
       for (int j = 0; j < n; ++j) add(__builtin_amdgcn_readlane(mine, j));
+    } else if (chained) {
+      int32_t last = -1;
+      for (int done = 0; done < n; done += 64) {
+        const int32_t batch = next_batch(last);
+        const int m = n - done < 64 ? n - done : 64;
+        for (int j = 0; j < m; ++j) add(__builtin_amdgcn_readlane(batch, j));
+        last = __builtin_amdgcn_readlane(batch, m - 1);
+      }
     } else {
       for (int64_t t0 = 0; t0 < M; t0 += 64) {
         const bool hit = t0 + lane < M && clamp_row(row_index[t0 + lane], n_rows) == r;
@@ -282,7 +327,10 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-int64_t slots_off(int64_t n_rows) { return ceil_div(4 * n_rows, 256) * 256; }
+int64_t pad256(int64_t n) { return ceil_div(n, 256) * 256; }
+// workspace: the rows' states, their slots, the entries' chain
+int64_t slots_off(int64_t n_rows) { return pad256(n_rows * static_cast<int64_t>(sizeof(RowState))); }
+int64_t next_off(int64_t n_rows) { return slots_off(n_rows) + pad256(4 * kSlots * n_rows); }
 
 }  // namespace
 }  // namespace mgq
@@ -308,8 +356,8 @@ extern "C" int mgq_quantize_rows_int8(const void* X, int dtype, int64_t rows, in
   return check_launch("quantize_rows_int8");
 }
 
-extern "C" int64_t mgq_rows_sum_workspace_size(int64_t n_rows) {
-  return slots_off(n_rows) + 4 * kSlots * n_rows;
+extern "C" int64_t mgq_rows_sum_workspace_size(int64_t n_entries, int64_t n_rows) {
+  return n_entries < 0 || n_rows < 0 ? 0 : next_off(n_rows) + 4 * n_entries;
 }
 
 extern "C" int mgq_rows_sum(const float* src, const int32_t* row_index, int64_t n_entries,
@@ -321,20 +369,23 @@ extern "C" int mgq_rows_sum(const float* src, const int32_t* row_index, int64_t 
   MGQ_REQUIRE(n_entries >= 0 && n_entries < (int64_t(1) << 31) && n_rows >= 0 &&
                   n_rows < (int64_t(1) << 31) && cols >= 0 && cols < (int64_t(1) << 30),
               MGQ_ERR_SHAPE, "rows_sum: bad shape");
-  const int64_t need = mgq_rows_sum_workspace_size(n_rows);
+  const int64_t need = mgq_rows_sum_workspace_size(n_entries, n_rows);
   MGQ_REQUIRE(workspace != nullptr && workspace_bytes >= need, MGQ_ERR_WORKSPACE,
               "rows_sum workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   if (n_rows == 0 || cols == 0) return MGQ_OK;
   hipStream_t s = as_stream(stream);
-  int32_t* count = static_cast<int32_t*>(workspace);
-  int32_t* slots = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + slots_off(n_rows));
-  rows_clear_kernel<<<elementwise_blocks(n_rows, 256), 256, 0, s>>>(count, n_rows);
+  char* ws = static_cast<char*>(workspace);
+  RowState* state = reinterpret_cast<RowState*>(ws);
+  int32_t* slots = reinterpret_cast<int32_t*>(ws + slots_off(n_rows));
+  int32_t* next = reinterpret_cast<int32_t*>(ws + next_off(n_rows));
+  rows_clear_kernel<<<elementwise_blocks(n_rows, 256), 256, 0, s>>>(state, n_rows);
+  if (n_entries > 0)
     rows_fill_kernel<<<elementwise_blocks(n_entries, 256), 256, 0, s>>>(row_index, n_entries, n_rows,
-                                                                        count, slots);
+                                                                        state, slots, next);
   for (int64_t r0 = 0; r0 < n_rows; r0 += kLaunchRows) {
     const int64_t rows = n_rows - r0 < kLaunchRows ? n_rows - r0 : kLaunchRows;
     rows_sum_kernel<<<static_cast<unsigned>(ceil_div(rows, 4)), 256, 0, s>>>(
-        src, row_index, n_entries, r0, n_rows, cols, count, slots, out, out_dtype);
+        src, row_index, n_entries, r0, n_rows, cols, state, slots, next, out, out_dtype);
   }
   return check_launch("rows_sum");
 }

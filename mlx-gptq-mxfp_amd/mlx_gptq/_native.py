@@ -94,7 +94,7 @@ SIGNATURES: dict[str, list] = {
     "mgq_grouped_wgrad_workspace_size": [_I64, _I64, _I64, _I64],
     "mgq_grouped_wgrad": [_VP, _INT, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _VP, _VP,
                           _INT, _VP, _I64, _VP],
-    "mgq_rows_sum_workspace_size": [_I64],
+    "mgq_rows_sum_workspace_size": [_I64, _I64],
     "mgq_rows_sum": [_VP, _VP, _I64, _I64, _I64, _VP, _INT, _VP, _I64, _VP],
     "mgq_mxfp_linear": [_VP, _I64, _I64, _VP, _I64, _VP, _VP, _INT, _I64, _I64, _I64, _VP, _VP,
                         _VP],

@@ -272,8 +272,8 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
     if gathered:
         out = torch.empty(int(n_rows), K, dtype=dy.dtype, device=dev)
         if out.numel():
-            ws = torch.empty(nat.load().mgq_rows_sum_workspace_size(int(n_rows)), dtype=torch.uint8,
-                             device=dev)
+            ws = torch.empty(nat.load().mgq_rows_sum_workspace_size(M, int(n_rows)),
+                             dtype=torch.uint8, device=dev)
             nat.call("mgq_rows_sum", dx.data_ptr(), idx.data_ptr(), M, int(n_rows), K,
                      out.data_ptr(), nat.dtype_code(out.dtype), ws.data_ptr(), ws.numel(), stream)
         dx = out
