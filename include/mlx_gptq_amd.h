@@ -412,6 +412,16 @@ int mgq_int8_linear(const int8_t* X, const float* x_scale, int64_t n_rows, int64
                     int64_t K, int64_t ldw, int64_t w_group, const int32_t* offsets, void* Y,
                     int out_dtype, void* stream);
 
+/* Which kernel one of the products above takes, on the host: tile[0] x tile[1]
+ * list entries x columns of the result a workgroup, tile[2] 0 the kernel for few
+ * rows, 1 a tile by loads straight into LDS, 2 a tile by way of registers.
+ * product: 0 mgq_grouped_linear in bf16, 1 in f16, 2 mgq_int8_linear, 3
+ * mgq_mxfp_linear with MXFP4 and 4 with MXFP8 words, 5 mgq_grouped_dgrad in bf16,
+ * 6 in f16 (X: dY). grouped: there are offsets. Of X and W only the address counts. */
+int mgq_linear_choice(int product, const void* X, int64_t ldx, int64_t n_entries, const void* W,
+                      int64_t n_groups, int64_t N, int64_t K, int64_t ldw, int64_t w_group,
+                      int grouped, int32_t* tile);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,8 +10,8 @@
 namespace mgq {
 namespace {
 
-// Which kernel and tile a product over rows takes: the one whose time by the
-// model below is least. The model was fitted to 980 products (all types, 1 .. 16384
+// Which kernel and tile a product over rows takes: of those whose grid holds it, the
+// one whose time by the model below is least. The model was fitted to 980 products (all types, 1 .. 16384
 // entries, 0 .. 128 groups, K 256 .. 14336, aligned and not) that were timed with each
 // of their 3 to 7 choices: the model's choice costs 1.7 % over the best one on
 // average and 64 % at worst, where the largest tile that the average group fills
@@ -39,8 +39,15 @@ constexpr TileTime kTileTimes[] = {
     {128, 256, true, 1.75, 3.2},
 };
 
+// A kernel of few rows (nq blocks of 16 entries) or a tile; neither where no kernel's
+// grid holds the product.
+struct RowsChoice {
+  int nq;
+  LinTileShape tile;
+};
+
 template <int OP, int KIND>
-int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
+RowsChoice choose_rows(const LinArgs& a) {
   const bool direct = lin_tile_direct(a, OP, KIND);
   const int64_t es = lin_esize<OP>();
   const double wb = OP == kOpMx4 ? 0.53 : OP == kOpMx8 ? 1.03 : es;  // bytes of a weight
@@ -51,9 +58,9 @@ int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
     return a.offsets ? fmax(1.0, M / rows + 0.575 * active) : ceil(M / rows);
   };
   double best = 1e300;
-  LinTileShape shape = {};
+  RowsChoice choice = {};
   for (const TileTime& t : kTileTimes) {
-    if (t.staged == direct) continue;
+    if (t.staged == direct || lin_tile_grid(a, t.rows, t.cols) >= kLinTileGrid) continue;
     double rounds = row_tiles(t.rows) * ceil(np / t.cols) / 256;
     rounds = rounds < 1 ? 1 : rounds + 0.617 * (ceil(rounds) - rounds);
     const double stage = t.stage * (wb < 1 ? 0.92 : 1.0);
@@ -61,27 +68,33 @@ int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
                                weight_bytes / (direct ? 12.5e6 : 8.1e6));
     if (us < best) {
       best = us;
-      shape = LinTileShape{t.rows, t.cols, t.staged};
+      choice.tile = LinTileShape{t.rows, t.cols, t.staged};
     }
   }
   if (KIND == kLinForward) {
     const uintptr_t bounds = lin_row_bounds(a, a.nc * es);
     const double cost = (bounds & 3) ? 2.72 : (bounds & 15) ? 1.14 : 1.0;
-    int few = 0;
     for (const int nq : {1, 2, 4}) {
-      const int rows = 16 * nq, cols = nq == 4 ? 32 : 16, batch = nq == 4 ? 4 : 8;
+      if (lin_few_grid(a, nq) >= kLinFewGrid) continue;
+      const int rows = 16 * nq, cols = lin_few_cols(nq), batch = nq == 4 ? 4 : 8;
       const double read = fmin(rows, ceil(M / active * (a.offsets && M > active ? 2.44 : 1.0)));
       const double l2 = row_tiles(rows) * ceil(np / cols) * (cols * wb + read * es) * nc * cost;
       const double chain = ceil(ceil(nc * es / 256) / batch) * batch * (nq + cols / 16) * 0.125 * cost;
       const double us = 5.45 + fmax(chain, fmax(l2 / 6.25e6, weight_bytes / 4.35e6));
       if (us < best) {
         best = us;
-        few = nq;
+        choice.nq = nq;
       }
     }
-    if (few) return lin_few_rows(a, OP, few, s, what);
   }
-  return lin_tile_rows(a, OP, KIND, shape, s, what);
+  return choice;
+}
+
+template <int OP, int KIND>
+int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
+  const RowsChoice c = choose_rows<OP, KIND>(a);
+  MGQ_REQUIRE(c.nq || c.tile.rows, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  return c.nq ? lin_few_rows(a, OP, c.nq, s, what) : lin_tile_rows(a, OP, KIND, c.tile, s, what);
 }
 
 int check_list(const char* what, const int32_t* offsets, const int32_t* row_index,
@@ -292,4 +305,45 @@ extern "C" int mgq_int8_linear(const int8_t* X, const float* x_scale, int64_t n_
   a.sw = w_scale;
   a.bias = bias;
   return run_rows<kOpI8, kLinForward>(a, as_stream(stream), what);
+}
+
+extern "C" int mgq_linear_choice(int product, const void* X, int64_t ldx, int64_t n_entries,
+                                 const void* W, int64_t n_groups, int64_t N, int64_t K, int64_t ldw,
+                                 int64_t w_group, int grouped, int32_t* tile) {
+  clear_error();
+  const char* what = "linear_choice";
+  MGQ_REQUIRE(product >= 0 && product <= 6, MGQ_ERR_VALUE, "%s: no such product", what);
+  const int32_t some_list = 0;  // stands for offsets: the choice does not read them
+  if (int rc = check_list(what, grouped ? &some_list : nullptr, nullptr, n_groups, n_entries, n_entries))
+    return rc;
+  if (int rc = check_dims(what, N, K)) return rc;
+  const bool dgrad = product >= 5, mx4 = product == kOpMx4, mx8 = product == kOpMx8;
+  const int es = product == kOpI8 ? 1 : 2;
+  LinArgs a = {};
+  a.P = static_cast<const char*>(W);
+  a.Q = static_cast<const char*>(X);
+  a.ldp = mx4 ? K / 2 : mx8 ? K : es * ldw;
+  a.ldq = es * ldx;
+  a.p_group = mx4 || mx8 ? a.ldp * N : es * w_group;
+  a.offsets = grouped ? &some_list : nullptr;
+  a.M = n_entries;
+  a.n_rows = n_entries;
+  a.G = static_cast<int>(n_groups);
+  a.np = static_cast<int>(dgrad ? K : N);
+  a.nc = static_cast<int>(dgrad ? N : K);
+  RowsChoice c;
+  switch (product) {
+    case 0: c = choose_rows<kOpBF16, kLinForward>(a); break;
+    case 1: c = choose_rows<kOpF16, kLinForward>(a); break;
+    case 2: c = choose_rows<kOpI8, kLinForward>(a); break;
+    case 3: c = choose_rows<kOpMx4, kLinForward>(a); break;
+    case 4: c = choose_rows<kOpMx8, kLinForward>(a); break;
+    case 5: c = choose_rows<kOpBF16, kLinDgrad>(a); break;
+    default: c = choose_rows<kOpF16, kLinDgrad>(a); break;
+  }
+  MGQ_REQUIRE(c.nq || c.tile.rows, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  tile[0] = c.nq ? 16 * c.nq : c.tile.rows;
+  tile[1] = c.nq ? lin_few_cols(c.nq) : c.tile.cols;
+  tile[2] = c.nq ? 0 : c.tile.staged ? 2 : 1;
+  return MGQ_OK;
 }

@@ -265,10 +265,11 @@ __global__ void __launch_bounds__(64 * kWaves) lin_few_kernel(const LinArgs a) {
   }
 }
 
-template <int OP, int NP, int NQ>
+template <int OP, int NQ>
 int launch(const LinArgs& a, hipStream_t s, const char* what) {
-  const int64_t grid = lin_row_tiles(a, 16 * NQ) * ceil_div(a.np, 16 * NP);
-  MGQ_REQUIRE(grid < (int64_t(1) << 24), MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  constexpr int NP = NQ == 4 ? 2 : 1;  // lin_few_cols(NQ) / 16
+  const int64_t grid = lin_few_grid(a, NQ);
+  MGQ_REQUIRE(grid < kLinFewGrid, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
   if ((lin_row_bounds(a, static_cast<int64_t>(a.nc) * lin_esize<OP>()) & 15) == 0)
     lin_few_kernel<OP, NP, NQ, true><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
   else
@@ -278,9 +279,9 @@ int launch(const LinArgs& a, hipStream_t s, const char* what) {
 
 template <int OP>
 int run(const LinArgs& a, int nq, hipStream_t s, const char* what) {
-  if (nq == 1) return launch<OP, 1, 1>(a, s, what);
-  if (nq == 2) return launch<OP, 1, 2>(a, s, what);
-  return launch<OP, 2, 4>(a, s, what);
+  if (nq == 1) return launch<OP, 1>(a, s, what);
+  if (nq == 2) return launch<OP, 2>(a, s, what);
+  return launch<OP, 4>(a, s, what);
 }
 
 }  // namespace

@@ -67,6 +67,11 @@ inline int64_t lin_row_tiles(const LinArgs& a, int bm) {
   return a.offsets ? a.M / bm + (segs < a.M ? segs : a.M) : ceil_div(a.M, bm);
 }
 
+inline int64_t lin_tile_grid(const LinArgs& a, int rows, int cols) {
+  return lin_row_tiles(a, rows) * ceil_div(a.np, cols);
+}
+constexpr int64_t kLinTileGrid = int64_t(1) << 23;  // 512 threads each, less than 2^32 in all
+
 // Output tile of a product over rows: 64, 128 or 256 entries by 256 columns, or
 // 64 by 128. staged: through registers (up to 128 entries).
 struct LinTileShape {

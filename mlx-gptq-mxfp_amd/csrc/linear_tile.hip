@@ -931,8 +931,7 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(const LinArgs a, const 
 template <int OP, int KIND, int FQ, int FP, bool STAGED>
 int launch(const LinArgs& a, const LinPlanArgs& pl, int64_t grid, hipStream_t s, const char* what) {
   const int64_t most = KIND == kLinWgrad || KIND == kLinWgradGather ? 2 * kCUs : grid;
-  // (a launch has less than 2^32 threads)
-  MGQ_REQUIRE(most < (int64_t(1) << 23) && grid < (int64_t(1) << 31), MGQ_ERR_SHAPE,
+  MGQ_REQUIRE(most < kLinTileGrid && grid < (int64_t(1) << 31), MGQ_ERR_SHAPE,
               "%s: too many output tiles", what);
   const unsigned blocks = static_cast<unsigned>(grid < most ? grid : most);
   lin_tile_kernel<OP, KIND, FQ, FP, STAGED><<<blocks, 512, 0, s>>>(a, pl);
@@ -941,7 +940,7 @@ int launch(const LinArgs& a, const LinPlanArgs& pl, int64_t grid, hipStream_t s,
 
 template <int OP, int KIND, int FQ, int FP, bool STAGED>
 int launch_rows(const LinArgs& a, hipStream_t s, const char* what) {
-  const int64_t grid = lin_row_tiles(a, 64 * FQ) * ceil_div(a.np, 128 * FP);
+  const int64_t grid = lin_tile_grid(a, 64 * FQ, 128 * FP);
   return launch<OP, KIND, FQ, FP, STAGED>(a, LinPlanArgs{}, grid, s, what);
 }
 

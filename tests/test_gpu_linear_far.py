@@ -64,3 +64,17 @@ def test_more_summed_rows_than_one_launch_holds():
     dx = linear.grouped_linear_dgrad(dy.to(DEV), w.to(DEV), row_index=at.to(DEV), n_rows=rows)
     want = torch.zeros(rows, dtype=torch.float64).index_add_(0, at.long(), 2.0 * dy.double()[:, 0])
     assert torch.equal(dx[:, 0].cpu().double(), want)
+
+
+def test_a_product_past_the_few_rows_kernels_launch():
+    """One entry for each of 4096 experts of 65536 rows: more workgroups of the kernel
+    for few rows than a launch holds, but not of a tile kernel. Sums of 16 products up
+    to 4 are exact in bf16."""
+    G, N, K = 4096, 65536, 16
+    g = torch.Generator(DEV).manual_seed(8)
+    w = torch.randint(-2, 3, (G, N, K), generator=g, device=DEV, dtype=torch.int8).to(torch.bfloat16)
+    x = torch.randint(-2, 3, (G, K), generator=g, device=DEV).to(torch.bfloat16)
+    y = linear.grouped_linear(x, w, torch.arange(G + 1, device=DEV, dtype=torch.int32), validate=False)
+    for a in range(0, G, 256):
+        want = (w[a : a + 256].float() * x[a : a + 256, None].float()).sum(-1)
+        assert torch.equal(y[a : a + 256].float(), want), a
