@@ -113,13 +113,17 @@ class ExpertMLP:
     def forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                 top_k_weights: torch.Tensor) -> torch.Tensor:
         """[T, H] -> [T, H]. The activation and the sum over a row's experts are
-        formed in fp32 and rounded to the rows' type."""
+        formed in fp32 and rounded to the rows' type. Assignments to no expert add
+        nothing, whatever their weight is."""
         T, k = top_k_index.shape
         r = route(top_k_index, self.num_experts)
         gate, up = self._product(hidden_states, self.gate_up, r.offsets, r.row_index).chunk(2, dim=-1)
         act = (F.silu(gate.float()) * up.float()).to(hidden_states.dtype)
         y = self._product(act, self.down, r.offsets)
         y = y[r.entry].view(T, k, y.shape[1]).float()
-        return (y * top_k_weights.float().unsqueeze(-1)).sum(1).to(hidden_states.dtype)
+        # (a row whose experts are all masked may come with weights of NaN)
+        dropped = (r.entry >= r.offsets[-1]).view(T, k)
+        weights = top_k_weights.float().masked_fill(dropped, 0.0)
+        return (y * weights.unsqueeze(-1)).sum(1).to(hidden_states.dtype)
 
     __call__ = forward
