@@ -15,6 +15,7 @@ from pathlib import Path
 
 import numpy as np
 import torch
+from torch import _C
 
 LIB_PATH = Path(__file__).resolve().parent / "libmlxgptq_hip.so"
 
@@ -168,12 +169,24 @@ def call(name: str, *args) -> None:
     """The entry point `name`, with the device of the stream that ends its
     arguments current."""
     fn = getattr(load(), name)
-    device = getattr(args[-1], "device", None)
-    if device is None or device == torch._C._cuda_getDevice():
-        check(fn(*args), name)
+    stream = args[-1]
+    if type(stream) is Stream and stream.device != _C._cuda_getDevice():
+        with torch.cuda.device(stream.device):
+            rc = fn(*args)
     else:
-        with torch.cuda.device(device):
-            check(fn(*args), name)
+        rc = fn(*args)
+    if rc:
+        check(rc, name)
+
+
+def launch(device: torch.device, name: str, *args) -> None:
+    """``call`` on the device's current stream, which ends the arguments."""
+    if device.index == _C._cuda_getDevice():
+        rc = getattr(load(), name)(*args, _C._cuda_getCurrentRawStream(device.index))
+        if rc:
+            check(rc, name)
+    else:
+        call(name, *args, stream_of(device))
 
 
 # --------------------------------------------------------------------------
@@ -223,15 +236,18 @@ def on_device(t: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 def stream_of(device: torch.device) -> Stream:
     """The device's current stream, for the last argument of ``call``."""
-    index = device.index if isinstance(device, torch.device) else torch.device(device).index
+    if not isinstance(device, torch.device):
+        device = torch.device(device)
+    index = device.index
     if index is None:
         index = torch.cuda.current_device()
-    handle = torch._C._cuda_getCurrentRawStream(index)
-    stream = _streams.get((index, handle))
-    if stream is None:
+    handle = _C._cuda_getCurrentRawStream(index)
+    try:
+        return _streams[index, handle]
+    except KeyError:
         stream = _streams[index, handle] = Stream(handle)
         stream.device = index
-    return stream
+        return stream
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

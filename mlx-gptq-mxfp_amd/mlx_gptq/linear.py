@@ -37,8 +37,10 @@ from torch.autograd import forward_ad
 
 from . import _native as nat
 
-_MX_BITS = {"mxfp4": 4, "mxfp8": 8}
+_MX_MODES = {"mxfp4": (4, nat.MODE_MXFP4), "mxfp8": (8, nat.MODE_MXFP8)}  # bits, code
 _HALF = (torch.bfloat16, torch.float16)
+_FLOATS = (torch.float32, *_HALF)
+_WORDS = (torch.int32, torch.uint32)
 
 
 # A single token's product takes a few microseconds, which the calls below reach
@@ -72,7 +74,8 @@ def _home(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
 
 def _ld(t: torch.Tensor) -> int:
     """Row pitch in elements (a single row's stride says nothing)."""
-    return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], 1)
+    shape = t.shape
+    return t.stride(-2) if shape[-2] > 1 else max(shape[-1], 1)
 
 
 def _weight3(fn: str, weight: torch.Tensor, offsets) -> torch.Tensor:
@@ -92,13 +95,14 @@ def _rows2(fn: str, name: str, x: torch.Tensor) -> None:
 
 
 def _integers(t: torch.Tensor) -> bool:
-    return not (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool)
+    dt = t.dtype
+    return dt is torch.int32 or not (dt.is_floating_point or dt.is_complex or dt is torch.bool)
 
 
 def _int32(t: torch.Tensor) -> torch.Tensor:
     """`t` in 32 bits. What lies past them stays out of range, as the kernels' clamps
     expect it."""
-    if t.dtype == torch.int32:
+    if t.dtype is torch.int32:
         return t
     if t.dtype == torch.int64:
         t = t.clamp(-(2**31), 2**31 - 1)
@@ -133,23 +137,29 @@ def _list(fn: str, offsets, row_index, groups: int, n_rows: int, dev: torch.devi
     return _dense(_int32(offsets), dev), row_index, entries
 
 
-def _check_half(fn: str, *tensors: torch.Tensor) -> None:
-    dt = tensors[0].dtype
-    if dt not in _HALF or any(t.dtype != dt for t in tensors):
+def _check_half(fn: str, a: torch.Tensor, b: torch.Tensor) -> None:
+    dt = a.dtype
+    if dt not in _HALF or b.dtype != dt:
         raise TypeError(f"{fn}: expects bfloat16 or float16 tensors of one type "
-                        f"(got {', '.join(str(t.dtype) for t in tensors)})")
+                        f"(got {dt}, {b.dtype})")
 
 
-def _check_tangents(fn: str, *tensors: torch.Tensor) -> None:
-    """No operand carries a forward-mode tangent (one comparison outside such a level)."""
+def _tracked(fn: str, *tensors: torch.Tensor) -> bool:
+    """Whether autograd would follow a result of `tensors`. Forward-mode tangents are
+    refused (outside their levels that costs one comparison)."""
     if forward_ad._current_level >= 0:
         for t in tensors:
             if forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{fn} has no forward-mode derivative")
+    for t in tensors:
+        if t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 class _NoGradient(torch.autograd.Function):
-    """A result that has no gradient, handed on with a backward that says so."""
+    """A result that has no gradient, handed on with a backward that raises, where the
+    plain result would read as a constant."""
 
     @staticmethod
     def forward(ctx, fn, out, *inputs):
@@ -160,14 +170,6 @@ class _NoGradient(torch.autograd.Function):
     def backward(ctx, dy):
         raise NotImplementedError(f"{ctx.fn} has no gradient: detach its inputs, or call it under "
                                   "torch.no_grad()")
-
-
-def _without_gradient(fn: str, out: torch.Tensor, *inputs: torch.Tensor) -> torch.Tensor:
-    """`out`, computed from `inputs`: a backward that reaches it raises, where a
-    plain result would read as a constant."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
-        return _NoGradient.apply(fn, out, *inputs)
-    return out
 
 
 def _forward(x, weight, offsets, row_index, validate):
@@ -184,9 +186,9 @@ def _forward(x, weight, offsets, row_index, validate):
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
     if M and N:
-        nat.call("mgq_grouped_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0], _ld(xd),
-                 nat.ptr(idx), M, wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off),
-                 y.data_ptr(), nat.stream_of(dev))
+        nat.launch(dev, "mgq_grouped_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0],
+                   _ld(xd), nat.ptr(idx), M, wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0),
+                   nat.ptr(off), y.data_ptr())
     return _home(y, x), off, idx
 
 
@@ -227,8 +229,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets=None,
     device were written again). The gradients have none themselves: a second
     derivative raises.
     """
-    _check_tangents("grouped_linear", x, weight)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if _tracked("grouped_linear", x, weight):
         return _GroupedLinear.apply(x, weight, offsets, row_index, validate)
     return _forward(x, weight, offsets, row_index, validate)[0]
 
@@ -243,7 +244,7 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
     required; rows that no entry reads are zero).
     """
     fn = "grouped_linear_dgrad"
-    _check_tangents(fn, dy, weight)
+    tracked = _tracked(fn, dy, weight)
     _check_half(fn, dy, weight)
     _rows2(fn, "dy", dy)
     w = _weight3(fn, weight, offsets)
@@ -262,11 +263,10 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
     gathered = idx is not None
     out_type = torch.float32 if gathered else dy.dtype
     dx = torch.empty(M, K, dtype=out_type, device=dev)
-    stream = nat.stream_of(dev)
     if M and K and N:
-        nat.call("mgq_grouped_dgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
-                 wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off), dx.data_ptr(),
-                 nat.dtype_code(out_type), stream)
+        nat.launch(dev, "mgq_grouped_dgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
+                   wd.data_ptr(), G, N, K, _ld(wd), wd.stride(0), nat.ptr(off), dx.data_ptr(),
+                   nat.dtype_code(out_type))
     elif N == 0:
         dx.zero_()
     if gathered:
@@ -274,10 +274,11 @@ def grouped_linear_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets=None,
         if out.numel():
             ws = torch.empty(nat.load().mgq_rows_sum_workspace_size(M, int(n_rows)),
                              dtype=torch.uint8, device=dev)
-            nat.call("mgq_rows_sum", dx.data_ptr(), idx.data_ptr(), M, int(n_rows), K,
-                     out.data_ptr(), nat.dtype_code(out.dtype), ws.data_ptr(), ws.numel(), stream)
+            nat.launch(dev, "mgq_rows_sum", dx.data_ptr(), idx.data_ptr(), M, int(n_rows), K,
+                       out.data_ptr(), nat.dtype_code(out.dtype), ws.data_ptr(), ws.numel())
         dx = out
-    return _without_gradient(fn, _home(dx, dy), dy, weight)
+    dx = _home(dx, dy)
+    return _NoGradient.apply(fn, dx, dy, weight) if tracked else dx
 
 
 def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
@@ -290,7 +291,7 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     once; zeros for a group without entries. At most 4096 groups.
     """
     fn = "grouped_linear_wgrad"
-    _check_tangents(fn, dy, x)
+    tracked = _tracked(fn, dy, x)
     _check_half(fn, dy, x)
     _rows2(fn, "dy", dy)
     _rows2(fn, "x", x)
@@ -310,12 +311,13 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     if N and K:
         size = nat.load().mgq_grouped_wgrad_workspace_size(M, G, N, K)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        nat.call("mgq_grouped_wgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
-                 xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), G, N, K, nat.ptr(off),
-                 dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size, nat.stream_of(dev))
+        nat.launch(dev, "mgq_grouped_wgrad", dyd.data_ptr(), nat.dtype_code(dy.dtype), M, _ld(dyd),
+                   xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), G, N, K, nat.ptr(off),
+                   dw.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), size)
     if offsets is None:
         dw = dw[0]
-    return _without_gradient(fn, _home(dw, dy), dy, x)
+    dw = _home(dw, dy)
+    return _NoGradient.apply(fn, dw, dy, x) if tracked else dw
 
 
 def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mode: str,
@@ -329,22 +331,23 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
     -> bf16 [entries, N]. The decoded weights are exact in bf16, the sums fp32.
     """
     fn = "mxfp_linear"
-    _check_tangents(fn, x)
-    if mode not in _MX_BITS:
+    tracked = _tracked(fn, x)
+    if mode not in _MX_MODES:
         raise ValueError(f"not a microscaling mode: {mode}")
-    if x.dtype != torch.bfloat16:
+    bits, code = _MX_MODES[mode]
+    if x.dtype is not torch.bfloat16:
         raise TypeError(f"{fn}: expects bfloat16 rows (got {x.dtype})")
-    if packed.dtype not in (torch.int32, torch.uint32) or scales.dtype != torch.uint8:
+    if packed.dtype not in _WORDS or scales.dtype is not torch.uint8:
         raise TypeError(f"{fn}: expects 32-bit words and uint8 scales "
                         f"(got {packed.dtype} and {scales.dtype})")
     _rows2(fn, "x", x)
     w, s = _weight3(fn, packed, offsets), _weight3(fn, scales, offsets)
     G, N, words = w.shape
-    K = words * 32 // _MX_BITS[mode]
+    K = words * 32 // bits
     if x.shape[1] != K or K % 32:
         raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the words hold {K} "
                              "(a multiple of 32)")
-    if tuple(s.shape) != (G, N, K // 32):
+    if s.shape != (G, N, K // 32):
         raise AssertionError(f"{fn}: scales must be {(G, N, K // 32)} (got {tuple(s.shape)})")
     dev = _device(x, packed, scales)
     xd = _pitched(x, dev)
@@ -352,10 +355,10 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
     if M and N:
-        nat.call("mgq_mxfp_linear", xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), M,
-                 wd.data_ptr(), sd.data_ptr(), nat.mode_code(mode), G, N, K, nat.ptr(off),
-                 y.data_ptr(), nat.stream_of(dev))
-    return _without_gradient(fn, _home(y, x), x)
+        nat.launch(dev, "mgq_mxfp_linear", xd.data_ptr(), xd.shape[0], _ld(xd), nat.ptr(idx), M,
+                   wd.data_ptr(), sd.data_ptr(), code, G, N, K, nat.ptr(off), y.data_ptr())
+    y = _home(y, x)
+    return _NoGradient.apply(fn, y, x) if tracked else y
 
 
 def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -365,8 +368,8 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     A zero row has scale 0 and zero codes. A row that holds a NaN or an infinity
     has scale NaN and zero codes, so products with it are NaN.
     """
-    _check_tangents("quantize_rows_int8", x)
-    if x.dtype not in (torch.float32, *_HALF):
+    tracked = _tracked("quantize_rows_int8", x)
+    if x.dtype not in _FLOATS:
         raise TypeError(f"quantize_rows_int8: expects float32, bfloat16 or float16 (got {x.dtype})")
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"quantize_rows_int8: rows of no elements ({tuple(x.shape)})")
@@ -375,9 +378,10 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     q = torch.empty(x.shape, dtype=torch.int8, device=dev)
     s = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     if rows.shape[0]:
-        nat.call("mgq_quantize_rows_int8", rows.data_ptr(), nat.dtype_code(x.dtype), rows.shape[0],
-                 rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr(), nat.stream_of(dev))
-    return _home(q, x), _without_gradient("quantize_rows_int8", _home(s, x), x)
+        nat.launch(dev, "mgq_quantize_rows_int8", rows.data_ptr(), nat.dtype_code(x.dtype),
+                   rows.shape[0], rows.shape[1], _ld(rows), q.data_ptr(), s.data_ptr())
+    q, s = _home(q, x), _home(s, x)
+    return q, _NoGradient.apply("quantize_rows_int8", s, x) if tracked else s
 
 
 def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
@@ -394,13 +398,13 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     """
     fn = "int8_linear"
     scaling = (x_scale, w_scale) if bias is None else (x_scale, w_scale, bias)
-    _check_tangents(fn, *scaling)
-    if x.dtype != torch.int8 or weight.dtype != torch.int8:
+    tracked = _tracked(fn, *scaling)
+    if x.dtype is not torch.int8 or weight.dtype is not torch.int8:
         raise TypeError(f"{fn}: expects int8 rows and weights (got {x.dtype} and {weight.dtype})")
-    for name, t in (("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias)):
-        if t is not None and t.dtype != torch.float32:
-            raise TypeError(f"{fn}: {name} must be float32 (got {t.dtype})")
-    if out_dtype not in (torch.float32, *_HALF):
+    for t in scaling:
+        if t.dtype is not torch.float32:
+            raise TypeError(f"{fn}: x_scale, w_scale and bias must be float32 (got {t.dtype})")
+    if out_dtype not in _FLOATS:
         raise TypeError(f"{fn}: the result is float32, bfloat16 or float16 (got {out_dtype})")
     _rows2(fn, "x", x)
     w = _weight3(fn, weight, offsets)
@@ -408,8 +412,8 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     if x.shape[1] != K:
         raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the weight {K}")
     per_channel = (N,) if offsets is None else (G, N)
-    if tuple(x_scale.shape) != (x.shape[0],) or tuple(w_scale.shape) != per_channel or (
-            bias is not None and tuple(bias.shape) != per_channel):
+    if x_scale.shape != (x.shape[0],) or w_scale.shape != per_channel or (
+            bias is not None and bias.shape != per_channel):
         raise AssertionError(f"{fn}: x_scale must be {(int(x.shape[0]),)}, w_scale and bias "
                              f"{per_channel}")
     dev = _device(x, weight)
@@ -419,8 +423,8 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
     if M and N:
-        nat.call("mgq_int8_linear", xd.data_ptr(), xs.data_ptr(), xd.shape[0], _ld(xd),
-                 nat.ptr(idx), M, wd.data_ptr(), ws.data_ptr(), nat.ptr(b), G, N, K, _ld(wd),
-                 wd.stride(0), nat.ptr(off), y.data_ptr(), nat.dtype_code(out_dtype),
-                 nat.stream_of(dev))
-    return _without_gradient(fn, _home(y, x), *scaling)
+        nat.launch(dev, "mgq_int8_linear", xd.data_ptr(), xs.data_ptr(), xd.shape[0], _ld(xd),
+                   nat.ptr(idx), M, wd.data_ptr(), ws.data_ptr(), nat.ptr(b), G, N, K, _ld(wd),
+                   wd.stride(0), nat.ptr(off), y.data_ptr(), nat.dtype_code(out_dtype))
+    y = _home(y, x)
+    return _NoGradient.apply(fn, y, *scaling) if tracked else y

@@ -94,11 +94,10 @@ def install(monkeypatch, device=torch.device("cpu")):
     """mlx_gptq.linear on host tensors; returns the list of calls made."""
     calls = []
 
-    def call(name, *args):
+    def launch(device, name, *args):
         calls.append(name)
-        globals()[name.removeprefix("mgq_")](*args)
+        globals()[name.removeprefix("mgq_")](*args, 0)
 
     monkeypatch.setattr(linear, "_device", lambda *tensors: device)
-    monkeypatch.setattr(nat, "stream_of", lambda dev: 0)
-    monkeypatch.setattr(nat, "call", call)
+    monkeypatch.setattr(nat, "launch", launch)
     return calls
