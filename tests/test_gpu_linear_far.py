@@ -13,6 +13,12 @@ DEV = torch.device("cuda", 0)
 ULP = 2.0**-8  # of bf16
 
 
+@pytest.fixture(autouse=True)
+def large_tensors_go_back():
+    yield
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("K", [1, 8])
 def test_more_rows_than_an_index_can_name(K):
     """Gathers from rows past 2^31 in all: the index names rows up to 2^31 - 1, by

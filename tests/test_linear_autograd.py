@@ -189,3 +189,17 @@ def test_only_what_the_gradient_reads_is_saved(calls, which):
     got, ref = (x.grad, want[0]) if which == "x" else (w.grad, want[1])
     assert bool(((got.float() - ref).abs() <= 2.0**-11 * ref.abs() + 2.0**-16).all())
     assert (w if which == "x" else x).grad is None
+
+
+def test_results_without_a_gradient_can_be_written_in_place(calls):
+    """A residual added in place, as to any operator's result."""
+    x = torch.ones(4, 32, dtype=torch.bfloat16, requires_grad=True)
+    for y in products(x):
+        before = y.detach().clone()
+        y += 2.0
+        y[0] = 0.0
+        assert torch.equal(y[1:].detach(), before[1:] + 2.0) and y.requires_grad
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            y.float().sum().backward()
+    q, s = linear.quantize_rows_int8(x)
+    s.mul_(2.0)
