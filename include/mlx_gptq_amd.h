@@ -365,7 +365,10 @@ int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy
 
 /* dW[g, n, k] = sum over the entries t of group g of dY[t, n] X[row(t), k];
  * zeros for a group without entries. out_dtype is dtype or f32. At most 4096
- * groups; the workspace is 256-byte aligned. */
+ * groups. The workspace is 256-byte aligned and holds the partial results of the
+ * longest groups: at most 2048 + tiles of one matrix (256 x 256) tiles of 256 KiB,
+ * 0.5 to 0.75 GiB for long lists, nothing but the plan for lists of up to 256
+ * entries. */
 int64_t mgq_grouped_wgrad_workspace_size(int64_t n_entries, int64_t n_groups, int64_t N,
                                          int64_t K);
 int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, int64_t lddy, const void* X,

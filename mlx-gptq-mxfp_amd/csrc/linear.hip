@@ -11,11 +11,15 @@ namespace mgq {
 namespace {
 
 // Which kernel and tile a product over rows takes: of those whose grid holds it, the
-// one whose time by the model below is least. The model was fitted to 980 products (all types, 1 .. 16384
-// entries, 0 .. 128 groups, K 256 .. 14336, aligned and not) that were timed with each
-// of their 3 to 7 choices: the model's choice costs 1.7 % over the best one on
-// average and 64 % at worst, where the largest tile that the average group fills
-// costs 33 % on average and tenfold at worst.
+// one whose time by the model below is least. The model was fitted to 980 products (all
+// types, 1 .. 16384 entries, 0 .. 128 groups, K 256 .. 14336, aligned and not) that were
+// timed with each of their 3 to 7 choices, called again and again on the same weights, so
+// that what fits the memory-side cache came from there. On these the model's choice costs
+// 1.7 % over the best one on average and 64 % at worst, where the largest tile that the
+// average group fills costs 33 % on average and tenfold at worst. (Pricing the few rows'
+// weight at 2.86 TB/s had 46 % at worst, but sent one token through 8 experts to a tile,
+// 16 instead of 11 us.) The worst are lists of some 3000 entries over 32 to 60 groups,
+// whose tiles the model counts below the groups' number.
 //
 //   large tiles: rounds of the 256 CUs x (stages x time of a stage + a fixed time
 //     for the tile's first loads and its results), or the weight's bytes at the

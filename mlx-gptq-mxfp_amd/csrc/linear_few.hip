@@ -2,7 +2,7 @@
 // small decoding batches), so the weight is read once and reading it is the
 // work.
 //
-// A workgroup computes 16 entries x 16 NP weight rows; its waves share the
+// A workgroup computes 16 NQ entries x 16 NP weight rows; its waves share the
 // contraction and add their sums through LDS in wave order. The weight goes from
 // memory into registers as the A operand of a 16x16 MFMA (lane l: row l % 16, a
 // 16-byte piece of it by l / 16), X from the caches as its B operand; nothing is
@@ -14,10 +14,14 @@
 // four quarters of a wave take four consecutive groups, so MFMA i of four
 // multiplies codes 8 i .. 8 i + 7 of each.
 //
-// Measured: one token through 8 of 128 experts [1536, 2048], bf16 11 us (4.6 TB/s of
-// weight, half of it from the memory-side cache), MXFP4 codes 8 us, of which a launch with its two dependent loads (offsets,
-// row index) takes 5; one row of int8 [14336, 4096] 13.5 us. A group's second 16
-// entries repeat its weight from L2; 64 entries in one workgroup (NQ = 4) load it once.
+// Measured, called again on the same weights (the 256 MB memory-side cache holds them):
+// one token through 8 of 128 experts [1536, 2048], bf16 11 us (4.6 TB/s of weight), MXFP4
+// codes 8 us, of which a launch with its two dependent loads (offsets, row index) takes 5;
+// one row of bf16 [14336, 4096] 22 us, and 44 us (2.7 TB/s) after 512 MiB were written
+// elsewhere. One row of int8 of that shape takes 12.6 us here (24.5 after the writes); the
+// time model prices it as 19 us and gives it to the 64 x 128 tile, which takes 15.0 (27.1).
+// A group's second 16 entries repeat its weight from L2; 64 entries in one workgroup
+// (NQ = 4) load it once.
 #include "linear_few.h"
 
 namespace mgq {

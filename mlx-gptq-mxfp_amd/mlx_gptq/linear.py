@@ -21,7 +21,8 @@ that belong to no group give zero rows. ``offsets=None`` is one dense weight
 (without its leading dimension). Offsets on the device stay there: with
 ``validate=False`` no call waits for the device, so a decoding loop can be
 captured in a graph. Offsets and indexes outside their ranges are clamped by the
-kernels, never followed; ``validate`` raises for them. Only ``grouped_linear``
+kernels, never followed; ``validate`` raises for them, and for offsets that decrease
+(unvalidated, those leave rows of the result unwritten). Only ``grouped_linear``
 is differentiable. The other calls run on tensors that require a gradient, but a
 backward that reaches their results raises, as forward-mode tangents do in every call.
 
@@ -288,7 +289,8 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     ([N, K] without offsets), of dy's type or ``out_dtype=torch.float32``.
 
     dy: [entries, N], x: [T, K]. fp32 sums over a group's entries, rounded
-    once; zeros for a group without entries. At most 4096 groups.
+    once; zeros for a group without entries. At most 4096 groups. A call takes up
+    to 0.75 GiB of workspace for the partial results of long groups.
     """
     fn = "grouped_linear_wgrad"
     tracked = _tracked(fn, dy, x)
