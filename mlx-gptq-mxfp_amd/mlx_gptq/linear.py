@@ -227,8 +227,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets=None,
     [entries, N]. fp32 sums, rounded once. Differentiable in x and weight: the
     gradients are ``grouped_linear_dgrad`` and ``grouped_linear_wgrad`` on the
     lists of the forward (autograd refuses a backward after int32 lists on the
-    device were written again). The gradients have none themselves: a second
-    derivative raises.
+    device, or the tensors they are views of, were written again). The gradients
+    have none themselves: a second derivative raises.
     """
     if _tracked("grouped_linear", x, weight):
         return _GroupedLinear.apply(x, weight, offsets, row_index, validate)
