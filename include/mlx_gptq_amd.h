@@ -335,7 +335,7 @@ int mgq_gptq_affine(float* W, const float* U, int64_t B, int64_t R, int64_t C, i
  * Matrix products with the weights -- mlx_gptq/linear.py                    *
  *                                                                           *
  * Not in the reference: the products a calibration forward, a fine-tuning   *
- * step or a serving program makes with dense, MXFP or int8 weights.         *
+ * step or a serving program makes with dense, MXFP, affine or int8 weights. *
  *                                                                           *
  * Group g owns the list entries [offsets[g], offsets[g + 1]) (offsets:      *
  * device int32 [n_groups + 1], or NULL for one group of all entries). Entry *
@@ -397,6 +397,19 @@ int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const int32_t* r
                     int64_t n_entries, const uint32_t* words, const uint8_t* scales, int mode,
                     int64_t n_groups, int64_t N, int64_t K, const int32_t* offsets, void* Y,
                     void* stream);
+
+/* Y[t, n] = sum_k X[row(t), k] (code[g, n, k] scales[g, n, k / group_size] +
+ * biases[g, n, k / group_size]), X and Y of dtype (bf16 or f16). words:
+ * [n_groups, N, K * bits / 32] as mgq_pack_q writes them (bits 2, 4 or 8), scales
+ * and biases: [n_groups, N, K / group_size] of param_dtype (f32/bf16/f16), all
+ * contiguous; group_size 32, 64 or 128, K a multiple of it. fp32 sums, rounded
+ * once: scale sum(x code) + bias sum(x) for every 32 values, so that |x| beyond
+ * 1e34 may overflow where the product with decoded weights would not. */
+int mgq_affine_linear(const void* X, int dtype, int64_t n_rows, int64_t ldx,
+                      const int32_t* row_index, int64_t n_entries, const uint32_t* words,
+                      const void* scales, const void* biases, int param_dtype, int bits,
+                      int64_t group_size, int64_t n_groups, int64_t N, int64_t K,
+                      const int32_t* offsets, void* Y, void* stream);
 
 /* q = rne(x / s) within +-127, s = max |x| of the row / 127 (fp32 quotients; a
  * subnormal s may be too small for its row, whose codes stop at 127). A zero row

@@ -1,0 +1,416 @@
+// The inner product that the kernels for a handful of rows share (affine_linear.hip,
+// experts_decode.hip): up to 16 NQ rows of 16-bit x times 16 NP weight rows in any
+// of the weight formats, over a part of the contraction.
+//
+// A 16x16x32 MFMA takes the x rows as its A operand and the weight rows as B, so a
+// lane ends up with four x rows (4 quad + e) of ONE weight row (lane % 16), and what
+// belongs to a weight row (its scales, its bias) is one number a lane.
+//
+// A step is 128 elements of the contraction, four MFMAs. Lane (r, quad) reads what it
+// needs of weight row r straight from memory:
+//   dense       four 16-byte pieces, elements 32 j + 8 quad of the step for MFMA j;
+//   MXFP        the 32 codes of the step's group `quad` and their scale byte, decoded
+//               to bf16 exactly; MFMA j takes codes 8 j .. 8 j + 7 of every group;
+//   affine      the 32 codes of the step's block `quad` and that block's scale s and
+//               bias b. Since w = q s + b,
+//                 sum_k x w = s sum_k x q + b sum_k x      over the ks of one group,
+//               and q is exact in 16 bits: the MFMAs multiply with q itself, another
+//               one with ones gives sum x in the same layout, and s and b are applied
+//               in fp32 once for each block of 32. For that an MFMA has to stay inside a
+//               block: a 4 x 4 transposition among the quads (permlane swaps) hands
+//               MFMA j the codes of block j, and broadcasts block j's s and b.
+// Up to four x rows (NE = 1) sit at A rows 0, 4, 8, 12, so that only one of a lane's
+// four results counts and s and b are applied to that one alone.
+#pragma once
+
+#include "linear_common.h"
+
+namespace mgq {
+
+enum FewFormat : int { kFewDense = 0, kFewMx4 = 1, kFewMx8 = 2, kFewAf2 = 3, kFewAf4 = 4, kFewAf8 = 5 };
+
+constexpr int kFewStep = 128;
+
+// A weight [groups, N, K] in its format.
+struct FewWeight {
+  const char* p;       // elements or codes
+  const char* s;       // MXFP: E8M0 bytes [groups, N, K / 32]; affine: scales [groups, N, K >> shift]
+  const char* b;       // affine: biases
+  int64_t ld, group;   // bytes from row to row, from group to group
+  int64_t n;           // rows of a group
+  int shift;           // affine: log2 of the values that share a scale
+  int type;            // affine: DType of scales and biases
+};
+
+// W: FewFormat, XT: kBF16 or kF16, SB: bytes of an affine scale (2 or 4).
+template <int W_, int XT_, int SB_ = 2>
+struct FewFmt {
+  static constexpr int W = W_, XT = XT_, SB = SB_;
+  static constexpr bool dense = W == kFewDense;
+  static constexpr bool mx = W == kFewMx4 || W == kFewMx8;
+  static constexpr bool affine = W >= kFewAf2;
+  static constexpr int bits = dense ? 16 : W == kFewAf2 ? 2 : W == kFewMx4 || W == kFewAf4 ? 4 : 8;
+  static constexpr int words = dense ? 16 : bits;  // 32-bit words of a lane and step
+  static constexpr int op = XT == kF16 ? kOpF16 : kOpBF16;
+};
+
+// Where a lane reads its weight row.
+struct FewRow {
+  const char* p;
+  const char* s;
+  const char* b;
+};
+
+template <class F>
+__device__ __forceinline__ FewRow few_row(const FewWeight& w, int64_t g, int64_t row, int K) {
+  FewRow r;
+  r.p = w.p + g * w.group + row * w.ld;
+  r.s = r.b = nullptr;
+  const int64_t at = g * w.n + row;
+  if constexpr (F::mx) r.s = w.s + at * (K / 32);
+  if constexpr (F::affine) {
+    r.s = w.s + at * (K >> w.shift) * F::SB;
+    r.b = w.b + at * (K >> w.shift) * F::SB;
+  }
+  return r;
+}
+
+// What a lane holds of a step: words, and the block's scale (and bias) as loaded.
+template <class F>
+struct FewStep {
+  uint32_t v[F::words];
+  uint32_t s, b;
+};
+
+struct __attribute__((packed, aligned(4))) few_u64_u_t {
+  uint32_t v[2];
+};
+
+// 16 bytes at any address.
+__device__ __forceinline__ lin_u32x4_t few_load16(const char* at) {
+  const lin_u128_u_t u = *reinterpret_cast<const lin_u128_u_t*>(at);
+  return lin_u32x4_t{u.v[0], u.v[1], u.v[2], u.v[3]};
+}
+// Elements k .. k + 7 of a 16-bit row of K, zeros from K on.
+__device__ __forceinline__ lin_u32x4_t few_cut16(const char* row, int k, int K) {
+  lin_u32x4_t r = {0, 0, 0, 0};
+  if (k + 8 <= K) return few_load16(row + 2 * static_cast<int64_t>(k));
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < K)
+      r[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k + i]) << (16 * (i & 1));
+  return r;
+}
+
+template <int BYTES>
+__device__ __forceinline__ uint32_t few_param(const char* at) {
+  if constexpr (BYTES == 2) return *reinterpret_cast<const uint16_t*>(at);
+  return *reinterpret_cast<const uint32_t*>(at);
+}
+
+// Step s of a row of K elements. Quantized rows (K % 32 == 0): a block past the row's
+// end reads the row's first one, and few_multiply discards it.
+template <class F>
+__device__ __forceinline__ void few_load(FewStep<F>& f, const FewRow& r, const FewWeight& w, int s,
+                                         int K) {
+  const int quad = (threadIdx.x & 63) >> 4;
+  if constexpr (F::dense) {
+    const int k0 = s * kFewStep + 8 * quad;
+    if ((s + 1) * kFewStep <= K) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const lin_u32x4_t u = few_load16(r.p + 2 * static_cast<int64_t>(k0 + 32 * j));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.v[4 * j + i] = u[i];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const lin_u32x4_t u = few_cut16(r.p, k0 + 32 * j, K);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.v[4 * j + i] = u[i];
+      }
+    }
+  } else {
+    int k0 = s * kFewStep + 32 * quad;
+    k0 = k0 < K ? k0 : 0;
+    const char* at = r.p + static_cast<int64_t>(k0 / 32) * (4 * F::bits);
+    if constexpr (F::bits == 2) {
+      const few_u64_u_t u = *reinterpret_cast<const few_u64_u_t*>(at);
+      f.v[0] = u.v[0];
+      f.v[1] = u.v[1];
+    } else {
+#pragma unroll
+      for (int h = 0; h < F::bits / 4; ++h) {
+        const lin_u32x4_t u = few_load16(at + 16 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.v[4 * h + i] = u[i];
+      }
+    }
+    if constexpr (F::mx) f.s = reinterpret_cast<const uint8_t*>(r.s)[k0 / 32];
+    if constexpr (F::affine) {
+      const int64_t g = k0 >> w.shift;
+      f.s = few_param<F::SB>(r.s + g * F::SB);
+      f.b = few_param<F::SB>(r.b + g * F::SB);
+    }
+  }
+}
+
+// x elements of MFMA j.
+template <class F>
+__device__ __forceinline__ int few_x_at(int s, int j) {
+  const int quad = (threadIdx.x & 63) >> 4;
+  return s * kFewStep + (F::mx ? 32 * quad + 8 * j : 32 * j + 8 * quad);
+}
+template <class F>
+__device__ __forceinline__ void few_load_x(lin_u32x4_t (&x)[4], const char* row, int s, int K) {
+  if ((s + 1) * kFewStep <= K) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = few_load16(row + 2 * static_cast<int64_t>(few_x_at<F>(s, j)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = few_x_at<F>(s, j);
+      if constexpr (F::dense)
+        x[j] = few_cut16(row, k, K);
+      else  // (whole pieces: K % 32 == 0)
+        x[j] = k < K ? few_load16(row + 2 * static_cast<int64_t>(k)) : lin_u32x4_t{0, 0, 0, 0};
+    }
+  }
+}
+
+template <class F>
+__device__ __forceinline__ lin_f32x4_t few_mfma(lin_u32x4_t x, lin_u32x4_t w, lin_f32x4_t c) {
+  if constexpr (F::XT == kF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lin_f16x8_t, x),
+                                                  __builtin_bit_cast(lin_f16x8_t, w), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8_t, x),
+                                                   __builtin_bit_cast(lin_bf16x8_t, w), c, 0, 0, 0);
+}
+
+// The four quads' values of v, each in every quad.
+__device__ __forceinline__ void few_spread(uint32_t v, uint32_t (&out)[4]) {
+  const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const auto lo = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+  out[0] = lo[0];
+  out[1] = lo[1];
+  out[2] = hi[0];
+  out[3] = hi[1];
+}
+// Word q of quad i, for word i of quad q: the 4 x 4 transposition among the quads.
+__device__ __forceinline__ void few_transpose(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  const auto u = __builtin_amdgcn_permlane32_swap(a, c, false, false);
+  const auto v = __builtin_amdgcn_permlane32_swap(b, d, false, false);
+  const auto p = __builtin_amdgcn_permlane16_swap(u[0], v[0], false, false);
+  const auto q = __builtin_amdgcn_permlane16_swap(u[1], v[1], false, false);
+  a = p[0];
+  b = p[1];
+  c = q[0];
+  d = q[1];
+}
+
+// Four codes (one a byte, below 16) as two pairs of 16-bit numbers. A byte below 16 is
+// the E4M3 number byte * 2^-9 (subnormals below 8, the first binade from 8 on), so the
+// scaled conversion of two E4M3 numbers returns the integers.
+template <int XT>
+__device__ __forceinline__ void few_small(uint32_t bytes, uint32_t& lo, uint32_t& hi) {
+  if constexpr (XT == kF16) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.0f, true));
+  } else {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 512.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 512.0f, true));
+  }
+}
+// Four 8-bit codes: whole numbers up to 255 are exact in both types.
+template <int XT>
+__device__ __forceinline__ void few_bytes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  lo = lin_pack2<XT>(static_cast<float>(w & 0xff), static_cast<float>((w >> 8) & 0xff));
+  hi = lin_pack2<XT>(static_cast<float>((w >> 16) & 0xff), static_cast<float>(w >> 24));
+}
+
+// The codes of an affine step after the transposition, ready to be decoded: eight codes
+// of block j for every lane, in the order of k = 32 j + 8 quad + 0..7.
+template <class F>
+__device__ __forceinline__ void few_arrange(FewStep<F>& f) {
+  if constexpr (F::bits == 4) {
+    few_transpose(f.v[0], f.v[1], f.v[2], f.v[3]);
+  } else if constexpr (F::bits == 8) {
+    few_transpose(f.v[0], f.v[2], f.v[4], f.v[6]);
+    few_transpose(f.v[1], f.v[3], f.v[5], f.v[7]);
+  }
+}
+template <class F>
+__device__ __forceinline__ lin_u32x4_t few_codes(const FewStep<F>& f, const uint32_t (&half)[4], int j) {
+  lin_u32x4_t r;
+  uint32_t a, b, c, d;
+  if constexpr (F::bits == 4) {
+    const uint32_t even = f.v[j] & 0x0f0f0f0fu, odd = (f.v[j] >> 4) & 0x0f0f0f0fu;
+    few_small<F::XT>(__builtin_amdgcn_perm(odd, even, 0x05010400u), a, b);
+    few_small<F::XT>(__builtin_amdgcn_perm(odd, even, 0x07030602u), c, d);
+  } else if constexpr (F::bits == 8) {
+    few_bytes<F::XT>(f.v[2 * j], a, b);
+    few_bytes<F::XT>(f.v[2 * j + 1], c, d);
+  } else {
+    // eight 2-bit codes: two a byte, then as above
+    const uint32_t n = (half[j] & 0xffu) | ((half[j] & 0xff00u) << 8);
+    const uint32_t lo4 = (n & 0x000f000fu) | ((n & 0x00f000f0u) << 4);
+    const uint32_t even = lo4 & 0x03030303u, odd = (lo4 >> 2) & 0x03030303u;
+    few_small<F::XT>(__builtin_amdgcn_perm(odd, even, 0x05010400u), a, b);
+    few_small<F::XT>(__builtin_amdgcn_perm(odd, even, 0x07030602u), c, d);
+  }
+  r[0] = a;
+  r[1] = b;
+  r[2] = c;
+  r[3] = d;
+  return r;
+}
+
+template <int SB>
+__device__ __forceinline__ uint32_t few_param_f32(uint32_t raw, int type) {
+  if constexpr (SB == 4) return raw;
+  return type == kF16 ? f2u(f16_to_f32(static_cast<uint16_t>(raw))) : raw << 16;
+}
+
+// acc[p][q] += the step's product of weight rows p with x rows q.
+template <class F, int NP, int NQ, int NE>
+__device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x4_t (&x)[NQ][4], int s,
+                                             int K, int type, lin_f32x4_t (&acc)[NP][NQ]) {
+  const bool whole = (s + 1) * kFewStep <= K;
+  if constexpr (F::dense) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const lin_u32x4_t w = {f[p].v[4 * j], f[p].v[4 * j + 1], f[p].v[4 * j + 2], f[p].v[4 * j + 3]};
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) acc[p][q] = few_mfma<F>(x[q][j], w, acc[p][q]);
+      }
+  } else if constexpr (F::mx) {
+    if (!whole) {  // (x is zero there, but a code may stand for no number)
+      const int quad = (threadIdx.x & 63) >> 4;
+      const uint32_t keep = s * kFewStep + 32 * quad < K ? 0xffffffffu : 0u;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+#pragma unroll
+        for (int i = 0; i < F::words; ++i) f[p].v[i] &= keep;
+        f[p].s &= keep;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        lin_u32x4_t w;
+        if constexpr (F::W == kFewMx4)
+          w = lin_decode_mx4(f[p].v[j], f[p].s);
+        else
+          w = lin_decode_mx8(f[p].v[2 * j], f[p].v[2 * j + 1], f[p].s);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) acc[p][q] = few_mfma<F>(x[q][j], w, acc[p][q]);
+      }
+  } else {
+    const uint32_t one = F::XT == kF16 ? 0x3c003c00u : 0x3f803f80u;
+    const lin_u32x4_t ones = {one, one, one, one};
+    const lin_f32x4_t zero = {0, 0, 0, 0};
+    uint32_t sc[NP][4], bi[NP][4], half[NP][4];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      few_spread(few_param_f32<F::SB>(f[p].s, type), sc[p]);
+      few_spread(few_param_f32<F::SB>(f[p].b, type), bi[p]);
+      few_arrange<F>(f[p]);
+      if constexpr (F::bits == 2) {
+        // 16 codes a word, words 0 and 1 of block `quad`: MFMA j's quads 0 and 1 take
+        // the halves of word 0 of block j, quads 2 and 3 those of word 1
+        const auto u = __builtin_amdgcn_permlane32_swap(f[p].v[0], f[p].v[1], false, false);
+        const auto a = __builtin_amdgcn_permlane16_swap(u[0], u[0], false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap(u[1], u[1], false, false);
+        const uint32_t up = 16 * ((threadIdx.x >> 4) & 1);
+        half[p][0] = (a[0] >> up) & 0xffffu;
+        half[p][1] = (a[1] >> up) & 0xffffu;
+        half[p][2] = (b[0] >> up) & 0xffffu;
+        half[p][3] = (b[1] >> up) & 0xffffu;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!whole && s * kFewStep + 32 * j >= K) break;
+      lin_f32x4_t sum[NQ];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) sum[q] = few_mfma<F>(x[q][j], ones, zero);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const lin_u32x4_t w = few_codes<F>(f[p], half[p], j);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const lin_f32x4_t d = few_mfma<F>(x[q][j], w, zero);
+#pragma unroll
+          for (int e = 0; e < NE; ++e) {
+            acc[p][q][e] = fmaf(u2f(sc[p][j]), d[e], acc[p][q][e]);
+            acc[p][q][e] = fmaf(u2f(bi[p][j]), sum[q][e], acc[p][q][e]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Steps [s_begin, s_end) of NP weight rows (a lane's own) with NQ x rows: BATCH steps'
+// weights are in flight beyond the ones being multiplied. Steps past the end repeat the
+// last one's loads, so that none depends on a branch.
+template <class F, int NP, int NQ, int NE, int BATCH>
+__device__ __forceinline__ void few_product(const FewRow (&row)[NP], const FewWeight& w,
+                                            const char* const (&x)[NQ], int K, int s_begin, int s_end,
+                                            lin_f32x4_t (&acc)[NP][NQ]) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) acc[p][q] = lin_f32x4_t{0, 0, 0, 0};
+  if (s_begin >= s_end) return;
+  FewStep<F> f[2][BATCH][NP];
+  lin_u32x4_t xv[BATCH][NQ][4];
+  auto load = [&](int k, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int at = s + i < s_end ? s + i : s_end - 1;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) few_load<F>(f[k][i][p], row[p], w, at, K);
+    }
+  };
+  auto load_x = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int at = s + i < s_end ? s + i : s_end - 1;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) few_load_x<F>(xv[i][q], x[q], at, K);
+    }
+  };
+  auto multiply = [&](int k, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (s + i < s_end) few_multiply<F, NP, NQ, NE>(f[k][i], xv[i], s + i, K, w.type, acc);
+  };
+  load(0, s_begin);
+  for (int s = s_begin; s < s_end; s += 2 * BATCH) {
+    load_x(s);
+    if (s + BATCH < s_end) load(1, s + BATCH);
+    multiply(0, s);
+    if (s + BATCH >= s_end) break;
+    load_x(s + BATCH);
+    if (s + 2 * BATCH < s_end) load(0, s + 2 * BATCH);
+    multiply(1, s + BATCH);
+  }
+}
+
+// Checks of a quantized weight's description, on the host.
+inline bool few_weight_ok(int format, int64_t K, int shift, int type) {
+  if (format == kFewDense) return true;
+  if (K % 32) return false;
+  if (format < kFewAf2) return true;
+  return shift >= 5 && shift <= 7 && K % (int64_t(1) << shift) == 0 &&
+         (type == kF32 || type == kBF16 || type == kF16);
+}
+
+}  // namespace mgq

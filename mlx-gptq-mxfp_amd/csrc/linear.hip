@@ -101,27 +101,6 @@ int run_rows(const LinArgs& a, hipStream_t s, const char* what) {
   return c.nq ? lin_few_rows(a, OP, c.nq, s, what) : lin_tile_rows(a, OP, KIND, c.tile, s, what);
 }
 
-int check_list(const char* what, const int32_t* offsets, const int32_t* row_index,
-               int64_t n_groups, int64_t n_entries, int64_t n_rows) {
-  MGQ_REQUIRE(n_groups >= 1 && n_groups <= (int64_t(1) << 20), MGQ_ERR_SHAPE,
-              "%s: %lld groups (1 .. 2^20)", what, (long long)n_groups);
-  MGQ_REQUIRE(offsets != nullptr || n_groups == 1, MGQ_ERR_VALUE,
-              "%s: offsets required for %lld groups", what, (long long)n_groups);
-  MGQ_REQUIRE(n_entries >= 0 && n_entries < (int64_t(1) << 31) - 4096, MGQ_ERR_SHAPE,
-              "%s: %lld list entries", what, (long long)n_entries);
-  MGQ_REQUIRE(n_rows >= 1 || n_entries == 0, MGQ_ERR_SHAPE, "%s: X has no rows", what);
-  MGQ_REQUIRE(row_index != nullptr || n_entries <= n_rows, MGQ_ERR_SHAPE,
-              "%s: %lld list entries but X has %lld rows", what, (long long)n_entries,
-              (long long)n_rows);
-  return MGQ_OK;
-}
-
-int check_dims(const char* what, int64_t N, int64_t K) {
-  MGQ_REQUIRE(N >= 1 && K >= 0 && N < (int64_t(1) << 30) && K < (int64_t(1) << 30), MGQ_ERR_SHAPE,
-              "%s: bad weight shape [%lld, %lld]", what, (long long)N, (long long)K);
-  return MGQ_OK;
-}
-
 }  // namespace
 }  // namespace mgq
 
@@ -134,8 +113,8 @@ extern "C" int mgq_grouped_linear(const void* X, int dtype, int64_t n_rows, int6
   clear_error();
   const char* what = "grouped_linear";
   MGQ_REQUIRE(dtype == kBF16 || dtype == kF16, MGQ_ERR_VALUE, "%s: bfloat16 or float16 only", what);
-  if (int rc = check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
-  if (int rc = check_dims(what, N, K)) return rc;
+  if (int rc = lin_check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
+  if (int rc = lin_check_dims(what, N, K)) return rc;
   MGQ_REQUIRE(ldx >= K && ldw >= K, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
   if (n_entries == 0) return MGQ_OK;
   LinArgs a = {};
@@ -168,8 +147,8 @@ extern "C" int mgq_grouped_dgrad(const void* dY, int dtype, int64_t n_entries, i
   MGQ_REQUIRE(dtype == kBF16 || dtype == kF16, MGQ_ERR_VALUE, "%s: bfloat16 or float16 only", what);
   MGQ_REQUIRE(out_dtype == dtype || out_dtype == kF32, MGQ_ERR_VALUE,
               "%s: the result has the operands' type or float32", what);
-  if (int rc = check_list(what, offsets, nullptr, n_groups, n_entries, n_entries)) return rc;
-  if (int rc = check_dims(what, N, K)) return rc;
+  if (int rc = lin_check_list(what, offsets, nullptr, n_groups, n_entries, n_entries)) return rc;
+  if (int rc = lin_check_dims(what, N, K)) return rc;
   MGQ_REQUIRE(lddy >= N && ldw >= K, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
   if (n_entries == 0 || K == 0) return MGQ_OK;
   LinArgs a = {};
@@ -208,8 +187,8 @@ extern "C" int mgq_grouped_wgrad(const void* dY, int dtype, int64_t n_entries, i
   MGQ_REQUIRE(dtype == kBF16 || dtype == kF16, MGQ_ERR_VALUE, "%s: bfloat16 or float16 only", what);
   MGQ_REQUIRE(out_dtype == dtype || out_dtype == kF32, MGQ_ERR_VALUE,
               "%s: the result has the operands' type or float32", what);
-  if (int rc = check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
-  if (int rc = check_dims(what, N, K)) return rc;
+  if (int rc = lin_check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
+  if (int rc = lin_check_dims(what, N, K)) return rc;
   MGQ_REQUIRE(lddy >= N && ldx >= K, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
   MGQ_REQUIRE(n_groups <= kLinPlanGroups, MGQ_ERR_SHAPE, "%s: %lld groups (at most %d)", what,
               (long long)n_groups, kLinPlanGroups);
@@ -245,8 +224,8 @@ extern "C" int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const
   const char* what = "mxfp_linear";
   MGQ_REQUIRE(mode == kMxfp4 || mode == kMxfp8, MGQ_ERR_VALUE, "%s: mode must be mxfp4 or mxfp8",
               what);
-  if (int rc = check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
-  if (int rc = check_dims(what, N, K)) return rc;
+  if (int rc = lin_check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
+  if (int rc = lin_check_dims(what, N, K)) return rc;
   MGQ_REQUIRE(K % kMxGroup == 0, MGQ_ERR_SHAPE, "%s: K = %lld is no multiple of 32", what,
               (long long)K);
   MGQ_REQUIRE(ldx >= K, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
@@ -282,8 +261,8 @@ extern "C" int mgq_int8_linear(const int8_t* X, const float* x_scale, int64_t n_
   const char* what = "int8_linear";
   MGQ_REQUIRE(out_dtype == kF32 || out_dtype == kBF16 || out_dtype == kF16, MGQ_ERR_VALUE,
               "%s: the result is float32, bfloat16 or float16", what);
-  if (int rc = check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
-  if (int rc = check_dims(what, N, K)) return rc;
+  if (int rc = lin_check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
+  if (int rc = lin_check_dims(what, N, K)) return rc;
   // |sum| <= 128 * 128 * K has to fit the int32 accumulator
   MGQ_REQUIRE(K <= 131071, MGQ_ERR_SHAPE, "%s: K = %lld exceeds 131071 (int32 sums)", what,
               (long long)K);
@@ -318,9 +297,10 @@ extern "C" int mgq_linear_choice(int product, const void* X, int64_t ldx, int64_
   const char* what = "linear_choice";
   MGQ_REQUIRE(product >= 0 && product <= 6, MGQ_ERR_VALUE, "%s: no such product", what);
   const int32_t some_list = 0;  // stands for offsets: the choice does not read them
-  if (int rc = check_list(what, grouped ? &some_list : nullptr, nullptr, n_groups, n_entries, n_entries))
+  if (int rc = lin_check_list(what, grouped ? &some_list : nullptr, nullptr, n_groups, n_entries,
+                              n_entries))
     return rc;
-  if (int rc = check_dims(what, N, K)) return rc;
+  if (int rc = lin_check_dims(what, N, K)) return rc;
   const bool dgrad = product >= 5, mx4 = product == kOpMx4, mx8 = product == kOpMx8;
   const int es = product == kOpI8 ? 1 : 2;
   LinArgs a = {};

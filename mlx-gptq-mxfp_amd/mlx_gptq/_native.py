@@ -102,6 +102,8 @@ SIGNATURES: dict[str, list] = {
     "mgq_quantize_rows_int8": [_VP, _INT, _I64, _I64, _I64, _VP, _VP, _VP],
     "mgq_int8_linear": [_VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _I64,
                         _I64, _VP, _VP, _INT, _VP],
+    "mgq_affine_linear": [_VP, _INT, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _INT, _INT, _I64, _I64,
+                          _I64, _I64, _VP, _VP, _VP],
     "mgq_linear_choice": [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64, _INT, _VP],
 }
 

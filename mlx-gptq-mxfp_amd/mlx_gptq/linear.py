@@ -1,14 +1,16 @@
-"""Matrix products with dense, MXFP and int8 weights on MI355X.
+"""Matrix products with dense, MXFP, affine and int8 weights on MI355X.
 
 What the solver's codes are multiplied with: the products of a calibration
 forward, a fine-tuning step or a serving program, for one weight or for every
 expert of a routed layer at once. The reference leaves these to torch and MLX;
-the kernels are csrc/linear*.hip.
+the kernels are csrc/linear*.hip and csrc/affine_linear.hip.
 
 * ``grouped_linear`` (bf16 or f16 weights, differentiable) with its two
   gradients ``grouped_linear_dgrad`` and ``grouped_linear_wgrad``;
 * ``mxfp_linear``: the same product with packed MXFP4 / MXFP8 weights, decoded
   inside the kernel;
+* ``affine_linear``: the same with packed 2-, 4- or 8-bit codes and a scale and a
+  bias for each group of 32, 64 or 128 values (MLX's affine grid);
 * ``quantize_rows_int8`` and ``int8_linear``: rows quantized to 8-bit integers
   with a scale each, and their product with 8-bit weights that have a scale for
   each output channel.
@@ -39,6 +41,8 @@ from torch.autograd import forward_ad
 from . import _native as nat
 
 _MX_MODES = {"mxfp4": (4, nat.MODE_MXFP4), "mxfp8": (8, nat.MODE_MXFP8)}  # bits, code
+_AFFINE_BITS = (2, 4, 8)
+_AFFINE_GROUPS = (32, 64, 128)
 _HALF = (torch.bfloat16, torch.float16)
 _FLOATS = (torch.float32, *_HALF)
 _WORDS = (torch.int32, torch.uint32)
@@ -361,6 +365,64 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
                    wd.data_ptr(), sd.data_ptr(), code, G, N, K, nat.ptr(off), y.data_ptr())
     y = _home(y, x)
     return _NoGradient.apply(fn, y, x) if tracked else y
+
+
+def affine_group(fn: str, cols: int, bits: int, packed: torch.Tensor, scales: torch.Tensor,
+                 biases: torch.Tensor) -> int:
+    """The group size of an affine weight [..., N, cols], its tensors checked."""
+    if bits not in _AFFINE_BITS:
+        raise ValueError(f"{fn}: bits must be one of {_AFFINE_BITS} (got {bits})")
+    if packed.dtype not in _WORDS:
+        raise TypeError(f"{fn}: expects 32-bit words (got {packed.dtype})")
+    if scales.dtype not in _FLOATS or biases.dtype != scales.dtype:
+        raise TypeError(f"{fn}: scales and biases must be float32, bfloat16 or float16 of one type "
+                        f"(got {scales.dtype} and {biases.dtype})")
+    shape = packed.shape
+    if not cols or cols * bits != shape[-1] * 32:
+        raise AssertionError(f"{fn}: x has {cols} columns, the words hold {shape[-1] * 32 // bits}")
+    n = scales.shape[-1] if scales.dim() else 0
+    group = cols // n if n and cols % n == 0 else 0
+    if group not in _AFFINE_GROUPS:
+        raise ValueError(f"{fn}: groups of 32, 64 or 128 values (got {n} scales for {cols})")
+    if scales.shape[:-1] != shape[:-1] or biases.shape != scales.shape:
+        raise AssertionError(f"{fn}: scales and biases must be {(*shape[:-1], n)} "
+                             f"(got {tuple(scales.shape)} and {tuple(biases.shape)})")
+    return group
+
+
+def affine_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
+                  bits: int, offsets=None, row_index: torch.Tensor | None = None,
+                  validate: bool = True) -> torch.Tensor:
+    """``grouped_linear`` with affine weights w = q * scale + bias.
+
+    x: [T, K] bf16 or f16, packed: [G, N, K * bits / 32] words as ``packing.pack_q``
+    lays them out (bits 2, 4 or 8), scales and biases: [G, N, K / group] float32,
+    bf16 or f16, as ``gptq.solve_gptq`` and ``grid.rtn_quantize`` return them, for
+    groups of 32, 64 or 128 values; without offsets all three lack the leading G.
+    -> [entries, N] of x's type. fp32 sums, rounded once; the weights are not rounded.
+    A row that holds an infinity, or values beyond 1e34, may give results that are no
+    numbers where the product with the decoded weight would be infinite.
+    """
+    fn = "affine_linear"
+    tracked = _tracked(fn, x, scales, biases)
+    if x.dtype not in _HALF:
+        raise TypeError(f"{fn}: expects bfloat16 or float16 rows (got {x.dtype})")
+    _rows2(fn, "x", x)
+    w = _weight3(fn, packed, offsets)
+    group = affine_group(fn, int(x.shape[1]), bits, packed, scales, biases)
+    G, N, _ = w.shape
+    dev = _device(x, packed, scales)
+    xd = _pitched(x, dev)
+    wd, sd, bd = _dense(w, dev), _dense(scales, dev), _dense(biases, dev)
+    off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    if M and N:
+        nat.launch(dev, "mgq_affine_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0],
+                   _ld(xd), nat.ptr(idx), M, wd.data_ptr(), sd.data_ptr(), bd.data_ptr(),
+                   nat.dtype_code(scales.dtype), bits, group, G, N, xd.shape[1], nat.ptr(off),
+                   y.data_ptr())
+    y = _home(y, x)
+    return _NoGradient.apply(fn, y, x, scales, biases) if tracked else y
 
 
 def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -76,6 +76,21 @@ def decode(q, scales, mode):
     return v * torch.exp2(scales.double() - 127).repeat_interleave(32, dim=-1)
 
 
+def affine(q, scales, biases):
+    """Codes [..., K], scales and biases [..., K / group] -> (float64 weights, the
+    magnitudes |q scale| + |bias| of their two terms)."""
+    group = q.shape[-1] // scales.shape[-1]
+    s, b = (t.double().repeat_interleave(group, dim=-1) for t in (scales, biases))
+    return q.double() * s + b, q.double() * s.abs() + b.abs()
+
+
+def affine_forward(x, q, scales, biases, offsets=None, row_index=None):
+    """(y, the sum of |x| (|q scale| + |bias|))."""
+    w, m = affine(q, scales, biases)
+    return (forward(x, w, offsets, row_index)[0],
+            forward(x.double().abs(), m, offsets, row_index)[0])
+
+
 def quantize_rows(x):
     """(codes, scales) with the quotients rounded to fp32 as defined."""
     f = x.double()
