@@ -438,6 +438,36 @@ int mgq_linear_choice(int product, const void* X, int64_t ldx, int64_t n_entries
                       int64_t n_groups, int64_t N, int64_t K, int64_t ldw, int64_t w_group,
                       int grouped, int32_t* tile);
 
+/* A routed layer's experts for a few rows -- mlx_gptq/experts.py ExpertMLP.decode:
+ *   out[t] = sum_j weights[t, j] down[e] act,  e = index[t, j],
+ *   act = silu(gate[e] x[t]) * (up[e] x[t]), rounded to dtype,
+ * sums in fp32, out rounded once. X: [T, H] of dtype (bf16 / f16; pitch ldx), index:
+ * [T, k] of 32 or 64 bits, weights: f32 [T, k], out: [T, H] of dtype. T <= 64, k <=
+ * 16. Assignments to no expert (outside [0, n_experts)) add nothing. `up` holds an
+ * expert's I gate rows, then its I up rows: [n_experts, 2 I, H]; `down`: [n_experts,
+ * H, I]. Each has a format of its own: dense (dtype, pitch ld and distance of two
+ * experts in elements), MXFP words with scale bytes (bf16 rows; group size 32), or
+ * affine words with scales and biases of param_dtype for groups of 32, 64 or 128
+ * values, laid out as in mgq_mxfp_linear and mgq_affine_linear. Two launches; every
+ * result is the same from call to call. The workspace is 256-byte aligned. */
+enum {
+  MGQ_WEIGHT_DENSE = 0,
+  MGQ_WEIGHT_MXFP4 = 1,
+  MGQ_WEIGHT_MXFP8 = 2,
+  MGQ_WEIGHT_AFFINE2 = 3,
+  MGQ_WEIGHT_AFFINE4 = 4,
+  MGQ_WEIGHT_AFFINE8 = 5
+};
+int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64_t I);
+int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t ldx, const void* index,
+                       int index_bits, const float* weights, int64_t k, int64_t n_experts, int64_t H,
+                       int64_t I, const void* up, int up_format, int64_t up_ld, int64_t up_expert,
+                       const void* up_scales, const void* up_biases, int64_t up_group,
+                       const void* down, int down_format, int64_t down_ld, int64_t down_expert,
+                       const void* down_scales, const void* down_biases, int64_t down_group,
+                       int param_dtype, void* out, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,85 @@
+// A routed layer's experts for a few rows, in two launches (experts_up.hip and
+// experts_down.hip):
+//
+//   act[i] = silu(Wg[e] x[t]) * (Wu[e] x[t])          for entry i = t k + j, e = index[i]
+//   out[t] = sum_j weights[t, j] Wd[e] act[t k + j]
+//
+// Entries whose expert is outside [0, E) add nothing.
+#pragma once
+
+#include "few_core.h"
+
+namespace mgq {
+
+constexpr int kDecodeRows = 64;     // rows of a call
+constexpr int kDecodeTopK = 16;     // experts of a row
+constexpr int kDecodeEntries = kDecodeRows * kDecodeTopK;
+
+struct DecodeArgs {
+  const char* x;
+  int64_t ldx;           // bytes
+  const void* index;     // [T, k] int32 or int64
+  const float* weights;  // [T, k]
+  FewWeight up, down;    // [E, 2 I, H] (gate rows first), [E, H, I]
+  char* act;             // workspace: [T k, I] of x's type
+  int32_t* plan;         // workspace: see decode_plan (experts_up.hip)
+  uint16_t* out;         // [T, H]
+  int index64;
+  int T, k, n;           // n = T k
+  int E, H, I;
+  int type;              // kBF16 or kF16
+};
+
+// The plan that the first launch leaves for the second one (T > 1): plan[0] items,
+// then the items, then the entries. An item is one expert with up to kDecodeItem of its
+// rows; entries of an item are (entry of act, weight as bits), each row once.
+struct DecodeItem {
+  int32_t expert;
+  uint16_t first, count;
+};
+struct DecodeEntry {
+  int32_t entry;
+  float weight;
+};
+constexpr int kDecodeItem = 16;
+constexpr int kDecodePlanHead = 16;  // bytes
+inline int64_t decode_plan_bytes(int64_t n) { return kDecodePlanHead + n * 16; }
+inline int64_t decode_act_bytes(int64_t n, int64_t I) { return (n * I * 2 + 255) / 256 * 256; }
+
+__device__ __forceinline__ int decode_expert(const DecodeArgs& a, int i) {
+  if (a.index64) {
+    const int64_t e = static_cast<const int64_t*>(a.index)[i];
+    return e >= 0 && e < a.E ? static_cast<int>(e) : -1;
+  }
+  const int32_t e = static_cast<const int32_t*>(a.index)[i];
+  return e >= 0 && e < a.E ? e : -1;
+}
+
+int decode_up(const DecodeArgs& a, int format, hipStream_t s, const char* what);
+int decode_down(const DecodeArgs& a, int format, hipStream_t s, const char* what);
+
+// f(FewFmt) for a weight's format, the rows' type and the scales' size.
+template <typename Fn>
+int decode_dispatch(int format, int type, int param_type, Fn&& f) {
+  const bool wide = param_type == kF32;
+#define MGQ_AFFINE(FMT)                                        \
+  if (type == kF16) {                                          \
+    if (wide) return f(FewFmt<FMT, kF16, 4>{});                \
+    return f(FewFmt<FMT, kF16, 2>{});                          \
+  }                                                            \
+  if (wide) return f(FewFmt<FMT, kBF16, 4>{});                 \
+  return f(FewFmt<FMT, kBF16, 2>{});
+  switch (format) {
+    case kFewDense:
+      if (type == kF16) return f(FewFmt<kFewDense, kF16>{});
+      return f(FewFmt<kFewDense, kBF16>{});
+    case kFewMx4: return f(FewFmt<kFewMx4, kBF16>{});
+    case kFewMx8: return f(FewFmt<kFewMx8, kBF16>{});
+    case kFewAf2: MGQ_AFFINE(kFewAf2)
+    case kFewAf4: MGQ_AFFINE(kFewAf4)
+    default: MGQ_AFFINE(kFewAf8)
+  }
+#undef MGQ_AFFINE
+}
+
+}  // namespace mgq

@@ -1,0 +1,166 @@
+// First launch of a routed layer for a few rows (experts_decode.h): gate and up
+// projection of every entry and their activation, and the plan for the second launch.
+//
+// A workgroup takes 16 gate rows and the 16 up rows beside them of one expert, with all
+// entries of that expert: its weight is read once (again for every further 16 entries).
+// The expert is that of list entry `slot`, whose workgroups end at once if an earlier
+// entry has the same one, or, where there are more entries than experts, expert `slot`.
+// The list is short enough for every wave to look through all of it.
+#include "experts_decode.h"
+
+namespace mgq {
+namespace {
+
+// One workgroup of 256: the entries in the experts' order. Thread e counts expert e's
+// rows by walking the list, the counts are summed up over the experts, and a second walk
+// writes. A row that names an expert twice is one entry with the sum of its weights.
+__device__ void decode_plan(const DecodeArgs& a, int16_t* ids, uint32_t* carry) {
+  typedef int16_t ids8_t __attribute__((ext_vector_type(8)));
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  DecodeItem* items = reinterpret_cast<DecodeItem*>(a.plan + kDecodePlanHead / 4);
+  DecodeEntry* entries = reinterpret_cast<DecodeEntry*>(items + a.n);
+  const uint32_t inv_k = 65536u / a.k + 1;  // i / k = i inv_k >> 16 (i < 1024, k <= 16)
+  // f(entry, row) for the entries of this round's expert `tid`
+  auto walk = [&](auto&& f) {
+    for (int i = 0; i < a.n; i += 8) {
+      const ids8_t v = *reinterpret_cast<const ids8_t*>(ids + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (v[j] == tid) f(i + j, static_cast<int>((i + j) * inv_k >> 16));
+    }
+  };
+  uint32_t base = 0;  // items << 16 | entries of the experts before this round's
+  for (int e0 = 0; e0 < a.E; e0 += 256) {
+    __syncthreads();
+    // (relative to the round, so that 16 bits hold any number of experts)
+    for (int i = tid; i < ((a.n + 7) & ~7); i += 256) {
+      const int e = i < a.n ? decode_expert(a, i) - e0 : -1;
+      ids[i] = static_cast<int16_t>(e >= 0 && e < 256 ? e : -1);
+    }
+    __syncthreads();
+    uint32_t count = 0;
+    int last = -1;
+    walk([&](int, int row) {
+      count += row != last;
+      last = row;
+    });
+    const uint32_t own = (count + kDecodeItem - 1) / kDecodeItem << 16 | count;
+    const uint32_t incl = lin_wave_scan(own);
+    if (lane == 63) carry[wave] = incl;
+    __syncthreads();
+    uint32_t before = base;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += carry[w];
+      base += carry[w];
+    }
+    before += incl - own;
+    int item = before >> 16, at = before & 0xffff;
+    for (uint32_t c = 0; c < count; c += kDecodeItem)
+      items[item++] = DecodeItem{e0 + tid, static_cast<uint16_t>(at + c),
+                                 static_cast<uint16_t>(count - c < kDecodeItem ? count - c : kDecodeItem)};
+    last = -1;
+    --at;
+    walk([&](int i, int row) {
+      const float w = a.weights[i];
+      if (row != last) {
+        last = row;
+        entries[++at] = DecodeEntry{i, w};
+      } else {
+        entries[at].weight += w;
+      }
+    });
+  }
+  if (tid == 0) a.plan[0] = static_cast<int32_t>(base >> 16);
+}
+
+constexpr int kWaves = 4;
+
+template <class F, int NE, int BATCH>
+__global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs a) {
+  constexpr int BM = NE == 1 ? 4 : 16;
+  __shared__ __attribute__((aligned(16))) int16_t list[kDecodeEntries];
+  __shared__ uint32_t carry[kWaves];
+  __shared__ lin_f32x4_t part[kWaves * 2 * 64];
+  int bid = blockIdx.x;
+  if (a.T > 1) {
+    if (bid == 0) {
+      decode_plan(a, list, carry);
+      return;
+    }
+    --bid;
+  }
+  const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (a.I + 15) / 16;
+  const int slot = bid / tiles, p = (bid - slot * tiles) * 16 + r16;
+  const bool by_expert = a.n > a.E;
+  const int expert = by_expert ? slot : __builtin_amdgcn_readfirstlane(decode_expert(a, slot));
+  if (expert < 0) return;
+  int count = 0;
+  for (int c = 0; c < a.n; c += 64) {
+    const bool hit = c + lane < a.n && decode_expert(a, c + lane) == expert;
+    const uint64_t mask = __ballot(hit);
+    if (!by_expert && count == 0 && mask && c + __builtin_ctzll(mask) < slot) return;
+    if (wave == 0 && hit)
+      list[count + __popcll(mask & ((uint64_t(1) << lane) - 1))] = static_cast<int16_t>(c + lane);
+    count += __popcll(mask);
+  }
+  if (count == 0) return;
+  __syncthreads();
+
+  FewRow row[2];
+  const int pc = p < a.I ? p : a.I - 1;
+  row[0] = few_row<F>(a.up, expert, pc, a.H);
+  row[1] = few_row<F>(a.up, expert, a.I + pc, a.H);
+  const int steps = (a.H + kFewStep - 1) / kFewStep;
+  for (int base = 0; base < count; base += BM) {
+    const int j = base + (NE == 1 ? r16 >> 2 : r16);
+    const int entry = list[j < count ? j : count - 1];
+    const char* const x[1] = {a.x + entry / a.k * a.ldx};
+    lin_f32x4_t acc[2][1];
+    few_product<F, 2, 1, NE, BATCH>(row, a.up, x, a.H, steps * wave / kWaves,
+                                    steps * (wave + 1) / kWaves, acc);
+    part[(2 * wave) * 64 + lane] = acc[0][0];
+    part[(2 * wave + 1) * 64 + lane] = acc[1][0];
+    __syncthreads();
+    if (wave == 0) {
+      lin_f32x4_t gate = part[lane], up = part[64 + lane];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        const lin_f32x4_t g = part[2 * w * 64 + lane], u = part[(2 * w + 1) * 64 + lane];
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          gate[e] += g[e];
+          up[e] += u[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const int i = base + (NE == 1 ? quad : 4 * quad + e);
+        // (16 bits: what the second product's MFMA takes)
+        if (i < count && p < a.I)
+          reinterpret_cast<uint16_t*>(a.act)[static_cast<int64_t>(list[i]) * a.I + p] =
+              lin_round16(gate[e] / (1.0f + expf(-gate[e])) * up[e], a.type);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+int decode_up(const DecodeArgs& a, int format, hipStream_t s, const char* what) {
+  const int64_t slots = a.n > a.E ? a.E : a.n;
+  const int64_t grid = slots * ceil_div(a.I, 16) + (a.T > 1);
+  MGQ_REQUIRE(grid < int64_t(1) << 24, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  return decode_dispatch(format, a.type, a.up.type, [&](auto f) {
+    using F = decltype(f);
+    if (a.T <= 4)
+      decode_up_kernel<F, 1, 2><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
+    else
+      decode_up_kernel<F, 4, 2><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
+    return check_launch(what);
+  });
+}
+
+}  // namespace mgq

@@ -34,6 +34,14 @@ MODE_AFFINE = 0
 MODE_MXFP4 = 1
 MODE_MXFP8 = 2
 
+# weight formats of mgq_experts_decode
+WEIGHT_DENSE = 0
+WEIGHT_MXFP4 = 1
+WEIGHT_MXFP8 = 2
+WEIGHT_AFFINE2 = 3
+WEIGHT_AFFINE4 = 4
+WEIGHT_AFFINE8 = 5
+
 CLIP_MINMAX = 0
 CLIP_MSE = 1
 
@@ -104,10 +112,16 @@ SIGNATURES: dict[str, list] = {
                         _I64, _VP, _VP, _INT, _VP],
     "mgq_affine_linear": [_VP, _INT, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _INT, _INT, _I64, _I64,
                           _I64, _I64, _VP, _VP, _VP],
+    # experts.py
+    "mgq_experts_decode_workspace_size": [_I64, _I64, _I64],
+    "mgq_experts_decode": [_VP, _INT, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _I64, _I64, _VP, _INT,
+                           _I64, _I64, _VP, _VP, _I64, _VP, _INT, _I64, _I64, _VP, _VP, _I64, _INT,
+                           _VP, _VP, _I64, _VP],
     "mgq_linear_choice": [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64, _INT, _VP],
 }
 
 _RESTYPES = {
+    "mgq_experts_decode_workspace_size": ctypes.c_int64,
     "mgq_grouped_wgrad_workspace_size": ctypes.c_int64,
     "mgq_rows_sum_workspace_size": ctypes.c_int64,
     "mgq_last_error": ctypes.c_char_p,

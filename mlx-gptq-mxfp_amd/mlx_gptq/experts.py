@@ -10,11 +10,16 @@ with weights that are
   the forward that feeds a calibration's next layer);
 * ``"mxfp4"`` / ``"mxfp8"``: the solver's or ``grid.rtn_quantize_mxfp``'s codes,
   packed;
+* ``"affine"``: 2-, 4- or 8-bit codes of the affine grid, packed, with a scale and a
+  bias for each group;
 * ``"int8"``: 8-bit weights with a scale for each output channel, rows quantized
   to 8 bits on the way into each product.
 
 Only dense experts are differentiable; in the other formats a backward that reaches
 the rows raises.
+
+``ExpertMLP.decode`` is the same layer for up to 64 rows in two launches, where
+``forward`` sorts the assignments and takes about 25.
 
 No call waits for the device: the routing stays there.
 """
@@ -26,6 +31,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
+from . import _native as nat
 from . import grid, linear, packing
 
 
@@ -59,12 +65,12 @@ def route(top_k_index: torch.Tensor, num_experts: int) -> Routing:
 class ExpertMLP:
     """Experts gate_up [E, 2 I, H] and down [E, H, I] in one of the formats.
 
-    ``gate_up`` and ``down`` are the weight itself (dense) or a pair: packed words
+    ``gate_up`` and ``down`` are the weight itself (dense), a pair: packed words
     and E8M0 scale bytes (mxfp4, mxfp8), int8 weights and fp32 channel scales
-    (int8), as linear.py takes them.
+    (int8), or packed words, scales and biases (affine), as linear.py takes them.
     """
 
-    MODES = ("dense", "mxfp4", "mxfp8", "int8")
+    MODES = ("dense", "mxfp4", "mxfp8", "int8", "affine")
 
     def __init__(self, gate_up, down, mode: str = "dense"):
         if mode not in self.MODES:
@@ -77,27 +83,34 @@ class ExpertMLP:
         self.num_experts = int(first.shape[0])
 
     @classmethod
-    def from_weights(cls, gate_up: torch.Tensor, down: torch.Tensor, mode: str = "dense"):
+    def from_weights(cls, gate_up: torch.Tensor, down: torch.Tensor, mode: str = "dense",
+                     bits: int = 4, group_size: int = 64):
         """Weights [E, out, in] rounded to the nearest in `mode`, without
-        calibration."""
+        calibration. ``bits`` and ``group_size`` are the affine grid's."""
         if mode == "dense":
             return cls(gate_up, down)
-        return cls(cls._nearest(gate_up, mode), cls._nearest(down, mode), mode)
+        return cls(*(cls._nearest(w, mode, bits, group_size) for w in (gate_up, down)), mode)
 
     @classmethod
-    def from_codes(cls, gate_up, down, mode: str):
+    def from_codes(cls, gate_up, down, mode: str, bits: int | None = None):
         """The solver's results: (q uint8 [E, out, in], scale bytes [E, out, in /
         32]) of each parameter, as ``gptq.solve_gptq`` returns them first and
-        second."""
-        if mode not in ("mxfp4", "mxfp8"):
-            raise ValueError(f"not a microscaling mode: {mode}")
-        bits = grid.mode_defaults(mode)[1]
-        return cls(*((packing.pack_q(q, bits), s) for q, s in (gate_up, down)), mode)
+        second; affine codes of ``bits`` bits (4 unless given) with scales and
+        biases, which it returns second and third."""
+        if mode not in ("mxfp4", "mxfp8", "affine"):
+            raise ValueError(f"not a grid of the solver: {mode}")
+        default = grid.mode_defaults(mode)[1]
+        if mode != "affine" and bits not in (None, default):
+            raise ValueError(f"{mode} codes have {default} bits (got {bits})")
+        return cls(*((packing.pack_q(w[0], bits or default), *w[1:]) for w in (gate_up, down)), mode)
 
     @staticmethod
-    def _nearest(w: torch.Tensor, mode: str):
+    def _nearest(w: torch.Tensor, mode: str, bits: int, group_size: int):
         if mode == "int8":
             return linear.quantize_rows_int8(w.detach())
+        if mode == "affine":
+            q, s, b, _ = grid.rtn_quantize(w, bits, group_size, storage_dtype=w.dtype)
+            return packing.pack_q(q, bits), s, b
         q, s, _, _ = grid.rtn_quantize_mxfp(w, mode)
         return packing.pack_q(q, grid.mode_defaults(mode)[1]), s
 
@@ -108,6 +121,9 @@ class ExpertMLP:
             q, s = linear.quantize_rows_int8(x)
             return linear.int8_linear(q, s, *weight, out_dtype=x.dtype, offsets=offsets,
                                       row_index=row_index, validate=False)
+        if self.mode == "affine":
+            bits = 32 * weight[0].shape[-1] // max(x.shape[1], 1)
+            return linear.affine_linear(x, *weight, bits, offsets, row_index, validate=False)
         return linear.mxfp_linear(x, *weight, self.mode, offsets, row_index, validate=False)
 
     def forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
@@ -127,3 +143,87 @@ class ExpertMLP:
         return (y * weights.unsqueeze(-1)).sum(1).to(hidden_states.dtype)
 
     __call__ = forward
+
+    def _decode_weight(self, weight, out_rows: int, cols: int, dtype: torch.dtype,
+                       dev: torch.device):
+        """(tensors kept alive, the weight's arguments of mgq_experts_decode, its scales'
+        type)."""
+        fn, E = "ExpertMLP.decode", self.num_experts
+        if self.mode == "dense":
+            if weight.dtype != dtype:
+                raise TypeError(f"{fn}: expects rows of the weights' type (got {dtype} and {weight.dtype})")
+            if weight.shape != (E, out_rows, cols):
+                raise AssertionError(f"{fn}: expects weights {(E, out_rows, cols)} "
+                                     f"(got {tuple(weight.shape)})")
+            w = linear._pitched(weight, dev)
+            return (w,), (w.data_ptr(), nat.WEIGHT_DENSE, linear._ld(w), w.stride(0), None, None, 0), None
+        bits = 32 * weight[0].shape[-1] // max(cols, 1)
+        if weight[0].shape[:-1] != (E, out_rows):
+            raise AssertionError(f"{fn}: expects weights {(E, out_rows, cols)} "
+                                 f"(words {tuple(weight[0].shape)})")
+        if self.mode == "affine":
+            group = linear.affine_group(fn, cols, bits, *weight)
+            code = {2: nat.WEIGHT_AFFINE2, 4: nat.WEIGHT_AFFINE4, 8: nat.WEIGHT_AFFINE8}[bits]
+        else:
+            linear.check_mxfp(fn, cols, self.mode, *weight)
+            group, code = 32, nat.WEIGHT_MXFP4 if self.mode == "mxfp4" else nat.WEIGHT_MXFP8
+        t = tuple(linear._dense(w, dev) for w in weight)
+        biases = t[2].data_ptr() if len(t) > 2 else None
+        return t, (t[0].data_ptr(), code, 0, 0, t[1].data_ptr(), biases, group), t[1].dtype
+
+    def decode(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
+               top_k_weights: torch.Tensor) -> torch.Tensor:
+        """``forward`` for up to 64 rows with up to 16 experts each, in two launches that
+        read the weights of the rows' experts once. [T, H] -> [T, H].
+
+        The activation is rounded to the rows' type, everything else is fp32 until the
+        result is rounded once (``forward`` also rounds between its products, so the two
+        agree within the type's precision only). Assignments to no expert add nothing. The
+        order of the sums depends on the sizes and the routing alone. int8 experts, whose
+        rows are quantized for each product, have ``forward`` only. Not differentiable.
+        """
+        fn = "ExpertMLP.decode"
+        if self.mode == "int8":
+            raise ValueError(f"{fn}: int8 experts are not supported, use forward")
+        x = hidden_states
+        dense = (self.gate_up, self.down) if self.mode == "dense" else ()
+        tracked = linear._tracked(fn, x, top_k_weights, *dense)
+        if x.dtype not in linear._HALF or (self.mode[:2] == "mx" and x.dtype is not torch.bfloat16):
+            raise TypeError(f"{fn}: expects bfloat16 rows, or float16 ones without MXFP weights "
+                            f"(got {x.dtype})")
+        linear._rows2(fn, "hidden_states", x)
+        T, H = x.shape
+        if top_k_index.dim() != 2 or top_k_index.shape[0] != T or not linear._integers(top_k_index):
+            raise ValueError(f"{fn}: top_k_index must be integers [{T}, k] "
+                             f"(got {tuple(top_k_index.shape)})")
+        k = top_k_index.shape[1]
+        if top_k_weights.shape != top_k_index.shape or not top_k_weights.dtype.is_floating_point:
+            raise ValueError(f"{fn}: top_k_weights must be numbers {(T, k)} "
+                             f"(got {tuple(top_k_weights.shape)})")
+        if T > 64 or not 1 <= k <= 16:
+            raise ValueError(f"{fn}: up to 64 rows with 1 to 16 experts each (got {(T, k)}); "
+                             "forward takes any number")
+        dev = linear._device(x, *(dense or self.gate_up[:1]))
+        first = self.gate_up if dense else self.gate_up[0]
+        inner = first.shape[1] // 2
+        up, up_args, param = self._decode_weight(self.gate_up, 2 * inner, H, x.dtype, dev)
+        down, down_args, other = self._decode_weight(self.down, H, inner, x.dtype, dev)
+        if param != other:
+            raise TypeError(f"{fn}: the scales of gate_up and down differ in type ({param}, {other})")
+        xd = linear._pitched(x, dev)
+        index = top_k_index
+        if index.dtype is not torch.int64:
+            index = linear._int32(index)
+        index = linear._dense(index, dev)
+        weights = linear._dense(top_k_weights.float(), dev)
+        out = torch.empty(T, H, dtype=x.dtype, device=dev)
+        if out.numel():
+            size = nat.load().mgq_experts_decode_workspace_size(T, k, inner)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
+            params = nat.DTYPE_BF16 if self.mode != "affine" else nat.dtype_code(param)
+            nat.launch(dev, "mgq_experts_decode", xd.data_ptr(), nat.dtype_code(x.dtype), T,
+                       linear._ld(xd), index.data_ptr(), 8 * index.element_size(), weights.data_ptr(),
+                       k, self.num_experts, H, inner, *up_args, *down_args, params, out.data_ptr(),
+                       ws.data_ptr(), size)
+        out = linear._home(out, x)
+        return linear._NoGradient.apply(fn, out, x, top_k_weights, *dense) if tracked else out

@@ -326,6 +326,19 @@ def grouped_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets=None,
     return _NoGradient.apply(fn, dw, dy, x) if tracked else dw
 
 
+def check_mxfp(fn: str, cols: int, mode: str, packed: torch.Tensor, scales: torch.Tensor) -> None:
+    """The tensors of an MXFP weight [..., N, cols]."""
+    if packed.dtype not in _WORDS or scales.dtype is not torch.uint8:
+        raise TypeError(f"{fn}: expects 32-bit words and uint8 scales "
+                        f"(got {packed.dtype} and {scales.dtype})")
+    *lead, words = packed.shape
+    K = words * 32 // _MX_MODES[mode][0]
+    if cols != K or K % 32:
+        raise AssertionError(f"{fn}: x has {cols} columns, the words hold {K} (a multiple of 32)")
+    if scales.shape != (*lead, K // 32):
+        raise AssertionError(f"{fn}: scales must be {(*lead, K // 32)} (got {tuple(scales.shape)})")
+
+
 def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mode: str,
                 offsets=None, row_index: torch.Tensor | None = None,
                 validate: bool = True) -> torch.Tensor:
@@ -340,21 +353,14 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
     tracked = _tracked(fn, x)
     if mode not in _MX_MODES:
         raise ValueError(f"not a microscaling mode: {mode}")
-    bits, code = _MX_MODES[mode]
+    code = _MX_MODES[mode][1]
     if x.dtype is not torch.bfloat16:
         raise TypeError(f"{fn}: expects bfloat16 rows (got {x.dtype})")
-    if packed.dtype not in _WORDS or scales.dtype is not torch.uint8:
-        raise TypeError(f"{fn}: expects 32-bit words and uint8 scales "
-                        f"(got {packed.dtype} and {scales.dtype})")
     _rows2(fn, "x", x)
     w, s = _weight3(fn, packed, offsets), _weight3(fn, scales, offsets)
-    G, N, words = w.shape
-    K = words * 32 // bits
-    if x.shape[1] != K or K % 32:
-        raise AssertionError(f"{fn}: x has {x.shape[1]} columns, the words hold {K} "
-                             "(a multiple of 32)")
-    if s.shape != (G, N, K // 32):
-        raise AssertionError(f"{fn}: scales must be {(G, N, K // 32)} (got {tuple(s.shape)})")
+    K = int(x.shape[1])
+    check_mxfp(fn, K, mode, w, s)
+    G, N, _ = w.shape
     dev = _device(x, packed, scales)
     xd = _pitched(x, dev)
     wd, sd = _dense(w, dev), _dense(s, dev)
