@@ -438,6 +438,24 @@ int mgq_linear_choice(int product, const void* X, int64_t ldx, int64_t n_entries
                       int64_t n_groups, int64_t N, int64_t K, int64_t ldw, int64_t w_group,
                       int grouped, int32_t* tile);
 
+/* The router's choice -- mlx_gptq/experts.py top_k_softmax: the k largest logits of
+ * each row, the lower index first among equal ones (a NaN counts as the largest, both
+ * zeros as equal), and w_j = exp(l_j - max l) / Z, Z the sum over the chosen
+ * (renormalize != 0) or over all experts, in fp32. Logits of -infinity are never
+ * chosen: where fewer than k are left, index is -1 and the weight 0. logits: [T, E] of
+ * dtype (f32/bf16/f16; pitch ld), index: i64 [T, k], weights: f32 [T, k]. E <= 1024,
+ * k <= 16 and E. */
+int mgq_top_k_softmax(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k,
+                      int renormalize, int64_t* index, float* weights, void* stream);
+
+/* dlogits [T, E] of dtype from dw = f32 [T, k], the gradient of the weights:
+ * renormalize: w_j (dw_j - sum_i w_i dw_i) where expert j was chosen, 0 elsewhere;
+ * otherwise [e chosen] w_e dw_e - p_e sum_i w_i dw_i with p the softmax of the row.
+ * Indexes outside [0, E) add nothing. */
+int mgq_top_k_softmax_grad(const float* dw, const void* logits, int dtype, int64_t T, int64_t E,
+                           int64_t ld, const int64_t* index, int64_t k, int renormalize,
+                           void* dlogits, void* stream);
+
 /* A routed layer's experts for a few rows -- mlx_gptq/experts.py ExpertMLP.decode:
  *   out[t] = sum_j weights[t, j] down[e] act,  e = index[t, j],
  *   act = silu(gate[e] x[t]) * (up[e] x[t]), rounded to dtype,

@@ -113,6 +113,8 @@ SIGNATURES: dict[str, list] = {
     "mgq_affine_linear": [_VP, _INT, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _INT, _INT, _I64, _I64,
                           _I64, _I64, _VP, _VP, _VP],
     # experts.py
+    "mgq_top_k_softmax": [_VP, _INT, _I64, _I64, _I64, _I64, _INT, _VP, _VP, _VP],
+    "mgq_top_k_softmax_grad": [_VP, _VP, _INT, _I64, _I64, _I64, _VP, _I64, _INT, _VP, _VP],
     "mgq_experts_decode_workspace_size": [_I64, _I64, _I64],
     "mgq_experts_decode": [_VP, _INT, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _I64, _I64, _VP, _INT,
                            _I64, _I64, _VP, _VP, _I64, _VP, _INT, _I64, _I64, _VP, _VP, _I64, _INT,

@@ -18,6 +18,8 @@ with weights that are
 Only dense experts are differentiable; in the other formats a backward that reaches
 the rows raises.
 
+``top_k_softmax`` is the router's choice that both take, with its gradient.
+
 ``ExpertMLP.decode`` is the same layer for up to 64 rows in two launches, where
 ``forward`` sorts the assignments and takes about 25.
 
@@ -33,6 +35,92 @@ import torch.nn.functional as F
 
 from . import _native as nat
 from . import grid, linear, packing
+
+
+MAX_TOP_K = 16
+MAX_EXPERTS = 1024
+
+
+def _check_logits(fn: str, logits: torch.Tensor, k: int) -> None:
+    if logits.dtype not in linear._FLOATS:
+        raise TypeError(f"{fn}: expects float32, bfloat16 or float16 logits (got {logits.dtype})")
+    linear._rows2(fn, "logits", logits)
+    E = logits.shape[1]
+    if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= min(E, MAX_TOP_K):
+        raise ValueError(f"{fn}: 1 to {MAX_TOP_K} of up to {MAX_EXPERTS} experts (got {k} of {E})")
+
+
+def _choose(logits: torch.Tensor, k: int, renormalize: bool):
+    dev = linear._device(logits)
+    x = linear._pitched(logits, dev)
+    T, E = x.shape
+    index = torch.empty(T, k, dtype=torch.int64, device=dev)
+    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
+    if T:
+        nat.launch(dev, "mgq_top_k_softmax", x.data_ptr(), nat.dtype_code(x.dtype), T, E,
+                   linear._ld(x), k, int(renormalize), index.data_ptr(), weights.data_ptr())
+    return linear._home(index, logits), linear._home(weights, logits)
+
+
+class _TopKSoftmax(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, renormalize):
+        index, weights = _choose(logits, k, renormalize)
+        ctx.renormalize = renormalize
+        ctx.save_for_backward(logits, index)
+        ctx.mark_non_differentiable(index)
+        return index, weights
+
+    @staticmethod
+    def backward(ctx, _, dw):
+        logits, index = ctx.saved_tensors
+        return top_k_softmax_grad(dw, logits, index, ctx.renormalize), None, None
+
+
+def top_k_softmax(logits: torch.Tensor, k: int,
+                  renormalize: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """The router's choice: (index int64 [T, k], weights float32 [T, k]).
+
+    The k largest logits of each row in descending order, the lower index first among
+    equal ones (a NaN counts as the largest), and the softmax's weights of these: over
+    the chosen (``renormalize``) or over all experts. logits: [T, E] float32, bf16 or
+    f16, E up to 1024, k up to 16. Logits of -infinity mask experts out: they are never
+    chosen, and where a row has fewer than k others the index is -1 (which ``route``,
+    ``ExpertMLP.forward`` and ``.decode`` take as no expert) and the weight 0.
+
+    The weights are differentiable in the logits (``top_k_softmax_grad``, which has no
+    derivative itself). Nothing waits for the device.
+    """
+    k = int(k)
+    _check_logits("top_k_softmax", logits, k)
+    if linear._tracked("top_k_softmax", logits):
+        return _TopKSoftmax.apply(logits, k, bool(renormalize))
+    return _choose(logits, k, renormalize)
+
+
+def top_k_softmax_grad(dw: torch.Tensor, logits: torch.Tensor, index: torch.Tensor,
+                       renormalize: bool = True) -> torch.Tensor:
+    """Gradient of ``top_k_softmax``'s weights with respect to the logits: [T, E] of
+    their type, computed in fp32 and rounded once. dw: [T, k], index: the choice."""
+    fn = "top_k_softmax_grad"
+    tracked = linear._tracked(fn, dw, logits)
+    if index.dim() != 2 or not linear._integers(index):
+        raise ValueError(f"{fn}: index must be integers [T, k] (got {tuple(index.shape)})")
+    _check_logits(fn, logits, int(index.shape[1]))
+    T, E = logits.shape
+    k = index.shape[1]
+    if index.shape[0] != T or dw.shape != index.shape or not dw.dtype.is_floating_point:
+        raise ValueError(f"{fn}: dw and index must be {(T, k)} "
+                         f"(got {tuple(dw.shape)} and {tuple(index.shape)})")
+    dev = linear._device(logits, dw)
+    x = linear._pitched(logits, dev)
+    d, i = linear._dense(dw.float(), dev), linear._dense(index.to(torch.int64), dev)
+    out = torch.empty(T, E, dtype=x.dtype, device=dev)
+    if T:
+        nat.launch(dev, "mgq_top_k_softmax_grad", d.data_ptr(), x.data_ptr(), nat.dtype_code(x.dtype),
+                   T, E, linear._ld(x), i.data_ptr(), k, int(renormalize), out.data_ptr())
+    out = linear._home(out, logits)
+    return linear._NoGradient.apply(fn, out, dw, logits) if tracked else out
 
 
 @dataclass
