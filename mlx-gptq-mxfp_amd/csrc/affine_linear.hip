@@ -5,7 +5,7 @@
 //
 // Few rows: a workgroup computes 16 NQ entries (4 where NE = 1) x 16 NP weight rows; its
 // waves share the contraction and add their sums through LDS in wave order.
-#include "few_core.h"
+#include "gemv_core.h"
 #include "linear_few.h"
 
 namespace mgq {
@@ -62,6 +62,71 @@ __global__ void __launch_bounds__(64 * WAVES) affine_few_kernel(const LinArgs a,
   }
 }
 
+// The same with the tiles of one entry block streamed: a workgroup takes 16 entries (4
+// where NE = 1) and `per` blocks of 16 weight rows, x stays in registers. The contraction
+// is at most 128 XS WAVES long.
+template <class F, int NE, int XS, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
+    affine_stream_kernel(const LinArgs a, const FewWeight w, const int per) {
+  constexpr int BM = NE == 1 ? 4 : 16;
+  __shared__ lin_f32x4_t part[2 * WAVES * 64];
+  LinTile t;
+  const int tiles = (a.np + 15) / 16;
+  if (!lin_find_tile<BM>(a, (tiles + per - 1) / per, &t)) return;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
+  const int t0 = t.pt * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  auto store = [&](int tile, const lin_f32x4_t& v) {
+    const int p = 16 * tile + r16;
+    if (p >= a.np) return;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const int64_t q = t.q0 + (NE == 1 ? quad : 4 * quad + e);
+      if (q < t.q_end)
+        reinterpret_cast<uint16_t*>(a.out)[q * a.ldo + p] = lin_round16(v[e], a.out_type);
+    }
+  };
+  if (t.g >= a.G) {  // (no group: zeros)
+    for (int i = t0 + (threadIdx.x >> 6); i < t1; i += WAVES) store(i, lin_f32x4_t{0, 0, 0, 0});
+    return;
+  }
+  const int64_t q = t.q0 + (NE == 1 ? r16 >> 2 : r16);
+  const char* x = a.Q + lin_row(a, q < t.q_end ? q : t.q_end - 1) * a.ldq;
+  few_stream<F, 1, NE, XS, WAVES>(
+      w, x, a.nc, t0, t1, part,
+      [&](int tile, FewRow(&row)[1]) {
+        const int p = 16 * tile + r16;
+        row[0] = few_row<F>(w, t.g, p < a.np ? p : a.np - 1, a.nc);
+      },
+      [&](int tile, const lin_f32x4_t(&sum)[1]) { store(tile, sum[0]); });
+}
+
+// Single entries: a wave takes one entry and R 64 / L weight rows.
+template <class F, int L, int R>
+__global__ void __launch_bounds__(256) affine_gemv_kernel(const LinArgs a, const FewWeight w) {
+  constexpr int RI = 64 / L, ROWS = R * RI;  // rows of a load, of a wave
+  LinTile t;
+  if (!lin_find_tile<1>(a, (a.np + 4 * ROWS - 1) / (4 * ROWS), &t)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int p0 = (4 * t.pt + wave) * ROWS;
+  if (p0 >= a.np) return;
+  auto first = [&](int r) { return p0 + r * RI < a.np - RI ? p0 + r * RI : a.np - RI; };
+  float acc[R], sum[gemv_sums<L, R>()];
+#pragma unroll
+  for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+  if (t.g < a.G)  // (no group: zeros)
+    gemv_add<F, L, R, 2>(acc, w, t.g, first, a.Q + lin_row(a, t.q0) * a.ldq, a.nc, 0,
+                         gemv_chunks<F, L>(a.nc));
+  gemv_reduce<L, R>(acc, sum);
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + t.q0 * a.ldo;
+#pragma unroll
+  for (int q = 0; q < gemv_sums<L, R>(); ++q)
+    if ((lane & 15) == q) {
+      const int r = gemv_row<L>(q, lane >> 4);
+      out[first(r / RI) + r % RI] = lin_round16(sum[q], a.out_type);
+    }
+}
+
 template <class F, int NP, int NQ, int NE, int WAVES, int BATCH>
 int launch_few(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
   const int64_t grid = lin_row_tiles(a, NE == 1 ? 4 : 16 * NQ) * ceil_div(a.np, 16 * NP);
@@ -70,9 +135,62 @@ int launch_few(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* 
       <<<static_cast<unsigned>(grid), 64 * WAVES, 0, s>>>(a, w);
   return check_launch(what);
 }
+template <class F>
+int launch_gemv(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
+  constexpr int R = 8;
+  const int lanes = gemv_lanes<F>(a.nc, a.np);
+  const int64_t grid = a.M * ceil_div(a.np, 4 * R * (64 / lanes));
+  MGQ_REQUIRE(grid < kLinFewGrid, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  const unsigned blocks = static_cast<unsigned>(grid);
+  if (lanes == 64) affine_gemv_kernel<F, 64, R><<<blocks, 256, 0, s>>>(a, w);
+  else if (lanes == 32) affine_gemv_kernel<F, 32, R><<<blocks, 256, 0, s>>>(a, w);
+  else affine_gemv_kernel<F, 16, R><<<blocks, 256, 0, s>>>(a, w);
+  return check_launch(what);
+}
+template <class F, int NE, int XS, int WAVES>
+int launch_stream(const LinArgs& a, const FewWeight& w, int per, hipStream_t s, const char* what) {
+  const int64_t grid = lin_row_tiles(a, NE == 1 ? 4 : 16) * ceil_div(ceil_div(a.np, 16), per);
+  MGQ_REQUIRE(grid < kLinFewGrid * 4 / WAVES, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  affine_stream_kernel<F, NE, XS, WAVES>
+      <<<static_cast<unsigned>(grid), 64 * WAVES, 0, s>>>(a, w, per);
+  return check_launch(what);
+}
+
+#ifdef AFFINE_FORCE
+extern "C" int mgq_force[4] = {0, 0, 0, 0};
+#endif
 
 template <class F>
 int run(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
+#ifdef AFFINE_FORCE
+  const int per = mgq_force[1];
+  switch (mgq_force[0]) {
+    case 1: return launch_few<F, 1, 1, 1, 4, 2>(a, w, s, what);
+    case 2: return launch_few<F, 1, 1, 4, 4, 2>(a, w, s, what);
+    case 3: return launch_few<F, 2, 4, 4, 4, 1>(a, w, s, what);
+    case 4: return launch_few<F, 2, 2, 4, 4, 1>(a, w, s, what);
+    case 5: return launch_gemv<F>(a, w, s, what);
+    case 10: return launch_stream<F, 1, 1, 8>(a, w, per, s, what);
+    case 11: return launch_stream<F, 1, 2, 8>(a, w, per, s, what);
+    case 12: return launch_stream<F, 1, 4, 8>(a, w, per, s, what);
+    case 13: return launch_stream<F, 1, 2, 16>(a, w, per, s, what);
+    case 14: return launch_stream<F, 1, 4, 4>(a, w, per, s, what);
+    case 20: return launch_stream<F, 4, 1, 8>(a, w, per, s, what);
+    case 21: return launch_stream<F, 4, 2, 8>(a, w, per, s, what);
+    case 22: return launch_stream<F, 4, 4, 8>(a, w, per, s, what);
+    case 23: return launch_stream<F, 4, 2, 16>(a, w, per, s, what);
+    case 24: return launch_stream<F, 4, 4, 4>(a, w, per, s, what);
+    case 30: case 31: case 32: case 33: {
+      LinArgs b = a;
+      b.P = w.p; b.Ps = reinterpret_cast<const uint8_t*>(w.s); b.Pb = reinterpret_cast<const uint8_t*>(w.b);
+      b.ldp = w.ld; b.p_group = w.group; b.p_shift = w.shift; b.p_type = w.type;
+      const int op = (F::XT == kF16 ? kOpAf2H : kOpAf2) + (F::W - kFewAf2);
+      const int r[4] = {256, 128, 64, 64}, c[4] = {256, 256, 256, 128};
+      const int i = mgq_force[0] - 30;
+      return lin_tile_affine(b, op, LinTileShape{r[i], c[i], mgq_force[2] != 0}, s, what);
+    }
+  }
+#endif
   if (a.M <= 4) return launch_few<F, 1, 1, 1, 4, 2>(a, w, s, what);
   if (a.M <= 16 || (a.offsets && a.M <= 16 * static_cast<int64_t>(a.G)))
     return launch_few<F, 1, 1, 4, 4, 2>(a, w, s, what);

@@ -7,7 +7,7 @@
 // Entries whose expert is outside [0, E) add nothing.
 #pragma once
 
-#include "few_core.h"
+#include "gemv_core.h"
 
 namespace mgq {
 

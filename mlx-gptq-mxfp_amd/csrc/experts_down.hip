@@ -5,14 +5,14 @@
 // workgroups. Its waves take the plan's items in turn (an expert with up to 16 of its
 // rows; parts of the contraction where there are fewer items than waves) and add what an
 // item gives each row into sums of their own in LDS; these are added in wave order. A
-// single row needs no plan: its items are its entries.
+// single row needs no plan: its items are its entries (gemv_core.h).
 #include "experts_decode.h"
 
 namespace mgq {
 namespace {
 
-template <class F, int NE, bool SINGLE, int WAVES, int BATCH>
-__global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArgs a, const int parts) {
+template <class F, int NE, int WAVES, int BATCH>
+__global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArgs a) {
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -20,48 +20,29 @@ __global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArg
   DecodeItem* items = reinterpret_cast<DecodeItem*>(lds + WAVES * a.T * 16);
   DecodeEntry* entries = reinterpret_cast<DecodeEntry*>(items + a.n);
   for (int i = lane; i < a.T * 16; i += 64) sums[i] = 0.0f;
-  int n_items = a.n;
-  if constexpr (!SINGLE) {
-    n_items = __builtin_amdgcn_readfirstlane(a.plan[0]);
-    const uint64_t* from = reinterpret_cast<const uint64_t*>(a.plan + kDecodePlanHead / 4);
-    for (int i = threadIdx.x; i < 2 * a.n; i += 64 * WAVES)
-      reinterpret_cast<uint64_t*>(items)[i] = from[i];
-  }
+  const int n_items = __builtin_amdgcn_readfirstlane(a.plan[0]);
+  const uint64_t* from = reinterpret_cast<const uint64_t*>(a.plan + kDecodePlanHead / 4);
+  for (int i = threadIdx.x; i < 2 * a.n; i += 64 * WAVES) reinterpret_cast<uint64_t*>(items)[i] = from[i];
   __syncthreads();
   const int h = blockIdx.x * 16 + r16, hc = h < a.H ? h : a.H - 1;
   const int steps = (a.I + kFewStep - 1) / kFewStep;
-  for (int u = wave; u < n_items * parts; u += WAVES) {
-    const int i = u / parts, part = u - i * parts;
-    int expert, first = 0, count = 1;
-    if constexpr (SINGLE) {
-      expert = __builtin_amdgcn_readfirstlane(decode_expert(a, i));
-      if (expert < 0) continue;
-    } else {
-      const DecodeItem it = items[i];
-      expert = __builtin_amdgcn_readfirstlane(it.expert);
-      first = __builtin_amdgcn_readfirstlane(it.first);
-      count = __builtin_amdgcn_readfirstlane(it.count);
-    }
+  for (int i = wave; i < n_items; i += WAVES) {
+    const DecodeItem it = items[i];
+    const int expert = __builtin_amdgcn_readfirstlane(it.expert);
+    const int first = __builtin_amdgcn_readfirstlane(it.first);
+    const int count = __builtin_amdgcn_readfirstlane(it.count);
     const FewRow row[1] = {few_row<F>(a.down, expert, hc, a.I)};
-    int entry = i;
-    if constexpr (!SINGLE) {
-      const int j = NE == 1 ? r16 >> 2 : r16;
-      entry = entries[first + (j < count ? j : count - 1)].entry;
-    }
+    const int own = NE == 1 ? r16 >> 2 : r16;
+    const int entry = entries[first + (own < count ? own : count - 1)].entry;
     const char* const x[1] = {a.act + static_cast<int64_t>(entry) * a.I * 2};
     lin_f32x4_t acc[1][1];
-    few_product<F, 1, 1, NE, BATCH>(row, a.down, x, a.I, steps * part / parts,
-                                    steps * (part + 1) / parts, acc);
-    if constexpr (SINGLE) {
-      if (quad == 0) sums[r16] += a.weights[i] * acc[0][0][0];
-    } else {
+    few_product<F, 1, 1, NE, BATCH>(row, a.down, x, a.I, 0, steps, acc);
 #pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const int j = NE == 1 ? quad : 4 * quad + e;
-        if (j < count) {  // (an item holds a row once: no two lanes add to one sum)
-          const DecodeEntry t = entries[first + j];
-          sums[t.entry / a.k * 16 + r16] += t.weight * acc[0][0][e];
-        }
+    for (int e = 0; e < NE; ++e) {
+      const int j = NE == 1 ? quad : 4 * quad + e;
+      if (j < count) {  // (an item holds a row once: no two lanes add to one sum)
+        const DecodeEntry t = entries[first + j];
+        sums[t.entry / a.k * 16 + r16] += t.weight * acc[0][0][e];
       }
     }
   }
@@ -76,14 +57,62 @@ __global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArg
   }
 }
 
-template <class F, int NE, bool SINGLE, int WAVES, int BATCH>
+template <class F, int NE, int WAVES, int BATCH>
 int launch(const DecodeArgs& a, hipStream_t s, const char* what) {
-  const int64_t steps = ceil_div(a.I, kFewStep);
-  int64_t parts = SINGLE ? WAVES / a.n : 1;
-  parts = parts < 1 ? 1 : parts > steps ? steps : parts;
-  const size_t lds = WAVES * a.T * 64 + (SINGLE ? 0 : 16 * a.n);
-  decode_down_kernel<F, NE, SINGLE, WAVES, BATCH>
-      <<<static_cast<unsigned>(ceil_div(a.H, 16)), 64 * WAVES, lds, s>>>(a, static_cast<int>(parts));
+  decode_down_kernel<F, NE, WAVES, BATCH>
+      <<<static_cast<unsigned>(ceil_div(a.H, 16)), 64 * WAVES, WAVES * a.T * 64 + 16 * a.n, s>>>(a);
+  return check_launch(what);
+}
+
+// A single row: a workgroup takes R 64 / L columns of the result, its waves the row's
+// experts in turn (parts of the contraction where there are fewer experts than waves).
+template <class F, int L, int R, int WAVES, int DEPTH>
+__global__ void __launch_bounds__(64 * WAVES) decode_down_single_kernel(const DecodeArgs a, const int parts) {
+  constexpr int RI = 64 / L, ROWS = R * RI, N = gemv_sums<L, R>();
+  __shared__ float sums[WAVES][ROWS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h0 = blockIdx.x * ROWS;
+  auto first = [&](int r) { return h0 + r * RI < a.H - RI ? h0 + r * RI : a.H - RI; };
+  const int chunks = gemv_chunks<F, L>(a.I);
+  float acc[R], sum[N];
+#pragma unroll
+  for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+  for (int u = wave; u < a.n * parts; u += WAVES) {
+    const int i = u / parts, part = u - i * parts;
+    const int expert = __builtin_amdgcn_readfirstlane(decode_expert(a, i));
+    if (expert < 0) continue;
+    const float weight = a.weights[i];
+    float one[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) one[r] = 0.0f;
+    gemv_add<F, L, R, DEPTH>(one, a.down, expert, first, a.act + static_cast<int64_t>(i) * a.I * 2, a.I,
+                             chunks * part / parts, chunks * (part + 1) / parts);
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = fmaf(weight, one[r], acc[r]);
+  }
+  gemv_reduce<L, R>(acc, sum);
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+    if ((lane & 15) == q) sums[wave][gemv_row<L>(q, lane >> 4)] = sum[q];
+  __syncthreads();
+  const int r = threadIdx.x;
+  if (r < ROWS) {
+    float v = sums[0][r];
+#pragma unroll
+    for (int o = 1; o < WAVES; ++o) v += sums[o][r];
+    a.out[first(r / RI) + r % RI] = lin_round16(v, a.type);
+  }
+}
+
+template <class F, int L>
+int launch_single(const DecodeArgs& a, hipStream_t s, const char* what) {
+  constexpr int R = L == 64 ? 8 : 4, WAVES = 8, DEPTH = F::dense ? 3 : 2;
+  const int chunks = gemv_chunks<F, L>(a.I);
+  int parts = WAVES / a.n;
+  parts = parts < 1 ? 1 : parts > chunks ? chunks : parts;
+  decode_down_single_kernel<F, L, R, WAVES, DEPTH>
+      <<<static_cast<unsigned>(ceil_div(a.H, R * (64 / L))), 64 * WAVES, 0, s>>>(a, parts);
   return check_launch(what);
 }
 
@@ -92,9 +121,14 @@ int launch(const DecodeArgs& a, hipStream_t s, const char* what) {
 int decode_down(const DecodeArgs& a, int format, hipStream_t s, const char* what) {
   return decode_dispatch(format, a.type, a.down.type, [&](auto f) {
     using F = decltype(f);
-    if (a.T == 1) return launch<F, 1, true, 16, 1>(a, s, what);
-    if (a.T <= 4) return launch<F, 1, false, 8, 2>(a, s, what);
-    return launch<F, 4, false, 8, 2>(a, s, what);
+    if (a.T == 1) {
+      const int lanes = gemv_lanes<F>(a.I, a.H);
+      return lanes == 64   ? launch_single<F, 64>(a, s, what)
+             : lanes == 32 ? launch_single<F, 32>(a, s, what)
+                           : launch_single<F, 16>(a, s, what);
+    }
+    if (a.T <= 4) return launch<F, 1, 8, 2>(a, s, what);
+    return launch<F, 4, 8, 2>(a, s, what);
   });
 }
 

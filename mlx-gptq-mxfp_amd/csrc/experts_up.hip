@@ -75,20 +75,21 @@ __device__ void decode_plan(const DecodeArgs& a, int16_t* ids, uint32_t* carry) 
 
 constexpr int kWaves = 4;
 
+__device__ __forceinline__ float decode_act(float gate, float up) {
+  return gate / (1.0f + expf(-gate)) * up;
+}
+
 template <class F, int NE, int BATCH>
 __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs a) {
   constexpr int BM = NE == 1 ? 4 : 16;
   __shared__ __attribute__((aligned(16))) int16_t list[kDecodeEntries];
   __shared__ uint32_t carry[kWaves];
   __shared__ lin_f32x4_t part[kWaves * 2 * 64];
-  int bid = blockIdx.x;
-  if (a.T > 1) {
-    if (bid == 0) {
-      decode_plan(a, list, carry);
-      return;
-    }
-    --bid;
+  if (blockIdx.x == 0) {
+    decode_plan(a, list, carry);
+    return;
   }
+  const int bid = blockIdx.x - 1;
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.I + 15) / 16;
@@ -140,21 +141,63 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
         // (16 bits: what the second product's MFMA takes)
         if (i < count && p < a.I)
           reinterpret_cast<uint16_t*>(a.act)[static_cast<int64_t>(list[i]) * a.I + p] =
-              lin_round16(gate[e] / (1.0f + expf(-gate[e])) * up[e], a.type);
+              lin_round16(decode_act(gate[e], up[e]), a.type);
       }
     }
     __syncthreads();
   }
 }
 
+// A single row: a wave takes one entry, R / 2 loads of gate rows and the up rows beside
+// them.
+template <class F, int L, int R, int DEPTH>
+__global__ void __launch_bounds__(64 * kWaves) decode_up_single_kernel(const DecodeArgs a) {
+  constexpr int RI = 64 / L, ROWS = R / 2 * RI, N = gemv_sums<L, R>();
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (a.I + kWaves * ROWS - 1) / (kWaves * ROWS);
+  const int entry = blockIdx.x / tiles;
+  const int i0 = ((blockIdx.x - entry * tiles) * kWaves + wave) * ROWS;
+  if (i0 >= a.I) return;
+  const int expert = __builtin_amdgcn_readfirstlane(decode_expert(a, entry));
+  if (expert < 0) return;
+  auto inner = [&](int r) { return i0 + r * RI < a.I - RI ? i0 + r * RI : a.I - RI; };
+  float acc[R], sum[N];
+#pragma unroll
+  for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+  gemv_add<F, L, R, DEPTH>(
+      acc, a.up, expert, [&](int r) { return r < R / 2 ? inner(r) : a.I + inner(r - R / 2); }, a.x, a.H,
+      0, gemv_chunks<F, L>(a.H));
+  gemv_reduce<L, R>(acc, sum);
+  uint16_t* act = reinterpret_cast<uint16_t*>(a.act) + static_cast<int64_t>(entry) * a.I;
+#pragma unroll
+  for (int q = 0; q < N / 2; ++q)
+    if ((lane & 15) == q) {
+      const int r = gemv_row<L>(q, lane >> 4);
+      act[inner(r / RI) + r % RI] = lin_round16(decode_act(sum[q], sum[q + N / 2]), a.type);
+    }
+}
+
+template <class F>
+int launch_single(const DecodeArgs& a, hipStream_t s, const char* what) {
+  constexpr int R = 8, DEPTH = F::dense ? 4 : 2;
+  const int lanes = gemv_lanes<F>(a.H, a.I);
+  const unsigned grid = static_cast<unsigned>(a.n * ceil_div(a.I, kWaves * R / 2 * (64 / lanes)));
+  if (lanes == 64) decode_up_single_kernel<F, 64, R, DEPTH><<<grid, 64 * kWaves, 0, s>>>(a);
+  else if (lanes == 32) decode_up_single_kernel<F, 32, R, DEPTH><<<grid, 64 * kWaves, 0, s>>>(a);
+  else decode_up_single_kernel<F, 16, R, DEPTH><<<grid, 64 * kWaves, 0, s>>>(a);
+  return check_launch(what);
+}
+
 }  // namespace
 
 int decode_up(const DecodeArgs& a, int format, hipStream_t s, const char* what) {
   const int64_t slots = a.n > a.E ? a.E : a.n;
-  const int64_t grid = slots * ceil_div(a.I, 16) + (a.T > 1);
+  const int64_t grid = slots * ceil_div(a.I, 16) + 1;
   MGQ_REQUIRE(grid < int64_t(1) << 24, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
   return decode_dispatch(format, a.type, a.up.type, [&](auto f) {
     using F = decltype(f);
+    if (a.T == 1) return launch_single<F>(a, s, what);
     if (a.T <= 4)
       decode_up_kernel<F, 1, 2><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
     else

@@ -404,6 +404,75 @@ __device__ __forceinline__ void few_product(const FewRow (&row)[NP], const FewWe
   }
 }
 
+// Waves hand LDS over without waiting for the loads that they have in flight into
+// registers (__syncthreads would, and with it for the next tile's weights).
+__device__ __forceinline__ void few_handover() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Tiles [t0, t1) of 16 NP weight rows, one after the other, times up to 16 x rows (a lane's
+// own: `x`). The workgroup's waves share the contraction, at most XS steps each, so that
+// the x rows stay in registers; the next tile's weights are in flight while one is
+// multiplied. rows(t, FewRow (&)[NP]) says where tile t's weight rows are, emit(t, sums)
+// takes its results in one of the waves. part: 2 WAVES NP 64 accumulators of LDS. Every wave
+// of the workgroup calls this with the same tiles.
+template <class F, int NP, int NE, int XS, int WAVES, typename Rows, typename Emit>
+__device__ __forceinline__ void few_stream(const FewWeight& w, const char* x, int K, int t0, int t1,
+                                           lin_f32x4_t* part, Rows&& rows, Emit&& emit) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int steps = (K + kFewStep - 1) / kFewStep;
+  const int s0 = steps * wave / WAVES, s1 = steps * (wave + 1) / WAVES;
+  FewStep<F> f[2][XS][NP];
+  auto load = [&](int k, int t) __attribute__((always_inline)) {
+    FewRow row[NP];
+    rows(t < t1 ? t : t1 - 1, row);
+#pragma unroll
+    for (int i = 0; i < XS; ++i) {
+      // (a step that is not this wave's repeats one that is, or the row's last)
+      const int at = s0 + i < s1 ? s0 + i : s1 > s0 ? s1 - 1 : steps - 1;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) few_load<F>(f[k][i][p], row[p], w, at, K);
+    }
+  };
+  load(0, t0);
+  lin_u32x4_t xv[XS][1][4];
+#pragma unroll
+  for (int i = 0; i < XS; ++i) few_load_x<F>(xv[i][0], x, s0 + i < s1 ? s0 + i : steps - 1, K);
+  auto tile = [&](int k, int t) __attribute__((always_inline)) {
+    if (t + 1 < t1) load(k ^ 1, t + 1);
+    lin_f32x4_t acc[NP][1];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) acc[p][0] = lin_f32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < XS; ++i)
+      if (s0 + i < s1) few_multiply<F, NP, 1, NE>(f[k][i], xv[i], s0 + i, K, w.type, acc);
+    lin_f32x4_t* own = part + k * (WAVES * NP * 64);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) own[(wave * NP + p) * 64 + lane] = acc[p][0];
+    few_handover();
+    // (the other half of `part` is free: who summed the last tile has come past the barrier)
+    if (wave == (t & (WAVES - 1))) {
+      lin_f32x4_t sum[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        sum[p] = own[p * 64 + lane];
+#pragma unroll
+        for (int o = 1; o < WAVES; ++o) {
+          const lin_f32x4_t v = own[(o * NP + p) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < NE; ++e) sum[p][e] += v[e];
+        }
+      }
+      emit(t, sum);
+    }
+  };
+  for (int t = t0; t < t1; t += 2) {
+    tile(0, t);
+    if (t + 1 < t1) tile(1, t + 1);
+  }
+}
+
 // Checks of a quantized weight's description, on the host.
 inline bool few_weight_ok(int format, int64_t K, int shift, int type) {
   if (format == kFewDense) return true;

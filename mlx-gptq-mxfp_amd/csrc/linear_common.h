@@ -18,13 +18,20 @@
 
 namespace mgq {
 
-// Operand types. The MX forms are the weight's; their other operand is bf16.
-enum LinOp : int { kOpBF16 = 0, kOpF16 = 1, kOpI8 = 2, kOpMx4 = 3, kOpMx8 = 4 };
+// Operand types. The MX and affine (2, 4 or 8 bits) forms are the weight's; their other
+// operand is bf16 (f16 in the H forms).
+enum LinOp : int {
+  kOpBF16 = 0, kOpF16 = 1, kOpI8 = 2, kOpMx4 = 3, kOpMx8 = 4,
+  kOpAf2 = 5, kOpAf4 = 6, kOpAf8 = 7, kOpAf2H = 8, kOpAf4H = 9, kOpAf8H = 10
+};
 
 struct LinArgs {
   const char* P;         // weight (forward, dgrad) or X (wgrad)
   const char* Q;         // X (forward) or dY
-  const uint8_t* Ps;     // E8M0 scale bytes of an MX weight [G, np, nc / 32]
+  const uint8_t* Ps;     // E8M0 scale bytes of an MX weight [G, np, nc / 32]; scales of an
+                         // affine one [G, np, nc >> p_shift]
+  const uint8_t* Pb;     // affine: biases, laid out like the scales
+  int p_shift, p_type;   // affine: log2 of the values that share a scale, type of both
   int64_t ldp, ldq;      // row pitches in bytes
   int64_t p_group;       // bytes from one group's weight to the next
   const int32_t* offsets;    // [G + 1], or null: one group of all entries
@@ -60,6 +67,21 @@ template <int OP>
 constexpr bool lin_is_mx() {
   return OP == kOpMx4 || OP == kOpMx8;
 }
+template <int OP>
+constexpr bool lin_is_affine() {
+  return OP >= kOpAf2;
+}
+template <int OP>
+constexpr bool lin_is_f16() {
+  return OP == kOpF16 || OP >= kOpAf2H;
+}
+// Bits of a weight's code.
+template <int OP>
+constexpr int lin_code_bits() {
+  return OP == kOpAf2 || OP == kOpAf2H                     ? 2
+         : OP == kOpMx4 || OP == kOpAf4 || OP == kOpAf4H ? 4
+                                                           : 8;
+}
 // Bytes of one element of the Q operand (and of a dense P operand).
 template <int OP>
 constexpr int lin_esize() {
@@ -85,7 +107,7 @@ __device__ __forceinline__ typename LinAcc<OP>::t32 lin_mfma32(lin_u32x4_t a, li
   if constexpr (OP == kOpI8)
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(lin_i32x4_t, a),
                                                  __builtin_bit_cast(lin_i32x4_t, b), c, 0, 0, 0);
-  else if constexpr (OP == kOpF16)
+  else if constexpr (lin_is_f16<OP>())
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lin_f16x8_t, a),
                                                   __builtin_bit_cast(lin_f16x8_t, b), c, 0, 0, 0);
   else
@@ -329,6 +351,35 @@ __device__ __forceinline__ uint32_t lin_pack2(float x, float y) {
     return __builtin_bit_cast(uint32_t,
                               lin_bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
   }
+}
+// Eight affine codes (the low 8 BITS bits of lo, then hi) -> q s + b in fp32, rounded to
+// 16 bits.
+template <int TYPE, int BITS>
+__device__ __forceinline__ lin_u32x4_t lin_decode_affine(uint32_t lo, uint32_t hi, float s, float b) {
+  uint32_t u[2];  // codes 0 2 4 6 and 1 3 5 7, one a byte (8 bits: 0..3 and 4..7)
+  if constexpr (BITS == 8) {
+    u[0] = lo;
+    u[1] = hi;
+  } else {
+    uint32_t n = lo;
+    if constexpr (BITS == 2) {
+      n = (n & 0xffu) | ((n & 0xff00u) << 8);
+      n = (n & 0x000f000fu) | ((n & 0x00f000f0u) << 4);
+    }
+    constexpr uint32_t mask = BITS == 4 ? 0x0f0f0f0fu : 0x03030303u;
+    u[0] = n & mask;
+    u[1] = (n >> BITS) & mask;
+  }
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int from = BITS == 8 ? i >> 2 : i & 1, at = BITS == 8 ? i & 3 : i >> 1;
+    w[i] = fmaf(static_cast<float>((u[from] >> (8 * at)) & 0xff), s, b);
+  }
+  lin_u32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = lin_pack2<TYPE>(w[2 * i], w[2 * i + 1]);
+  return r;
 }
 __device__ __forceinline__ uint16_t lin_round16(float v, int type) {
   return type == kF16 ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);

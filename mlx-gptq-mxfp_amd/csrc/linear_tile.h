@@ -83,6 +83,7 @@ struct LinTileShape {
 bool lin_tile_direct(const LinArgs& a, int op, int kind);
 int lin_tile_rows(const LinArgs& a, int op, int kind, LinTileShape t, hipStream_t s,
                   const char* what);
+int lin_tile_affine(const LinArgs& a, int op, LinTileShape t, hipStream_t s, const char* what);
 int64_t lin_tile_wgrad_bytes(int64_t M, int64_t G, int64_t N, int64_t K);
 int lin_tile_wgrad(const LinArgs& a, int op, void* workspace, hipStream_t s, const char* what);
 
