@@ -463,11 +463,8 @@ int mgq_top_k_softmax_grad(const float* dw, const void* logits, int dtype, int64
  * [T, k] of 32 or 64 bits, weights: f32 [T, k], out: [T, H] of dtype. T <= 64, k <=
  * 16. Assignments to no expert (outside [0, n_experts)) add nothing. `up` holds an
  * expert's I gate rows, then its I up rows: [n_experts, 2 I, H]; `down`: [n_experts,
- * H, I]. Each has a format of its own: dense (dtype, pitch ld and distance of two
- * experts in elements), MXFP words with scale bytes (bf16 rows; group size 32), or
- * affine words with scales and biases of param_dtype for groups of 32, 64 or 128
- * values, laid out as in mgq_mxfp_linear and mgq_affine_linear. Two launches; every
- * result is the same from call to call. The workspace is 256-byte aligned. */
+ * H, I]. Each has a format of its own, see mgq_weight. Two launches; every result is
+ * the same from call to call. The workspace is 256-byte aligned. */
 enum {
   MGQ_WEIGHT_DENSE = 0,
   MGQ_WEIGHT_MXFP4 = 1,
@@ -476,15 +473,20 @@ enum {
   MGQ_WEIGHT_AFFINE4 = 4,
   MGQ_WEIGHT_AFFINE8 = 5
 };
+typedef struct {
+  const void* data;    /* elements of the rows' dtype, or words as mgq_pack_q writes them */
+  const void* scales;  /* MXFP (bf16 rows only): E8M0 bytes; affine: scales */
+  const void* biases;  /* affine */
+  int64_t ld, expert;  /* dense: row pitch, distance of two experts' weights, in elements */
+  int64_t group;       /* affine: values that share a scale, 32, 64 or 128 */
+  int format;          /* MGQ_WEIGHT_* */
+  int param_dtype;     /* affine: type of scales and biases (f32/bf16/f16) */
+} mgq_weight;          /* (device pointers in a struct on the host, read during the call) */
 int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64_t I);
 int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t ldx, const void* index,
                        int index_bits, const float* weights, int64_t k, int64_t n_experts, int64_t H,
-                       int64_t I, const void* up, int up_format, int64_t up_ld, int64_t up_expert,
-                       const void* up_scales, const void* up_biases, int64_t up_group,
-                       const void* down, int down_format, int64_t down_ld, int64_t down_expert,
-                       const void* down_scales, const void* down_biases, int64_t down_group,
-                       int param_dtype, void* out, void* workspace, int64_t workspace_bytes,
-                       void* stream);
+                       int64_t I, const mgq_weight* up, const mgq_weight* down, void* out,
+                       void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

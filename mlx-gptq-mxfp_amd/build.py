@@ -50,7 +50,10 @@ COMMON_FLAGS = [
 # Hessian kernel keeps the default, which puts its accumulators in AGPRs.
 _VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 EXTRA_FLAGS = {"gptq_mxfp.hip": _VGPR_FORM, "chol_full.hip": _VGPR_FORM,
-               "gptq_affine.hip": _VGPR_FORM}
+               "gptq_affine.hip": _VGPR_FORM,
+               # (results that are scaled right away)
+               "affine_linear.hip": _VGPR_FORM, "experts_up.hip": _VGPR_FORM,
+               "experts_down.hip": _VGPR_FORM}
 
 
 def hipcc() -> str:

@@ -25,10 +25,8 @@ __global__ void __launch_bounds__(64 * WAVES) affine_few_kernel(const LinArgs a,
 
   FewRow row[NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int p = p0 + 16 * i + r16;
-    row[i] = few_row<F>(w, g, p < a.np ? p : a.np - 1, a.nc);
-  }
+  for (int i = 0; i < NP; ++i)
+    row[i] = few_row<F>(w, g, p0 + 16 * i < a.np ? p0 + 16 * i : p0, a.nc);
   const char* x[NQ];
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
@@ -60,44 +58,6 @@ __global__ void __launch_bounds__(64 * WAVES) affine_few_kernel(const LinArgs a,
         reinterpret_cast<uint16_t*>(a.out)[q * a.ldo + p] = lin_round16(sum[e], a.out_type);
     }
   }
-}
-
-// The same with the tiles of one entry block streamed: a workgroup takes 16 entries (4
-// where NE = 1) and `per` blocks of 16 weight rows, x stays in registers. The contraction
-// is at most 128 XS WAVES long.
-template <class F, int NE, int XS, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES)
-    affine_stream_kernel(const LinArgs a, const FewWeight w, const int per) {
-  constexpr int BM = NE == 1 ? 4 : 16;
-  __shared__ lin_f32x4_t part[2 * WAVES * 64];
-  LinTile t;
-  const int tiles = (a.np + 15) / 16;
-  if (!lin_find_tile<BM>(a, (tiles + per - 1) / per, &t)) return;
-  const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
-  const int t0 = t.pt * per, t1 = t0 + per < tiles ? t0 + per : tiles;
-  auto store = [&](int tile, const lin_f32x4_t& v) {
-    const int p = 16 * tile + r16;
-    if (p >= a.np) return;
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const int64_t q = t.q0 + (NE == 1 ? quad : 4 * quad + e);
-      if (q < t.q_end)
-        reinterpret_cast<uint16_t*>(a.out)[q * a.ldo + p] = lin_round16(v[e], a.out_type);
-    }
-  };
-  if (t.g >= a.G) {  // (no group: zeros)
-    for (int i = t0 + (threadIdx.x >> 6); i < t1; i += WAVES) store(i, lin_f32x4_t{0, 0, 0, 0});
-    return;
-  }
-  const int64_t q = t.q0 + (NE == 1 ? r16 >> 2 : r16);
-  const char* x = a.Q + lin_row(a, q < t.q_end ? q : t.q_end - 1) * a.ldq;
-  few_stream<F, 1, NE, XS, WAVES>(
-      w, x, a.nc, t0, t1, part,
-      [&](int tile, FewRow(&row)[1]) {
-        const int p = 16 * tile + r16;
-        row[0] = few_row<F>(w, t.g, p < a.np ? p : a.np - 1, a.nc);
-      },
-      [&](int tile, const lin_f32x4_t(&sum)[1]) { store(tile, sum[0]); });
 }
 
 // Single entries: a wave takes one entry and R 64 / L weight rows.
@@ -147,15 +107,6 @@ int launch_gemv(const LinArgs& a, const FewWeight& w, hipStream_t s, const char*
   else affine_gemv_kernel<F, 16, R><<<blocks, 256, 0, s>>>(a, w);
   return check_launch(what);
 }
-template <class F, int NE, int XS, int WAVES>
-int launch_stream(const LinArgs& a, const FewWeight& w, int per, hipStream_t s, const char* what) {
-  const int64_t grid = lin_row_tiles(a, NE == 1 ? 4 : 16) * ceil_div(ceil_div(a.np, 16), per);
-  MGQ_REQUIRE(grid < kLinFewGrid * 4 / WAVES, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  affine_stream_kernel<F, NE, XS, WAVES>
-      <<<static_cast<unsigned>(grid), 64 * WAVES, 0, s>>>(a, w, per);
-  return check_launch(what);
-}
-
 #ifdef AFFINE_FORCE
 extern "C" int mgq_force[4] = {0, 0, 0, 0};
 #endif
@@ -170,16 +121,15 @@ int run(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
     case 3: return launch_few<F, 2, 4, 4, 4, 1>(a, w, s, what);
     case 4: return launch_few<F, 2, 2, 4, 4, 1>(a, w, s, what);
     case 5: return launch_gemv<F>(a, w, s, what);
-    case 10: return launch_stream<F, 1, 1, 8>(a, w, per, s, what);
-    case 11: return launch_stream<F, 1, 2, 8>(a, w, per, s, what);
-    case 12: return launch_stream<F, 1, 4, 8>(a, w, per, s, what);
-    case 13: return launch_stream<F, 1, 2, 16>(a, w, per, s, what);
-    case 14: return launch_stream<F, 1, 4, 4>(a, w, per, s, what);
-    case 20: return launch_stream<F, 4, 1, 8>(a, w, per, s, what);
-    case 21: return launch_stream<F, 4, 2, 8>(a, w, per, s, what);
-    case 22: return launch_stream<F, 4, 4, 8>(a, w, per, s, what);
-    case 23: return launch_stream<F, 4, 2, 16>(a, w, per, s, what);
-    case 24: return launch_stream<F, 4, 4, 4>(a, w, per, s, what);
+    case 6: return launch_few<F, 1, 1, 1, 4, 4>(a, w, s, what);
+    case 7: return launch_few<F, 1, 1, 4, 4, 4>(a, w, s, what);
+    case 8: return launch_few<F, 2, 1, 4, 4, 2>(a, w, s, what);
+    case 9: return launch_few<F, 4, 1, 4, 4, 2>(a, w, s, what);
+    case 10: return launch_few<F, 4, 1, 4, 4, 1>(a, w, s, what);
+    case 11: return launch_few<F, 1, 1, 4, 8, 2>(a, w, s, what);
+    case 12: return launch_few<F, 2, 1, 4, 8, 2>(a, w, s, what);
+    case 13: return launch_few<F, 4, 2, 4, 4, 1>(a, w, s, what);
+    case 14: return launch_few<F, 4, 4, 4, 4, 1>(a, w, s, what);
     case 30: case 31: case 32: case 33: {
       LinArgs b = a;
       b.P = w.p; b.Ps = reinterpret_cast<const uint8_t*>(w.s); b.Pb = reinterpret_cast<const uint8_t*>(w.b);
@@ -198,6 +148,9 @@ int run(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
 }
 template <int XT, int SB>
 int run_bits(int bits, const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
+#ifdef AFFINE_FORCE
+  return bits == 8 ? run<FewFmt<kFewAf8, kBF16, 2>>(a, w, s, what) : run<FewFmt<kFewAf4, kBF16, 2>>(a, w, s, what);
+#endif
   if (bits == 2) return run<FewFmt<kFewAf2, XT, SB>>(a, w, s, what);
   if (bits == 4) return run<FewFmt<kFewAf4, XT, SB>>(a, w, s, what);
   return run<FewFmt<kFewAf8, XT, SB>>(a, w, s, what);

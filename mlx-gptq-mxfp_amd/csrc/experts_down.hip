@@ -24,14 +24,14 @@ __global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArg
   const uint64_t* from = reinterpret_cast<const uint64_t*>(a.plan + kDecodePlanHead / 4);
   for (int i = threadIdx.x; i < 2 * a.n; i += 64 * WAVES) reinterpret_cast<uint64_t*>(items)[i] = from[i];
   __syncthreads();
-  const int h = blockIdx.x * 16 + r16, hc = h < a.H ? h : a.H - 1;
+  const int h0 = blockIdx.x * 16;
   const int steps = (a.I + kFewStep - 1) / kFewStep;
   for (int i = wave; i < n_items; i += WAVES) {
     const DecodeItem it = items[i];
     const int expert = __builtin_amdgcn_readfirstlane(it.expert);
     const int first = __builtin_amdgcn_readfirstlane(it.first);
     const int count = __builtin_amdgcn_readfirstlane(it.count);
-    const FewRow row[1] = {few_row<F>(a.down, expert, hc, a.I)};
+    const FewRow row[1] = {few_row<F>(a.down, expert, h0, a.I)};
     const int own = NE == 1 ? r16 >> 2 : r16;
     const int entry = entries[first + (own < count ? own : count - 1)].entry;
     const char* const x[1] = {a.act + static_cast<int64_t>(entry) * a.I * 2};
@@ -143,11 +143,7 @@ extern "C" int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64
 
 extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t ldx, const void* index,
                                   int index_bits, const float* weights, int64_t k, int64_t n_experts,
-                                  int64_t H, int64_t I, const void* up, int up_format, int64_t up_ld,
-                                  int64_t up_expert, const void* up_scales, const void* up_biases,
-                                  int64_t up_group, const void* down, int down_format, int64_t down_ld,
-                                  int64_t down_expert, const void* down_scales,
-                                  const void* down_biases, int64_t down_group, int param_dtype,
+                                  int64_t H, int64_t I, const mgq_weight* up, const mgq_weight* down,
                                   void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   clear_error();
   const char* what = "experts_decode";
@@ -162,32 +158,33 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
   MGQ_REQUIRE(H >= 1 && I >= 1 && H < (int64_t(1) << 29) && I < (int64_t(1) << 29), MGQ_ERR_SHAPE,
               "%s: bad layer sizes %lld, %lld", what, (long long)H, (long long)I);
   MGQ_REQUIRE(ldx >= H, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
-  auto weight = [&](const void* p, int format, int64_t ld, int64_t expert, const void* s,
-                    const void* b, int64_t group, int64_t n, int64_t cols, FewWeight* w) -> int {
+  auto weight = [&](const mgq_weight& m, int64_t n, int64_t cols, FewWeight* w) -> int {
+    const int format = m.format;
     MGQ_REQUIRE(format >= kFewDense && format <= kFewAf8, MGQ_ERR_VALUE, "%s: no such weight format",
                 what);
     MGQ_REQUIRE(dtype == kBF16 || (format != kFewMx4 && format != kFewMx8), MGQ_ERR_VALUE,
                 "%s: MXFP weights take bfloat16 rows", what);
-    w->p = static_cast<const char*>(p);
+    w->p = static_cast<const char*>(m.data);
     w->n = n;
     if (format == kFewDense) {
-      MGQ_REQUIRE(ld >= cols, MGQ_ERR_SHAPE, "%s: a weight's pitch is shorter than its row", what);
-      w->ld = 2 * ld;
-      w->group = 2 * expert;
+      MGQ_REQUIRE(m.ld >= cols && m.ld < (int64_t(1) << 29), MGQ_ERR_SHAPE,
+                  "%s: a weight's pitch is shorter than its row, or 2^29 elements", what);
+      w->ld = 2 * m.ld;
+      w->group = 2 * m.expert;
       return MGQ_OK;
     }
-    w->s = static_cast<const char*>(s);
-    w->b = static_cast<const char*>(b);
+    w->s = static_cast<const char*>(m.scales);
+    w->b = static_cast<const char*>(m.biases);
     const int bits = format == kFewAf2 ? 2 : format == kFewMx4 || format == kFewAf4 ? 4 : 8;
+    int64_t group = kMxGroup;
     if (format >= kFewAf2) {
+      group = m.group;
       MGQ_REQUIRE(group == 32 || group == 64 || group == 128, MGQ_ERR_VALUE,
                   "%s: groups of 32, 64 or 128 values", what);
-      MGQ_REQUIRE(param_dtype == kF32 || param_dtype == kBF16 || param_dtype == kF16, MGQ_ERR_VALUE,
-                  "%s: scales and biases are float32, bfloat16 or float16", what);
+      MGQ_REQUIRE(m.param_dtype == kF32 || m.param_dtype == kBF16 || m.param_dtype == kF16,
+                  MGQ_ERR_VALUE, "%s: scales and biases are float32, bfloat16 or float16", what);
       w->shift = group == 32 ? 5 : group == 64 ? 6 : 7;
-      w->type = param_dtype;
-    } else {
-      group = kMxGroup;
+      w->type = m.param_dtype;
     }
     MGQ_REQUIRE(cols % group == 0, MGQ_ERR_SHAPE, "%s: %lld columns are no multiple of the group size",
                 what, (long long)cols);
@@ -196,11 +193,8 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
     return MGQ_OK;
   };
   DecodeArgs a = {};
-  if (int rc = weight(up, up_format, up_ld, up_expert, up_scales, up_biases, up_group, 2 * I, H, &a.up))
-    return rc;
-  if (int rc = weight(down, down_format, down_ld, down_expert, down_scales, down_biases, down_group, H, I,
-                      &a.down))
-    return rc;
+  if (int rc = weight(*up, 2 * I, H, &a.up)) return rc;
+  if (int rc = weight(*down, H, I, &a.down)) return rc;
   const int64_t need = mgq_experts_decode_workspace_size(T, k, I);
   MGQ_REQUIRE(workspace_bytes >= need, MGQ_ERR_WORKSPACE, "%s: workspace %lld < %lld bytes", what,
               (long long)workspace_bytes, (long long)need);
@@ -221,6 +215,6 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
   a.I = static_cast<int>(I);
   a.type = dtype;
   hipStream_t s = as_stream(stream);
-  if (int rc = decode_up(a, up_format, s, what)) return rc;
-  return decode_down(a, down_format, s, what);
+  if (int rc = decode_up(a, up->format, s, what)) return rc;
+  return decode_down(a, down->format, s, what);
 }

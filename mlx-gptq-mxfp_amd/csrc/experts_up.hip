@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.I + 15) / 16;
-  const int slot = bid / tiles, p = (bid - slot * tiles) * 16 + r16;
+  const int slot = bid / tiles, p0 = (bid - slot * tiles) * 16, p = p0 + r16;
   const bool by_expert = a.n > a.E;
   const int expert = by_expert ? slot : __builtin_amdgcn_readfirstlane(decode_expert(a, slot));
   if (expert < 0) return;
@@ -110,9 +110,9 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
   __syncthreads();
 
   FewRow row[2];
-  const int pc = p < a.I ? p : a.I - 1;
-  row[0] = few_row<F>(a.up, expert, pc, a.H);
-  row[1] = few_row<F>(a.up, expert, a.I + pc, a.H);
+  // (a gate row past the last one is an up row, whose result is not stored)
+  row[0] = few_row<F>(a.up, expert, p0, a.H);
+  row[1] = few_row<F>(a.up, expert, a.I + p0, a.H);
   const int steps = (a.H + kFewStep - 1) / kFewStep;
   for (int base = 0; base < count; base += BM) {
     const int j = base + (NE == 1 ? r16 >> 2 : r16);

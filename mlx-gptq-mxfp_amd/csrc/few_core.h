@@ -54,25 +54,32 @@ struct FewFmt {
   static constexpr int op = XT == kF16 ? kOpF16 : kOpBF16;
 };
 
-// Where a lane reads its weight row.
+// Where a lane reads weight row p0 + lane % 16 (the last one of the weight past its end):
+// addresses that are the same in all lanes, and the lane's offsets from them.
 struct FewRow {
   const char* p;
   const char* s;
   const char* b;
+  uint32_t lp, ls;
 };
 
 template <class F>
-__device__ __forceinline__ FewRow few_row(const FewWeight& w, int64_t g, int64_t row, int K) {
-  FewRow r;
-  r.p = w.p + g * w.group + row * w.ld;
-  r.s = r.b = nullptr;
-  const int64_t at = g * w.n + row;
-  if constexpr (F::mx) r.s = w.s + at * (K / 32);
-  if constexpr (F::affine) {
-    r.s = w.s + at * (K >> w.shift) * F::SB;
-    r.b = w.b + at * (K >> w.shift) * F::SB;
+__device__ __forceinline__ FewRow few_row(const FewWeight& w, int64_t g, int p0, int K) {
+  const uint32_t r16 = threadIdx.x & 15, quad = (threadIdx.x >> 4) & 3;
+  const uint32_t left = static_cast<uint32_t>(w.n) - 1 - p0, r = r16 < left ? r16 : left;
+  FewRow row;
+  row.p = w.p + g * w.group + p0 * w.ld;
+  row.lp = r * static_cast<uint32_t>(w.ld) + quad * (F::dense ? 16 : 4 * F::bits);
+  row.s = row.b = nullptr;
+  row.ls = 0;
+  if constexpr (!F::dense) {
+    const uint32_t n = F::mx ? K / 32 : K >> w.shift;
+    const int64_t at = (g * w.n + p0) * n * (F::mx ? 1 : F::SB);
+    row.s = w.s + at;
+    row.ls = r * n * (F::mx ? 1 : F::SB);
+    if constexpr (F::affine) row.b = w.b + at;
   }
-  return r;
+  return row;
 }
 
 // What a lane holds of a step: words, and the block's scale (and bias) as loaded.
@@ -108,74 +115,70 @@ __device__ __forceinline__ uint32_t few_param(const char* at) {
   return *reinterpret_cast<const uint32_t*>(at);
 }
 
-// Step s of a row of K elements. Quantized rows (K % 32 == 0): a block past the row's
-// end reads the row's first one, and few_multiply discards it.
-template <class F>
+// Step s of a weight row. WHOLE: the row holds all 128 elements of it; otherwise zeros
+// follow the row's end (dense), or a block past it reads the row's first one and
+// few_multiply discards it (quantized, K % 32 == 0).
+template <class F, bool WHOLE>
 __device__ __forceinline__ void few_load(FewStep<F>& f, const FewRow& r, const FewWeight& w, int s,
                                          int K) {
-  const int quad = (threadIdx.x & 63) >> 4;
+  const uint32_t quad = (threadIdx.x >> 4) & 3;
   if constexpr (F::dense) {
-    const int k0 = s * kFewStep + 8 * quad;
-    if ((s + 1) * kFewStep <= K) {
+    const uint32_t at = r.lp + static_cast<uint32_t>(s) * (2 * kFewStep);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const lin_u32x4_t u = few_load16(r.p + 2 * static_cast<int64_t>(k0 + 32 * j));
+    for (int j = 0; j < 4; ++j) {
+      lin_u32x4_t u;
+      if constexpr (WHOLE)
+        u = few_load16(r.p + static_cast<uint64_t>(at + 64 * j));
+      else
+        u = few_cut16(r.p + static_cast<uint64_t>(r.lp) - 16 * quad, s * kFewStep + 32 * j + 8 * quad, K);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f.v[4 * j + i] = u[i];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const lin_u32x4_t u = few_cut16(r.p, k0 + 32 * j, K);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f.v[4 * j + i] = u[i];
-      }
+      for (int i = 0; i < 4; ++i) f.v[4 * j + i] = u[i];
     }
   } else {
-    int k0 = s * kFewStep + 32 * quad;
-    k0 = k0 < K ? k0 : 0;
-    const char* at = r.p + static_cast<int64_t>(k0 / 32) * (4 * F::bits);
+    uint32_t k0 = s * kFewStep + 32 * quad, at = r.lp + static_cast<uint32_t>(s) * (16 * F::bits);
+    if constexpr (!WHOLE) {
+      const bool inside = k0 < static_cast<uint32_t>(K);
+      at = inside ? at : r.lp - quad * (4 * F::bits);
+      k0 = inside ? k0 : 0;
+    }
+    const char* from = r.p + static_cast<uint64_t>(at);
     if constexpr (F::bits == 2) {
-      const few_u64_u_t u = *reinterpret_cast<const few_u64_u_t*>(at);
+      const few_u64_u_t u = *reinterpret_cast<const few_u64_u_t*>(from);
       f.v[0] = u.v[0];
       f.v[1] = u.v[1];
     } else {
 #pragma unroll
       for (int h = 0; h < F::bits / 4; ++h) {
-        const lin_u32x4_t u = few_load16(at + 16 * h);
+        const lin_u32x4_t u = few_load16(from + 16 * h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) f.v[4 * h + i] = u[i];
       }
     }
-    if constexpr (F::mx) f.s = reinterpret_cast<const uint8_t*>(r.s)[k0 / 32];
-    if constexpr (F::affine) {
-      const int64_t g = k0 >> w.shift;
-      f.s = few_param<F::SB>(r.s + g * F::SB);
-      f.b = few_param<F::SB>(r.b + g * F::SB);
+    if constexpr (F::mx) {
+      f.s = *reinterpret_cast<const uint8_t*>(r.s + static_cast<uint64_t>(r.ls + k0 / 32));
+    } else {
+      const uint32_t g = r.ls + (k0 >> w.shift) * F::SB;
+      f.s = few_param<F::SB>(r.s + static_cast<uint64_t>(g));
+      f.b = few_param<F::SB>(r.b + static_cast<uint64_t>(g));
     }
   }
 }
 
-// x elements of MFMA j.
-template <class F>
-__device__ __forceinline__ int few_x_at(int s, int j) {
-  const int quad = (threadIdx.x & 63) >> 4;
-  return s * kFewStep + (F::mx ? 32 * quad + 8 * j : 32 * j + 8 * quad);
-}
-template <class F>
+// A lane's x elements of a step's MFMAs. `row` is the lane's x row.
+template <class F, bool WHOLE>
 __device__ __forceinline__ void few_load_x(lin_u32x4_t (&x)[4], const char* row, int s, int K) {
-  if ((s + 1) * kFewStep <= K) {
+  const int quad = (threadIdx.x >> 4) & 3;
+  const int k0 = s * kFewStep + (F::mx ? 32 : 8) * quad;
+  constexpr int step = F::mx ? 8 : 32;
+  const char* at = row + 2 * static_cast<int64_t>(k0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = few_load16(row + 2 * static_cast<int64_t>(few_x_at<F>(s, j)));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = few_x_at<F>(s, j);
-      if constexpr (F::dense)
-        x[j] = few_cut16(row, k, K);
-      else  // (whole pieces: K % 32 == 0)
-        x[j] = k < K ? few_load16(row + 2 * static_cast<int64_t>(k)) : lin_u32x4_t{0, 0, 0, 0};
-    }
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (WHOLE)
+      x[j] = few_load16(at + 2 * step * j);
+    else if constexpr (F::dense)
+      x[j] = few_cut16(row, k0 + step * j, K);
+    else  // (whole pieces: K % 32 == 0)
+      x[j] = k0 + step * j < K ? few_load16(at + 2 * step * j) : lin_u32x4_t{0, 0, 0, 0};
   }
 }
 
@@ -275,10 +278,9 @@ __device__ __forceinline__ uint32_t few_param_f32(uint32_t raw, int type) {
 }
 
 // acc[p][q] += the step's product of weight rows p with x rows q.
-template <class F, int NP, int NQ, int NE>
+template <class F, int NP, int NQ, int NE, bool WHOLE>
 __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x4_t (&x)[NQ][4], int s,
                                              int K, int type, lin_f32x4_t (&acc)[NP][NQ]) {
-  const bool whole = (s + 1) * kFewStep <= K;
   if constexpr (F::dense) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -289,7 +291,7 @@ __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x
         for (int q = 0; q < NQ; ++q) acc[p][q] = few_mfma<F>(x[q][j], w, acc[p][q]);
       }
   } else if constexpr (F::mx) {
-    if (!whole) {  // (x is zero there, but a code may stand for no number)
+    if constexpr (!WHOLE) {  // (x is zero there, but a code may stand for no number)
       const int quad = (threadIdx.x & 63) >> 4;
       const uint32_t keep = s * kFewStep + 32 * quad < K ? 0xffffffffu : 0u;
 #pragma unroll
@@ -336,7 +338,7 @@ __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (!whole && s * kFewStep + 32 * j >= K) break;
+      if (!WHOLE && s * kFewStep + 32 * j >= K) break;
       lin_f32x4_t sum[NQ];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) sum[q] = few_mfma<F>(x[q][j], ones, zero);
@@ -358,8 +360,9 @@ __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x
 }
 
 // Steps [s_begin, s_end) of NP weight rows (a lane's own) with NQ x rows: BATCH steps'
-// weights are in flight beyond the ones being multiplied. Steps past the end repeat the
-// last one's loads, so that none depends on a branch.
+// weights are in flight beyond the ones being multiplied. Steps past the last whole one
+// repeat its loads, so that none depends on a branch; a step that the rows end in comes
+// last, by itself.
 template <class F, int NP, int NQ, int NE, int BATCH>
 __device__ __forceinline__ void few_product(const FewRow (&row)[NP], const FewWeight& w,
                                             const char* const (&x)[NQ], int K, int s_begin, int s_end,
@@ -368,108 +371,50 @@ __device__ __forceinline__ void few_product(const FewRow (&row)[NP], const FewWe
   for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int q = 0; q < NQ; ++q) acc[p][q] = lin_f32x4_t{0, 0, 0, 0};
-  if (s_begin >= s_end) return;
-  FewStep<F> f[2][BATCH][NP];
-  lin_u32x4_t xv[BATCH][NQ][4];
-  auto load = [&](int k, int s) __attribute__((always_inline)) {
+  const int whole = K / kFewStep, end = s_end < whole ? s_end : whole;
+  if (s_begin < end) {
+    FewStep<F> f[2][BATCH][NP];
+    lin_u32x4_t xv[BATCH][NQ][4];
+    auto load = [&](int k, int s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int at = s + i < s_end ? s + i : s_end - 1;
+      for (int i = 0; i < BATCH; ++i) {
+        const int at = s + i < end ? s + i : end - 1;
 #pragma unroll
-      for (int p = 0; p < NP; ++p) few_load<F>(f[k][i][p], row[p], w, at, K);
-    }
-  };
-  auto load_x = [&](int s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int at = s + i < s_end ? s + i : s_end - 1;
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) few_load_x<F>(xv[i][q], x[q], at, K);
-    }
-  };
-  auto multiply = [&](int k, int s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i)
-      if (s + i < s_end) few_multiply<F, NP, NQ, NE>(f[k][i], xv[i], s + i, K, w.type, acc);
-  };
-  load(0, s_begin);
-  for (int s = s_begin; s < s_end; s += 2 * BATCH) {
-    load_x(s);
-    if (s + BATCH < s_end) load(1, s + BATCH);
-    multiply(0, s);
-    if (s + BATCH >= s_end) break;
-    load_x(s + BATCH);
-    if (s + 2 * BATCH < s_end) load(0, s + 2 * BATCH);
-    multiply(1, s + BATCH);
-  }
-}
-
-// Waves hand LDS over without waiting for the loads that they have in flight into
-// registers (__syncthreads would, and with it for the next tile's weights).
-__device__ __forceinline__ void few_handover() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
-// Tiles [t0, t1) of 16 NP weight rows, one after the other, times up to 16 x rows (a lane's
-// own: `x`). The workgroup's waves share the contraction, at most XS steps each, so that
-// the x rows stay in registers; the next tile's weights are in flight while one is
-// multiplied. rows(t, FewRow (&)[NP]) says where tile t's weight rows are, emit(t, sums)
-// takes its results in one of the waves. part: 2 WAVES NP 64 accumulators of LDS. Every wave
-// of the workgroup calls this with the same tiles.
-template <class F, int NP, int NE, int XS, int WAVES, typename Rows, typename Emit>
-__device__ __forceinline__ void few_stream(const FewWeight& w, const char* x, int K, int t0, int t1,
-                                           lin_f32x4_t* part, Rows&& rows, Emit&& emit) {
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int steps = (K + kFewStep - 1) / kFewStep;
-  const int s0 = steps * wave / WAVES, s1 = steps * (wave + 1) / WAVES;
-  FewStep<F> f[2][XS][NP];
-  auto load = [&](int k, int t) __attribute__((always_inline)) {
-    FewRow row[NP];
-    rows(t < t1 ? t : t1 - 1, row);
-#pragma unroll
-    for (int i = 0; i < XS; ++i) {
-      // (a step that is not this wave's repeats one that is, or the row's last)
-      const int at = s0 + i < s1 ? s0 + i : s1 > s0 ? s1 - 1 : steps - 1;
-#pragma unroll
-      for (int p = 0; p < NP; ++p) few_load<F>(f[k][i][p], row[p], w, at, K);
-    }
-  };
-  load(0, t0);
-  lin_u32x4_t xv[XS][1][4];
-#pragma unroll
-  for (int i = 0; i < XS; ++i) few_load_x<F>(xv[i][0], x, s0 + i < s1 ? s0 + i : steps - 1, K);
-  auto tile = [&](int k, int t) __attribute__((always_inline)) {
-    if (t + 1 < t1) load(k ^ 1, t + 1);
-    lin_f32x4_t acc[NP][1];
-#pragma unroll
-    for (int p = 0; p < NP; ++p) acc[p][0] = lin_f32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < XS; ++i)
-      if (s0 + i < s1) few_multiply<F, NP, 1, NE>(f[k][i], xv[i], s0 + i, K, w.type, acc);
-    lin_f32x4_t* own = part + k * (WAVES * NP * 64);
-#pragma unroll
-    for (int p = 0; p < NP; ++p) own[(wave * NP + p) * 64 + lane] = acc[p][0];
-    few_handover();
-    // (the other half of `part` is free: who summed the last tile has come past the barrier)
-    if (wave == (t & (WAVES - 1))) {
-      lin_f32x4_t sum[NP];
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        sum[p] = own[p * 64 + lane];
-#pragma unroll
-        for (int o = 1; o < WAVES; ++o) {
-          const lin_f32x4_t v = own[(o * NP + p) * 64 + lane];
-#pragma unroll
-          for (int e = 0; e < NE; ++e) sum[p][e] += v[e];
-        }
+        for (int p = 0; p < NP; ++p) few_load<F, true>(f[k][i][p], row[p], w, at, K);
       }
-      emit(t, sum);
+    };
+    auto load_x = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int at = s + i < end ? s + i : end - 1;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) few_load_x<F, true>(xv[i][q], x[q], at, K);
+      }
+    };
+    auto multiply = [&](int k, int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i)
+        if (s + i < end) few_multiply<F, NP, NQ, NE, true>(f[k][i], xv[i], s + i, K, w.type, acc);
+    };
+    load(0, s_begin);
+    for (int s = s_begin; s < end; s += 2 * BATCH) {
+      load_x(s);
+      if (s + BATCH < end) load(1, s + BATCH);
+      multiply(0, s);
+      if (s + BATCH >= end) break;
+      load_x(s + BATCH);
+      if (s + 2 * BATCH < end) load(0, s + 2 * BATCH);
+      multiply(1, s + BATCH);
     }
-  };
-  for (int t = t0; t < t1; t += 2) {
-    tile(0, t);
-    if (t + 1 < t1) tile(1, t + 1);
+  }
+  if (s_end > whole && s_begin < s_end) {
+    FewStep<F> f[NP];
+    lin_u32x4_t xv[NQ][4];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) few_load<F, false>(f[p], row[p], w, whole, K);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) few_load_x<F, false>(xv[q], x[q], whole, K);
+    few_multiply<F, NP, NQ, NE, false>(f, xv, whole, K, w.type, acc);
   }
 }
 

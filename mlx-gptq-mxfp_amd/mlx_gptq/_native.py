@@ -52,6 +52,14 @@ _F32 = ctypes.c_float
 _F64 = ctypes.c_double
 _SZ = ctypes.c_size_t
 
+
+class Weight(ctypes.Structure):
+    """mgq_weight: a layer's weight for mgq_experts_decode."""
+
+    _fields_ = [("data", _VP), ("scales", _VP), ("biases", _VP), ("ld", _I64), ("expert", _I64),
+                ("group", _I64), ("format", _INT), ("param_dtype", _INT)]
+
+
 # name -> argtypes (every entry point returns int status unless listed in _RESTYPES)
 SIGNATURES: dict[str, list] = {
     "mgq_version": [],
@@ -116,8 +124,7 @@ SIGNATURES: dict[str, list] = {
     "mgq_top_k_softmax": [_VP, _INT, _I64, _I64, _I64, _I64, _INT, _VP, _VP, _VP],
     "mgq_top_k_softmax_grad": [_VP, _VP, _INT, _I64, _I64, _I64, _VP, _I64, _INT, _VP, _VP],
     "mgq_experts_decode_workspace_size": [_I64, _I64, _I64],
-    "mgq_experts_decode": [_VP, _INT, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _I64, _I64, _VP, _INT,
-                           _I64, _I64, _VP, _VP, _I64, _VP, _INT, _I64, _I64, _VP, _VP, _I64, _INT,
+    "mgq_experts_decode": [_VP, _INT, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _I64, _I64, _VP, _VP,
                            _VP, _VP, _I64, _VP],
     "mgq_linear_choice": [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64, _INT, _VP],
 }

@@ -28,6 +28,7 @@ No call waits for the device: the routing stays there.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -150,6 +151,40 @@ def route(top_k_index: torch.Tensor, num_experts: int) -> Routing:
     return Routing(offsets, row_index, entry)
 
 
+class _DecodeWeights:
+    """What ExpertMLP.decode passes of its weights."""
+
+    def __init__(self, cols, dtype, device, inner, up, down, gate_up, down_weight, tensors):
+        self.cols, self.dtype, self.device, self.inner = cols, dtype, device, inner
+        self.type_code = nat.dtype_code(dtype)
+        self.up, self.down = up, down
+        self.up_ptr, self.down_ptr = ctypes.addressof(up), ctypes.addressof(down)
+        self.given = gate_up, down_weight
+        # copies (of host weights, or of ones whose rows do not lie one after the other) go
+        # with this call: only weights described where they are stand for the next one
+        flat = [t for w in self.given for t in ((w,) if isinstance(w, torch.Tensor) else w)]
+        ptrs = [t.data_ptr() for t in tensors]
+        self.in_place = ptrs == [t.data_ptr() for t in flat]
+        self.tensors, self.layout = tensors, [(t, t.data_ptr(), t.shape, t.stride()) for t in flat]
+        self._sizes: dict[tuple[int, int], int] = {}
+
+    def current(self, layer) -> bool:
+        if not self.in_place or layer.gate_up is not self.given[0] or layer.down is not self.given[1]:
+            return False
+        for t, ptr, shape, stride in self.layout:
+            if t.data_ptr() != ptr or t.shape != shape or t.stride() != stride:
+                return False
+        return True
+
+    def workspace(self, T: int, k: int) -> int:
+        try:
+            return self._sizes[T, k]
+        except KeyError:
+            size = nat.load().mgq_experts_decode_workspace_size(T, k, self.inner)
+            self._sizes[T, k] = size
+            return size
+
+
 class ExpertMLP:
     """Experts gate_up [E, 2 I, H] and down [E, H, I] in one of the formats.
 
@@ -169,6 +204,7 @@ class ExpertMLP:
         if first.dim() != 3 or first.shape[1] % 2:
             raise ValueError(f"ExpertMLP: gate_up must be [E, 2 I, H] (got {tuple(first.shape)})")
         self.num_experts = int(first.shape[0])
+        self._described: _DecodeWeights | None = None
 
     @classmethod
     def from_weights(cls, gate_up: torch.Tensor, down: torch.Tensor, mode: str = "dense",
@@ -234,8 +270,7 @@ class ExpertMLP:
 
     def _decode_weight(self, weight, out_rows: int, cols: int, dtype: torch.dtype,
                        dev: torch.device):
-        """(tensors kept alive, the weight's arguments of mgq_experts_decode, its scales'
-        type)."""
+        """(nat.Weight, its tensors) for rows of `cols` of `dtype`."""
         fn, E = "ExpertMLP.decode", self.num_experts
         if self.mode == "dense":
             if weight.dtype != dtype:
@@ -244,20 +279,39 @@ class ExpertMLP:
                 raise AssertionError(f"{fn}: expects weights {(E, out_rows, cols)} "
                                      f"(got {tuple(weight.shape)})")
             w = linear._pitched(weight, dev)
-            return (w,), (w.data_ptr(), nat.WEIGHT_DENSE, linear._ld(w), w.stride(0), None, None, 0), None
+            return nat.Weight(w.data_ptr(), None, None, linear._ld(w), w.stride(0), 0,
+                              nat.WEIGHT_DENSE, 0), (w,)
         bits = 32 * weight[0].shape[-1] // max(cols, 1)
         if weight[0].shape[:-1] != (E, out_rows):
             raise AssertionError(f"{fn}: expects weights {(E, out_rows, cols)} "
                                  f"(words {tuple(weight[0].shape)})")
+        params = 0
         if self.mode == "affine":
-            group = linear.affine_group(fn, cols, bits, *weight)
+            packed, scales, biases = weight
+            group = linear.affine_dims(fn, cols, bits, packed.shape, packed.dtype, scales.shape,
+                                       scales.dtype, biases.shape, biases.dtype, True)[2]
             code = {2: nat.WEIGHT_AFFINE2, 4: nat.WEIGHT_AFFINE4, 8: nat.WEIGHT_AFFINE8}[bits]
+            params = nat.dtype_code(scales.dtype)
         else:
             linear.check_mxfp(fn, cols, self.mode, *weight)
             group, code = 32, nat.WEIGHT_MXFP4 if self.mode == "mxfp4" else nat.WEIGHT_MXFP8
         t = tuple(linear._dense(w, dev) for w in weight)
-        biases = t[2].data_ptr() if len(t) > 2 else None
-        return t, (t[0].data_ptr(), code, 0, 0, t[1].data_ptr(), biases, group), t[1].dtype
+        return nat.Weight(t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr() if len(t) > 2 else None,
+                          0, 0, group, code, params), t
+
+    def _decode_weights(self, cols: int, dtype: torch.dtype, dev: torch.device):
+        """Both weights as mgq_experts_decode takes them: described once, and again for
+        other rows or when a tensor is no longer the one described."""
+        d = self._described
+        if d is not None and d.cols == cols and d.dtype is dtype and d.device == dev and d.current(self):
+            return d
+        gate_up, down = self.gate_up, self.down
+        inner = (gate_up if self.mode == "dense" else gate_up[0]).shape[1] // 2
+        up, up_tensors = self._decode_weight(gate_up, 2 * inner, cols, dtype, dev)
+        dn, dn_tensors = self._decode_weight(down, cols, inner, dtype, dev)
+        self._described = _DecodeWeights(cols, dtype, dev, inner, up, dn, gate_up, down,
+                                         up_tensors + dn_tensors)
+        return self._described
 
     def decode(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                top_k_weights: torch.Tensor) -> torch.Tensor:
@@ -292,26 +346,21 @@ class ExpertMLP:
             raise ValueError(f"{fn}: up to 64 rows with 1 to 16 experts each (got {(T, k)}); "
                              "forward takes any number")
         dev = linear._device(x, *(dense or self.gate_up[:1]))
-        first = self.gate_up if dense else self.gate_up[0]
-        inner = first.shape[1] // 2
-        up, up_args, param = self._decode_weight(self.gate_up, 2 * inner, H, x.dtype, dev)
-        down, down_args, other = self._decode_weight(self.down, H, inner, x.dtype, dev)
-        if param != other:
-            raise TypeError(f"{fn}: the scales of gate_up and down differ in type ({param}, {other})")
+        d = self._decode_weights(H, x.dtype, dev)
         xd = linear._pitched(x, dev)
         index = top_k_index
         if index.dtype is not torch.int64:
             index = linear._int32(index)
         index = linear._dense(index, dev)
-        weights = linear._dense(top_k_weights.float(), dev)
+        weights = top_k_weights if top_k_weights.dtype is torch.float32 else top_k_weights.float()
+        weights = linear._dense(weights, dev)
         out = torch.empty(T, H, dtype=x.dtype, device=dev)
-        if out.numel():
-            size = nat.load().mgq_experts_decode_workspace_size(T, k, inner)
+        if T and H:
+            size = d.workspace(T, k)
             ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            params = nat.DTYPE_BF16 if self.mode != "affine" else nat.dtype_code(param)
-            nat.launch(dev, "mgq_experts_decode", xd.data_ptr(), nat.dtype_code(x.dtype), T,
-                       linear._ld(xd), index.data_ptr(), 8 * index.element_size(), weights.data_ptr(),
-                       k, self.num_experts, H, inner, *up_args, *down_args, params, out.data_ptr(),
+            nat.launch(dev, "mgq_experts_decode", xd.data_ptr(), d.type_code, T, linear._ld(xd),
+                       index.data_ptr(), 64 if index.dtype is torch.int64 else 32, weights.data_ptr(),
+                       k, self.num_experts, H, d.inner, d.up_ptr, d.down_ptr, out.data_ptr(),
                        ws.data_ptr(), size)
         out = linear._home(out, x)
         return linear._NoGradient.apply(fn, out, x, top_k_weights, *dense) if tracked else out

@@ -34,6 +34,8 @@ staged through the current HIP device, as in the other modules.
 
 from __future__ import annotations
 
+import functools
+
 import numpy as np
 import torch
 from torch.autograd import forward_ad
@@ -373,27 +375,33 @@ def mxfp_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, mod
     return _NoGradient.apply(fn, y, x) if tracked else y
 
 
-def affine_group(fn: str, cols: int, bits: int, packed: torch.Tensor, scales: torch.Tensor,
-                 biases: torch.Tensor) -> int:
-    """The group size of an affine weight [..., N, cols], its tensors checked."""
+@functools.lru_cache(maxsize=1024)
+def affine_dims(fn: str, cols: int, bits: int, words: torch.Size, word_type: torch.dtype,
+                scales: torch.Size, scale_type: torch.dtype, biases: torch.Size,
+                bias_type: torch.dtype, grouped: bool) -> tuple[int, int, int]:
+    """(groups, rows, group size) of an affine weight for rows of `cols`, its tensors'
+    shapes and types checked. (Remembered by these: a single token's product takes about
+    as long as the checks.)"""
     if bits not in _AFFINE_BITS:
         raise ValueError(f"{fn}: bits must be one of {_AFFINE_BITS} (got {bits})")
-    if packed.dtype not in _WORDS:
-        raise TypeError(f"{fn}: expects 32-bit words (got {packed.dtype})")
-    if scales.dtype not in _FLOATS or biases.dtype != scales.dtype:
+    if word_type not in _WORDS:
+        raise TypeError(f"{fn}: expects 32-bit words (got {word_type})")
+    if scale_type not in _FLOATS or bias_type != scale_type:
         raise TypeError(f"{fn}: scales and biases must be float32, bfloat16 or float16 of one type "
-                        f"(got {scales.dtype} and {biases.dtype})")
-    shape = packed.shape
-    if not cols or cols * bits != shape[-1] * 32:
-        raise AssertionError(f"{fn}: x has {cols} columns, the words hold {shape[-1] * 32 // bits}")
-    n = scales.shape[-1] if scales.dim() else 0
+                        f"(got {scale_type} and {bias_type})")
+    if len(words) != 2 + grouped:
+        with_, dims = ("with", "[G, N, K]") if grouped else ("without", "[N, K]")
+        raise ValueError(f"{fn}: {with_} offsets the weight is {dims} (got words {tuple(words)})")
+    if not cols or cols * bits != words[-1] * 32:
+        raise AssertionError(f"{fn}: x has {cols} columns, the words hold {words[-1] * 32 // bits}")
+    n = scales[-1] if scales else 0
     group = cols // n if n and cols % n == 0 else 0
     if group not in _AFFINE_GROUPS:
         raise ValueError(f"{fn}: groups of 32, 64 or 128 values (got {n} scales for {cols})")
-    if scales.shape[:-1] != shape[:-1] or biases.shape != scales.shape:
-        raise AssertionError(f"{fn}: scales and biases must be {(*shape[:-1], n)} "
-                             f"(got {tuple(scales.shape)} and {tuple(biases.shape)})")
-    return group
+    if scales[:-1] != words[:-1] or biases != scales:
+        raise AssertionError(f"{fn}: scales and biases must be {(*words[:-1], n)} "
+                             f"(got {tuple(scales)} and {tuple(biases)})")
+    return (words[0] if grouped else 1), words[-2], group
 
 
 def affine_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
@@ -414,19 +422,23 @@ def affine_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, b
     if x.dtype not in _HALF:
         raise TypeError(f"{fn}: expects bfloat16 or float16 rows (got {x.dtype})")
     _rows2(fn, "x", x)
-    w = _weight3(fn, packed, offsets)
-    group = affine_group(fn, int(x.shape[1]), bits, packed, scales, biases)
-    G, N, _ = w.shape
+    T, K = x.shape
+    st = scales.dtype
+    G, N, group = affine_dims(fn, K, bits, packed.shape, packed.dtype, scales.shape, st, biases.shape,
+                              biases.dtype, offsets is not None)
     dev = _device(x, packed, scales)
     xd = _pitched(x, dev)
-    wd, sd, bd = _dense(w, dev), _dense(scales, dev), _dense(biases, dev)
-    off, idx, M = _list(fn, offsets, row_index, G, int(x.shape[0]), dev, validate)
+    wd, sd, bd = _dense(packed, dev), _dense(scales, dev), _dense(biases, dev)
+    off = idx = None
+    M = T
+    if offsets is not None or row_index is not None:
+        off, idx, M = _list(fn, offsets, row_index, G, T, dev, validate)
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
     if M and N:
-        nat.launch(dev, "mgq_affine_linear", xd.data_ptr(), nat.dtype_code(x.dtype), xd.shape[0],
-                   _ld(xd), nat.ptr(idx), M, wd.data_ptr(), sd.data_ptr(), bd.data_ptr(),
-                   nat.dtype_code(scales.dtype), bits, group, G, N, xd.shape[1], nat.ptr(off),
-                   y.data_ptr())
+        nat.launch(dev, "mgq_affine_linear", xd.data_ptr(), nat.dtype_code(x.dtype), T, _ld(xd),
+                   None if idx is None else idx.data_ptr(), M, wd.data_ptr(), sd.data_ptr(),
+                   bd.data_ptr(), nat.dtype_code(st), bits, group, G, N, K,
+                   None if off is None else off.data_ptr(), y.data_ptr())
     y = _home(y, x)
     return _NoGradient.apply(fn, y, x, scales, biases) if tracked else y
 

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -45,7 +47,7 @@ def call(layer, x=(3, 64), index=(3, 2), weights=None, dtype=BF, index_type=torc
 
 def test_what_is_taken_reaches_the_launch():
     for layer in (dense(), words("mxfp4"), words("mxfp8", bits=8), words("affine"),
-                  words("affine", bits=2, params=F32)):
+                  words("affine", bits=2, params=F32), words("affine", down_params=F32)):
         with pytest.raises(RuntimeError, match="launched"):
             call(layer)
     with pytest.raises(RuntimeError, match="launched"):
@@ -70,7 +72,6 @@ def test_what_is_taken_reaches_the_launch():
     (lambda: words("mxfp4"), dict(dtype=F16), TypeError),
     (lambda: words("mxfp4"), dict(x=(3, 32)), AssertionError),
     (lambda: words("affine"), dict(x=(3, 32)), ValueError),
-    (lambda: words("affine", params=BF, down_params=F32), {}, TypeError),
     (lambda: ExpertMLP((torch.zeros(4, 64, 64, dtype=torch.int8), torch.zeros(4, 64)),
                        (torch.zeros(4, 64, 32, dtype=torch.int8), torch.zeros(4, 64)), "int8"), {},
      ValueError),
@@ -93,23 +94,53 @@ def test_formats_of_a_layer():
 
 
 OK = dict(X=16, dtype=nat.DTYPE_BF16, T=3, ldx=64, index=16, index_bits=64, weights=16, k=2, E=4, H=64,
-          I=32, up=16, up_format=nat.WEIGHT_AFFINE4, up_ld=0, up_expert=0, up_scales=16, up_biases=16,
-          up_group=32, down=16, down_format=nat.WEIGHT_DENSE, down_ld=32, down_expert=2048,
-          down_scales=None, down_biases=None, down_group=0, params=nat.DTYPE_BF16, out=16, ws=16,
-          ws_bytes=1 << 20, stream=None)
+          I=32, up=None, down=None, out=16, ws=16, ws_bytes=1 << 20, stream=None)
+UP = dict(data=16, scales=16, biases=16, ld=0, expert=0, group=32, format=nat.WEIGHT_AFFINE4,
+          param_dtype=nat.DTYPE_BF16)
+DOWN = dict(data=16, scales=None, biases=None, ld=32, expert=2048, group=0, format=nat.WEIGHT_DENSE,
+            param_dtype=0)
+
+
+def entry(up=None, down=None, **change):
+    u, d = nat.Weight(**{**UP, **(up or {})}), nat.Weight(**{**DOWN, **(down or {})})
+    args = {**OK, "up": ctypes.addressof(u), "down": ctypes.addressof(d), **change}
+    return nat.load().mgq_experts_decode(*args.values())
 
 
 @pytest.mark.parametrize("change,status", [
     (dict(dtype=nat.DTYPE_F32), nat.ERR_VALUE), (dict(index_bits=16), nat.ERR_VALUE),
     (dict(T=65), nat.ERR_SHAPE), (dict(k=17), nat.ERR_SHAPE), (dict(k=0), nat.ERR_SHAPE),
     (dict(E=0), nat.ERR_SHAPE), (dict(I=0), nat.ERR_SHAPE), (dict(ldx=63), nat.ERR_SHAPE),
-    (dict(up_format=6), nat.ERR_VALUE), (dict(up_group=16), nat.ERR_VALUE),
-    (dict(params=7), nat.ERR_VALUE), (dict(H=96, ldx=96, up_group=64), nat.ERR_SHAPE),
-    (dict(down_ld=31), nat.ERR_SHAPE), (dict(down_format=nat.WEIGHT_MXFP4, I=48), nat.ERR_SHAPE),
-    (dict(dtype=nat.DTYPE_F16, down_format=nat.WEIGHT_MXFP8), nat.ERR_VALUE),
+    (dict(up=dict(format=6)), nat.ERR_VALUE), (dict(up=dict(group=16)), nat.ERR_VALUE),
+    (dict(up=dict(param_dtype=7)), nat.ERR_VALUE),
+    (dict(H=96, ldx=96, up=dict(group=64)), nat.ERR_SHAPE),
+    (dict(down=dict(ld=31)), nat.ERR_SHAPE), (dict(down=dict(ld=1 << 29)), nat.ERR_SHAPE),
+    (dict(down=dict(format=nat.WEIGHT_MXFP4), I=48), nat.ERR_SHAPE),
+    (dict(dtype=nat.DTYPE_F16, down=dict(format=nat.WEIGHT_MXFP8)), nat.ERR_VALUE),
     (dict(ws_bytes=100), nat.ERR_WORKSPACE)])
 def test_entry_point_returns_a_status(change, status):
-    entry = nat.load().mgq_experts_decode
-    assert entry(*{**OK, **change}.values()) == status
+    assert entry(**change) == status
     assert "experts_decode" in nat.last_error()
-    assert entry(*{**OK, "T": 0}.values()) == nat.OK
+    assert entry(T=0) == nat.OK
+
+
+def test_the_weights_are_described_anew_when_they_change():
+    """A tensor put in another's place, moved or reshaped is seen; one that is written is
+    the same."""
+    layer = dense()
+    cpu = torch.device("cpu")
+    first = layer._decode_weights(64, BF, cpu)
+    layer.gate_up.fill_(1.0)
+    assert layer._decode_weights(64, BF, cpu) is first
+    layer.gate_up = layer.gate_up.clone()
+    second = layer._decode_weights(64, BF, cpu)
+    assert second is not first and second.up.data == layer.gate_up.data_ptr()
+    layer.down.data = layer.down.data.clone()
+    third = layer._decode_weights(64, BF, cpu)
+    assert third is not second and third.down.data == layer.down.data_ptr()
+    with pytest.raises(AssertionError):
+        layer._decode_weights(32, BF, cpu)
+    # copies are made again for every call
+    layer.down = torch.zeros(4, 32, 64, dtype=BF).transpose(1, 2)
+    a = layer._decode_weights(64, BF, cpu)
+    assert layer._decode_weights(64, BF, cpu) is not a
