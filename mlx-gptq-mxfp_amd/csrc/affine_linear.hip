@@ -11,10 +11,11 @@
 namespace mgq {
 namespace {
 
-template <class F, int NP, int NQ, int NE, int WAVES, int BATCH>
+template <class F, int NP, int NQ, int NE, int WAVES, int DEPTH>
 __global__ void __launch_bounds__(64 * WAVES) affine_few_kernel(const LinArgs a, const FewWeight w) {
   constexpr int BM = NE == 1 ? 4 : 16 * NQ;
   __shared__ lin_f32x4_t part[WAVES * NP * NQ * 64];
+  __shared__ __attribute__((aligned(16))) char params[WAVES * few_lds<F, NP>()];
   LinTile t;
   if (!lin_find_tile<BM>(a, (a.np + 16 * NP - 1) / (16 * NP), &t)) return;
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
@@ -34,8 +35,8 @@ __global__ void __launch_bounds__(64 * WAVES) affine_few_kernel(const LinArgs a,
     x[j] = a.Q + lin_row(a, q < t.q_end ? q : t.q_end - 1) * a.ldq;
   }
   lin_f32x4_t acc[NP][NQ];
-  few_product<F, NP, NQ, NE, BATCH>(row, w, x, a.nc, steps * wave / WAVES, steps * (wave + 1) / WAVES,
-                                    acc);
+  few_product<F, NP, NQ, NE, DEPTH>(row, w, x, a.nc, steps * wave / WAVES, steps * (wave + 1) / WAVES,
+                                    params + wave * few_lds<F, NP>(), acc);
 #pragma unroll
   for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -87,11 +88,11 @@ __global__ void __launch_bounds__(256) affine_gemv_kernel(const LinArgs a, const
     }
 }
 
-template <class F, int NP, int NQ, int NE, int WAVES, int BATCH>
+template <class F, int NP, int NQ, int NE, int WAVES, int DEPTH>
 int launch_few(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
   const int64_t grid = lin_row_tiles(a, NE == 1 ? 4 : 16 * NQ) * ceil_div(a.np, 16 * NP);
   MGQ_REQUIRE(grid < kLinFewGrid * 4 / WAVES, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  affine_few_kernel<F, NP, NQ, NE, WAVES, BATCH>
+  affine_few_kernel<F, NP, NQ, NE, WAVES, DEPTH>
       <<<static_cast<unsigned>(grid), 64 * WAVES, 0, s>>>(a, w);
   return check_launch(what);
 }
@@ -116,20 +117,21 @@ int run(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
 #ifdef AFFINE_FORCE
   const int per = mgq_force[1];
   switch (mgq_force[0]) {
-    case 1: return launch_few<F, 1, 1, 1, 4, 2>(a, w, s, what);
-    case 2: return launch_few<F, 1, 1, 4, 4, 2>(a, w, s, what);
-    case 3: return launch_few<F, 2, 4, 4, 4, 1>(a, w, s, what);
-    case 4: return launch_few<F, 2, 2, 4, 4, 1>(a, w, s, what);
     case 5: return launch_gemv<F>(a, w, s, what);
-    case 6: return launch_few<F, 1, 1, 1, 4, 4>(a, w, s, what);
-    case 7: return launch_few<F, 1, 1, 4, 4, 4>(a, w, s, what);
-    case 8: return launch_few<F, 2, 1, 4, 4, 2>(a, w, s, what);
+    case 1: return launch_few<F, 1, 1, 1, 4, 4>(a, w, s, what);
+    case 2: return launch_few<F, 2, 1, 1, 4, 4>(a, w, s, what);
+    case 3: return launch_few<F, 4, 1, 1, 4, 4>(a, w, s, what);
+    case 6: return launch_few<F, 1, 1, 4, 4, 4>(a, w, s, what);
+    case 7: return launch_few<F, 2, 1, 4, 4, 2>(a, w, s, what);
+    case 8: return launch_few<F, 2, 1, 4, 4, 4>(a, w, s, what);
     case 9: return launch_few<F, 4, 1, 4, 4, 2>(a, w, s, what);
-    case 10: return launch_few<F, 4, 1, 4, 4, 1>(a, w, s, what);
-    case 11: return launch_few<F, 1, 1, 4, 8, 2>(a, w, s, what);
-    case 12: return launch_few<F, 2, 1, 4, 8, 2>(a, w, s, what);
-    case 13: return launch_few<F, 4, 2, 4, 4, 1>(a, w, s, what);
-    case 14: return launch_few<F, 4, 4, 4, 4, 1>(a, w, s, what);
+    case 10: return launch_few<F, 4, 1, 4, 4, 4>(a, w, s, what);
+    case 11: return launch_few<F, 4, 1, 4, 8, 2>(a, w, s, what);
+    case 12: return launch_few<F, 4, 1, 4, 8, 4>(a, w, s, what);
+    case 13: return launch_few<F, 4, 2, 4, 4, 2>(a, w, s, what);
+    case 14: return launch_few<F, 4, 2, 4, 4, 3>(a, w, s, what);
+    case 15: return launch_few<F, 4, 4, 4, 4, 2>(a, w, s, what);
+    case 16: return launch_few<F, 2, 4, 4, 4, 2>(a, w, s, what);
     case 30: case 31: case 32: case 33: {
       LinArgs b = a;
       b.P = w.p; b.Ps = reinterpret_cast<const uint8_t*>(w.s); b.Pb = reinterpret_cast<const uint8_t*>(w.b);

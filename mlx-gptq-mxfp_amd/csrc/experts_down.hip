@@ -11,9 +11,10 @@
 namespace mgq {
 namespace {
 
-template <class F, int NE, int WAVES, int BATCH>
+template <class F, int NE, int WAVES, int DEPTH>
 __global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArgs a) {
   extern __shared__ float lds[];
+  __shared__ __attribute__((aligned(16))) char params[F::dense ? 16 : WAVES * few_lds<F, 1>()];
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float* sums = lds + wave * a.T * 16;  // [T][16]
@@ -36,7 +37,7 @@ __global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArg
     const int entry = entries[first + (own < count ? own : count - 1)].entry;
     const char* const x[1] = {a.act + static_cast<int64_t>(entry) * a.I * 2};
     lin_f32x4_t acc[1][1];
-    few_product<F, 1, 1, NE, BATCH>(row, a.down, x, a.I, 0, steps, acc);
+    few_product<F, 1, 1, NE, DEPTH>(row, a.down, x, a.I, 0, steps, params + wave * few_lds<F, 1>(), acc);
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const int j = NE == 1 ? quad : 4 * quad + e;
@@ -57,9 +58,9 @@ __global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArg
   }
 }
 
-template <class F, int NE, int WAVES, int BATCH>
+template <class F, int NE, int WAVES, int DEPTH>
 int launch(const DecodeArgs& a, hipStream_t s, const char* what) {
-  decode_down_kernel<F, NE, WAVES, BATCH>
+  decode_down_kernel<F, NE, WAVES, DEPTH>
       <<<static_cast<unsigned>(ceil_div(a.H, 16)), 64 * WAVES, WAVES * a.T * 64 + 16 * a.n, s>>>(a);
   return check_launch(what);
 }
@@ -127,8 +128,8 @@ int decode_down(const DecodeArgs& a, int format, hipStream_t s, const char* what
              : lanes == 32 ? launch_single<F, 32>(a, s, what)
                            : launch_single<F, 16>(a, s, what);
     }
-    if (a.T <= 4) return launch<F, 1, 8, 2>(a, s, what);
-    return launch<F, 4, 8, 2>(a, s, what);
+    if (a.T <= 4) return launch<F, 1, 8, 3>(a, s, what);
+    return launch<F, 4, 8, 3>(a, s, what);
   });
 }
 

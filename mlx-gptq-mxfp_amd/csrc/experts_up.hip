@@ -79,12 +79,13 @@ __device__ __forceinline__ float decode_act(float gate, float up) {
   return gate / (1.0f + expf(-gate)) * up;
 }
 
-template <class F, int NE, int BATCH>
+template <class F, int NE, int DEPTH>
 __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs a) {
   constexpr int BM = NE == 1 ? 4 : 16;
   __shared__ __attribute__((aligned(16))) int16_t list[kDecodeEntries];
   __shared__ uint32_t carry[kWaves];
   __shared__ lin_f32x4_t part[kWaves * 2 * 64];
+  __shared__ __attribute__((aligned(16))) char params[F::dense ? 16 : kWaves * few_lds<F, 2>()];
   if (blockIdx.x == 0) {
     decode_plan(a, list, carry);
     return;
@@ -119,8 +120,9 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
     const int entry = list[j < count ? j : count - 1];
     const char* const x[1] = {a.x + entry / a.k * a.ldx};
     lin_f32x4_t acc[2][1];
-    few_product<F, 2, 1, NE, BATCH>(row, a.up, x, a.H, steps * wave / kWaves,
-                                    steps * (wave + 1) / kWaves, acc);
+    few_product<F, 2, 1, NE, DEPTH>(row, a.up, x, a.H, steps * wave / kWaves,
+                                    steps * (wave + 1) / kWaves,
+                                    params + wave * few_lds<F, 2>(), acc);
     part[(2 * wave) * 64 + lane] = acc[0][0];
     part[(2 * wave + 1) * 64 + lane] = acc[1][0];
     __syncthreads();

@@ -11,14 +11,16 @@
 //   dense       four 16-byte pieces, elements 32 j + 8 quad of the step for MFMA j;
 //   MXFP        the 32 codes of the step's group `quad` and their scale byte, decoded
 //               to bf16 exactly; MFMA j takes codes 8 j .. 8 j + 7 of every group;
-//   affine      the 32 codes of the step's block `quad` and that block's scale s and
-//               bias b. Since w = q s + b,
+//   affine      the 32 codes of the step's block `quad`. Since w = q s + b,
 //                 sum_k x w = s sum_k x q + b sum_k x      over the ks of one group,
 //               and q is exact in 16 bits: the MFMAs multiply with q itself, another
 //               one with ones gives sum x in the same layout, and s and b are applied
-//               in fp32 once for each block of 32. For that an MFMA has to stay inside a
-//               block: a 4 x 4 transposition among the quads (permlane swaps) hands
-//               MFMA j the codes of block j, and broadcasts block j's s and b.
+//               in fp32 once for each block of 32 (of 64 for longer groups). For that an
+//               MFMA has to stay inside a block: a 4 x 4 transposition among the quads
+//               (permlane swaps) hands MFMA j the codes of block j.
+// Scales come through LDS, 16 groups of a row at a time: a load of the two bytes that a
+// step needs of each of 16 rows costs as much as the step's codes (a 14336 x 4096 weight of
+// 4 bits times 16 rows: 22 us with such loads, 14 without any).
 // Up to four x rows (NE = 1) sit at A rows 0, 4, 8, 12, so that only one of a lane's
 // four results counts and s and b are applied to that one alone.
 #pragma once
@@ -82,11 +84,10 @@ __device__ __forceinline__ FewRow few_row(const FewWeight& w, int64_t g, int p0,
   return row;
 }
 
-// What a lane holds of a step: words, and the block's scale (and bias) as loaded.
+// What a lane holds of a step.
 template <class F>
 struct FewStep {
   uint32_t v[F::words];
-  uint32_t s, b;
 };
 
 struct __attribute__((packed, aligned(4))) few_u64_u_t {
@@ -119,8 +120,7 @@ __device__ __forceinline__ uint32_t few_param(const char* at) {
 // follow the row's end (dense), or a block past it reads the row's first one and
 // few_multiply discards it (quantized, K % 32 == 0).
 template <class F, bool WHOLE>
-__device__ __forceinline__ void few_load(FewStep<F>& f, const FewRow& r, const FewWeight& w, int s,
-                                         int K) {
+__device__ __forceinline__ void few_load(FewStep<F>& f, const FewRow& r, int s, int K) {
   const uint32_t quad = (threadIdx.x >> 4) & 3;
   if constexpr (F::dense) {
     const uint32_t at = r.lp + static_cast<uint32_t>(s) * (2 * kFewStep);
@@ -135,11 +135,10 @@ __device__ __forceinline__ void few_load(FewStep<F>& f, const FewRow& r, const F
       for (int i = 0; i < 4; ++i) f.v[4 * j + i] = u[i];
     }
   } else {
-    uint32_t k0 = s * kFewStep + 32 * quad, at = r.lp + static_cast<uint32_t>(s) * (16 * F::bits);
+    uint32_t at = r.lp + static_cast<uint32_t>(s) * (16 * F::bits);
     if constexpr (!WHOLE) {
-      const bool inside = k0 < static_cast<uint32_t>(K);
+      const bool inside = s * kFewStep + 32 * quad < static_cast<uint32_t>(K);
       at = inside ? at : r.lp - quad * (4 * F::bits);
-      k0 = inside ? k0 : 0;
     }
     const char* from = r.p + static_cast<uint64_t>(at);
     if constexpr (F::bits == 2) {
@@ -153,13 +152,6 @@ __device__ __forceinline__ void few_load(FewStep<F>& f, const FewRow& r, const F
 #pragma unroll
         for (int i = 0; i < 4; ++i) f.v[4 * h + i] = u[i];
       }
-    }
-    if constexpr (F::mx) {
-      f.s = *reinterpret_cast<const uint8_t*>(r.s + static_cast<uint64_t>(r.ls + k0 / 32));
-    } else {
-      const uint32_t g = r.ls + (k0 >> w.shift) * F::SB;
-      f.s = few_param<F::SB>(r.s + static_cast<uint64_t>(g));
-      f.b = few_param<F::SB>(r.b + static_cast<uint64_t>(g));
     }
   }
 }
@@ -192,16 +184,6 @@ __device__ __forceinline__ lin_f32x4_t few_mfma(lin_u32x4_t x, lin_u32x4_t w, li
                                                    __builtin_bit_cast(lin_bf16x8_t, w), c, 0, 0, 0);
 }
 
-// The four quads' values of v, each in every quad.
-__device__ __forceinline__ void few_spread(uint32_t v, uint32_t (&out)[4]) {
-  const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  const auto lo = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
-  const auto hi = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
-  out[0] = lo[0];
-  out[1] = lo[1];
-  out[2] = hi[0];
-  out[3] = hi[1];
-}
 // Word q of quad i, for word i of quad q: the 4 x 4 transposition among the quads.
 __device__ __forceinline__ void few_transpose(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
   const auto u = __builtin_amdgcn_permlane32_swap(a, c, false, false);
@@ -271,16 +253,92 @@ __device__ __forceinline__ lin_u32x4_t few_codes(const FewStep<F>& f, const uint
   return r;
 }
 
+// Scales of 16 groups of a wave's weight rows in LDS, the wave's own: affine (s, b) as two
+// floats, MXFP the bytes. A lane brings four groups of its row from memory.
+constexpr int kFewGroups = 16;
+template <class F>
+constexpr int few_pitch() {  // bytes of a row
+  return F::mx ? kFewGroups + 4 : 8 * (kFewGroups + 1);
+}
+template <class F, int NP>
+constexpr int few_lds() {  // bytes of a wave
+  return F::dense ? 0 : NP * 16 * few_pitch<F>();
+}
+template <class F>
+struct FewParams {
+  uint32_t s[F::affine ? F::SB : 1], b[F::affine ? F::SB : 1];  // four groups
+};
+template <int B>
+struct __attribute__((packed, aligned(B))) few_params_u_t {
+  uint32_t v[B];
+};
+// Four values of B bytes from g on of a row of n, those past its end like its last.
+template <int B>
+__device__ __forceinline__ void few_fetch4(const char* row, int g, int n, uint32_t (&v)[B]) {
+  if (g + 4 <= n) {
+    const few_params_u_t<B> u =
+        *reinterpret_cast<const few_params_u_t<B>*>(row + static_cast<uint64_t>(g) * B);
+#pragma unroll
+    for (int i = 0; i < B; ++i) v[i] = u.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < B; ++i) v[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const char* at = row + static_cast<uint64_t>(g + i < n ? g + i : n - 1) * B;
+      if constexpr (B == 1)
+        v[0] |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t*>(at)) << (8 * i);
+      else if constexpr (B == 2)
+        v[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at)) << (16 * (i & 1));
+      else
+        v[i] = *reinterpret_cast<const uint32_t*>(at);
+    }
+  }
+}
+template <class F>
+__device__ __forceinline__ void few_fetch(FewParams<F>& f, const FewRow& r, int g0, int n) {
+  const int g = g0 + 4 * static_cast<int>((threadIdx.x >> 4) & 3);
+  few_fetch4<F::affine ? F::SB : 1>(r.s + static_cast<uint64_t>(r.ls), g, n, f.s);
+  if constexpr (F::affine) few_fetch4<F::SB>(r.b + static_cast<uint64_t>(r.ls), g, n, f.b);
+}
 template <int SB>
 __device__ __forceinline__ uint32_t few_param_f32(uint32_t raw, int type) {
   if constexpr (SB == 4) return raw;
   return type == kF16 ? f2u(f16_to_f32(static_cast<uint16_t>(raw))) : raw << 16;
 }
+// Into LDS (the wave's reads of what was there are done: LDS serves a wave in order; the
+// fences keep the compiler to that).
+template <class F, int NP>
+__device__ __forceinline__ void few_stage(const FewParams<F> (&f)[NP], int type, char* lds) {
+  const int r16 = threadIdx.x & 15, quad = (threadIdx.x >> 4) & 3;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    char* row = lds + (16 * p + r16) * few_pitch<F>();
+    if constexpr (F::mx) {
+      *reinterpret_cast<uint32_t*>(row + 4 * quad) = f[p].s[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t s = F::SB == 4 ? f[p].s[i] : f[p].s[i / 2] >> (16 * (i & 1)) & 0xffff;
+        const uint32_t b = F::SB == 4 ? f[p].b[i] : f[p].b[i / 2] >> (16 * (i & 1)) & 0xffff;
+        *reinterpret_cast<uint2*>(row + 8 * (4 * quad + i)) =
+            uint2{few_param_f32<F::SB>(s, type), few_param_f32<F::SB>(b, type)};
+      }
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
-// acc[p][q] += the step's product of weight rows p with x rows q.
+// acc[p][q] += the step's product of weight rows p with x rows q. `first`: the group of
+// element 0 of the step, counted from the first one in LDS.
 template <class F, int NP, int NQ, int NE, bool WHOLE>
 __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x4_t (&x)[NQ][4], int s,
-                                             int K, int type, lin_f32x4_t (&acc)[NP][NQ]) {
+                                             int K, int shift, int first, const char* lds,
+                                             lin_f32x4_t (&acc)[NP][NQ]) {
+  const int r16 = threadIdx.x & 15, quad = (threadIdx.x >> 4) & 3;
   if constexpr (F::dense) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -291,14 +349,17 @@ __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x
         for (int q = 0; q < NQ; ++q) acc[p][q] = few_mfma<F>(x[q][j], w, acc[p][q]);
       }
   } else if constexpr (F::mx) {
+    uint32_t scale[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+      scale[p] = *reinterpret_cast<const uint8_t*>(lds + (16 * p + r16) * few_pitch<F>() + first + quad);
     if constexpr (!WHOLE) {  // (x is zero there, but a code may stand for no number)
-      const int quad = (threadIdx.x & 63) >> 4;
       const uint32_t keep = s * kFewStep + 32 * quad < K ? 0xffffffffu : 0u;
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
 #pragma unroll
         for (int i = 0; i < F::words; ++i) f[p].v[i] &= keep;
-        f[p].s &= keep;
+        scale[p] &= keep;
       }
     }
 #pragma unroll
@@ -307,9 +368,9 @@ __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x
       for (int p = 0; p < NP; ++p) {
         lin_u32x4_t w;
         if constexpr (F::W == kFewMx4)
-          w = lin_decode_mx4(f[p].v[j], f[p].s);
+          w = lin_decode_mx4(f[p].v[j], scale[p]);
         else
-          w = lin_decode_mx8(f[p].v[2 * j], f[p].v[2 * j + 1], f[p].s);
+          w = lin_decode_mx8(f[p].v[2 * j], f[p].v[2 * j + 1], scale[p]);
 #pragma unroll
         for (int q = 0; q < NQ; ++q) acc[p][q] = few_mfma<F>(x[q][j], w, acc[p][q]);
       }
@@ -317,11 +378,9 @@ __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x
     const uint32_t one = F::XT == kF16 ? 0x3c003c00u : 0x3f803f80u;
     const lin_u32x4_t ones = {one, one, one, one};
     const lin_f32x4_t zero = {0, 0, 0, 0};
-    uint32_t sc[NP][4], bi[NP][4], half[NP][4];
+    uint32_t half[NP][4];
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      few_spread(few_param_f32<F::SB>(f[p].s, type), sc[p]);
-      few_spread(few_param_f32<F::SB>(f[p].b, type), bi[p]);
       few_arrange<F>(f[p]);
       if constexpr (F::bits == 2) {
         // 16 codes a word, words 0 and 1 of block `quad`: MFMA j's quads 0 and 1 take
@@ -329,92 +388,118 @@ __device__ __forceinline__ void few_multiply(FewStep<F> (&f)[NP], const lin_u32x
         const auto u = __builtin_amdgcn_permlane32_swap(f[p].v[0], f[p].v[1], false, false);
         const auto a = __builtin_amdgcn_permlane16_swap(u[0], u[0], false, false);
         const auto b = __builtin_amdgcn_permlane16_swap(u[1], u[1], false, false);
-        const uint32_t up = 16 * ((threadIdx.x >> 4) & 1);
+        const uint32_t up = 16 * (quad & 1);
         half[p][0] = (a[0] >> up) & 0xffffu;
         half[p][1] = (a[1] >> up) & 0xffffu;
         half[p][2] = (b[0] >> up) & 0xffffu;
         half[p][3] = (b[1] >> up) & 0xffffu;
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (!WHOLE && s * kFewStep + 32 * j >= K) break;
+    // blocks j .. j + N - 1 lie in one group
+    auto blocks = [&](int j, auto n) __attribute__((always_inline)) {
+      constexpr int N = decltype(n)::value;
       lin_f32x4_t sum[NQ];
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) sum[q] = few_mfma<F>(x[q][j], ones, zero);
+      for (int q = 0; q < NQ; ++q) {
+        sum[q] = few_mfma<F>(x[q][j], ones, zero);
+        if constexpr (N == 2) sum[q] = few_mfma<F>(x[q][j + 1], ones, sum[q]);
+      }
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        const lin_u32x4_t w = few_codes<F>(f[p], half[p], j);
+        const float2 sb = *reinterpret_cast<const float2*>(
+            lds + (16 * p + r16) * few_pitch<F>() + 8 * (first + (32 * j >> shift)));
+        const lin_u32x4_t w0 = few_codes<F>(f[p], half[p], j);
+        lin_u32x4_t w1;
+        if constexpr (N == 2) w1 = few_codes<F>(f[p], half[p], j + 1);
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          const lin_f32x4_t d = few_mfma<F>(x[q][j], w, zero);
+          lin_f32x4_t d = few_mfma<F>(x[q][j], w0, zero);
+          if constexpr (N == 2) d = few_mfma<F>(x[q][j + 1], w1, d);
 #pragma unroll
           for (int e = 0; e < NE; ++e) {
-            acc[p][q][e] = fmaf(u2f(sc[p][j]), d[e], acc[p][q][e]);
-            acc[p][q][e] = fmaf(u2f(bi[p][j]), sum[q][e], acc[p][q][e]);
+            acc[p][q][e] = fmaf(sb.x, d[e], acc[p][q][e]);
+            acc[p][q][e] = fmaf(sb.y, sum[q][e], acc[p][q][e]);
           }
         }
+      }
+    };
+    if (WHOLE && shift > 5) {
+      blocks(0, std::integral_constant<int, 2>{});
+      blocks(2, std::integral_constant<int, 2>{});
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!WHOLE && s * kFewStep + 32 * j >= K) break;
+        blocks(j, std::integral_constant<int, 1>{});
       }
     }
   }
 }
 
-// Steps [s_begin, s_end) of NP weight rows (a lane's own) with NQ x rows: BATCH steps'
-// weights are in flight beyond the ones being multiplied. Steps past the last whole one
-// repeat its loads, so that none depends on a branch; a step that the rows end in comes
-// last, by itself.
-template <class F, int NP, int NQ, int NE, int BATCH>
+// Steps [s_begin, s_end) of NP weight rows (a lane's own) with NQ x rows. The operands of
+// DEPTH - 1 steps are in flight beyond the one being multiplied: x too, whose trip from L2
+// would otherwise be waited for in every step. A step that the rows end in comes last, by
+// itself. lds: few_lds<F, NP>() bytes of the wave's own.
+template <class F, int NP, int NQ, int NE, int DEPTH>
 __device__ __forceinline__ void few_product(const FewRow (&row)[NP], const FewWeight& w,
                                             const char* const (&x)[NQ], int K, int s_begin, int s_end,
-                                            lin_f32x4_t (&acc)[NP][NQ]) {
+                                            char* lds, lin_f32x4_t (&acc)[NP][NQ]) {
 #pragma unroll
   for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int q = 0; q < NQ; ++q) acc[p][q] = lin_f32x4_t{0, 0, 0, 0};
+  if (s_begin >= s_end) return;
   const int whole = K / kFewStep, end = s_end < whole ? s_end : whole;
-  if (s_begin < end) {
-    FewStep<F> f[2][BATCH][NP];
-    lin_u32x4_t xv[BATCH][NQ][4];
-    auto load = [&](int k, int s) __attribute__((always_inline)) {
+  const int shift = F::affine ? w.shift : 5, groups = K >> shift;
+  const int period = (kFewGroups << shift) / kFewStep;  // steps of the groups in LDS
+  int group = s_begin * kFewStep >> shift;              // the first one there
+  FewParams<F> par[NP];
+  auto fetch = [&](int g) __attribute__((always_inline)) {
+    if constexpr (!F::dense) {
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int at = s + i < end ? s + i : end - 1;
-#pragma unroll
-        for (int p = 0; p < NP; ++p) few_load<F, true>(f[k][i][p], row[p], w, at, K);
+      for (int p = 0; p < NP; ++p) few_fetch<F>(par[p], row[p], g, groups);
+    }
+  };
+  // before step s: its groups into LDS, the next ones on their way
+  auto stage = [&](int s) __attribute__((always_inline)) {
+    if constexpr (!F::dense) {
+      if (((s - s_begin) & (period - 1)) == 0) {
+        few_stage<F, NP>(par, w.type, lds);
+        group = s * kFewStep >> shift;
+        if (s + period < s_end) fetch((s + period) * kFewStep >> shift);
       }
-    };
-    auto load_x = [&](int s) __attribute__((always_inline)) {
+    }
+  };
+  FewStep<F> f[DEPTH][NP];
+  lin_u32x4_t xv[DEPTH][NQ][4];
+  auto load = [&](int d, int s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int at = s + i < end ? s + i : end - 1;
+    for (int p = 0; p < NP; ++p) few_load<F, true>(f[d][p], row[p], s, K);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) few_load_x<F, true>(xv[i][q], x[q], at, K);
-      }
-    };
-    auto multiply = [&](int k, int s) __attribute__((always_inline)) {
+    for (int q = 0; q < NQ; ++q) few_load_x<F, true>(xv[d][q], x[q], s, K);
+  };
+  fetch(group);
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i)
-        if (s + i < end) few_multiply<F, NP, NQ, NE, true>(f[k][i], xv[i], s + i, K, w.type, acc);
-    };
-    load(0, s_begin);
-    for (int s = s_begin; s < end; s += 2 * BATCH) {
-      load_x(s);
-      if (s + BATCH < end) load(1, s + BATCH);
-      multiply(0, s);
-      if (s + BATCH >= end) break;
-      load_x(s + BATCH);
-      if (s + 2 * BATCH < end) load(0, s + 2 * BATCH);
-      multiply(1, s + BATCH);
+  for (int d = 0; d < DEPTH - 1; ++d)
+    if (s_begin + d < end) load(d, s_begin + d);
+  for (int s = s_begin; s < end; s += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (s + d >= end) break;
+      if (s + d + DEPTH - 1 < end) load((d + DEPTH - 1) % DEPTH, s + d + DEPTH - 1);
+      stage(s + d);
+      few_multiply<F, NP, NQ, NE, true>(f[d], xv[d], s + d, K, shift,
+                                        ((s + d) * kFewStep >> shift) - group, lds, acc);
     }
   }
-  if (s_end > whole && s_begin < s_end) {
-    FewStep<F> f[NP];
-    lin_u32x4_t xv[NQ][4];
+  if (s_end > whole) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) few_load<F, false>(f[p], row[p], w, whole, K);
+    for (int p = 0; p < NP; ++p) few_load<F, false>(f[0][p], row[p], whole, K);
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) few_load_x<F, false>(xv[q], x[q], whole, K);
-    few_multiply<F, NP, NQ, NE, false>(f, xv, whole, K, w.type, acc);
+    for (int q = 0; q < NQ; ++q) few_load_x<F, false>(xv[0][q], x[q], whole, K);
+    stage(whole);
+    few_multiply<F, NP, NQ, NE, false>(f[0], xv[0], whole, K, shift, (whole * kFewStep >> shift) - group,
+                                       lds, acc);
   }
 }
 
