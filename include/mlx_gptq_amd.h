@@ -403,13 +403,22 @@ int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const int32_t* r
  * [n_groups, N, K * bits / 32] as mgq_pack_q writes them (bits 2, 4 or 8), scales
  * and biases: [n_groups, N, K / group_size] of param_dtype (f32/bf16/f16), all
  * contiguous; group_size 32, 64 or 128, K a multiple of it. fp32 sums, rounded
- * once: scale sum(x code) + bias sum(x) for every 32 values, so that |x| beyond
- * 1e34 may overflow where the product with decoded weights would not. */
+ * once. Few rows: scale sum(x code) + bias sum(x) for every 32 or 64 values, so that
+ * |x| beyond 1e34 may overflow where the product with decoded weights would not.
+ * Many rows: the decoded weights are rounded to dtype (mgq_affine_choice). */
 int mgq_affine_linear(const void* X, int dtype, int64_t n_rows, int64_t ldx,
                       const int32_t* row_index, int64_t n_entries, const uint32_t* words,
                       const void* scales, const void* biases, int param_dtype, int bits,
                       int64_t group_size, int64_t n_groups, int64_t N, int64_t K,
                       const int32_t* offsets, void* Y, void* stream);
+
+/* Which kernel mgq_affine_linear takes, on the host: kernel[0] 0 the one for single
+ * entries, 1 a form of the one for few rows (its number in kernel[1]), 2 or 3 a tile of
+ * kernel[1] x kernel[2] list entries x columns by loads straight into LDS or by way of
+ * registers. Tiles round the decoded weights to X's type, the others do not round them.
+ * Of X and words only the address counts. */
+int mgq_affine_choice(const void* X, int64_t ldx, int64_t n_entries, const uint32_t* words, int bits,
+                      int64_t n_groups, int64_t N, int64_t K, int grouped, int32_t* kernel);
 
 /* q = rne(x / s) within +-127, s = max |x| of the row / 127 (fp32 quotients; a
  * subnormal s may be too small for its row, whose codes stop at 127). A zero row

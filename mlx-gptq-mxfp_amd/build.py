@@ -52,7 +52,8 @@ _VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 EXTRA_FLAGS = {"gptq_mxfp.hip": _VGPR_FORM, "chol_full.hip": _VGPR_FORM,
                "gptq_affine.hip": _VGPR_FORM,
                # (results that are scaled right away)
-               "affine_linear.hip": _VGPR_FORM, "experts_up.hip": _VGPR_FORM,
+               "affine_bits2.hip": _VGPR_FORM, "affine_bits4.hip": _VGPR_FORM,
+               "affine_bits8.hip": _VGPR_FORM, "experts_up.hip": _VGPR_FORM,
                "experts_down.hip": _VGPR_FORM}
 
 

@@ -1,0 +1,10 @@
+// Few rows times affine weights of 8 bits.
+#include "affine_few.h"
+
+namespace mgq {
+
+int affine_few_bits8(const LinArgs& a, const FewWeight& w, int choice, hipStream_t s, const char* what) {
+  return run_types<kFewAf8>(a, w, choice, s, what);
+}
+
+}  // namespace mgq

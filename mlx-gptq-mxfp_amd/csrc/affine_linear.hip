@@ -1,161 +1,116 @@
 // Products with affine weights, y[t, n] = sum_k x[r(t), k] (q[g, n, k] s + b) with a scale
 // s and a bias b for each group of 32, 64 or 128 values of a weight row and 2-, 4- or
 // 8-bit codes q, packed low bits first. The list of entries t and its groups g are those of
-// linear_common.h, the arithmetic is few_core.h's.
-//
-// Few rows: a workgroup computes 16 NQ entries (4 where NE = 1) x 16 NP weight rows; its
-// waves share the contraction and add their sums through LDS in wave order.
-#include "gemv_core.h"
+// linear_common.h. Here are the entry point and the choice of kernel: affine_few.h for few
+// rows, the tile kernel of the other products (affine_tile.hip) for many.
+#include <math.h>
+
+#include "affine_few_choice.h"
 #include "linear_few.h"
 
 namespace mgq {
 namespace {
 
-template <class F, int NP, int NQ, int NE, int WAVES, int DEPTH>
-__global__ void __launch_bounds__(64 * WAVES) affine_few_kernel(const LinArgs a, const FewWeight w) {
-  constexpr int BM = NE == 1 ? 4 : 16 * NQ;
-  __shared__ lin_f32x4_t part[WAVES * NP * NQ * 64];
-  __shared__ __attribute__((aligned(16))) char params[WAVES * few_lds<F, NP>()];
-  LinTile t;
-  if (!lin_find_tile<BM>(a, (a.np + 16 * NP - 1) / (16 * NP), &t)) return;
-  const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int p0 = t.pt * 16 * NP;
-  const int steps = t.g < a.G ? (a.nc + kFewStep - 1) / kFewStep : 0;  // (no group: zeros)
-  const int64_t g = t.g < a.G ? t.g : 0;
-
-  FewRow row[NP];
-#pragma unroll
-  for (int i = 0; i < NP; ++i)
-    row[i] = few_row<F>(w, g, p0 + 16 * i < a.np ? p0 + 16 * i : p0, a.nc);
-  const char* x[NQ];
-#pragma unroll
-  for (int j = 0; j < NQ; ++j) {
-    const int64_t q = t.q0 + (NE == 1 ? r16 >> 2 : 16 * j + r16);
-    x[j] = a.Q + lin_row(a, q < t.q_end ? q : t.q_end - 1) * a.ldq;
-  }
-  lin_f32x4_t acc[NP][NQ];
-  few_product<F, NP, NQ, NE, DEPTH>(row, w, x, a.nc, steps * wave / WAVES, steps * (wave + 1) / WAVES,
-                                    params + wave * few_lds<F, NP>(), acc);
-#pragma unroll
-  for (int i = 0; i < NP; ++i)
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) part[((wave * NP + i) * NQ + j) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  for (int blk = wave; blk < NP * NQ; blk += WAVES) {
-    lin_f32x4_t sum = part[blk * 64 + lane];
-#pragma unroll
-    for (int o = 1; o < WAVES; ++o) {
-      const lin_f32x4_t v = part[(o * NP * NQ + blk) * 64 + lane];
-#pragma unroll
-      for (int e = 0; e < NE; ++e) sum[e] += v[e];
-    }
-    const int p = p0 + 16 * (blk / NQ) + r16;
-    if (p >= a.np) continue;
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const int64_t q = t.q0 + (NE == 1 ? quad : 16 * (blk % NQ) + 4 * quad + e);
-      if (q < t.q_end)
-        reinterpret_cast<uint16_t*>(a.out)[q * a.ldo + p] = lin_round16(sum[e], a.out_type);
-    }
-  }
-}
-
-// Single entries: a wave takes one entry and R 64 / L weight rows.
-template <class F, int L, int R>
-__global__ void __launch_bounds__(256) affine_gemv_kernel(const LinArgs a, const FewWeight w) {
-  constexpr int RI = 64 / L, ROWS = R * RI;  // rows of a load, of a wave
-  LinTile t;
-  if (!lin_find_tile<1>(a, (a.np + 4 * ROWS - 1) / (4 * ROWS), &t)) return;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int p0 = (4 * t.pt + wave) * ROWS;
-  if (p0 >= a.np) return;
-  auto first = [&](int r) { return p0 + r * RI < a.np - RI ? p0 + r * RI : a.np - RI; };
-  float acc[R], sum[gemv_sums<L, R>()];
-#pragma unroll
-  for (int r = 0; r < R; ++r) acc[r] = 0.0f;
-  if (t.g < a.G)  // (no group: zeros)
-    gemv_add<F, L, R, 2>(acc, w, t.g, first, a.Q + lin_row(a, t.q0) * a.ldq, a.nc, 0,
-                         gemv_chunks<F, L>(a.nc));
-  gemv_reduce<L, R>(acc, sum);
-  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + t.q0 * a.ldo;
-#pragma unroll
-  for (int q = 0; q < gemv_sums<L, R>(); ++q)
-    if ((lane & 15) == q) {
-      const int r = gemv_row<L>(q, lane >> 4);
-      out[first(r / RI) + r % RI] = lin_round16(sum[q], a.out_type);
-    }
-}
-
-template <class F, int NP, int NQ, int NE, int WAVES, int DEPTH>
-int launch_few(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
-  const int64_t grid = lin_row_tiles(a, NE == 1 ? 4 : 16 * NQ) * ceil_div(a.np, 16 * NP);
-  MGQ_REQUIRE(grid < kLinFewGrid * 4 / WAVES, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  affine_few_kernel<F, NP, NQ, NE, WAVES, DEPTH>
-      <<<static_cast<unsigned>(grid), 64 * WAVES, 0, s>>>(a, w);
-  return check_launch(what);
-}
-template <class F>
-int launch_gemv(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
-  constexpr int R = 8;
-  const int lanes = gemv_lanes<F>(a.nc, a.np);
-  const int64_t grid = a.M * ceil_div(a.np, 4 * R * (64 / lanes));
-  MGQ_REQUIRE(grid < kLinFewGrid, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
-  const unsigned blocks = static_cast<unsigned>(grid);
-  if (lanes == 64) affine_gemv_kernel<F, 64, R><<<blocks, 256, 0, s>>>(a, w);
-  else if (lanes == 32) affine_gemv_kernel<F, 32, R><<<blocks, 256, 0, s>>>(a, w);
-  else affine_gemv_kernel<F, 16, R><<<blocks, 256, 0, s>>>(a, w);
-  return check_launch(what);
-}
 #ifdef AFFINE_FORCE
 extern "C" int mgq_force[4] = {0, 0, 0, 0};
 #endif
 
-template <class F>
-int run(const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
-#ifdef AFFINE_FORCE
-  const int per = mgq_force[1];
-  switch (mgq_force[0]) {
-    case 5: return launch_gemv<F>(a, w, s, what);
-    case 1: return launch_few<F, 1, 1, 1, 4, 4>(a, w, s, what);
-    case 2: return launch_few<F, 2, 1, 1, 4, 4>(a, w, s, what);
-    case 3: return launch_few<F, 4, 1, 1, 4, 4>(a, w, s, what);
-    case 6: return launch_few<F, 1, 1, 4, 4, 4>(a, w, s, what);
-    case 7: return launch_few<F, 2, 1, 4, 4, 2>(a, w, s, what);
-    case 8: return launch_few<F, 2, 1, 4, 4, 4>(a, w, s, what);
-    case 9: return launch_few<F, 4, 1, 4, 4, 2>(a, w, s, what);
-    case 10: return launch_few<F, 4, 1, 4, 4, 4>(a, w, s, what);
-    case 11: return launch_few<F, 4, 1, 4, 8, 2>(a, w, s, what);
-    case 12: return launch_few<F, 4, 1, 4, 8, 4>(a, w, s, what);
-    case 13: return launch_few<F, 4, 2, 4, 4, 2>(a, w, s, what);
-    case 14: return launch_few<F, 4, 2, 4, 4, 3>(a, w, s, what);
-    case 15: return launch_few<F, 4, 4, 4, 4, 2>(a, w, s, what);
-    case 16: return launch_few<F, 2, 4, 4, 4, 2>(a, w, s, what);
-    case 30: case 31: case 32: case 33: {
-      LinArgs b = a;
-      b.P = w.p; b.Ps = reinterpret_cast<const uint8_t*>(w.s); b.Pb = reinterpret_cast<const uint8_t*>(w.b);
-      b.ldp = w.ld; b.p_group = w.group; b.p_shift = w.shift; b.p_type = w.type;
-      const int op = (F::XT == kF16 ? kOpAf2H : kOpAf2) + (F::W - kFewAf2);
-      const int r[4] = {256, 128, 64, 64}, c[4] = {256, 256, 256, 128};
-      const int i = mgq_force[0] - 30;
-      return lin_tile_affine(b, op, LinTileShape{r[i], c[i], mgq_force[2] != 0}, s, what);
+int run_tile(LinArgs a, const FewWeight& w, int bits, LinTileShape t, hipStream_t s, const char* what) {
+  a.P = w.p;
+  a.Ps = reinterpret_cast<const uint8_t*>(w.s);
+  a.Pb = reinterpret_cast<const uint8_t*>(w.b);
+  a.ldp = w.ld;
+  a.p_group = w.group;
+  a.p_shift = w.shift;
+  a.p_type = w.type;
+  const int op = (a.out_type == kF16 ? kOpAf2H : kOpAf2) + (bits == 8 ? 2 : bits == 4 ? 1 : 0);
+  return lin_tile_affine(a, op, t, s, what);
+}
+int run_few(const LinArgs& a, const FewWeight& w, int bits, int choice, hipStream_t s, const char* what) {
+  if (bits == 2) return affine_few_bits2(a, w, choice, s, what);
+  if (bits == 4) return affine_few_bits4(a, w, choice, s, what);
+  return affine_few_bits8(a, w, choice, s, what);
+}
+
+// The kernel whose time by the model below is least, of those whose grid holds the
+// product. Times are of 4-bit codes with a scale for 64 values (one MI355X, called again and
+// again with weights that had left the caches):
+//   few rows: the steps of 128 values that a wave takes, one after the other, at the time
+//     of a step for a wave alone on its SIMD or for the waves that share it (a form's
+//     numbers in affine_few_choice.h);
+//   single entries: chunks of 64 pieces of eight rows, 1.65 us each;
+//   tiles: the stages of 64 values, rounds of the 256 CUs; 2.2 instead of 1.7 us for
+//     the largest tile when every CU has one.
+// Groups of unknown lengths are taken as in the other products (linear.hip). 14336 x 4096, 4
+// bits: 1 entry 11 us (0), 4 entries 12.7 (1), 16 entries 15.6 (4; the largest tile 114), 64
+// entries 28.8 (10; the smallest tile 58.7), 512 entries 103 (128 x 256; form 10: 210).
+struct Choice {
+  int few;
+  LinTileShape tile;
+};
+Choice choose(const LinArgs& a, const FewWeight& w, int bits) {
+  const double M = static_cast<double>(a.M), active = a.offsets ? (a.G < a.M ? a.G : M) : 1;
+  const double steps = ceil_div(a.nc, kFewStep);
+  auto row_tiles = [&](int rows) {
+    return a.offsets ? fmax(1.0, M / rows + 0.575 * active) : ceil(M / rows);
+  };
+  Choice c = {};
+  double best = 1e300;
+  auto offer = [&](double us, int few, LinTileShape tile) {
+    if (us < best) {
+      best = us;
+      c = Choice{few, tile};
+    }
+  };
+  if (a.M * ceil_div(a.np, 32) < kLinFewGrid) {
+    const double chunks = ceil_div(a.nc, bits == 8 ? 1024 : 2048);
+    offer(5 + chunks * 1.65 * fmax(1.0, M * ceil_div(a.np, 8) / 1024.0), 0, LinTileShape{});
+  }
+#define MGQ_OFFER(n, NP, NQ, NE, WAVES, KS, depth, alone, shared)                      \
+  {                                                                                    \
+    constexpr int rows = NE == 1 ? 4 : 16 * NQ, cols = 16 * NP * (WAVES / KS);          \
+    if (lin_row_tiles(a, rows) * ceil_div(a.np, cols) < kLinFewGrid * 4 / WAVES) {       \
+      const double on_simd = row_tiles(rows) * ceil_div(a.np, cols) * WAVES / 1024;      \
+      offer(5 + ceil(steps / KS) * fmax(alone, shared * (on_simd + ceil(on_simd)) / 2),  \
+            n, LinTileShape{});                                                         \
+    }                                                                                  \
+  }
+  MGQ_AFFINE_SHAPES(MGQ_OFFER)
+#undef MGQ_OFFER
+  // (a piece of 16 bytes of 2-bit codes holds 64 values: the rows have to)
+  if (bits != 2 || a.nc % 64 == 0) {
+    LinArgs t = a;
+    t.P = w.p;
+    t.ldp = w.ld;
+    t.p_group = w.group;
+    const bool staged = !lin_tile_direct(t, kOpAf4, kLinForward);
+    struct {
+      int rows, cols;
+      double stage;
+    } const tiles[] = {{64, 128, 0.86}, {64, 256, 1.25}, {128, 256, 1.4}, {256, 256, 1.7}};
+    for (const auto& v : tiles) {
+      if ((staged && v.rows == 256) || lin_tile_grid(a, v.rows, v.cols) >= kLinTileGrid) continue;
+      const double rounds = row_tiles(v.rows) * ceil_div(a.np, v.cols) / 256;
+      const double full = rounds > 1 ? (v.rows == 256 ? 1.3 : 1.15) : 1.0;
+      offer(5 + (rounds < 1 ? 1 : rounds + 0.617 * (ceil(rounds) - rounds)) *
+                    (ceil_div(a.nc, 64) * v.stage * full * (staged ? 1.3 : 1.0) + 3),
+            0, LinTileShape{v.rows, v.cols, staged});
     }
   }
-#endif
-  if (a.M <= 4) return launch_few<F, 1, 1, 1, 4, 2>(a, w, s, what);
-  if (a.M <= 16 || (a.offsets && a.M <= 16 * static_cast<int64_t>(a.G)))
-    return launch_few<F, 1, 1, 4, 4, 2>(a, w, s, what);
-  return launch_few<F, 2, 4, 4, 4, 1>(a, w, s, what);
+  return c;
 }
-template <int XT, int SB>
-int run_bits(int bits, const LinArgs& a, const FewWeight& w, hipStream_t s, const char* what) {
+
+int run(const LinArgs& a, const FewWeight& w, int bits, hipStream_t s, const char* what) {
 #ifdef AFFINE_FORCE
-  return bits == 8 ? run<FewFmt<kFewAf8, kBF16, 2>>(a, w, s, what) : run<FewFmt<kFewAf4, kBF16, 2>>(a, w, s, what);
+  if (mgq_force[0] >= 100) {
+    const int r[4] = {256, 128, 64, 64}, c[4] = {256, 256, 256, 128}, i = mgq_force[0] - 100;
+    return run_tile(a, w, bits, LinTileShape{r[i], c[i], mgq_force[2] != 0}, s, what);
+  }
+  return run_few(a, w, bits, mgq_force[0], s, what);
 #endif
-  if (bits == 2) return run<FewFmt<kFewAf2, XT, SB>>(a, w, s, what);
-  if (bits == 4) return run<FewFmt<kFewAf4, XT, SB>>(a, w, s, what);
-  return run<FewFmt<kFewAf8, XT, SB>>(a, w, s, what);
+  const Choice c = choose(a, w, bits);
+  if (c.tile.rows) return run_tile(a, w, bits, c.tile, s, what);
+  return run_few(a, w, bits, c.few, s, what);
 }
 
 }  // namespace
@@ -205,10 +160,35 @@ extern "C" int mgq_affine_linear(const void* X, int dtype, int64_t n_rows, int64
   w.n = N;
   w.shift = group_size == 32 ? 5 : group_size == 64 ? 6 : 7;
   w.type = param_dtype;
-  hipStream_t s = as_stream(stream);
-  if (dtype == kF16)
-    return param_dtype == kF32 ? run_bits<kF16, 4>(bits, a, w, s, what)
-                               : run_bits<kF16, 2>(bits, a, w, s, what);
-  return param_dtype == kF32 ? run_bits<kBF16, 4>(bits, a, w, s, what)
-                             : run_bits<kBF16, 2>(bits, a, w, s, what);
+  return run(a, w, bits, as_stream(stream), what);
+}
+
+extern "C" int mgq_affine_choice(const void* X, int64_t ldx, int64_t n_entries, const uint32_t* words,
+                                 int bits, int64_t n_groups, int64_t N, int64_t K, int grouped,
+                                 int32_t* kernel) {
+  clear_error();
+  const char* what = "affine_choice";
+  MGQ_REQUIRE(bits == 2 || bits == 4 || bits == 8, MGQ_ERR_VALUE, "%s: bits must be 2, 4 or 8", what);
+  const int32_t some_list = 0;  // stands for offsets: the choice does not read them
+  if (int rc = lin_check_list(what, grouped ? &some_list : nullptr, nullptr, n_groups, n_entries, n_entries))
+    return rc;
+  if (int rc = lin_check_dims(what, N, K)) return rc;
+  LinArgs a = {};
+  a.Q = static_cast<const char*>(X);
+  a.ldq = 2 * ldx;
+  a.offsets = grouped ? &some_list : nullptr;
+  a.M = n_entries;
+  a.n_rows = n_entries;
+  a.G = static_cast<int>(n_groups);
+  a.np = static_cast<int>(N);
+  a.nc = static_cast<int>(K);
+  FewWeight w = {};
+  w.p = reinterpret_cast<const char*>(words);
+  w.ld = K / 8 * bits;
+  w.group = w.ld * N;
+  const Choice c = choose(a, w, bits);
+  kernel[0] = c.tile.rows ? (c.tile.staged ? 3 : 2) : c.few ? 1 : 0;
+  kernel[1] = c.tile.rows ? c.tile.rows : c.few;
+  kernel[2] = c.tile.cols;
+  return MGQ_OK;
 }

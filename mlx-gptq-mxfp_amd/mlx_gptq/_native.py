@@ -120,6 +120,7 @@ SIGNATURES: dict[str, list] = {
                         _I64, _VP, _VP, _INT, _VP],
     "mgq_affine_linear": [_VP, _INT, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _INT, _INT, _I64, _I64,
                           _I64, _I64, _VP, _VP, _VP],
+    "mgq_affine_choice": [_VP, _I64, _I64, _VP, _INT, _I64, _I64, _I64, _INT, _VP],
     # experts.py
     "mgq_top_k_softmax": [_VP, _INT, _I64, _I64, _I64, _I64, _INT, _VP, _VP, _VP],
     "mgq_top_k_softmax_grad": [_VP, _VP, _INT, _I64, _I64, _I64, _VP, _I64, _INT, _VP, _VP],

@@ -6,14 +6,19 @@ additions of its block, two fused multiply-adds of each of the K / 32 blocks and
 additions of eight partial sums, each within 2^-23 of its operands' magnitudes (twice
 2^-24, which also covers truncating adders): (K / 16 + 48) 2^-23 m, less than the bound
 (K + 48) 2^-23 m used here. Rounding to the rows' type adds half a step: 2^-8 relative
-for bf16, 2^-11 for f16 with half of its subnormal step, 2^-25.
+for bf16, 2^-11 for f16 with half of its subnormal step, 2^-25. The tile kernel (many
+rows) rounds q scale + bias to the rows' type before it multiplies, half a step of every
+weight: UNIT sum|x| |q scale + bias| more, which `mag` is at least as large as.
 """
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
+from mlx_gptq import _native as nat
 from mlx_gptq import gptq, grid, linear, packing
 from oracle import linear_ref as ref
 
@@ -38,9 +43,12 @@ def rows(T, K, dtype, seed=1):
     return torch.randn(T, K, generator=g).to(TYPES[dtype])
 
 
-def close(got, want, mag, K, what=None):
+def close(got, want, mag, K, what=None, rounded=None):
+    """rounded: sum|x| |w| where the kernel rounds the weights."""
     d = (got.cpu().double() - want).abs()
     tol = (K + 48) * 2.0**-23 * mag + UNIT[got.dtype] * want.abs() * 1.01 + STEP[got.dtype]
+    if rounded is not None:
+        tol = tol + 1.01 * UNIT[got.dtype] * rounded + STEP[got.dtype] * K * 8
     bad = ~(d <= tol)
     assert not bool(bad.any()), (what, int(bad.sum()), float((d - tol).max()),
                                  torch.nonzero(bad)[:4].tolist())
@@ -54,6 +62,37 @@ def product(x, q, s, b, bits, offsets=None, row_index=None, **kw):
     return linear.affine_linear(x.to(DEV), words, s.to(DEV), b.to(DEV), bits, offsets, idx, **kw)
 
 
+SINGLE, FEW, TILE, STAGED = range(4)
+
+
+def kernel(x, words, bits, G, N, offsets, M=None):
+    """mgq_affine_choice of a call on these device tensors."""
+    out = (ctypes.c_int32 * 3)()
+    nat.call("mgq_affine_choice", x.data_ptr(), x.stride(0) if x.shape[0] > 1 else x.shape[1],
+             x.shape[0] if M is None else M, words.data_ptr(), bits, G, N, x.shape[1],
+             int(offsets is not None), ctypes.addressof(out))
+    return tuple(out)
+
+
+def check(x, q, s, b, bits, offsets=None, row_index=None, what=None, words=None):
+    """The product of these (x may be on the device) against float64; which kernel it took."""
+    G, N, K = q.shape
+    x = x.to(DEV)
+    if words is None:
+        words = packing.pack_q((q if offsets is not None else q[0]).to(DEV), bits)
+    pick = (lambda t: t.to(DEV)) if offsets is not None else (lambda t: t[0].to(DEV))
+    idx = None if row_index is None else row_index.to(DEV)
+    y = linear.affine_linear(x, words, pick(s), pick(b), bits, offsets, idx)
+    took = kernel(x, words, bits, G, N, offsets, y.shape[0])
+    host = x.cpu()
+    want, mag = ref.affine_forward(host, q, s, b, offsets, row_index)
+    rounded = None
+    if took[0] >= TILE:
+        rounded = ref.forward(host, ref.affine(q, s, b)[0], offsets, row_index)[1]
+    close(y, want, mag, K, what, rounded)
+    return y, took
+
+
 FORMS = [(bits, group, dtype, params) for bits in (2, 4, 8) for group in (32, 64, 128)
          for dtype in ("bf16", "f16") for params in ("bf16", "f16", "f32")]
 
@@ -64,8 +103,7 @@ def test_every_form(bits, group, dtype, params):
     N, K = 40, 3 * group + (128 if group < 128 else 0)
     q, s, b = weight(1, N, K, bits, group, params)
     for T in (1, 3, 5, 16, 30, 70, 300):
-        x = rows(T, K, dtype)
-        close(product(x, q, s, b, bits), *ref.affine_forward(x, q, s, b), K, T)
+        check(rows(T, K, dtype), q, s, b, bits, what=T)
 
 
 @pytest.mark.parametrize("bits", [2, 4, 8])
@@ -79,7 +117,7 @@ def test_codes_stand_in_their_places(bits, dtype):
     q[0, 0] = (torch.arange(K) % 2**bits).to(torch.uint8)
     s, b = torch.ones(1, 19, K // 32), torch.zeros(1, 19, K // 32)
     x = torch.eye(K).to(TYPES[dtype])
-    for T in (1, 4, 16, K):
+    for T in (1, 4, 16, K):  # (whole numbers: the tile's rounding keeps them too)
         y = product(x[K - T:], q, s, b, bits)
         assert torch.equal(y.cpu().double(), q[0].double().T[K - T:])
 
@@ -93,8 +131,7 @@ SIZES = [(1, 1, 32), (1, 17, 32), (2, 16, 96), (4, 33, 1056), (5, 130, 160), (16
 @pytest.mark.parametrize("bits", [4, 8])
 def test_sizes(T, N, K, bits):
     q, s, b = weight(1, N, K, bits, 32, "bf16", seed=T)
-    x = rows(T, K, "bf16")
-    close(product(x, q, s, b, bits), *ref.affine_forward(x, q, s, b), K)
+    check(rows(T, K, "bf16"), q, s, b, bits)
 
 
 # groups' counts, rows of x (0: not gathered), entries of no group in front and behind
@@ -124,8 +161,7 @@ def test_groups(name, bits, group, dtype):
     idx = None
     if gathered:
         idx = torch.randint(0, T, (M,), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
-    y = product(x, q, s, b, bits, off, idx)
-    close(y, *ref.affine_forward(x, q, s, b, off, idx), K, name)
+    y, _ = check(x, q, s, b, bits, off, idx, name)
     if before:
         assert not bool(y[:before].any()) and not bool(y[off[-1]:].any())
 
@@ -141,12 +177,11 @@ def test_strides_and_alignment(T):
     words.copy_(packing.pack_q(q[0].to(DEV), bits).view(torch.int32))
     for start in (0, 1, 5, 8):
         x = wide[:, start:start + K]
-        y = linear.affine_linear(x, words, s[0].to(DEV), b[0].to(DEV), bits)
-        close(y, *ref.affine_forward(x.cpu(), q, s, b), K, start)
+        check(x, q, s, b, bits, what=start, words=words)
     # scales and biases that are views, words given as uint32
     sb = torch.stack((s[0], b[0]), dim=-1).to(DEV)
     y = linear.affine_linear(x, words.view(torch.uint32), sb[..., 0], sb[..., 1], bits)
-    close(y, *ref.affine_forward(x.cpu(), q, s, b), K)
+    assert torch.equal(y, linear.affine_linear(x, words, s[0].to(DEV), b[0].to(DEV), bits))
 
 
 @pytest.mark.parametrize("T", [3, 40, 200])
@@ -154,8 +189,7 @@ def test_a_bias_far_from_its_scale(T):
     """Weights 100 +- 8 steps: the terms cancel in neither order of the sum."""
     q, s, b = weight(1, 33, 512, 4, 64, "f32")
     b = torch.full_like(b, 100.0)
-    x = rows(T, 512, "bf16")
-    close(product(x, q, s, b, 4), *ref.affine_forward(x, q, s, b), 512)
+    check(rows(T, 512, "bf16"), q, s, b, 4)
 
 
 @pytest.mark.parametrize("T", [1, 20, 150])
@@ -165,9 +199,10 @@ def test_a_row_that_is_no_number_stays_alone(T):
     x[T // 2, 7] = torch.nan
     y = product(x, q, s, b, 4).cpu()
     assert bool(y[T // 2].isnan().all())
+    clean = x.clone()
+    clean[T // 2] = 0
     keep = [t for t in range(T) if t != T // 2]
-    want, mag = ref.affine_forward(x[keep], q, s, b)
-    close(y[keep], want, mag, 96)
+    assert torch.equal(y[keep], check(clean, q, s, b, 4)[0].cpu()[keep])
     s[0, 3, 1] = torch.nan  # and so does a weight row
     y = product(rows(T, 96, "bf16"), q, s, b, 4)
     assert y.isnan().all(dim=0).nonzero().flatten().tolist() == [3]
