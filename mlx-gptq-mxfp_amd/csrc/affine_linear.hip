@@ -37,10 +37,10 @@ int run_few(const LinArgs& a, const FewWeight& w, int bits, int choice, hipStrea
 // again with weights that had left the caches):
 //   few rows: the steps of 128 values that a wave takes, one after the other, at the time
 //     of a step for a wave alone on its SIMD or for the waves that share it (a form's
-//     numbers in affine_few_choice.h);
+//     numbers in affine_few_choice.h), three more where workgroups follow one another;
 //   single entries: chunks of 64 pieces of eight rows, 1.65 us each;
-//   tiles: the stages of 64 values, rounds of the 256 CUs; 2.2 instead of 1.7 us for
-//     the largest tile when every CU has one.
+//   tiles: the stages of 64 values, rounds of the 256 CUs; up to 1.45 times as much when
+//     every CU has one.
 // Groups of unknown lengths are taken as in the other products (linear.hip). 14336 x 4096, 4
 // bits: 1 entry 11 us (0), 4 entries 12.7 (1), 16 entries 15.6 (4; the largest tile 114), 64
 // entries 28.8 (10; the smallest tile 58.7), 512 entries 103 (128 x 256; form 10: 210).
@@ -71,7 +71,9 @@ Choice choose(const LinArgs& a, const FewWeight& w, int bits) {
     constexpr int rows = NE == 1 ? 4 : 16 * NQ, cols = 16 * NP * (WAVES / KS);          \
     if (lin_row_tiles(a, rows) * ceil_div(a.np, cols) < kLinFewGrid * 4 / WAVES) {       \
       const double on_simd = row_tiles(rows) * ceil_div(a.np, cols) * WAVES / 1024;      \
-      offer(5 + ceil(steps / KS) * fmax(alone, shared * (on_simd + ceil(on_simd)) / 2),  \
+      const double more = on_simd > 1 ? 3 * (1 - 1 / on_simd) : 0;                       \
+      offer(5 + (ceil(steps / KS) + more) *                                              \
+                    fmax(alone, shared * (on_simd + ceil(on_simd)) / 2),                 \
             n, LinTileShape{});                                                         \
     }                                                                                  \
   }
@@ -86,12 +88,13 @@ Choice choose(const LinArgs& a, const FewWeight& w, int bits) {
     const bool staged = !lin_tile_direct(t, kOpAf4, kLinForward);
     struct {
       int rows, cols;
-      double stage;
-    } const tiles[] = {{64, 128, 0.86}, {64, 256, 1.25}, {128, 256, 1.4}, {256, 256, 1.7}};
+      double stage, full;
+    } const tiles[] = {{64, 128, 0.64, 1.05}, {64, 256, 1.05, 1.0}, {128, 256, 1.22, 1.29},
+                       {256, 256, 1.5, 1.45}};
     for (const auto& v : tiles) {
       if ((staged && v.rows == 256) || lin_tile_grid(a, v.rows, v.cols) >= kLinTileGrid) continue;
       const double rounds = row_tiles(v.rows) * ceil_div(a.np, v.cols) / 256;
-      const double full = rounds > 1 ? (v.rows == 256 ? 1.3 : 1.15) : 1.0;
+      const double full = rounds > 1 ? v.full : 1.0;
       offer(5 + (rounds < 1 ? 1 : rounds + 0.617 * (ceil(rounds) - rounds)) *
                     (ceil_div(a.nc, 64) * v.stage * full * (staged ? 1.3 : 1.0) + 3),
             0, LinTileShape{v.rows, v.cols, staged});
