@@ -491,7 +491,7 @@ typedef struct {
   int format;          /* MGQ_WEIGHT_* */
   int param_dtype;     /* affine: type of scales and biases (f32/bf16/f16) */
 } mgq_weight;          /* (device pointers in a struct on the host, read during the call) */
-int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64_t I);
+int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64_t H, int64_t I);
 int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t ldx, const void* index,
                        int index_bits, const float* weights, int64_t k, int64_t n_experts, int64_t H,
                        int64_t I, const mgq_weight* up, const mgq_weight* down, void* out,

@@ -23,11 +23,14 @@ struct DecodeArgs {
   FewWeight up, down;    // [E, 2 I, H] (gate rows first), [E, H, I]
   char* act;             // workspace: [T k, I] of x's type
   int32_t* plan;         // workspace: see decode_plan (experts_up.hip)
+  int32_t* counts;       // workspace: parts of a column tile that are done
+  float* sums;           // workspace: [parts, T, H]
   uint16_t* out;         // [T, H]
   int index64;
   int T, k, n;           // n = T k
   int E, H, I;
   int type;              // kBF16 or kF16
+  int parts, tiles;      // of the second launch
 };
 
 // The plan that the first launch leaves for the second one (T > 1): plan[0] items,
@@ -43,8 +46,20 @@ struct DecodeEntry {
 };
 constexpr int kDecodeItem = 16;
 constexpr int kDecodePlanHead = 16;  // bytes
-inline int64_t decode_plan_bytes(int64_t n) { return kDecodePlanHead + n * 16; }
-inline int64_t decode_act_bytes(int64_t n, int64_t I) { return (n * I * 2 + 255) / 256 * 256; }
+
+// The second launch: 32 columns of the result a workgroup, whose items `decode_parts`
+// workgroups share; what each gives goes through the workspace.
+constexpr int kDecodeCols = 32;
+inline int decode_tiles(int64_t H) { return static_cast<int>((H + kDecodeCols - 1) / kDecodeCols); }
+inline int decode_parts(int64_t n, int64_t H) {
+  const int64_t fill = 512 / decode_tiles(H), most = n / 8;  // two workgroups a CU, two items a wave
+  const int64_t p = fill < most ? fill : most;
+  return static_cast<int>(p < 1 ? 1 : p > 8 ? 8 : p);
+}
+inline int64_t decode_round(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+inline int64_t decode_act_bytes(int64_t n, int64_t I) { return decode_round(n * I * 2); }
+inline int64_t decode_plan_bytes(int64_t n) { return decode_round(kDecodePlanHead + n * 16); }
+inline int64_t decode_count_bytes(int64_t H) { return decode_round(4 * int64_t(decode_tiles(H))); }
 
 __device__ __forceinline__ int decode_expert(const DecodeArgs& a, int i) {
   if (a.index64) {

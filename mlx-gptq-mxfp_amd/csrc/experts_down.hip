@@ -1,67 +1,204 @@
 // Second launch of a routed layer for a few rows (experts_decode.h): down projection and
 // the weighted sum over each row's experts, and the entry point of both.
 //
-// A workgroup computes 16 columns of the result for all rows, so that no sum crosses
-// workgroups. Its waves take the plan's items in turn (an expert with up to 16 of its
-// rows; parts of the contraction where there are fewer items than waves) and add what an
-// item gives each row into sums of their own in LDS; these are added in wave order. A
-// single row needs no plan: its items are its entries (gemv_core.h).
+// A workgroup computes 32 columns of the result for all rows. Its waves take the plan's items
+// in turn (an expert with up to 16 of its rows) and add what an item gives each row into sums
+// of their own in LDS; these are added in wave order. Where the columns alone would leave
+// CUs without work, several workgroups share the items of a column tile and the last one of
+// them to come adds their sums, in a fixed order. A single row needs no plan: its items are
+// its entries (gemv_core.h).
 #include "experts_decode.h"
 
 namespace mgq {
 namespace {
 
-template <class F, int NE, int WAVES, int DEPTH>
-__global__ void __launch_bounds__(64 * WAVES) decode_down_kernel(const DecodeArgs a) {
+constexpr int kWaves = 4;
+
+template <class F, int NE, int DEPTH>
+__global__ void __launch_bounds__(64 * kWaves) decode_down_kernel(const DecodeArgs a) {
+  constexpr int NP = kDecodeCols / 16;
   extern __shared__ float lds[];
-  __shared__ __attribute__((aligned(16))) char params[F::dense ? 16 : WAVES * few_lds<F, 1>()];
+  __shared__ __attribute__((aligned(16))) char params[F::dense ? 16 : kWaves * few_lds<F, NP>()];
+  __shared__ int32_t done;
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float* sums = lds + wave * a.T * 16;  // [T][16]
-  DecodeItem* items = reinterpret_cast<DecodeItem*>(lds + WAVES * a.T * 16);
+  const int tile = blockIdx.x / a.parts, part = blockIdx.x - tile * a.parts;
+  const int h0 = tile * kDecodeCols;
+  float* sums = lds + wave * a.T * kDecodeCols;  // [T][32]
+  DecodeItem* items = reinterpret_cast<DecodeItem*>(lds + kWaves * a.T * kDecodeCols);
   DecodeEntry* entries = reinterpret_cast<DecodeEntry*>(items + a.n);
-  for (int i = lane; i < a.T * 16; i += 64) sums[i] = 0.0f;
+  char* own_params = params + (F::dense ? 0 : wave * few_lds<F, NP>());
+  for (int i = lane; i < a.T * kDecodeCols; i += 64) sums[i] = 0.0f;
   const int n_items = __builtin_amdgcn_readfirstlane(a.plan[0]);
   const uint64_t* from = reinterpret_cast<const uint64_t*>(a.plan + kDecodePlanHead / 4);
-  for (int i = threadIdx.x; i < 2 * a.n; i += 64 * WAVES) reinterpret_cast<uint64_t*>(items)[i] = from[i];
+  for (int i = threadIdx.x; i < 2 * a.n; i += 64 * kWaves) reinterpret_cast<uint64_t*>(items)[i] = from[i];
   __syncthreads();
-  const int h0 = blockIdx.x * 16;
-  const int steps = (a.I + kFewStep - 1) / kFewStep;
-  for (int i = wave; i < n_items; i += WAVES) {
-    const DecodeItem it = items[i];
-    const int expert = __builtin_amdgcn_readfirstlane(it.expert);
-    const int first = __builtin_amdgcn_readfirstlane(it.first);
-    const int count = __builtin_amdgcn_readfirstlane(it.count);
-    const FewRow row[1] = {few_row<F>(a.down, expert, h0, a.I)};
+
+  const int whole = a.I / kFewStep, steps = (a.I + kFewStep - 1) / kFewStep;
+  const int shift = F::affine ? a.down.shift : 5, groups = a.I >> shift;
+  const int period = (kFewGroups << shift) / kFewStep;
+  const int unit0 = part * kWaves + wave, stride = a.parts * kWaves;
+  auto rows_of = [&](int u, FewRow(&row)[NP]) {
+    const int expert = __builtin_amdgcn_readfirstlane(items[u].expert);
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+      row[p] = few_row<F>(a.down, expert, h0 + 16 * p < a.H ? h0 + 16 * p : a.H - 1, a.I);
+  };
+  auto x_of = [&](int u) {
+    const int first = __builtin_amdgcn_readfirstlane(items[u].first);
+    const int count = __builtin_amdgcn_readfirstlane(items[u].count);
     const int own = NE == 1 ? r16 >> 2 : r16;
     const int entry = entries[first + (own < count ? own : count - 1)].entry;
-    const char* const x[1] = {a.act + static_cast<int64_t>(entry) * a.I * 2};
-    lin_f32x4_t acc[1][1];
-    few_product<F, 1, 1, NE, DEPTH>(row, a.down, x, a.I, 0, steps, params + wave * few_lds<F, 1>(), acc);
+    return static_cast<const char*>(a.act) + static_cast<int64_t>(entry) * a.I * 2;
+  };
+  // an item's sums to its rows
+  auto add = [&](int u, const lin_f32x4_t(&acc)[NP][1]) {
+    const int first = __builtin_amdgcn_readfirstlane(items[u].first);
+    const int count = __builtin_amdgcn_readfirstlane(items[u].count);
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const int j = NE == 1 ? quad : 4 * quad + e;
       if (j < count) {  // (an item holds a row once: no two lanes add to one sum)
         const DecodeEntry t = entries[first + j];
-        sums[t.entry / a.k * 16 + r16] += t.weight * acc[0][0][e];
+        float* to = sums + t.entry / a.k * kDecodeCols + r16;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) to[16 * p] += t.weight * acc[p][0][e];
+      }
+    }
+  };
+  if (whole == 0) {
+    for (int u = unit0; u < n_items; u += stride) {
+      FewRow row[NP];
+      rows_of(u, row);
+      const char* const x[1] = {x_of(u)};
+      lin_f32x4_t acc[NP][1];
+      few_product<F, NP, 1, NE, 2>(row, a.down, x, a.I, 0, steps, own_params, acc);
+      add(u, acc);
+    }
+  } else if (unit0 < n_items) {
+    // The wave's items one after the other as one stream of steps, so that the next item's
+    // operands are on their way while one ends.
+    FewStep<F> f[DEPTH][NP];
+    lin_u32x4_t xv[DEPTH][1][4];
+    FewRow load_row[NP], row[NP];
+    FewParams<F> par[NP];
+    int lu = unit0, ls = 0;  // what is loaded next
+    rows_of(lu, load_row);
+    const char* lx = x_of(lu);
+    auto load = [&](int d) __attribute__((always_inline)) {
+      if (lu >= n_items) return;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) few_load<F, true>(f[d][p], load_row[p], ls, a.I);
+      few_load_x<F, true>(xv[d][0], lx, ls, a.I);
+      if (++ls == whole) {
+        ls = 0;
+        lu += stride;
+        if (lu < n_items) {
+          rows_of(lu, load_row);
+          lx = x_of(lu);
+        }
+      }
+    };
+    auto fetch = [&](const FewRow(&r)[NP], int g) __attribute__((always_inline)) {
+      if constexpr (!F::dense) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) few_fetch<F>(par[p], r[p], g, groups);
+      }
+    };
+    int u = unit0, s = 0, group = 0;
+    rows_of(u, row);
+    fetch(row, 0);
+    lin_f32x4_t acc[NP][1];
+    auto clear = [&]() {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) acc[p][0] = lin_f32x4_t{0, 0, 0, 0};
+    };
+    clear();
+    auto stage = [&](int at) __attribute__((always_inline)) {
+      if constexpr (!F::dense) {
+        if ((at & (period - 1)) == 0) {
+          few_stage<F, NP>(par, a.down.type, own_params);
+          group = at * kFewStep >> shift;
+          if (at + period < steps) {
+            fetch(row, (at + period) * kFewStep >> shift);
+          } else if (u + stride < n_items) {
+            FewRow next[NP];
+            rows_of(u + stride, next);
+            fetch(next, 0);
+          }
+        }
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) load(d);
+    const int total = (n_items - unit0 + stride - 1) / stride * whole;
+    for (int at = 0; at < total; at += DEPTH) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        if (at + d >= total) break;
+        load((d + DEPTH - 1) % DEPTH);
+        stage(s);
+        few_multiply<F, NP, 1, NE, true>(f[d], xv[d], s, a.I, shift, (s * kFewStep >> shift) - group,
+                                         own_params, acc);
+        if (++s < whole) continue;
+        if (whole < steps) {
+          FewStep<F> tail[NP];
+          lin_u32x4_t tx[1][4];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) few_load<F, false>(tail[p], row[p], whole, a.I);
+          few_load_x<F, false>(tx[0], x_of(u), whole, a.I);
+          stage(whole);
+          few_multiply<F, NP, 1, NE, false>(tail, tx, whole, a.I, shift, (whole * kFewStep >> shift) - group,
+                                            own_params, acc);
+        }
+        add(u, acc);
+        clear();
+        s = 0;
+        u += stride;
+        if (u < n_items) rows_of(u, row);
       }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.T * 16; i += 64 * WAVES) {
-    const int col = blockIdx.x * 16 + (i & 15);
-    if (col >= a.H) continue;
+  const int outputs = a.T * kDecodeCols;
+  auto wave_sum = [&](int i) {
     float sum = lds[i];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) sum += lds[w * a.T * 16 + i];
-    a.out[static_cast<int64_t>(i >> 4) * a.H + col] = lin_round16(sum, a.type);
+    for (int w = 1; w < kWaves; ++w) sum += lds[w * outputs + i];
+    return sum;
+  };
+  auto store = [&](int i, float v) {
+    const int col = h0 + i % kDecodeCols;
+    if (col < a.H) a.out[static_cast<int64_t>(i / kDecodeCols) * a.H + col] = lin_round16(v, a.type);
+  };
+  if (a.parts == 1) {
+    for (int i = threadIdx.x; i < outputs; i += 64 * kWaves) store(i, wave_sum(i));
+    return;
+  }
+  // The workgroup that comes last adds the parts, in their order. They go past the XCDs'
+  // L2s in stores and loads of their own, each waited for: a fence would write back and
+  // invalidate the whole L2 for every workgroup (158 instead of 69 us for 64 rows of MXFP8).
+  float* mine = a.sums + (static_cast<int64_t>(tile) * a.parts + part) * outputs;
+  for (int i = threadIdx.x; i < outputs; i += 64 * kWaves)
+    __hip_atomic_store(mine + i, wave_sum(i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  lds_handover();  // every wave's stores have arrived
+  if (threadIdx.x == 0)
+    done = __hip_atomic_fetch_add(a.counts + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (done != a.parts - 1) return;
+  const float* all = a.sums + static_cast<int64_t>(tile) * a.parts * outputs;
+  for (int i = threadIdx.x; i < outputs; i += 64 * kWaves) {
+    float sum = 0.0f;
+    for (int o = 0; o < a.parts; ++o)
+      sum += __hip_atomic_load(all + o * outputs + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    store(i, sum);
   }
 }
 
-template <class F, int NE, int WAVES, int DEPTH>
+template <class F, int NE>
 int launch(const DecodeArgs& a, hipStream_t s, const char* what) {
-  decode_down_kernel<F, NE, WAVES, DEPTH>
-      <<<static_cast<unsigned>(ceil_div(a.H, 16)), 64 * WAVES, WAVES * a.T * 64 + 16 * a.n, s>>>(a);
+  decode_down_kernel<F, NE, 3><<<static_cast<unsigned>(a.tiles * a.parts), 64 * kWaves,
+                                 kWaves * a.T * kDecodeCols * 4 + 16 * a.n, s>>>(a);
   return check_launch(what);
 }
 
@@ -128,8 +265,7 @@ int decode_down(const DecodeArgs& a, int format, hipStream_t s, const char* what
              : lanes == 32 ? launch_single<F, 32>(a, s, what)
                            : launch_single<F, 16>(a, s, what);
     }
-    if (a.T <= 4) return launch<F, 1, 8, 3>(a, s, what);
-    return launch<F, 4, 8, 3>(a, s, what);
+    return a.T <= 4 ? launch<F, 1>(a, s, what) : launch<F, 4>(a, s, what);
   });
 }
 
@@ -137,9 +273,11 @@ int decode_down(const DecodeArgs& a, int format, hipStream_t s, const char* what
 
 using namespace mgq;
 
-extern "C" int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64_t I) {
-  if (T < 1 || k < 1 || I < 1) return 0;
-  return decode_act_bytes(T * k, I) + decode_plan_bytes(T * k);
+extern "C" int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64_t H, int64_t I) {
+  if (T < 1 || k < 1 || H < 1 || I < 1) return 0;
+  const int64_t n = T * k, parts = decode_parts(n, H);
+  return decode_act_bytes(n, I) + decode_plan_bytes(n) + decode_count_bytes(H) +
+         (parts > 1 ? parts * T * decode_tiles(H) * kDecodeCols * 4 : 0);
 }
 
 extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t ldx, const void* index,
@@ -196,7 +334,7 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
   DecodeArgs a = {};
   if (int rc = weight(*up, 2 * I, H, &a.up)) return rc;
   if (int rc = weight(*down, H, I, &a.down)) return rc;
-  const int64_t need = mgq_experts_decode_workspace_size(T, k, I);
+  const int64_t need = mgq_experts_decode_workspace_size(T, k, H, I);
   MGQ_REQUIRE(workspace_bytes >= need, MGQ_ERR_WORKSPACE, "%s: workspace %lld < %lld bytes", what,
               (long long)workspace_bytes, (long long)need);
   if (T == 0) return MGQ_OK;
@@ -207,6 +345,8 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
   a.weights = weights;
   a.act = static_cast<char*>(workspace);
   a.plan = reinterpret_cast<int32_t*>(a.act + decode_act_bytes(T * k, I));
+  a.counts = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(a.plan) + decode_plan_bytes(T * k));
+  a.sums = reinterpret_cast<float*>(reinterpret_cast<char*>(a.counts) + decode_count_bytes(H));
   a.out = static_cast<uint16_t*>(out);
   a.T = static_cast<int>(T);
   a.k = static_cast<int>(k);
@@ -215,6 +355,8 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
   a.H = static_cast<int>(H);
   a.I = static_cast<int>(I);
   a.type = dtype;
+  a.parts = decode_parts(T * k, H);
+  a.tiles = decode_tiles(H);
   hipStream_t s = as_stream(stream);
   if (int rc = decode_up(a, up->format, s, what)) return rc;
   return decode_down(a, down->format, s, what);

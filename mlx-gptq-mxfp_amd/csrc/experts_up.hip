@@ -71,6 +71,7 @@ __device__ void decode_plan(const DecodeArgs& a, int16_t* ids, uint32_t* carry) 
     });
   }
   if (tid == 0) a.plan[0] = static_cast<int32_t>(base >> 16);
+  for (int i = tid; i < a.tiles; i += 256) a.counts[i] = 0;
 }
 
 constexpr int kWaves = 4;
@@ -79,12 +80,13 @@ __device__ __forceinline__ float decode_act(float gate, float up) {
   return gate / (1.0f + expf(-gate)) * up;
 }
 
-template <class F, int NE, int DEPTH>
+// KS waves share the contraction; the others take 16 gate rows each.
+template <class F, int NE, int KS, int DEPTH>
 __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs a) {
-  constexpr int BM = NE == 1 ? 4 : 16;
+  constexpr int BM = NE == 1 ? 4 : 16, BP = 16 * (kWaves / KS);
   __shared__ __attribute__((aligned(16))) int16_t list[kDecodeEntries];
   __shared__ uint32_t carry[kWaves];
-  __shared__ lin_f32x4_t part[kWaves * 2 * 64];
+  __shared__ lin_f32x4_t part[KS > 1 ? kWaves * 2 * 64 : 1];
   __shared__ __attribute__((aligned(16))) char params[F::dense ? 16 : kWaves * few_lds<F, 2>()];
   if (blockIdx.x == 0) {
     decode_plan(a, list, carry);
@@ -93,50 +95,63 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
   const int bid = blockIdx.x - 1;
   const int lane = threadIdx.x & 63, r16 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = (a.I + 15) / 16;
-  const int slot = bid / tiles, p0 = (bid - slot * tiles) * 16, p = p0 + r16;
+  const int tiles = (a.I + BP - 1) / BP, kw = wave % KS;
+  const int slot = bid / tiles, p0 = (bid - slot * tiles) * BP + wave / KS * 16, p = p0 + r16;
   const bool by_expert = a.n > a.E;
   const int expert = by_expert ? slot : __builtin_amdgcn_readfirstlane(decode_expert(a, slot));
   if (expert < 0) return;
   int count = 0;
-  for (int c = 0; c < a.n; c += 64) {
-    const bool hit = c + lane < a.n && decode_expert(a, c + lane) == expert;
-    const uint64_t mask = __ballot(hit);
-    if (!by_expert && count == 0 && mask && c + __builtin_ctzll(mask) < slot) return;
-    if (wave == 0 && hit)
-      list[count + __popcll(mask & ((uint64_t(1) << lane) - 1))] = static_cast<int16_t>(c + lane);
-    count += __popcll(mask);
+  for (int c0 = 0; c0 < a.n; c0 += 512) {
+    int ids[8];  // (loaded together: the list is the first thing that is waited for)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int i = c0 + 64 * c + lane;
+      ids[c] = i < a.n ? decode_expert(a, i) : -1;
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint64_t mask = __ballot(ids[c] == expert);
+      const int i0 = c0 + 64 * c;
+      if (!by_expert && count == 0 && mask && i0 + __builtin_ctzll(mask) < slot) return;
+      if (wave == 0 && ids[c] == expert)
+        list[count + __popcll(mask & ((uint64_t(1) << lane) - 1))] = static_cast<int16_t>(i0 + lane);
+      count += __popcll(mask);
+    }
   }
   if (count == 0) return;
   __syncthreads();
 
   FewRow row[2];
   // (a gate row past the last one is an up row, whose result is not stored)
-  row[0] = few_row<F>(a.up, expert, p0, a.H);
-  row[1] = few_row<F>(a.up, expert, a.I + p0, a.H);
+  const int pc = p0 < a.I ? p0 : a.I - 1;
+  row[0] = few_row<F>(a.up, expert, pc, a.H);
+  row[1] = few_row<F>(a.up, expert, a.I + pc, a.H);
   const int steps = (a.H + kFewStep - 1) / kFewStep;
   for (int base = 0; base < count; base += BM) {
     const int j = base + (NE == 1 ? r16 >> 2 : r16);
     const int entry = list[j < count ? j : count - 1];
     const char* const x[1] = {a.x + entry / a.k * a.ldx};
     lin_f32x4_t acc[2][1];
-    few_product<F, 2, 1, NE, DEPTH>(row, a.up, x, a.H, steps * wave / kWaves,
-                                    steps * (wave + 1) / kWaves,
+    few_product<F, 2, 1, NE, DEPTH>(row, a.up, x, a.H, steps * kw / KS, steps * (kw + 1) / KS,
                                     params + wave * few_lds<F, 2>(), acc);
-    part[(2 * wave) * 64 + lane] = acc[0][0];
-    part[(2 * wave + 1) * 64 + lane] = acc[1][0];
-    __syncthreads();
-    if (wave == 0) {
-      lin_f32x4_t gate = part[lane], up = part[64 + lane];
+    lin_f32x4_t gate = acc[0][0], up = acc[1][0];
+    if constexpr (KS > 1) {
+      part[(2 * wave) * 64 + lane] = gate;
+      part[(2 * wave + 1) * 64 + lane] = up;
+      __syncthreads();
+      if (kw == 0) {
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) {
-        const lin_f32x4_t g = part[2 * w * 64 + lane], u = part[(2 * w + 1) * 64 + lane];
+        for (int w = 1; w < KS; ++w) {
+          const lin_f32x4_t g = part[2 * (wave + w) * 64 + lane], u = part[(2 * (wave + w) + 1) * 64 + lane];
 #pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          gate[e] += g[e];
-          up[e] += u[e];
+          for (int e = 0; e < NE; ++e) {
+            gate[e] += g[e];
+            up[e] += u[e];
+          }
         }
       }
+    }
+    if (kw == 0) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         const int i = base + (NE == 1 ? quad : 4 * quad + e);
@@ -146,7 +161,7 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
               lin_round16(decode_act(gate[e], up[e]), a.type);
       }
     }
-    __syncthreads();
+    if constexpr (KS > 1) __syncthreads();
   }
 }
 
@@ -191,20 +206,22 @@ int launch_single(const DecodeArgs& a, hipStream_t s, const char* what) {
   return check_launch(what);
 }
 
+template <class F, int NE, int KS>
+int launch(const DecodeArgs& a, hipStream_t s, const char* what) {
+  const int64_t grid = (a.n > a.E ? a.E : a.n) * ceil_div(a.I, 16 * (kWaves / KS)) + 1;
+  MGQ_REQUIRE(grid < int64_t(1) << 24, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  decode_up_kernel<F, NE, KS, 2><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
+  return check_launch(what);
+}
+
 }  // namespace
 
 int decode_up(const DecodeArgs& a, int format, hipStream_t s, const char* what) {
-  const int64_t slots = a.n > a.E ? a.E : a.n;
-  const int64_t grid = slots * ceil_div(a.I, 16) + 1;
-  MGQ_REQUIRE(grid < int64_t(1) << 24, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
   return decode_dispatch(format, a.type, a.up.type, [&](auto f) {
     using F = decltype(f);
     if (a.T == 1) return launch_single<F>(a, s, what);
-    if (a.T <= 4)
-      decode_up_kernel<F, 1, 2><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
-    else
-      decode_up_kernel<F, 4, 2><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a);
-    return check_launch(what);
+    if (a.T <= 4) return launch<F, 1, 4>(a, s, what);
+    return launch<F, 4, 2>(a, s, what);
   });
 }
 

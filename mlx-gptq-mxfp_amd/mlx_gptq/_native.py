@@ -124,7 +124,7 @@ SIGNATURES: dict[str, list] = {
     # experts.py
     "mgq_top_k_softmax": [_VP, _INT, _I64, _I64, _I64, _I64, _INT, _VP, _VP, _VP],
     "mgq_top_k_softmax_grad": [_VP, _VP, _INT, _I64, _I64, _I64, _VP, _I64, _INT, _VP, _VP],
-    "mgq_experts_decode_workspace_size": [_I64, _I64, _I64],
+    "mgq_experts_decode_workspace_size": [_I64, _I64, _I64, _I64],
     "mgq_experts_decode": [_VP, _INT, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _I64, _I64, _VP, _VP,
                            _VP, _VP, _I64, _VP],
     "mgq_linear_choice": [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64, _INT, _VP],

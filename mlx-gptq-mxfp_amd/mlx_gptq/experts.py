@@ -180,7 +180,7 @@ class _DecodeWeights:
         try:
             return self._sizes[T, k]
         except KeyError:
-            size = nat.load().mgq_experts_decode_workspace_size(T, k, self.inner)
+            size = nat.load().mgq_experts_decode_workspace_size(T, k, self.cols, self.inner)
             self._sizes[T, k] = size
             return size
 
