@@ -3,75 +3,101 @@
 //
 // A workgroup takes 16 gate rows and the 16 up rows beside them of one expert, with all
 // entries of that expert: its weight is read once (again for every further 16 entries).
-// The expert is that of list entry `slot`, whose workgroups end at once if an earlier
-// entry has the same one, or, where there are more entries than experts, expert `slot`.
-// The list is short enough for every wave to look through all of it.
+// Only the device knows how many experts the rows have: a workgroup finds the slot-th of
+// them in the list, which is short enough for every wave to look through, and those past
+// the last one end there (they come last, where they hold up nobody).
 #include "experts_decode.h"
 
 namespace mgq {
 namespace {
 
-// One workgroup of 256: the entries in the experts' order. Thread e counts expert e's
-// rows by walking the list, the counts are summed up over the experts, and a second walk
-// writes. A row that names an expert twice is one entry with the sum of its weights.
-__device__ void decode_plan(const DecodeArgs& a, int16_t* ids, uint32_t* carry) {
-  typedef int16_t ids8_t __attribute__((ext_vector_type(8)));
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// One workgroup of 256: the entries in the order (expert, place in the list), by counting
+// for each how many come before it, and the items that they fall into. A row that names an
+// expert twice is one entry with the sum of its weights. `keys` and `sorted` are LDS for
+// kDecodeEntries each.
+__device__ void decode_plan(const DecodeArgs& a, int32_t* keys, int32_t* sorted) {
+  constexpr int kOwn = kDecodeEntries / 256;  // entries of a thread
+  constexpr int32_t kNone = 0x7fffffff;
+  const int tid = threadIdx.x, n4 = (a.n + 3) / 4;
   DecodeItem* items = reinterpret_cast<DecodeItem*>(a.plan + kDecodePlanHead / 4);
   DecodeEntry* entries = reinterpret_cast<DecodeEntry*>(items + a.n);
-  const uint32_t inv_k = 65536u / a.k + 1;  // i / k = i inv_k >> 16 (i < 1024, k <= 16)
-  // f(entry, row) for the entries of this round's expert `tid`
-  auto walk = [&](auto&& f) {
-    for (int i = 0; i < a.n; i += 8) {
-      const ids8_t v = *reinterpret_cast<const ids8_t*>(ids + i);
+  int32_t key[kOwn];
+  float weight[kOwn];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (v[j] == tid) f(i + j, static_cast<int>((i + j) * inv_k >> 16));
-    }
-  };
-  uint32_t base = 0;  // items << 16 | entries of the experts before this round's
-  for (int e0 = 0; e0 < a.E; e0 += 256) {
-    __syncthreads();
-    // (relative to the round, so that 16 bits hold any number of experts)
-    for (int i = tid; i < ((a.n + 7) & ~7); i += 256) {
-      const int e = i < a.n ? decode_expert(a, i) - e0 : -1;
-      ids[i] = static_cast<int16_t>(e >= 0 && e < 256 ? e : -1);
-    }
-    __syncthreads();
-    uint32_t count = 0;
-    int last = -1;
-    walk([&](int, int row) {
-      count += row != last;
-      last = row;
-    });
-    const uint32_t own = (count + kDecodeItem - 1) / kDecodeItem << 16 | count;
-    const uint32_t incl = lin_wave_scan(own);
-    if (lane == 63) carry[wave] = incl;
-    __syncthreads();
-    uint32_t before = base;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += carry[w];
-      base += carry[w];
-    }
-    before += incl - own;
-    int item = before >> 16, at = before & 0xffff;
-    for (uint32_t c = 0; c < count; c += kDecodeItem)
-      items[item++] = DecodeItem{e0 + tid, static_cast<uint16_t>(at + c),
-                                 static_cast<uint16_t>(count - c < kDecodeItem ? count - c : kDecodeItem)};
-    last = -1;
-    --at;
-    walk([&](int i, int row) {
-      const float w = a.weights[i];
-      if (row != last) {
-        last = row;
-        entries[++at] = DecodeEntry{i, w};
-      } else {
-        entries[at].weight += w;
-      }
-    });
+  for (int r = 0; r < kOwn; ++r) {
+    const int i = tid + 256 * r;
+    key[r] = i < a.n ? decode_expert(a, i) : -1;
+    weight[r] = i < a.n ? a.weights[i] : 0.0f;
+    keys[i] = key[r];
+    sorted[i] = kNone;
   }
-  if (tid == 0) a.plan[0] = static_cast<int32_t>(base >> 16);
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kOwn; ++r) {
+    const int i = tid + 256 * r, e = key[r];
+    if (256 * r >= a.n || e < 0) {
+      key[r] = kNone;
+      continue;
+    }
+    bool again = false;
+    const int row = i / a.k * a.k;
+    for (int j = row; j < row + a.k; ++j)
+      if (j != i && keys[j] == e) {
+        again |= j < i;
+        weight[r] += a.weights[j];
+      }
+    key[r] = again ? kNone : e * kDecodeEntries + i;  // (at most 2^20 experts)
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kOwn; ++r) keys[tid + 256 * r] = key[r];
+  __syncthreads();
+  int place[kOwn] = {};
+  for (int j = 0; j < n4; ++j) {
+    const int4 v = reinterpret_cast<const int4*>(keys)[j];
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r)
+      if (256 * r < a.n) place[r] += (v.x < key[r]) + (v.y < key[r]) + (v.z < key[r]) + (v.w < key[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < kOwn; ++r)
+    if (key[r] != kNone) {
+      sorted[place[r]] = key[r];
+      entries[place[r]] = DecodeEntry{key[r] % kDecodeEntries, weight[r]};
+    }
   for (int i = tid; i < a.tiles; i += 256) a.counts[i] = 0;
+  __syncthreads();
+  if (tid >= 64) return;
+  // an item starts at every kDecodeItem-th entry of an expert
+  int32_t* firsts = keys;
+  int n_items = 0, total = 0, run = 0;
+  for (int c = 0; c < a.n; c += 64) {
+    const int p = c + tid;
+    const int32_t v = p < a.n ? sorted[p] : kNone;
+    const int expert = v / kDecodeEntries;
+    const uint64_t upto = ~uint64_t(0) >> (63 - tid);
+    const uint64_t starts = __ballot(v != kNone && (p == 0 || sorted[p - 1] / kDecodeEntries != expert));
+    const uint64_t before = starts & upto;
+    const int start = before ? c + 63 - __builtin_clzll(before) : run;
+    const bool opens = v != kNone && (p - start) % kDecodeItem == 0;
+    const uint64_t open = __ballot(opens);
+    if (opens) {
+      const int item = n_items + __popcll(open & (upto >> 1));
+      firsts[item] = p;
+      items[item].expert = expert;
+    }
+    n_items += __popcll(open);
+    total += __popcll(__ballot(v != kNone));
+    if (starts) run = c + 63 - __builtin_clzll(starts);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (int i = tid; i < n_items; i += 64) {
+    const int first = firsts[i], end = i + 1 < n_items ? firsts[i + 1] : total;
+    items[i].first = static_cast<uint16_t>(first);
+    items[i].count = static_cast<uint16_t>(end - first);
+  }
+  if (tid == 0) a.plan[0] = n_items;
 }
 
 constexpr int kWaves = 4;
@@ -80,16 +106,18 @@ __device__ __forceinline__ float decode_act(float gate, float up) {
   return gate / (1.0f + expf(-gate)) * up;
 }
 
+constexpr int kTable = kDecodeEntries;  // experts whose first entries LDS holds
+
 // KS waves share the contraction; the others take 16 gate rows each.
 template <class F, int NE, int KS, int DEPTH>
 __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs a) {
   constexpr int BM = NE == 1 ? 4 : 16, BP = 16 * (kWaves / KS);
-  __shared__ __attribute__((aligned(16))) int16_t list[kDecodeEntries];
-  __shared__ uint32_t carry[kWaves];
+  // (the plan's keys and their order; the list of the workgroup's entries and the table)
+  __shared__ __attribute__((aligned(16))) int32_t list[kDecodeEntries], first_of[kTable];
   __shared__ lin_f32x4_t part[KS > 1 ? kWaves * 2 * 64 : 1];
   __shared__ __attribute__((aligned(16))) char params[F::dense ? 16 : kWaves * few_lds<F, 2>()];
   if (blockIdx.x == 0) {
-    decode_plan(a, list, carry);
+    decode_plan(a, list, first_of);
     return;
   }
   const int bid = blockIdx.x - 1;
@@ -97,28 +125,50 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.I + BP - 1) / BP, kw = wave % KS;
   const int slot = bid / tiles, p0 = (bid - slot * tiles) * BP + wave / KS * 16, p = p0 + r16;
-  const bool by_expert = a.n > a.E;
-  const int expert = by_expert ? slot : __builtin_amdgcn_readfirstlane(decode_expert(a, slot));
+  constexpr int kChunks = kDecodeEntries / 64;
+  int ids[kChunks];  // the list, loaded at once: it is the first thing that is waited for
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    const int i = 64 * c + lane;
+    ids[c] = 64 * c < a.n && i < a.n ? decode_expert(a, i) : -1;
+  }
+  // this workgroup's expert
+  int expert = -1;
+  if (a.E <= kTable) {
+    // the slot-th entry that is its expert's first one
+    for (int i = threadIdx.x; i < a.E; i += 64 * kWaves) first_of[i] = kDecodeEntries;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+      if (c % kWaves == wave && ids[c] >= 0) atomicMin(first_of + ids[c], 64 * c + lane);
+    __syncthreads();
+    int seen = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const bool leads = ids[c] >= 0 && first_of[ids[c]] == 64 * c + lane;
+      const uint64_t mask = __ballot(leads);
+      const int before = seen + __popcll(mask & ((uint64_t(1) << lane) - 1));
+      const uint64_t hit = __ballot(leads && before == slot);
+      if (hit) expert = __builtin_amdgcn_readlane(ids[c], __builtin_ctzll(hit));
+      seen += __popcll(mask);
+    }
+  } else {
+    // entry `slot`'s, if no entry before it has the same one
+    const int mine = __builtin_amdgcn_readfirstlane(decode_expert(a, slot));
+    bool earlier = mine < 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) earlier |= __ballot(ids[c] == mine && 64 * c + lane < slot) != 0;
+    if (!earlier) expert = mine;
+  }
   if (expert < 0) return;
   int count = 0;
-  for (int c0 = 0; c0 < a.n; c0 += 512) {
-    int ids[8];  // (loaded together: the list is the first thing that is waited for)
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const int i = c0 + 64 * c + lane;
-      ids[c] = i < a.n ? decode_expert(a, i) : -1;
-    }
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const uint64_t mask = __ballot(ids[c] == expert);
-      const int i0 = c0 + 64 * c;
-      if (!by_expert && count == 0 && mask && i0 + __builtin_ctzll(mask) < slot) return;
-      if (wave == 0 && ids[c] == expert)
-        list[count + __popcll(mask & ((uint64_t(1) << lane) - 1))] = static_cast<int16_t>(i0 + lane);
-      count += __popcll(mask);
-    }
+  for (int c = 0; c < kChunks; ++c) {
+    const uint64_t mask = __ballot(ids[c] == expert);
+    if (wave == 0 && ids[c] == expert)
+      list[count + __popcll(mask & ((uint64_t(1) << lane) - 1))] = 64 * c + lane;
+    count += __popcll(mask);
   }
-  if (count == 0) return;
   __syncthreads();
 
   FewRow row[2];
@@ -221,7 +271,7 @@ int decode_up(const DecodeArgs& a, int format, hipStream_t s, const char* what) 
     using F = decltype(f);
     if (a.T == 1) return launch_single<F>(a, s, what);
     if (a.T <= 4) return launch<F, 1, 4>(a, s, what);
-    return launch<F, 4, 2>(a, s, what);
+    return a.n <= 64 ? launch<F, 4, 4>(a, s, what) : launch<F, 4, 2>(a, s, what);
   });
 }
 
