@@ -125,50 +125,64 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.I + BP - 1) / BP, kw = wave % KS;
   const int slot = bid / tiles, p0 = (bid - slot * tiles) * BP + wave / KS * 16, p = p0 + r16;
-  constexpr int kChunks = kDecodeEntries / 64;
-  int ids[kChunks];  // the list, loaded at once: it is the first thing that is waited for
+  // The list goes through registers, in halves of a fixed size that most calls need one of.
+  constexpr int kChunks = 8;
+  const int halves = (a.n + 64 * kChunks - 1) / (64 * kChunks);
+  int ids[kChunks];
+  auto load_ids = [&](int half) {
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const int i = 64 * c + lane;
-    ids[c] = 64 * c < a.n && i < a.n ? decode_expert(a, i) : -1;
-  }
+    for (int c = 0; c < kChunks; ++c) {
+      const int i = 64 * (kChunks * half + c) + lane;
+      ids[c] = -1;
+      if (64 * (kChunks * half + c) < a.n && i < a.n) ids[c] = decode_expert(a, i);
+    }
+  };
+  // f(chunk of ids, first place) for the chunks there are
+  auto chunks = [&](auto&& f) {
+    for (int half = 0; half < halves; ++half) {
+      if (halves > 1) load_ids(half);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int i0 = 64 * (kChunks * half + c);
+        if (i0 >= a.n) break;
+        f(ids[c], i0);
+      }
+    }
+  };
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  if (halves == 1) load_ids(0);
   // this workgroup's expert
   int expert = -1;
   if (a.E <= kTable) {
     // the slot-th entry that is its expert's first one
     for (int i = threadIdx.x; i < a.E; i += 64 * kWaves) first_of[i] = kDecodeEntries;
     __syncthreads();
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      if (c % kWaves == wave && ids[c] >= 0) atomicMin(first_of + ids[c], 64 * c + lane);
+    chunks([&](int id, int i0) {
+      if (i0 / 64 % kWaves == wave && id >= 0) atomicMin(first_of + id, i0 + lane);
+    });
     __syncthreads();
     int seen = 0;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const bool leads = ids[c] >= 0 && first_of[ids[c]] == 64 * c + lane;
+    chunks([&](int id, int i0) {
+      const bool leads = id >= 0 && first_of[id] == i0 + lane;
       const uint64_t mask = __ballot(leads);
-      const int before = seen + __popcll(mask & ((uint64_t(1) << lane) - 1));
-      const uint64_t hit = __ballot(leads && before == slot);
-      if (hit) expert = __builtin_amdgcn_readlane(ids[c], __builtin_ctzll(hit));
+      const uint64_t hit = __ballot(leads && seen + __popcll(mask & below) == slot);
+      if (hit) expert = __builtin_amdgcn_readlane(id, __builtin_ctzll(hit));
       seen += __popcll(mask);
-    }
+    });
   } else {
     // entry `slot`'s, if no entry before it has the same one
     const int mine = __builtin_amdgcn_readfirstlane(decode_expert(a, slot));
     bool earlier = mine < 0;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) earlier |= __ballot(ids[c] == mine && 64 * c + lane < slot) != 0;
+    chunks([&](int id, int i0) { earlier |= __ballot(id == mine && i0 + lane < slot) != 0; });
     if (!earlier) expert = mine;
   }
   if (expert < 0) return;
   int count = 0;
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const uint64_t mask = __ballot(ids[c] == expert);
-    if (wave == 0 && ids[c] == expert)
-      list[count + __popcll(mask & ((uint64_t(1) << lane) - 1))] = 64 * c + lane;
+  chunks([&](int id, int i0) {
+    const uint64_t mask = __ballot(id == expert);
+    if (wave == 0 && id == expert) list[count + __popcll(mask & below)] = i0 + lane;
     count += __popcll(mask);
-  }
+  });
   __syncthreads();
 
   FewRow row[2];
@@ -271,7 +285,7 @@ int decode_up(const DecodeArgs& a, int format, hipStream_t s, const char* what) 
     using F = decltype(f);
     if (a.T == 1) return launch_single<F>(a, s, what);
     if (a.T <= 4) return launch<F, 1, 4>(a, s, what);
-    return a.n <= 64 ? launch<F, 4, 4>(a, s, what) : launch<F, 4, 2>(a, s, what);
+    return a.n <= 64 ? launch<F, 4, 4>(a, s, what) : launch<F, 4, 1>(a, s, what);
   });
 }
 
