@@ -148,12 +148,32 @@ __global__ void __launch_bounds__(256) top_k_kernel(const RouterArgs a) {
     typename K::type key[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) key[i] = K::make(bits[i], element<VEC>(l, i));
+    // Eight keys of a lane in descending order: its largest is then in its first register,
+    // and a choice that was this lane's moves the others up.
+    constexpr bool SORTED = VPL <= 8;
+    if constexpr (SORTED) {
+      static_assert(VPL == 8, "network of eight");
+      auto order = [&](int i, int j) {
+        const typename K::type x = key[i], y = key[j];
+        key[i] = x > y ? x : y;
+        key[j] = x > y ? y : x;
+      };
+      // Batcher's odd-even merge of eight
+      order(0, 1); order(2, 3); order(4, 5); order(6, 7);
+      order(0, 2); order(1, 3); order(4, 6); order(5, 7);
+      order(1, 2); order(5, 6);
+      order(0, 4); order(1, 5); order(2, 6); order(3, 7);
+      order(2, 4); order(3, 5);
+      order(1, 2); order(3, 4); order(5, 6);
+    }
     typename K::type mine = 0;  // lane j keeps choice j
     float m = 0, z = 0;
     for (int j = 0; j < a.k; ++j) {
       typename K::type best = key[0];
+      if constexpr (!SORTED) {
 #pragma unroll
-      for (int i = 1; i < VPL; ++i) best = key[i] > best ? key[i] : best;
+        for (int i = 1; i < VPL; ++i) best = key[i] > best ? key[i] : best;
+      }
       best = row_max(best);
       if (j == 0) {
         m = best > 0 ? K::value(best) : 0.0f;
@@ -163,8 +183,15 @@ __global__ void __launch_bounds__(256) top_k_kernel(const RouterArgs a) {
         }
       }
       if (l == j) mine = best;
+      if constexpr (SORTED) {
+        const bool own = key[0] == best;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) key[i] = key[i] == best ? 0 : key[i];
+        for (int i = 0; i + 1 < VPL; ++i) key[i] = own ? key[i + 1] : key[i];
+        key[VPL - 1] = own ? 0 : key[VPL - 1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) key[i] = key[i] == best ? 0 : key[i];
+      }
     }
     const bool some = mine > 0;
     const float w = some ? expf(K::value(mine) - m) : 0.0f;
@@ -179,6 +206,12 @@ __global__ void __launch_bounds__(256) top_k_kernel(const RouterArgs a) {
 template <int TYPE, int VEC, int VPL, bool RENORM>
 __global__ void __launch_bounds__(256) top_k_grad_kernel(const RouterArgs a) {
   constexpr int ES = TYPE == kF32 ? 4 : 2;
+  // What the chosen experts get, at its place of the row: each row its own part, written
+  // and read by the 16 lanes that share it (one wave). Short rows only.
+  constexpr bool PLACED = VPL <= 16;
+  constexpr int PITCH = VPL * kLanes + 4;  // (the four rows of a wave start in other banks)
+  __shared__ __attribute__((aligned(16))) float placed[PLACED ? 256 / kLanes * PITCH : 4];
+  float* const place = placed + (PLACED ? threadIdx.x / kLanes * PITCH : 0);
   const int l = threadIdx.x & (kLanes - 1);
   const int64_t rows = static_cast<int64_t>(gridDim.x) * (256 / kLanes);
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * (256 / kLanes); r0 < a.T; r0 += rows) {
@@ -224,16 +257,46 @@ __global__ void __launch_bounds__(256) top_k_grad_kernel(const RouterArgs a) {
     const float wd = w != 0.0f ? w * dw : 0.0f;
     const float dot = row_sum(wd);
     const float add = !RENORM ? wd : w != 0.0f ? w * (dw - dot) : 0.0f;
+    const float scale = RENORM || z == 0.0f ? 0.0f : -dot / z;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) p[i] = RENORM || z == 0.0f ? 0.0f : -(p[i] / z) * dot;
+    for (int i = 0; i < VPL; ++i) p[i] = RENORM || z == 0.0f ? 0.0f : p[i] * scale;
+    // An index that stands twice in a row gets the sum, in the order of the row.
+    bool again = false;
+    float sum = add;
     static_for<kMaxTopK>([&](auto j) {
       if (j < a.k) {
         const int e = row_lane<j>(chosen);
         const float v = row_lane<j>(add);
+        if constexpr (PLACED) {
+          if (e == chosen && j != l) {
+            again |= j < l;
+            sum += v;
+          }
+        } else {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) p[i] += element<VEC>(l, i) == e ? v : 0.0f;
+          for (int i = 0; i < VPL; ++i) p[i] += element<VEC>(l, i) == e ? v : 0.0f;
+        }
       }
     });
+    if constexpr (PLACED) {
+      // (LDS serves a wave in order; the fences keep the compiler to that)
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < VPL; i += 4) *reinterpret_cast<float4*>(place + 4 * l + 64 * (i / 4)) = float4{0, 0, 0, 0};
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (chosen >= 0 && !again) place[chosen] = sum;
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int i = 0; i < VPL; i += VEC) {
+        const int e = element<VEC>(l, i);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p[i + j] += place[e + j];
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
     if (r >= a.T) continue;
     char* out = a.dlogits + t * a.E * ES;
 #pragma unroll
