@@ -137,9 +137,6 @@ int run(const LinArgs& a, const FewWeight& w, int choice, hipStream_t s, const c
 }
 template <int FORMAT>
 int run_types(const LinArgs& a, const FewWeight& w, int choice, hipStream_t s, const char* what) {
-#ifdef AFFINE_FORCE
-  return run<FewFmt<FORMAT, kBF16, 2>>(a, w, choice, s, what);
-#endif
   const bool f16 = a.out_type == kF16, wide = w.type == kF32;
   if (f16) return wide ? run<FewFmt<FORMAT, kF16, 4>>(a, w, choice, s, what)
                        : run<FewFmt<FORMAT, kF16, 2>>(a, w, choice, s, what);

@@ -11,10 +11,6 @@
 namespace mgq {
 namespace {
 
-#ifdef AFFINE_FORCE
-extern "C" int mgq_force[4] = {0, 0, 0, 0};
-#endif
-
 int run_tile(LinArgs a, const FewWeight& w, int bits, LinTileShape t, hipStream_t s, const char* what) {
   a.P = w.p;
   a.Ps = reinterpret_cast<const uint8_t*>(w.s);
@@ -104,13 +100,6 @@ Choice choose(const LinArgs& a, const FewWeight& w, int bits) {
 }
 
 int run(const LinArgs& a, const FewWeight& w, int bits, hipStream_t s, const char* what) {
-#ifdef AFFINE_FORCE
-  if (mgq_force[0] >= 100) {
-    const int r[4] = {256, 128, 64, 64}, c[4] = {256, 256, 256, 128}, i = mgq_force[0] - 100;
-    return run_tile(a, w, bits, LinTileShape{r[i], c[i], mgq_force[2] != 0}, s, what);
-  }
-  return run_few(a, w, bits, mgq_force[0], s, what);
-#endif
   const Choice c = choose(a, w, bits);
   if (c.tile.rows) return run_tile(a, w, bits, c.tile, s, what);
   return run_few(a, w, bits, c.few, s, what);

@@ -53,7 +53,6 @@ struct FewFmt {
   static constexpr bool affine = W >= kFewAf2;
   static constexpr int bits = dense ? 16 : W == kFewAf2 ? 2 : W == kFewMx4 || W == kFewAf4 ? 4 : 8;
   static constexpr int words = dense ? 16 : bits;  // 32-bit words of a lane and step
-  static constexpr int op = XT == kF16 ? kOpF16 : kOpBF16;
 };
 
 // Where a lane reads weight row p0 + lane % 16 (the last one of the weight past its end):
@@ -501,15 +500,6 @@ __device__ __forceinline__ void few_product(const FewRow (&row)[NP], const FewWe
     few_multiply<F, NP, NQ, NE, false>(f[0], xv[0], whole, K, shift, (whole * kFewStep >> shift) - group,
                                        lds, acc);
   }
-}
-
-// Checks of a quantized weight's description, on the host.
-inline bool few_weight_ok(int format, int64_t K, int shift, int type) {
-  if (format == kFewDense) return true;
-  if (K % 32) return false;
-  if (format < kFewAf2) return true;
-  return shift >= 5 && shift <= 7 && K % (int64_t(1) << shift) == 0 &&
-         (type == kF32 || type == kBF16 || type == kF16);
 }
 
 }  // namespace mgq

@@ -165,14 +165,14 @@ class _DecodeWeights:
         flat = [t for w in self.given for t in ((w,) if isinstance(w, torch.Tensor) else w)]
         ptrs = [t.data_ptr() for t in tensors]
         self.in_place = ptrs == [t.data_ptr() for t in flat]
-        self.tensors, self.layout = tensors, [(t, t.data_ptr(), t.shape, t.stride()) for t in flat]
+        self.tensors, self.layout = tensors, [(t, t.data_ptr(), t.dtype, t.shape, t.stride()) for t in flat]
         self._sizes: dict[tuple[int, int], int] = {}
 
     def current(self, layer) -> bool:
         if not self.in_place or layer.gate_up is not self.given[0] or layer.down is not self.given[1]:
             return False
-        for t, ptr, shape, stride in self.layout:
-            if t.data_ptr() != ptr or t.shape != shape or t.stride() != stride:
+        for t, ptr, dtype, shape, stride in self.layout:
+            if t.data_ptr() != ptr or t.dtype is not dtype or t.shape != shape or t.stride() != stride:
                 return False
         return True
 
@@ -193,11 +193,13 @@ class ExpertMLP:
     (int8), or packed words, scales and biases (affine), as linear.py takes them.
     """
 
-    MODES = ("dense", "mxfp4", "mxfp8", "int8", "affine")
+    MODES = ("dense", "mxfp4", "mxfp8", "int8")  # one grid each
+    GRID_MODES = ("affine",)                      # `bits` and a group size choose the grid
 
     def __init__(self, gate_up, down, mode: str = "dense"):
-        if mode not in self.MODES:
-            raise ValueError(f"unsupported expert mode: {mode} ({', '.join(self.MODES)})")
+        if mode not in self.MODES + self.GRID_MODES:
+            raise ValueError(f"unsupported expert mode: {mode} "
+                             f"({', '.join(self.MODES + self.GRID_MODES)})")
         self.mode = mode
         self.gate_up, self.down = gate_up, down
         first = gate_up if mode == "dense" else gate_up[0]
