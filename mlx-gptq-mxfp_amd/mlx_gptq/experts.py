@@ -228,6 +228,11 @@ class ExpertMLP:
         default = grid.mode_defaults(mode)[1]
         if mode != "affine" and bits not in (None, default):
             raise ValueError(f"{mode} codes have {default} bits (got {bits})")
+        given = 3 if mode == "affine" else 2
+        if len(gate_up) != given or len(down) != given:
+            raise ValueError(f"from_codes: {mode} weights are codes and scales"
+                             + (" and biases" if given == 3 else "")
+                             + f" (got {len(gate_up)} and {len(down)} tensors)")
         return cls(*((packing.pack_q(w[0], bits or default), *w[1:]) for w in (gate_up, down)), mode)
 
     @staticmethod
