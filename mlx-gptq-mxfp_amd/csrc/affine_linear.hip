@@ -126,8 +126,8 @@ extern "C" int mgq_affine_linear(const void* X, int dtype, int64_t n_rows, int64
               "%s: group_size must be 32, 64 or 128", what);
   if (int rc = lin_check_list(what, offsets, row_index, n_groups, n_entries, n_rows)) return rc;
   if (int rc = lin_check_dims(what, N, K)) return rc;
-  MGQ_REQUIRE(K % group_size == 0, MGQ_ERR_SHAPE, "%s: K = %lld is no multiple of the group size", what,
-              (long long)K);
+  MGQ_REQUIRE(K > 0 && K % group_size == 0, MGQ_ERR_SHAPE,
+              "%s: K = %lld is no multiple of the group size", what, (long long)K);
   MGQ_REQUIRE(ldx >= K, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
   if (n_entries == 0) return MGQ_OK;
   LinArgs a = {};
@@ -165,6 +165,7 @@ extern "C" int mgq_affine_choice(const void* X, int64_t ldx, int64_t n_entries, 
   if (int rc = lin_check_list(what, grouped ? &some_list : nullptr, nullptr, n_groups, n_entries, n_entries))
     return rc;
   if (int rc = lin_check_dims(what, N, K)) return rc;
+  MGQ_REQUIRE(K > 0 && K % 32 == 0, MGQ_ERR_SHAPE, "%s: K = %lld is no multiple of 32", what, (long long)K);
   LinArgs a = {};
   a.Q = static_cast<const char*>(X);
   a.ldq = 2 * ldx;

@@ -312,21 +312,27 @@ __device__ __forceinline__ void few_stage(const FewParams<F> (&f)[NP], int type,
   const int r16 = threadIdx.x & 15, quad = (threadIdx.x >> 4) & 3;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
+  auto put = [&](auto as_f32) __attribute__((always_inline)) {
 #pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    char* row = lds + (16 * p + r16) * few_pitch<F>();
-    if constexpr (F::mx) {
-      *reinterpret_cast<uint32_t*>(row + 4 * quad) = f[p].s[0];
-    } else {
+    for (int p = 0; p < NP; ++p) {
+      char* row = lds + (16 * p + r16) * few_pitch<F>();
+      if constexpr (F::mx) {
+        *reinterpret_cast<uint32_t*>(row + 4 * quad) = f[p].s[0];
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t s = F::SB == 4 ? f[p].s[i] : f[p].s[i / 2] >> (16 * (i & 1)) & 0xffff;
-        const uint32_t b = F::SB == 4 ? f[p].b[i] : f[p].b[i / 2] >> (16 * (i & 1)) & 0xffff;
-        *reinterpret_cast<uint2*>(row + 8 * (4 * quad + i)) =
-            uint2{few_param_f32<F::SB>(s, type), few_param_f32<F::SB>(b, type)};
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t s = F::SB == 4 ? f[p].s[i] : f[p].s[i / 2] >> (16 * (i & 1)) & 0xffff;
+          const uint32_t b = F::SB == 4 ? f[p].b[i] : f[p].b[i / 2] >> (16 * (i & 1)) & 0xffff;
+          *reinterpret_cast<uint2*>(row + 8 * (4 * quad + i)) = uint2{as_f32(s), as_f32(b)};
+        }
       }
     }
-  }
+  };
+  // (one branch on the type, not one a value)
+  if (F::SB == 2 && type == kF16)
+    put([](uint32_t v) { return f2u(f16_to_f32(static_cast<uint16_t>(v))); });
+  else
+    put([](uint32_t v) { return F::SB == 2 ? v << 16 : v; });
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }

@@ -51,7 +51,8 @@ def test_entry_point_returns_a_status():
     entry = nat.load().mgq_affine_linear
     for change, status in ((dict(dtype=nat.DTYPE_F32), nat.ERR_VALUE), (dict(param_dtype=5), nat.ERR_VALUE),
                            (dict(bits=3), nat.ERR_VALUE), (dict(group_size=16), nat.ERR_VALUE),
-                           (dict(K=96), nat.ERR_SHAPE), (dict(ldx=63), nat.ERR_SHAPE),
+                           (dict(K=96), nat.ERR_SHAPE), (dict(K=0), nat.ERR_SHAPE),
+                           (dict(ldx=63), nat.ERR_SHAPE),
                            (dict(n_groups=2), nat.ERR_VALUE), (dict(n_entries=5), nat.ERR_SHAPE),
                            (dict(n_rows=0), nat.ERR_SHAPE), (dict(N=1 << 31), nat.ERR_SHAPE),
                            (dict(n_entries=1 << 30, n_rows=1 << 30, N=1 << 29), nat.ERR_SHAPE)):

@@ -265,3 +265,70 @@ def test_offsets_out_of_range_are_clamped():
     idx = torch.tensor([0, 7, -2, 3, 5, 100], dtype=torch.int32)
     y = product(x, q, s, b, 4, off, idx, validate=False)
     close(y, *ref.affine_forward(x, q, s, b, [0, 3, 6], idx.clamp(0, 5)), 64)
+
+
+# a call that reaches each form (M, N, K, G, bits, bytes that the rows are off 16)
+REACHED = {
+    (SINGLE, 0, 0): (1, 4096, 736, 0, 4, 0), (FEW, 1, 0): (32, 100, 32, 32, 4, 2),
+    (FEW, 2, 0): (1, 16, 32, 0, 4, 2), (FEW, 3, 0): (600, 40, 512, 16, 2, 0),
+    (FEW, 4, 0): (8, 6000, 512, 2, 4, 0), (FEW, 5, 0): (200, 40, 32, 0, 2, 0),
+    (FEW, 6, 0): (600, 40, 32, 16, 8, 0), (FEW, 7, 0): (600, 40, 160, 16, 2, 2),
+    (FEW, 8, 0): (200, 257, 512, 32, 4, 2), (FEW, 9, 0): (600, 257, 512, 32, 2, 2),
+    (FEW, 10, 0): (300, 1001, 512, 16, 4, 2), (FEW, 11, 0): (40, 4096, 32, 16, 4, 2),
+    (TILE, 64, 128): (300, 6000, 1024, 0, 8, 0), (TILE, 64, 256): (300, 6000, 32, 8, 8, 0),
+    (TILE, 128, 256): (128, 6000, 32, 16, 4, 0), (TILE, 256, 256): (200, 6000, 32, 16, 8, 0),
+    (STAGED, 64, 256): (300, 6000, 32, 8, 8, 2), (STAGED, 128, 256): (600, 4096, 32, 16, 8, 2),
+}
+
+
+@pytest.mark.parametrize("form", sorted(REACHED))
+@pytest.mark.parametrize("dtype,params", [("bf16", "bf16"), ("f16", "f32")])
+def test_every_kernel_is_reached(form, dtype, params):
+    M, N, K, G, bits, off16 = REACHED[form]
+    q, s, b = weight(max(G, 1), N, K, bits, 32, params, seed=M)
+    store = torch.zeros(M * K + 8, dtype=TYPES[dtype], device=DEV)
+    x = store[off16 // 2:off16 // 2 + M * K].view(M, K)
+    x.copy_(rows(M, K, dtype))
+    off = None
+    if G:  # uneven groups, the third one empty where there is one
+        cuts = torch.randint(0, M + 1, (G - 1,), generator=torch.Generator().manual_seed(2)).sort().values
+        off = [0, *cuts.tolist(), M]
+        if G > 3:
+            off[3] = off[2]
+    _, took = check(x, q, s, b, bits, off)
+    assert took == form
+
+
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_far_rows_and_weights(M):
+    """Rows, weights, scales and results whose places pass 2^32 bytes."""
+    G, N, K, tail = 3, 1 << 20, 4096, 40
+    T = (1 << 19) + 70000  # rows of 8 KiB
+    g = torch.Generator().manual_seed(M)
+    words = torch.zeros(G, N, K // 8, dtype=torch.int32, device=DEV)
+    s = torch.zeros(G, N, K // 32, dtype=torch.float32, device=DEV)
+    b = torch.zeros(G, N, K // 32, dtype=torch.float32, device=DEV)
+    q, sl, bl = weight(1, tail, K, 4, 32, "f32")
+    words[2, -tail:] = packing.pack_q(q[0].to(DEV), 4).view(torch.int32)
+    s[2, -tail:], b[2, -tail:] = sl[0].to(DEV), bl[0].to(DEV)
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device=DEV)
+    used = torch.randint(T - 60000, T, (M,), generator=g)
+    used[-1] = T - 1
+    x[used.to(DEV)] = rows(M, K, "bf16").to(DEV)
+    idx = used.to(torch.int32).to(DEV)
+    off = torch.tensor([0, 0, 0, M], dtype=torch.int32, device=DEV)
+    y = linear.affine_linear(x, words, s, b, 4, off, idx)
+    took = kernel(x, words, 4, G, N, off, M)
+    few = x[used.to(DEV)].cpu()
+    want, mag = ref.affine_forward(few, q, sl, bl)
+    rounded = ref.forward(few, ref.affine(q, sl, bl)[0])[1] if took[0] >= TILE else None
+    close(y[:, -tail:], want, mag, K, took, rounded)
+    assert not bool(y[:, :-tail].any())
+
+
+def test_the_choice_refuses_what_the_product_refuses():
+    out = (ctypes.c_int32 * 3)()
+    for args in ((3, 1, 16, 64), (4, 2, 16, 64), (4, 1, 1 << 31, 64), (4, 1, 16, 0)):
+        bits, G, N, K = args
+        with pytest.raises((ValueError, AssertionError)):
+            nat.call("mgq_affine_choice", 16, 64, 4, 16, bits, G, N, K, 0, ctypes.addressof(out))

@@ -260,3 +260,38 @@ def test_a_gradient_raises():
     y = layer.mlp.decode(x.requires_grad_(), index, weights)
     with pytest.raises(NotImplementedError, match="decode"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("T,k", [(2, 16), (20, 3), (64, 16)])
+def test_more_experts_than_a_table_of_them_holds(T, k):
+    layer = Layer("affine", 1500, 32, 32, group=32)
+    x, index, weights = layer.inputs(T, k)
+    index[:, 0] = 1499
+    index[0] = torch.arange(k) % 2 + 1030  # (a row with two experts, many times)
+    layer.check(x, index, weights)
+
+
+@pytest.mark.parametrize("T", [1, 3, 20])
+def test_far_weights(T):
+    """An expert whose weights start behind 2^32 bytes, against float64 on the device."""
+    E, H, I = 5, 16384, 16384
+    up = torch.empty(E, 2 * I, H, dtype=torch.bfloat16, device=DEV).normal_(0, H**-0.5)
+    down = torch.empty(E, H, I, dtype=torch.bfloat16, device=DEV).normal_(0, I**-0.5)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV)
+    weights = torch.rand(T, 1, generator=g).to(DEV) + 0.5
+    y = ExpertMLP(up, down).decode(x, torch.full((T, 1), E - 1, device=DEV), weights)
+    w, xd = up[-1].double(), x.double()
+    h, eh = xd @ w.T, (H + 48) * 2.0**-23 * (xd.abs() @ w.abs().T)
+    del w
+    gate, u, eg, eu = h[:, :I], h[:, I:], eh[:, :I], eh[:, I:]
+    a = torch.nn.functional.silu(gate) * u
+    ea = 1.1 * eg * (u.abs() + eu) + (gate.abs() + eg) * eu + 2.0**-20 * a.abs()
+    ea = ea + 2.0**-8 * 1.01 * (a.abs() + ea)
+    w = down[-1].double()
+    want = a @ w.T
+    err = ea @ w.abs().T + (I + 48) * 2.0**-23 * ((a.abs() + ea) @ w.abs().T)
+    want, err = weights.double() * want, weights.double() * (err * 1.01 + 2.0**-20 * want.abs())
+    bound = err + 2.0**-8 * 1.01 * (want.abs() + err)
+    d = (y.double() - want).abs()
+    assert bool((d <= bound).all()), float((d - bound).max())
