@@ -1,5 +1,5 @@
-// The inner product that the kernels for a handful of rows share (affine_linear.hip,
-// experts_decode.hip): up to 16 NQ rows of 16-bit x times 16 NP weight rows in any
+// The inner product that the kernels for a handful of rows share (affine_few.h,
+// experts_up.hip, experts_down.hip): up to 16 NQ rows of 16-bit x times 16 NP weight rows in any
 // of the weight formats, over a part of the contraction.
 //
 // A 16x16x32 MFMA takes the x rows as its A operand and the weight rows as B, so a

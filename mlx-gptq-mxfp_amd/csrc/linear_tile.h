@@ -1,4 +1,4 @@
-// The large-tile kernels' host side (linear_tile.hip) and wgrad's work list.
+// The large-tile kernels' host side (linear_tile.hip, linear_tile_kernel.h) and wgrad's work list.
 #pragma once
 
 #include "linear_common.h"

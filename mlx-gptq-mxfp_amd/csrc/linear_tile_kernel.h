@@ -20,6 +20,10 @@
 //   - Transposed operands keep contraction rows (64 of them) in LDS as they are
 //     in memory; ds_read_b64_tr_b16 hands a lane one column of four rows. The
 //     64-byte block b of row t sits at b ^ (t % 4).
+//   - Affine codes (2, 4 or 8 bits, a scale and a bias for 32, 64 or 128 values) stay codes
+//     in LDS like MX ones; q s + b is formed in fp32 and rounded once to x's type, which
+//     the MFMA needs: 8 fused multiply-adds and 4 packed roundings for 8 codes, which the
+//     MFMAs of a tile do not cover (8191 x 14336 x 4096, 4 bits: 963 us, 1000 TFLOP/s).
 //   - An MX weight's codes stay codes in LDS (32 or 64 bytes a row and stage, and
 //     its two scale bytes widened to dwords). Half-wave h of the MFMA takes the
 //     stage's elements 32 h .. 32 h + 31, one MX group, so a lane needs one scale

@@ -10,6 +10,12 @@
 // instructions), a wave four rows. A logit becomes an unsigned key whose order is (logit,
 // then lower index first); logits of -infinity (experts that the row may not use) get
 // key 0 and are never chosen.
+//
+// Bound by instructions, not by bytes: 65536 rows of 128 bf16 logits with k = 8 take 14.3 us
+// (23 MB) and the gradient 13.0 us (40 MB), 1.6 and 3.1 TB/s. Eight keys of a lane are sorted
+// once (16 us where each choice looked through all of them); the gradient's chosen terms
+// go to their places through LDS (15.5 us where every lane compared its experts with all k).
+// One row: 2.8 us, a launch.
 #include "linear_common.h"
 
 namespace mgq {
