@@ -128,6 +128,8 @@ extern "C" int mgq_affine_linear(const void* X, int dtype, int64_t n_rows, int64
   if (int rc = lin_check_dims(what, N, K)) return rc;
   MGQ_REQUIRE(K > 0 && K % group_size == 0, MGQ_ERR_SHAPE,
               "%s: K = %lld is no multiple of the group size", what, (long long)K);
+  MGQ_REQUIRE(K / 8 * bits <= kFewRowBytes, MGQ_ERR_SHAPE, "%s: rows of K = %lld codes pass 2^28 bytes",
+              what, (long long)K);
   MGQ_REQUIRE(ldx >= K, MGQ_ERR_SHAPE, "%s: a row pitch is shorter than a row", what);
   if (n_entries == 0) return MGQ_OK;
   LinArgs a = {};

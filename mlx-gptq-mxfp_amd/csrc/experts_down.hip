@@ -310,8 +310,8 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
     w->p = static_cast<const char*>(m.data);
     w->n = n;
     if (format == kFewDense) {
-      MGQ_REQUIRE(m.ld >= cols && m.ld < (int64_t(1) << 29), MGQ_ERR_SHAPE,
-                  "%s: a weight's pitch is shorter than its row, or 2^29 elements", what);
+      MGQ_REQUIRE(m.ld >= cols && m.ld <= kFewRowBytes / 2, MGQ_ERR_SHAPE,
+                  "%s: a weight's pitch is shorter than its row, or passes 2^28 bytes", what);
       w->ld = 2 * m.ld;
       w->group = 2 * m.expert;
       return MGQ_OK;
@@ -332,6 +332,7 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
     MGQ_REQUIRE(cols % group == 0, MGQ_ERR_SHAPE, "%s: %lld columns are no multiple of the group size",
                 what, (long long)cols);
     w->ld = cols / 8 * bits;
+    MGQ_REQUIRE(w->ld <= kFewRowBytes, MGQ_ERR_SHAPE, "%s: a weight's rows pass 2^28 bytes", what);
     w->group = w->ld * n;
     return MGQ_OK;
   };

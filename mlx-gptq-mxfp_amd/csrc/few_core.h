@@ -44,6 +44,9 @@ struct FewWeight {
   int type;            // affine: DType of scales and biases
 };
 
+// Bytes of a weight row at most: a lane's offset from the first of sixteen rows is 32 bits.
+constexpr int64_t kFewRowBytes = int64_t(1) << 28;
+
 // W: FewFormat, XT: kBF16 or kF16, SB: bytes of an affine scale (2 or 4).
 template <int W_, int XT_, int SB_ = 2>
 struct FewFmt {

@@ -336,7 +336,8 @@ class ExpertMLP:
             raise ValueError(f"{fn}: int8 experts are not supported, use forward")
         x = hidden_states
         dense = (self.gate_up, self.down) if self.mode == "dense" else ()
-        tracked = linear._tracked(fn, x, top_k_weights, *dense)
+        floats = (*self.gate_up[1:], *self.down[1:]) if self.mode == "affine" else dense
+        tracked = linear._tracked(fn, x, top_k_weights, *floats)
         if x.dtype not in linear._HALF or (self.mode[:2] == "mx" and x.dtype is not torch.bfloat16):
             raise TypeError(f"{fn}: expects bfloat16 rows, or float16 ones without MXFP weights "
                             f"(got {x.dtype})")
@@ -370,4 +371,4 @@ class ExpertMLP:
                        k, self.num_experts, H, d.inner, d.up_ptr, d.down_ptr, out.data_ptr(),
                        ws.data_ptr(), size)
         out = linear._home(out, x)
-        return linear._NoGradient.apply(fn, out, x, top_k_weights, *dense) if tracked else out
+        return linear._NoGradient.apply(fn, out, x, top_k_weights, *floats) if tracked else out

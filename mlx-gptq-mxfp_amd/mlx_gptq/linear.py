@@ -35,6 +35,7 @@ staged through the current HIP device, as in the other modules.
 from __future__ import annotations
 
 import functools
+import operator
 
 import numpy as np
 import torch
@@ -426,6 +427,7 @@ def affine_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, b
     _rows2(fn, "x", x)
     T, K = x.shape
     st = scales.dtype
+    bits = operator.index(bits)
     G, N, group = affine_dims(fn, K, bits, packed.shape, packed.dtype, scales.shape, st, biases.shape,
                               biases.dtype, offsets is not None)
     dev = _device(x, packed, scales)

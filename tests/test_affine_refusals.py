@@ -26,6 +26,7 @@ def call(x=(4, 64), words=(3, 8), scales=(3, 2), biases=None, bits=4, x_type=BF,
     ({"types": (torch.int32, torch.int32)}, TypeError),
     ({"bits": 3}, ValueError),
     ({"bits": 16}, ValueError),
+    ({"bits": 4.0}, TypeError),
     ({"bits": 8}, AssertionError),
     ({"x": (4, 65)}, AssertionError),
     ({"x": (4, 0), "words": (3, 0), "scales": (3, 0)}, AssertionError),
@@ -53,6 +54,7 @@ def test_entry_point_returns_a_status():
                            (dict(bits=3), nat.ERR_VALUE), (dict(group_size=16), nat.ERR_VALUE),
                            (dict(K=96), nat.ERR_SHAPE), (dict(K=0), nat.ERR_SHAPE),
                            (dict(ldx=63), nat.ERR_SHAPE),
+                           (dict(bits=8, K=(1 << 28) + 64, ldx=1 << 29), nat.ERR_SHAPE),
                            (dict(n_groups=2), nat.ERR_VALUE), (dict(n_entries=5), nat.ERR_SHAPE),
                            (dict(n_rows=0), nat.ERR_SHAPE), (dict(N=1 << 31), nat.ERR_SHAPE),
                            (dict(n_entries=1 << 30, n_rows=1 << 30, N=1 << 29), nat.ERR_SHAPE)):

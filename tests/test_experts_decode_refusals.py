@@ -115,6 +115,9 @@ def entry(up=None, down=None, **change):
     (dict(up=dict(param_dtype=7)), nat.ERR_VALUE),
     (dict(H=96, ldx=96, up=dict(group=64)), nat.ERR_SHAPE),
     (dict(down=dict(ld=31)), nat.ERR_SHAPE), (dict(down=dict(ld=1 << 29)), nat.ERR_SHAPE),
+    (dict(down=dict(ld=(1 << 27) + 1)), nat.ERR_SHAPE),
+    (dict(H=(1 << 28) + 64, ldx=1 << 29, up=dict(format=nat.WEIGHT_AFFINE8), ws_bytes=1 << 40),
+     nat.ERR_SHAPE),
     (dict(down=dict(format=nat.WEIGHT_MXFP4), I=48), nat.ERR_SHAPE),
     (dict(dtype=nat.DTYPE_F16, down=dict(format=nat.WEIGHT_MXFP8)), nat.ERR_VALUE),
     (dict(ws_bytes=100), nat.ERR_WORKSPACE)])

@@ -262,6 +262,15 @@ def test_a_gradient_raises():
         y.sum().backward()
 
 
+def test_a_gradient_of_the_scales_raises():
+    layer = Layer("affine", 4, 32, 32)
+    x, index, weights = (t.to(DEV) for t in layer.inputs(3, 2))
+    layer.mlp.gate_up[1].requires_grad_()
+    y = layer.mlp.decode(x, index, weights)
+    with pytest.raises(NotImplementedError, match="decode"):
+        y.sum().backward()
+
+
 @pytest.mark.parametrize("T,k", [(2, 16), (20, 3), (64, 16)])
 def test_more_experts_than_a_table_of_them_holds(T, k):
     layer = Layer("affine", 1500, 32, 32, group=32)
