@@ -159,20 +159,27 @@ class _DecodeWeights:
         self.type_code = nat.dtype_code(dtype)
         self.up, self.down = up, down
         self.up_ptr, self.down_ptr = ctypes.addressof(up), ctypes.addressof(down)
-        self.given = gate_up, down_weight
         # copies (of host weights, or of ones whose rows do not lie one after the other) go
         # with this call: only weights described where they are stand for the next one
-        flat = [t for w in self.given for t in ((w,) if isinstance(w, torch.Tensor) else w)]
+        flat = self._flat(gate_up, down_weight)
         ptrs = [t.data_ptr() for t in tensors]
         self.in_place = ptrs == [t.data_ptr() for t in flat]
         self.tensors, self.layout = tensors, [(t, t.data_ptr(), t.dtype, t.shape, t.stride()) for t in flat]
         self._sizes: dict[tuple[int, int], int] = {}
 
+    @staticmethod
+    def _flat(gate_up, down):
+        return (gate_up, down) if isinstance(gate_up, torch.Tensor) else (*gate_up, *down)
+
     def current(self, layer) -> bool:
-        if not self.in_place or layer.gate_up is not self.given[0] or layer.down is not self.given[1]:
+        """Whether these are the tensors that the layer holds now, where they were: one may
+        have taken another's place on the layer, or in a list of them that stayed."""
+        now = self._flat(layer.gate_up, layer.down)
+        if not self.in_place or len(now) != len(self.layout):
             return False
-        for t, ptr, dtype, shape, stride in self.layout:
-            if t.data_ptr() != ptr or t.dtype is not dtype or t.shape != shape or t.stride() != stride:
+        for t, (old, ptr, dtype, shape, stride) in zip(now, self.layout):
+            if (t is not old or t.data_ptr() != ptr or t.dtype is not dtype or t.shape != shape
+                    or t.stride() != stride):
                 return False
         return True
 

@@ -1,0 +1,57 @@
+"""ExpertMLP.decode describes its weights once for all calls: what it keeps between them,
+and what makes it describe them anew. No device work."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mlx_gptq import _native as nat
+from mlx_gptq import linear
+from mlx_gptq.experts import ExpertMLP
+
+BF, I32 = torch.bfloat16, torch.int32
+CPU = torch.device("cpu")
+
+
+@pytest.fixture(autouse=True)
+def launches(monkeypatch):
+    """The launches' arguments; host tensors pass as the device's."""
+    made = []
+    monkeypatch.setattr(linear, "_device", lambda *tensors: CPU)
+    monkeypatch.setattr(nat, "launch", lambda dev, name, *args: made.append((name, *args)))
+    return made
+
+
+def weight(n, k, mode, E=4, bits=4):
+    if mode == "dense":
+        return torch.zeros(E, n, k, dtype=BF)
+    packed = torch.zeros(E, n, k * bits // 32, dtype=I32)
+    if mode == "affine":
+        return [packed, *(torch.zeros(E, n, k // 32, dtype=BF) for _ in range(2))]
+    return [packed, torch.zeros(E, n, k // 32, dtype=torch.uint8)]
+
+
+def layer_of(mode, H=64, I=32):
+    return ExpertMLP(weight(2 * I, H, mode), weight(H, I, mode), mode)
+
+
+def decode(layer, T=3, H=64):
+    return layer.decode(torch.zeros(T, H, dtype=BF), torch.zeros(T, 2, dtype=torch.int64),
+                        torch.zeros(T, 2))
+
+
+@pytest.mark.parametrize("mode,place", [("mxfp4", 0), ("mxfp4", 1), ("affine", 0), ("affine", 1),
+                                        ("affine", 2)])
+@pytest.mark.parametrize("which", ["gate_up", "down"])
+def test_a_tensor_replaced_in_a_list_is_seen(mode, place, which):
+    layer = layer_of(mode)
+    first = layer._decode_weights(64, BF, CPU)
+    assert layer._decode_weights(64, BF, CPU) is first
+    weights = getattr(layer, which)
+    weights[place] = weights[place].clone()
+    again = layer._decode_weights(64, BF, CPU)
+    assert again is not first
+    described = again.up if which == "gate_up" else again.down
+    assert (described.data, described.scales, described.biases)[place] == weights[place].data_ptr()
+    assert layer._decode_weights(64, BF, CPU) is again
