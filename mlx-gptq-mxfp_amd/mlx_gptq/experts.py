@@ -323,9 +323,9 @@ class ExpertMLP:
         inner = (gate_up if self.mode == "dense" else gate_up[0]).shape[1] // 2
         up, up_tensors = self._decode_weight(gate_up, 2 * inner, cols, dtype, dev)
         dn, dn_tensors = self._decode_weight(down, cols, inner, dtype, dev)
-        self._described = _DecodeWeights(cols, dtype, dev, inner, up, dn, gate_up, down,
-                                         up_tensors + dn_tensors)
-        return self._described
+        d = _DecodeWeights(cols, dtype, dev, inner, up, dn, gate_up, down, up_tensors + dn_tensors)
+        self._described = d
+        return d
 
     def decode(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                top_k_weights: torch.Tensor) -> torch.Tensor:

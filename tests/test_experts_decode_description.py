@@ -55,3 +55,25 @@ def test_a_tensor_replaced_in_a_list_is_seen(mode, place, which):
     described = again.up if which == "gate_up" else again.down
     assert (described.data, described.scales, described.biases)[place] == weights[place].data_ptr()
     assert layer._decode_weights(64, BF, CPU) is again
+
+
+def test_calls_at_once_take_their_own_description(monkeypatch):
+    """Two threads: while one stores its description, the other stores one of other rows."""
+
+    class Shared(ExpertMLP):
+        other = None
+
+        def __setattr__(self, name, value):
+            super().__setattr__(name, value)
+            if name == "_described" and value is not None and self.other is not None:
+                super().__setattr__(name, self.other)
+
+    layer = Shared(weight(64, 64, "dense"), weight(64, 32, "dense"))
+    other = layer._decode_weights(64, BF, CPU)
+    layer.gate_up, layer.down = weight(64, 64, "dense"), weight(64, 32, "dense")
+    layer.other = other
+    passed = []
+    monkeypatch.setattr(nat, "launch", lambda dev, name, *args: passed.append(
+        (nat.Weight.from_address(args[11]).data, nat.Weight.from_address(args[12]).data)))
+    decode(layer)
+    assert passed == [(layer.gate_up.data_ptr(), layer.down.data_ptr())]
