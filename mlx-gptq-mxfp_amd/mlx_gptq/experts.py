@@ -29,6 +29,7 @@ No call waits for the device: the routing stays there.
 from __future__ import annotations
 
 import ctypes
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -152,33 +153,27 @@ def route(top_k_index: torch.Tensor, num_experts: int) -> Routing:
 
 
 class _DecodeWeights:
-    """What ExpertMLP.decode passes of its weights."""
+    """What ExpertMLP.decode passes of its weights. It keeps none of the layer's tensors
+    alive; copies (of host weights, or of ones whose rows do not lie one after the other)
+    are its own, and such a description serves one call only."""
 
-    def __init__(self, cols, dtype, device, inner, up, down, gate_up, down_weight, tensors):
+    def __init__(self, cols, dtype, device, inner, up, down, given, passed):
         self.cols, self.dtype, self.device, self.inner = cols, dtype, device, inner
         self.type_code = nat.dtype_code(dtype)
         self.up, self.down = up, down
         self.up_ptr, self.down_ptr = ctypes.addressof(up), ctypes.addressof(down)
-        # copies (of host weights, or of ones whose rows do not lie one after the other) go
-        # with this call: only weights described where they are stand for the next one
-        flat = self._flat(gate_up, down_weight)
-        ptrs = [t.data_ptr() for t in tensors]
-        self.in_place = ptrs == [t.data_ptr() for t in flat]
-        self.tensors, self.layout = tensors, [(t, t.data_ptr(), t.dtype, t.shape, t.stride()) for t in flat]
+        self.in_place = [t.data_ptr() for t in passed] == [t.data_ptr() for t in given]
+        self.copies = () if self.in_place else passed
+        self.layout = [(weakref.ref(t), t.data_ptr(), t.dtype, t.shape, t.stride()) for t in given]
         self._sizes: dict[tuple[int, int], int] = {}
 
-    @staticmethod
-    def _flat(gate_up, down):
-        return (gate_up, down) if isinstance(gate_up, torch.Tensor) else (*gate_up, *down)
-
-    def current(self, layer) -> bool:
-        """Whether these are the tensors that the layer holds now, where they were: one may
+    def current(self, now) -> bool:
+        """Whether the layer's tensors, `now`, are those described, where they were: one may
         have taken another's place on the layer, or in a list of them that stayed."""
-        now = self._flat(layer.gate_up, layer.down)
-        if not self.in_place or len(now) != len(self.layout):
+        if len(now) != len(self.layout):
             return False
         for t, (old, ptr, dtype, shape, stride) in zip(now, self.layout):
-            if (t is not old or t.data_ptr() != ptr or t.dtype is not dtype or t.shape != shape
+            if (old() is not t or t.data_ptr() != ptr or t.dtype is not dtype or t.shape != shape
                     or t.stride() != stride):
                 return False
         return True
@@ -316,15 +311,19 @@ class ExpertMLP:
     def _decode_weights(self, cols: int, dtype: torch.dtype, dev: torch.device):
         """Both weights as mgq_experts_decode takes them: described once, and again for
         other rows or when a tensor is no longer the one described."""
-        d = self._described
-        if d is not None and d.cols == cols and d.dtype is dtype and d.device == dev and d.current(self):
-            return d
         gate_up, down = self.gate_up, self.down
+        given = (gate_up, down) if self.mode == "dense" else (*gate_up, *down)
+        d = self._described
+        if (d is not None and d.cols == cols and d.dtype is dtype and d.device == dev
+                and d.current(given)):
+            return d
+        # (before new copies are made, and if an error follows)
+        self._described = None
         inner = (gate_up if self.mode == "dense" else gate_up[0]).shape[1] // 2
         up, up_tensors = self._decode_weight(gate_up, 2 * inner, cols, dtype, dev)
         dn, dn_tensors = self._decode_weight(down, cols, inner, dtype, dev)
-        d = _DecodeWeights(cols, dtype, dev, inner, up, dn, gate_up, down, up_tensors + dn_tensors)
-        self._described = d
+        d = _DecodeWeights(cols, dtype, dev, inner, up, dn, given, up_tensors + dn_tensors)
+        self._described = d if d.in_place else None
         return d
 
     def decode(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,

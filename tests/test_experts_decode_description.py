@@ -3,6 +3,8 @@ and what makes it describe them anew. No device work."""
 
 from __future__ import annotations
 
+import weakref
+
 import pytest
 import torch
 
@@ -77,3 +79,36 @@ def test_calls_at_once_take_their_own_description(monkeypatch):
         (nat.Weight.from_address(args[11]).data, nat.Weight.from_address(args[12]).data)))
     decode(layer)
     assert passed == [(layer.gate_up.data_ptr(), layer.down.data_ptr())]
+
+
+@pytest.mark.parametrize("mode", ["dense", "mxfp4", "affine"])
+def test_copies_go_with_their_call(mode, launches, monkeypatch):
+    """Weights that had to be copied: no copy outlives its call."""
+    layer = layer_of(mode)
+    turned = layer.gate_up if mode == "dense" else layer.gate_up[0]
+    turned = turned.transpose(1, 2).contiguous().transpose(1, 2)
+    layer.gate_up = turned if mode == "dense" else [turned, *layer.gate_up[1:]]
+    copies = []
+    contiguous = torch.Tensor.contiguous
+
+    def contiguous_seen(t):
+        out = contiguous(t)
+        if out is not t:
+            copies.append(weakref.ref(out))
+        return out
+
+    monkeypatch.setattr(torch.Tensor, "contiguous", contiguous_seen)
+    for calls in (1, 2):
+        decode(layer)
+        assert len(launches) == len(copies) == calls
+        assert all(c() is None for c in copies)
+
+
+@pytest.mark.parametrize("mode", ["dense", "mxfp4", "affine"])
+def test_a_replaced_weight_is_let_go(mode):
+    layer = layer_of(mode)
+    decode(layer)
+    old = weakref.ref(layer.gate_up if mode == "dense" else layer.gate_up[0])
+    layer.gate_up = weight(64, 64, mode)
+    assert old() is None
+    decode(layer)
