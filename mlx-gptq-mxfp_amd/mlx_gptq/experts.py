@@ -198,6 +198,8 @@ class ExpertMLP:
     MODES = ("dense", "mxfp4", "mxfp8", "int8")  # one grid each
     GRID_MODES = ("affine",)                      # `bits` and a group size choose the grid
 
+    _described: _DecodeWeights | None = None
+
     def __init__(self, gate_up, down, mode: str = "dense"):
         if mode not in self.MODES + self.GRID_MODES:
             raise ValueError(f"unsupported expert mode: {mode} "
@@ -208,7 +210,10 @@ class ExpertMLP:
         if first.dim() != 3 or first.shape[1] % 2:
             raise ValueError(f"ExpertMLP: gate_up must be [E, 2 I, H] (got {tuple(first.shape)})")
         self.num_experts = int(first.shape[0])
-        self._described: _DecodeWeights | None = None
+
+    def __getstate__(self):
+        # (addresses of this process's tensors: a copy describes its own)
+        return {name: value for name, value in self.__dict__.items() if name != "_described"}
 
     @classmethod
     def from_weights(cls, gate_up: torch.Tensor, down: torch.Tensor, mode: str = "dense",

@@ -3,6 +3,8 @@ and what makes it describe them anew. No device work."""
 
 from __future__ import annotations
 
+import copy
+import pickle
 import weakref
 
 import pytest
@@ -112,3 +114,18 @@ def test_a_replaced_weight_is_let_go(mode):
     layer.gate_up = weight(64, 64, mode)
     assert old() is None
     decode(layer)
+
+
+@pytest.mark.parametrize("mode", ["dense", "mxfp4", "affine"])
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda layer: pickle.loads(pickle.dumps(layer))],
+                         ids=["copy", "deepcopy", "pickle"])
+def test_a_layer_that_has_decoded_can_be_copied(mode, how, launches):
+    layer = layer_of(mode)
+    decode(layer)
+    twin = how(layer)
+    assert (twin.mode, twin.num_experts) == (mode, 4)
+    decode(twin)
+    own = twin.gate_up if mode == "dense" else twin.gate_up[0]
+    assert nat.Weight.from_address(launches[1][12]).data == own.data_ptr()
+    decode(layer)
+    assert launches[2][12] == launches[0][12]
