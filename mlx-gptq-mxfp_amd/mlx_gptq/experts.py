@@ -252,7 +252,8 @@ class ExpertMLP:
         q, s, _, _ = grid.rtn_quantize_mxfp(w, mode)
         return packing.pack_q(q, grid.mode_defaults(mode)[1]), s
 
-    def _product(self, x, weight, offsets, row_index=None):
+    def _product(self, x, weight, offsets, row_index=None, cols=None):
+        """x times a weight, whose rows have `cols` values (as many as x unless given)."""
         if self.mode == "dense":
             return linear.grouped_linear(x, weight, offsets, row_index, validate=False)
         if self.mode == "int8":
@@ -260,7 +261,7 @@ class ExpertMLP:
             return linear.int8_linear(q, s, *weight, out_dtype=x.dtype, offsets=offsets,
                                       row_index=row_index, validate=False)
         if self.mode == "affine":
-            bits = 32 * weight[0].shape[-1] // max(x.shape[1], 1)
+            bits = 32 * weight[0].shape[-1] // max(x.shape[1] if cols is None else cols, 1)
             return linear.affine_linear(x, *weight, bits, offsets, row_index, validate=False)
         return linear.mxfp_linear(x, *weight, self.mode, offsets, row_index, validate=False)
 
@@ -271,9 +272,13 @@ class ExpertMLP:
         nothing, whatever their weight is."""
         T, k = top_k_index.shape
         r = route(top_k_index, self.num_experts)
-        gate, up = self._product(hidden_states, self.gate_up, r.offsets, r.row_index).chunk(2, dim=-1)
+        # (each weight's rows are as long as the other one says)
+        up_rows, down_rows = ((w if self.mode == "dense" else w[0]).shape[1]
+                              for w in (self.gate_up, self.down))
+        gate, up = self._product(hidden_states, self.gate_up, r.offsets, r.row_index,
+                                 down_rows).chunk(2, dim=-1)
         act = (F.silu(gate.float()) * up.float()).to(hidden_states.dtype)
-        y = self._product(act, self.down, r.offsets)
+        y = self._product(act, self.down, r.offsets, cols=up_rows // 2)
         y = y[r.entry].view(T, k, y.shape[1]).float()
         # (a row whose experts are all masked may come with weights of NaN)
         dropped = (r.entry >= r.offsets[-1]).view(T, k)
