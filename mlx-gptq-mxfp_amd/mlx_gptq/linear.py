@@ -112,8 +112,11 @@ def _int32(t: torch.Tensor) -> torch.Tensor:
     expect it."""
     if t.dtype is torch.int32:
         return t
-    if t.dtype == torch.int64:
-        t = t.clamp(-(2**31), 2**31 - 1)
+    if t.dtype in (torch.int64, torch.uint64, torch.uint32):
+        wide = t.to(torch.int64)
+        if t.dtype is torch.uint64:  # (2^63 and more read as negative numbers)
+            wide = wide.masked_fill(wide < 0, 2**31 - 1)
+        t = wide.clamp(-(2**31), 2**31 - 1)
     return t.to(torch.int32)
 
 
