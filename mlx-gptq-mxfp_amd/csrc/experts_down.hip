@@ -307,6 +307,7 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
                 what);
     MGQ_REQUIRE(dtype == kBF16 || (format != kFewMx4 && format != kFewMx8), MGQ_ERR_VALUE,
                 "%s: MXFP weights take bfloat16 rows", what);
+    MGQ_REQUIRE(m.data != nullptr, MGQ_ERR_VALUE, "%s: a weight has no elements", what);
     w->p = static_cast<const char*>(m.data);
     w->n = n;
     if (format == kFewDense) {
@@ -333,15 +334,20 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
                 what, (long long)cols);
     w->ld = cols / 8 * bits;
     MGQ_REQUIRE(w->ld <= kFewRowBytes, MGQ_ERR_SHAPE, "%s: a weight's rows pass 2^28 bytes", what);
+    MGQ_REQUIRE(m.scales != nullptr && (format < kFewAf2 || m.biases != nullptr), MGQ_ERR_VALUE,
+                "%s: a weight has no scales, or an affine one no biases", what);
     w->group = w->ld * n;
     return MGQ_OK;
   };
+  MGQ_REQUIRE(up != nullptr && down != nullptr, MGQ_ERR_VALUE, "%s: a weight's description is missing",
+              what);
   DecodeArgs a = {};
   if (int rc = weight(*up, 2 * I, H, &a.up)) return rc;
   if (int rc = weight(*down, H, I, &a.down)) return rc;
   const int64_t need = mgq_experts_decode_workspace_size(T, k, H, I);
-  MGQ_REQUIRE(workspace_bytes >= need, MGQ_ERR_WORKSPACE, "%s: workspace %lld < %lld bytes", what,
-              (long long)workspace_bytes, (long long)need);
+  MGQ_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), MGQ_ERR_WORKSPACE,
+              "%s: workspace %lld < %lld bytes", what, (long long)(workspace ? workspace_bytes : 0),
+              (long long)need);
   if (T == 0) return MGQ_OK;
   a.x = static_cast<const char*>(X);
   a.ldx = 2 * ldx;
