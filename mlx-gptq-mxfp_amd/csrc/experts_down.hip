@@ -247,15 +247,30 @@ __global__ void __launch_bounds__(64 * WAVES) decode_down_single_kernel(const De
   }
 }
 
+constexpr int kSingleWaves = 8;
+constexpr int single_loads(int lanes) { return lanes == 64 ? 8 : 4; }
+
 template <class F, int L>
 int launch_single(const DecodeArgs& a, hipStream_t s, const char* what) {
-  constexpr int R = L == 64 ? 8 : 4, WAVES = 8, DEPTH = F::dense ? 3 : 2;
+  constexpr int R = single_loads(L), WAVES = kSingleWaves, DEPTH = F::dense ? 3 : 2;
   const int chunks = gemv_chunks<F, L>(a.I);
   int parts = WAVES / a.n;
   parts = parts < 1 ? 1 : parts > chunks ? chunks : parts;
   decode_down_single_kernel<F, L, R, WAVES, DEPTH>
       <<<static_cast<unsigned>(ceil_div(a.H, R * (64 / L))), 64 * WAVES, 0, s>>>(a, parts);
   return check_launch(what);
+}
+
+// Less than 2^32 threads (of several rows always: H < 2^29 are less than 2^24 tiles).
+int check_grid(const DecodeArgs& a, int format, const char* what) {
+  if (a.T > 1) return MGQ_OK;
+  return decode_dispatch(format, a.type, a.down.type, [&](auto f) {
+    const int lanes = gemv_lanes<decltype(f)>(a.I, a.H);
+    const int64_t blocks = ceil_div(a.H, single_loads(lanes) * (64 / lanes));
+    MGQ_REQUIRE(blocks < (int64_t(1) << 32) / (64 * kSingleWaves), MGQ_ERR_SHAPE,
+                "%s: too many output tiles", what);
+    return static_cast<int>(MGQ_OK);
+  });
 }
 
 }  // namespace
@@ -368,6 +383,7 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
   a.type = dtype;
   a.parts = decode_parts(T * k, H);
   a.tiles = decode_tiles(H);
+  if (int rc = check_grid(a, down->format, what)) return rc;  // (before the first launch)
   hipStream_t s = as_stream(stream);
   if (int rc = decode_up(a, up->format, s, what)) return rc;
   return decode_down(a, down->format, s, what);

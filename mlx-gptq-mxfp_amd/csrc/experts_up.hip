@@ -271,7 +271,9 @@ template <class F>
 int launch_single(const DecodeArgs& a, hipStream_t s, const char* what) {
   constexpr int R = 8, DEPTH = F::dense ? 4 : 2;
   const int lanes = gemv_lanes<F>(a.H, a.I);
-  const unsigned grid = static_cast<unsigned>(a.n * ceil_div(a.I, kWaves * R / 2 * (64 / lanes)));
+  const int64_t blocks = a.n * ceil_div(a.I, kWaves * R / 2 * (64 / lanes));
+  MGQ_REQUIRE(blocks < int64_t(1) << 24, MGQ_ERR_SHAPE, "%s: too many output tiles", what);
+  const unsigned grid = static_cast<unsigned>(blocks);
   if (lanes == 64) decode_up_single_kernel<F, 64, R, DEPTH><<<grid, 64 * kWaves, 0, s>>>(a);
   else if (lanes == 32) decode_up_single_kernel<F, 32, R, DEPTH><<<grid, 64 * kWaves, 0, s>>>(a);
   else decode_up_single_kernel<F, 16, R, DEPTH><<<grid, 64 * kWaves, 0, s>>>(a);

@@ -32,3 +32,16 @@ def test_a_description_that_is_missing(missing):
     args = {**OK, "up": ctypes.addressof(w), "down": ctypes.addressof(w), missing: None}
     assert nat.load().mgq_experts_decode(*args.values()) == nat.ERR_VALUE
     assert "experts_decode" in nat.last_error()
+
+
+@pytest.mark.parametrize("change", [
+    # one row: 16 experts of 2^27 gate rows, 64 to a workgroup of 256
+    dict(T=1, H=1, I=1 << 27, ldx=1, k=16, E=16, up=dict(format=nat.WEIGHT_DENSE, ld=1, expert=1 << 28),
+         down=dict(ld=1 << 27)),
+    # 2^27 columns of the result, 16 to a workgroup of 512
+    dict(T=1, H=1 << 27, I=1, ldx=1 << 27, k=1, E=1,
+         up=dict(format=nat.WEIGHT_DENSE, ld=1 << 27, expert=1 << 28), down=dict(ld=1)),
+])
+def test_more_workgroups_than_a_launch_holds(change):
+    assert entry(ws_bytes=1 << 50, **change) == nat.ERR_SHAPE
+    assert "too many output tiles" in nat.last_error()
