@@ -467,7 +467,8 @@ int mgq_top_k_softmax_grad(const float* dw, const void* logits, int dtype, int64
 
 /* A routed layer's experts for a few rows -- mlx_gptq/experts.py ExpertMLP.decode:
  *   out[t] = sum_j weights[t, j] down[e] act,  e = index[t, j],
- *   act = silu(gate[e] x[t]) * (up[e] x[t]), rounded to dtype,
+ *   act = silu(gate[e] x[t]) * (up[e] x[t]), rounded to dtype (T <= 8: and what that
+ *   lost, rounded, added),
  * sums in fp32, out rounded once. X: [T, H] of dtype (bf16 / f16; pitch ldx), index:
  * [T, k] of 32 or 64 bits, weights: f32 [T, k], out: [T, H] of dtype. T <= 64, k <=
  * 16. Assignments to no expert (outside [0, n_experts)) add nothing. `up` holds an

@@ -14,6 +14,14 @@ namespace mgq {
 constexpr int kDecodeRows = 64;     // rows of a call
 constexpr int kDecodeTopK = 16;     // experts of a row
 constexpr int kDecodeEntries = kDecodeRows * kDecodeTopK;
+// Rows of a call up to which the activation goes from one launch to the other as the sum of
+// two 16-bit numbers: itself rounded, and what that lost, rounded (2^-17 of it is lost in bf16,
+// 2^-22 in f16, where one number loses about what rounding the result does). The second
+// product's MFMA has rows to spare for them as long as an expert has at most 8 of the call's
+// 64. Above, one number: an MFMA for each part makes 16 rows of 4-bit codes 45.4 us instead of
+// 42.4 and 64 rows of MXFP8 192 instead of 177 (128 experts of 768 x 2048); experts cut into
+// eights of their rows instead take 47.5 and 184.
+constexpr int kDecodePartRows = 8;
 
 struct DecodeArgs {
   const char* x;
@@ -21,7 +29,7 @@ struct DecodeArgs {
   const void* index;     // [T, k] int32 or int64
   const float* weights;  // [T, k]
   FewWeight up, down;    // [E, 2 I, H] (gate rows first), [E, H, I]
-  char* act;             // workspace: [T k, I] of x's type
+  uint16_t* act;         // workspace: [T k, act_parts, I] of x's type
   int32_t* plan;         // workspace: see decode_plan (experts_up.hip)
   int32_t* counts;       // workspace: parts of a column tile that are done
   float* sums;           // workspace: [parts, T, H]
@@ -30,6 +38,7 @@ struct DecodeArgs {
   int T, k, n;           // n = T k
   int E, H, I;
   int type;              // kBF16 or kF16
+  int act_parts;         // 2 up to kDecodePartRows rows
   int parts, tiles;      // of the second launch
 };
 
@@ -57,9 +66,22 @@ inline int decode_parts(int64_t n, int64_t H) {
   return static_cast<int>(p < 1 ? 1 : p > 8 ? 8 : p);
 }
 inline int64_t decode_round(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-inline int64_t decode_act_bytes(int64_t n, int64_t I) { return decode_round(n * I * 2); }
+inline int decode_act_parts(int64_t T) { return T <= kDecodePartRows ? 2 : 1; }
+inline int64_t decode_act_bytes(int64_t T, int64_t k, int64_t I) {
+  return decode_round(T * k * decode_act_parts(T) * I * 2);
+}
 inline int64_t decode_plan_bytes(int64_t n) { return decode_round(kDecodePlanHead + n * 16); }
 inline int64_t decode_count_bytes(int64_t H) { return decode_round(4 * int64_t(decode_tiles(H))); }
+
+// The activation of entry `i` at p (an infinity, or no number, in one part).
+__device__ __forceinline__ void decode_store_act(const DecodeArgs& a, int i, int p, float v) {
+  const uint16_t high = lin_round16(v, a.type);
+  uint16_t* row = a.act + static_cast<int64_t>(i) * a.act_parts * a.I + p;
+  row[0] = high;
+  if (a.act_parts == 1) return;
+  const float left = v - (a.type == kF16 ? f16_to_f32(high) : bf16_to_f32(high));
+  row[a.I] = fabsf(left) < INFINITY ? lin_round16(left, a.type) : 0;
+}
 
 __device__ __forceinline__ int decode_expert(const DecodeArgs& a, int i) {
   if (a.index64) {

@@ -18,6 +18,8 @@ namespace {
 
 constexpr int kWaves = 4;
 
+// Where the activation has two parts, both are rows of the MFMA: up to 4 rows in the call
+// (NE = 2) row 4 j + i is part i of an item's row j, otherwise row 8 i + j is.
 template <class F, int NE, int DEPTH>
 __global__ void __launch_bounds__(64 * kWaves) decode_down_kernel(const DecodeArgs a) {
   constexpr int NP = kDecodeCols / 16;
@@ -51,22 +53,39 @@ __global__ void __launch_bounds__(64 * kWaves) decode_down_kernel(const DecodeAr
   auto x_of = [&](int u) {
     const int first = __builtin_amdgcn_readfirstlane(items[u].first);
     const int count = __builtin_amdgcn_readfirstlane(items[u].count);
-    const int own = NE == 1 ? r16 >> 2 : r16;
-    const int entry = entries[first + (own < count ? own : count - 1)].entry;
-    return static_cast<const char*>(a.act) + static_cast<int64_t>(entry) * a.I * 2;
+    const bool two = NE == 2 || a.act_parts == 2;
+    const int own = NE == 2 ? r16 >> 2 : two ? r16 & 7 : r16;
+    const int part = NE == 2 ? r16 & 1 : two ? r16 >> 3 : 0;
+    const int64_t entry = entries[first + (own < count ? own : count - 1)].entry;
+    return reinterpret_cast<const char*>(a.act + (entry * (two ? 2 : 1) + part) * a.I);
   };
   // an item's sums to its rows
   auto add = [&](int u, const lin_f32x4_t(&acc)[NP][1]) {
     const int first = __builtin_amdgcn_readfirstlane(items[u].first);
     const int count = __builtin_amdgcn_readfirstlane(items[u].count);
+    constexpr int N = NE == 2 ? 1 : NE;
+    float v[NP][N];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const int j = NE == 1 ? quad : 4 * quad + e;
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[p][e] = NE == 2 ? acc[p][0][0] + acc[p][0][1] : acc[p][0][e];
+    if (NE == 4 && a.act_parts == 2) {  // (the upper half of the wave has the other parts)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const auto s = __builtin_amdgcn_permlane32_swap(f2u(v[p][e]), f2u(v[p][e]), false, false);
+          v[p][e] = u2f(s[0]) + u2f(s[1]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int j = NE == 2 ? quad : 4 * quad + e;
       if (j < count) {  // (an item holds a row once: no two lanes add to one sum)
         const DecodeEntry t = entries[first + j];
         float* to = sums + t.entry / a.k * kDecodeCols + r16;
 #pragma unroll
-        for (int p = 0; p < NP; ++p) to[16 * p] += t.weight * acc[p][0][e];
+        for (int p = 0; p < NP; ++p) to[16 * p] += t.weight * v[p][e];
       }
     }
   };
@@ -228,8 +247,9 @@ __global__ void __launch_bounds__(64 * WAVES) decode_down_single_kernel(const De
     float one[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) one[r] = 0.0f;
-    gemv_add<F, L, R, DEPTH>(one, a.down, expert, first, a.act + static_cast<int64_t>(i) * a.I * 2, a.I,
-                             chunks * part / parts, chunks * (part + 1) / parts);
+    gemv_add<F, L, R, DEPTH, 2>(one, a.down, expert, first,
+                                reinterpret_cast<const char*>(a.act + static_cast<int64_t>(i) * 2 * a.I),
+                                a.I, chunks * part / parts, chunks * (part + 1) / parts);
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r] = fmaf(weight, one[r], acc[r]);
   }
@@ -284,7 +304,7 @@ int decode_down(const DecodeArgs& a, int format, hipStream_t s, const char* what
              : lanes == 32 ? launch_single<F, 32>(a, s, what)
                            : launch_single<F, 16>(a, s, what);
     }
-    return a.T <= 4 ? launch<F, 1>(a, s, what) : launch<F, 4>(a, s, what);
+    return a.T <= 4 ? launch<F, 2>(a, s, what) : launch<F, 4>(a, s, what);
   });
 }
 
@@ -295,7 +315,7 @@ using namespace mgq;
 extern "C" int64_t mgq_experts_decode_workspace_size(int64_t T, int64_t k, int64_t H, int64_t I) {
   if (T < 1 || k < 1 || H < 1 || I < 1) return 0;
   const int64_t n = T * k, parts = decode_parts(n, H);
-  return decode_act_bytes(n, I) + decode_plan_bytes(n) + decode_count_bytes(H) +
+  return decode_act_bytes(T, k, I) + decode_plan_bytes(n) + decode_count_bytes(H) +
          (parts > 1 ? parts * T * decode_tiles(H) * kDecodeCols * 4 : 0);
 }
 
@@ -369,8 +389,9 @@ extern "C" int mgq_experts_decode(const void* X, int dtype, int64_t T, int64_t l
   a.index = index;
   a.index64 = index_bits == 64;
   a.weights = weights;
-  a.act = static_cast<char*>(workspace);
-  a.plan = reinterpret_cast<int32_t*>(a.act + decode_act_bytes(T * k, I));
+  a.act = static_cast<uint16_t*>(workspace);
+  a.act_parts = decode_act_parts(T);
+  a.plan = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + decode_act_bytes(T, k, I));
   a.counts = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(a.plan) + decode_plan_bytes(T * k));
   a.sums = reinterpret_cast<float*>(reinterpret_cast<char*>(a.counts) + decode_count_bytes(H));
   a.out = static_cast<uint16_t*>(out);

@@ -227,10 +227,7 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_kernel(const DecodeArgs
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         const int i = base + (NE == 1 ? quad : 4 * quad + e);
-        // (16 bits: what the second product's MFMA takes)
-        if (i < count && p < a.I)
-          reinterpret_cast<uint16_t*>(a.act)[static_cast<int64_t>(list[i]) * a.I + p] =
-              lin_round16(decode_act(gate[e], up[e]), a.type);
+        if (i < count && p < a.I) decode_store_act(a, list[i], p, decode_act(gate[e], up[e]));
       }
     }
     if constexpr (KS > 1) __syncthreads();
@@ -258,12 +255,11 @@ __global__ void __launch_bounds__(64 * kWaves) decode_up_single_kernel(const Dec
       acc, a.up, expert, [&](int r) { return r < R / 2 ? inner(r) : a.I + inner(r - R / 2); }, a.x, a.H,
       0, gemv_chunks<F, L>(a.H));
   gemv_reduce<L, R>(acc, sum);
-  uint16_t* act = reinterpret_cast<uint16_t*>(a.act) + static_cast<int64_t>(entry) * a.I;
 #pragma unroll
   for (int q = 0; q < N / 2; ++q)
     if ((lane & 15) == q) {
       const int r = gemv_row<L>(q, lane >> 4);
-      act[inner(r / RI) + r % RI] = lin_round16(decode_act(sum[q], sum[q + N / 2]), a.type);
+      decode_store_act(a, entry, inner(r / RI) + r % RI, decode_act(sum[q], sum[q + N / 2]));
     }
 }
 

@@ -84,13 +84,17 @@ __device__ __forceinline__ lin_u32x4_t gemv_pairs(uint32_t v) {
   return r;
 }
 
-// The piece's product.
-template <class F>
-__device__ __forceinline__ float gemv_multiply(const GemvPiece<F>& f, const GemvX<F>& x, int type) {
+// The piece's product with x, the sum of its XS parts.
+template <class F, int XS>
+__device__ __forceinline__ float gemv_multiply(const GemvPiece<F>& f, const GemvX<F> (&x)[XS], int type) {
   float r = 0;
+  auto add = [&](uint32_t w, int pair) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < XS; ++i) r = gemv_dot2<F::XT>(w, x[i].v[pair], r);
+  };
   if constexpr (F::dense) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r = gemv_dot2<F::XT>(f.v[i], x.v[i], r);
+    for (int i = 0; i < 4; ++i) add(f.v[i], i);
   } else if constexpr (F::mx) {
 #pragma unroll
     for (int i = 0; i < gemv_words<F>(); i += F::W == kFewMx8 ? 2 : 1) {
@@ -101,7 +105,7 @@ __device__ __forceinline__ float gemv_multiply(const GemvPiece<F>& f, const Gemv
         w = lin_decode_mx8(f.v[i], f.v[i + 1], f.s);
       const int at = F::W == kFewMx4 ? 4 * i : 2 * i;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r = gemv_dot2<F::XT>(w[j], x.v[at + j], r);
+      for (int j = 0; j < 4; ++j) add(w[j], at + j);
     }
   } else {
     if constexpr (F::bits == 8) {
@@ -109,8 +113,8 @@ __device__ __forceinline__ float gemv_multiply(const GemvPiece<F>& f, const Gemv
       for (int i = 0; i < 4; ++i) {
         uint32_t lo, hi;
         few_bytes<F::XT>(f.v[i], lo, hi);
-        r = gemv_dot2<F::XT>(lo, x.v[2 * i], r);
-        r = gemv_dot2<F::XT>(hi, x.v[2 * i + 1], r);
+        add(lo, 2 * i);
+        add(hi, 2 * i + 1);
       }
     } else if constexpr (F::bits == 4) {
 #pragma unroll
@@ -119,7 +123,7 @@ __device__ __forceinline__ float gemv_multiply(const GemvPiece<F>& f, const Gemv
         few_small<F::XT>(f.v[i] & 0x0f0f0f0fu, p[0], p[1]);
         few_small<F::XT>((f.v[i] >> 4) & 0x0f0f0f0fu, p[2], p[3]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r = gemv_dot2<F::XT>(p[j], x.v[4 * i + j], r);
+        for (int j = 0; j < 4; ++j) add(p[j], 4 * i + j);
       }
     } else {
       // a 2-bit code in four bits is the E2M1 number code / 2
@@ -129,44 +133,50 @@ __device__ __forceinline__ float gemv_multiply(const GemvPiece<F>& f, const Gemv
         const lin_u32x4_t e = gemv_pairs<F::XT>(even), o = gemv_pairs<F::XT>(odd);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          r = gemv_dot2<F::XT>(e[2 * j], x.v[8 * i + 4 * j], r);
-          r = gemv_dot2<F::XT>(e[2 * j + 1], x.v[8 * i + 4 * j + 1], r);
-          r = gemv_dot2<F::XT>(o[2 * j], x.v[8 * i + 4 * j + 2], r);
-          r = gemv_dot2<F::XT>(o[2 * j + 1], x.v[8 * i + 4 * j + 3], r);
+          add(e[2 * j], 8 * i + 4 * j);
+          add(e[2 * j + 1], 8 * i + 4 * j + 1);
+          add(o[2 * j], 8 * i + 4 * j + 2);
+          add(o[2 * j + 1], 8 * i + 4 * j + 3);
         }
       }
     }
     r = u2f(few_param_f32<F::SB>(f.s, type)) * r;
-    r = fmaf(u2f(few_param_f32<F::SB>(f.b, type)), x.sum, r);
+    float sum = x[0].sum;
+#pragma unroll
+    for (int i = 1; i < XS; ++i) sum += x[i].sum;
+    r = fmaf(u2f(few_param_f32<F::SB>(f.b, type)), sum, r);
   }
   return r;
 }
 
 // acc[i] += (this lane's part of) weight rows first(i) + lane / L times x, over the chunks
 // [c0, c1) of L pieces each; a row has gemv_chunks of them. first(i) is the same in all
-// lanes and leaves 64 / L rows to the weight's end. The weights of DEPTH - 1 chunks are in
-// flight beyond the one being multiplied.
+// lanes and leaves 64 / L rows to the weight's end. x is the sum of XS rows of K, one after the
+// other. The weights of DEPTH - 1 chunks are in flight beyond the one being multiplied.
 template <class F, int L>
 __host__ __device__ inline int gemv_chunks(int K) {
   constexpr int E = L * gemv_elems<F>();
   return (K + E - 1) / E;
 }
-template <class F, int L, int R, int DEPTH, typename First>
+template <class F, int L, int R, int DEPTH, int XS = 1, typename First>
 __device__ __forceinline__ void gemv_add(float (&acc)[R], const FewWeight& w, int64_t g, First&& first,
                                          const char* x, int K, int c0, int c1) {
   constexpr int E = gemv_elems<F>();
   const int lane = threadIdx.x & 63;
   const uint32_t sub = lane / L;  // row of the instruction's rows
   GemvPiece<F> f[DEPTH][R];
-  GemvX<F> xv[DEPTH];
+  GemvX<F> xv[DEPTH][XS];
   auto load = [&](int d, int c) __attribute__((always_inline)) {
     const int k0 = (c * L + (lane & (L - 1))) * E;
     const bool whole = (c + 1) * L * E <= K;
     if constexpr (F::dense) {
       if (whole) {
-        const lin_u32x4_t u = few_load16(x + 2 * static_cast<int64_t>(k0));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[d].v[i] = u[i];
+        for (int p = 0; p < XS; ++p) {
+          const lin_u32x4_t u = few_load16(x + 2 * (static_cast<int64_t>(p) * K + k0));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xv[d][p].v[i] = u[i];
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const char* base = w.p + g * w.group + first(r) * w.ld;
@@ -175,9 +185,12 @@ __device__ __forceinline__ void gemv_add(float (&acc)[R], const FewWeight& w, in
           for (int i = 0; i < 4; ++i) f[d][r].v[i] = v[i];
         }
       } else {
-        const lin_u32x4_t u = few_cut16(x, k0, K);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[d].v[i] = u[i];
+        for (int p = 0; p < XS; ++p) {
+          const lin_u32x4_t u = few_cut16(x + 2 * static_cast<int64_t>(p) * K, k0, K);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xv[d][p].v[i] = u[i];
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const lin_u32x4_t v = few_cut16(w.p + g * w.group + (first(r) + sub) * w.ld, k0, K);
@@ -188,11 +201,14 @@ __device__ __forceinline__ void gemv_add(float (&acc)[R], const FewWeight& w, in
     } else {
       const uint32_t kc = k0 < K ? k0 : 0;  // (a lane past the row's end reads its first piece)
 #pragma unroll
-      for (int h = 0; h < E / 8; ++h) {
-        const lin_u32x4_t u = few_load16(x + static_cast<uint64_t>(2u * kc + 16u * h));
+      for (int p = 0; p < XS; ++p)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[d].v[4 * h + i] = u[i];
-      }
+        for (int h = 0; h < E / 8; ++h) {
+          const lin_u32x4_t u =
+              few_load16(x + 2 * static_cast<int64_t>(p) * K + static_cast<uint64_t>(2u * kc + 16u * h));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xv[d][p].v[4 * h + i] = u[i];
+        }
       const uint32_t at = sub * static_cast<uint32_t>(w.ld) + kc / 32 * (4 * F::bits) + kc % 32 * F::bits / 8;
       const int n = F::affine ? K >> w.shift : K / 32;  // scales of a row
       const uint32_t ps = (sub * n + (F::affine ? kc >> w.shift : kc / 32)) * (F::affine ? F::SB : 1);
@@ -220,11 +236,12 @@ __device__ __forceinline__ void gemv_add(float (&acc)[R], const FewWeight& w, in
     }
   };
   auto multiply = [&](int d, int c) __attribute__((always_inline)) {
-    gemv_arrange<F>(xv[d]);
+#pragma unroll
+    for (int p = 0; p < XS; ++p) gemv_arrange<F>(xv[d][p]);
     const bool inside = F::dense || (c * L + (lane & (L - 1))) * E < K;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float v = gemv_multiply<F>(f[d][r], xv[d], w.type);
+      const float v = gemv_multiply<F, XS>(f[d][r], xv[d], w.type);
       acc[r] += inside ? v : 0.0f;
     }
   };

@@ -341,9 +341,10 @@ class ExpertMLP:
         """``forward`` for up to 64 rows with up to 16 experts each, in two launches that
         read the weights of the rows' experts once. [T, H] -> [T, H].
 
-        The activation is rounded to the rows' type, everything else is fp32 until the
-        result is rounded once (``forward`` also rounds between its products, so the two
-        agree within the type's precision only). Assignments to no expert add nothing. The
+        For up to 8 rows the activation keeps twice the bits of the rows' type, for more it
+        is rounded to it; everything else is fp32 until the result is rounded once
+        (``forward`` also rounds between its products, so the two agree within the type's
+        precision only). Assignments to no expert add nothing. The
         order of the sums depends on the sizes and the routing alone. int8 experts, whose
         rows are quantized for each product, have ``forward`` only. Not differentiable.
         """
