@@ -29,6 +29,7 @@ No call waits for the device: the routing stays there.
 from __future__ import annotations
 
 import ctypes
+import operator
 import weakref
 from dataclasses import dataclass
 
@@ -93,7 +94,7 @@ def top_k_softmax(logits: torch.Tensor, k: int,
     The weights are differentiable in the logits (``top_k_softmax_grad``, which has no
     derivative itself). Nothing waits for the device.
     """
-    k = int(k)
+    k = operator.index(k)
     _check_logits("top_k_softmax", logits, k)
     if linear._tracked("top_k_softmax", logits):
         return _TopKSoftmax.apply(logits, k, bool(renormalize))
