@@ -207,8 +207,10 @@ int lin_tile_rows(const LinArgs& a, int op, int kind, LinTileShape t, hipStream_
     case kOpI8: return pick_rows<kOpI8, kLinForward>(a, t, s, what);
     case kOpMx4: return pick_rows<kOpMx4, kLinForward>(a, t, s, what);
     case kOpMx8: return pick_rows<kOpMx8, kLinForward>(a, t, s, what);
-    default: return lin_tile_affine(a, op, t, s, what);
+    default: break;
   }
+  set_error("%s: no such operands", what);  // (affine ones have lin_tile_affine)
+  return MGQ_ERR_VALUE;
 }
 
 int64_t lin_tile_wgrad_bytes(int64_t M, int64_t G, int64_t N, int64_t K) {
