@@ -405,7 +405,8 @@ int mgq_mxfp_linear(const void* X, int64_t n_rows, int64_t ldx, const int32_t* r
  * contiguous; group_size 32, 64 or 128, K a multiple of it. fp32 sums, rounded
  * once. Few rows: scale sum(x code) + bias sum(x) for every 32 or 64 values, so that
  * |x| beyond 1e34 may overflow where the product with decoded weights would not.
- * Many rows: the decoded weights are rounded to dtype (mgq_affine_choice). */
+ * Many rows: the decoded weights are rounded to dtype, past 65504 to an infinity in
+ * f16 (mgq_affine_choice). */
 int mgq_affine_linear(const void* X, int dtype, int64_t n_rows, int64_t ldx,
                       const int32_t* row_index, int64_t n_entries, const uint32_t* words,
                       const void* scales, const void* biases, int param_dtype, int bits,

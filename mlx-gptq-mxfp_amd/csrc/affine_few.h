@@ -6,12 +6,13 @@
 // order, times row blocks.
 // affine_gemv_kernel: single entries (gemv_core.h).
 //
-// Bound by the instructions that decode: a step of 128 values times 32 rows takes a wave
-// about 160 vector instructions (2.1 ns each on a SIMD), and by the wait for a step's
-// codes where a SIMD has one wave. 14336 x 4096, 4 bits: 10.5 us for one entry (33 MB, 3.1
-// TB/s); 128 experts of 1536 x 2048, 512 entries: 72 us (228 MB, 3.2 TB/s; 63 with weights
-// that are cached, so memory is not what it waits for). More than one step in flight beyond
-// the one that is multiplied took the same time.
+// Bound by waits with few waves a SIMD. 128 experts of 1536 x 2048, 4 bits, 512 entries take
+// 72 us (228 MB, 3.2 TB/s), of which the 17.6 million vector instructions (about 160 for a
+// step of 128 values times 32 rows) are 29 at four cycles on 1024 SIMDs; its waves, three to a
+// SIMD at 148 registers, wait for 55 % of their cycles. With cached weights it takes 63, so
+// most of the wait is not memory's; more than one step in flight beyond the one that is
+// multiplied took the same time. 14336 x 4096, 4 bits, one entry: 10.5 us (33 MB, 3.1 TB/s),
+// 3.3 of them vector instructions.
 #pragma once
 
 #include "affine_few_choice.h"

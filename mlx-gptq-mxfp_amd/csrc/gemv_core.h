@@ -3,7 +3,9 @@
 // L lanes (64, 32 or 16) share a weight row, 16 bytes (8 for 2-bit codes) each, so that a
 // load instruction reads 64 / L rows in contiguous pieces of up to 1 KB: 5.3 TB/s of cold
 // weight measured against 4.4 where sixteen rows are read 64 bytes at a time, as an MFMA
-// operand wants them. A lane multiplies its codes with the x values beside them (two
+// operand wants them, both by loads alone. With the products the kernels reach 4.3 to 4.5 TB/s
+// of bf16 and 3.1 of 4-bit codes, launch included, whose two waves a SIMD (174 registers) keep
+// less in flight. A lane multiplies its codes with the x values beside them (two
 // products an instruction, fp32 sums); scales and biases apply to the lane's sum, since its
 // codes lie in one group. The lanes' sums of a row are added once, at the end.
 #pragma once

@@ -23,7 +23,11 @@
 //   - Affine codes (2, 4 or 8 bits, a scale and a bias for 32, 64 or 128 values) stay codes
 //     in LDS like MX ones; q s + b is formed in fp32 and rounded once to x's type, which
 //     the MFMA needs: 8 fused multiply-adds and 4 packed roundings for 8 codes, which the
-//     MFMAs of a tile do not cover (8191 x 14336 x 4096, 4 bits: 963 us, 1000 TFLOP/s).
+//     MFMAs of a tile do not cover (8191 x 14336 x 4096, 4 bits: 963 us, 1000 TFLOP/s, which
+//     is about the 485 us of its vector instructions and the 382 of its MFMAs one after the
+//     other). Rounded weights are what a dense weight of x's type is. Without that rounding
+//     (codes to the MFMA, s and b applied to a sum for every group) a 32 x 32 block would take
+//     32 more multiply-adds for 64 values, as many cycles as its four MFMAs.
 //   - An MX weight's codes stay codes in LDS (32 or 64 bytes a row and stage, and
 //     its two scale bytes widened to dwords). Half-wave h of the MFMA takes the
 //     stage's elements 32 h .. 32 h + 31, one MX group, so a lane needs one scale

@@ -15,6 +15,9 @@
 // (23 MB) and the gradient 13.0 us (40 MB), 1.6 and 3.1 TB/s. Eight keys of a lane are sorted
 // once (16 us where each choice looked through all of them); the gradient's chosen terms
 // go to their places through LDS (15.5 us where every lane compared its experts with all k).
+// More than 128 experts are looked through for every choice: 65536 rows of 256, 512 and 1024
+// take 21, 36 and 86 us in bf16 (renormalized, k = 8) and 38, 84 and 297 in fp32, whose 64-bit
+// keys of 1024 experts leave room for one wave a SIMD; the gradient 14, 25 and 49 (21, 32 and 78).
 // One row: 2.8 us, a launch.
 #include "linear_common.h"
 

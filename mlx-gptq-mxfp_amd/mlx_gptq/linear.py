@@ -419,9 +419,10 @@ def affine_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, b
     groups of 32, 64 or 128 values; without offsets all three lack the leading G.
     -> [entries, N] of x's type. fp32 sums, rounded once. For few rows (up to some 128 a
     group, as measured) the weights are not rounded, as q * scale and bias enter the sum
-    apart; for more they are rounded to x's type, like a dense weight of it. A row that holds
-    an infinity, or values beyond 1e34, may give results that are no numbers where the
-    product with the decoded weight would be infinite.
+    apart; for more they are rounded to x's type, like a dense weight of it (in float16 a
+    weight past 65504 is then infinite). For few rows a row that holds an infinity, or
+    values beyond 1e34, may give results that are no numbers where the product with the
+    decoded weight would be infinite.
     """
     fn = "affine_linear"
     tracked = _tracked(fn, x, scales, biases)
