@@ -1,9 +1,10 @@
 """A routed layer from calibration to its quantized forward.
 
 Captures the inputs of a fused-expert module, solves its two parameters with
-GPTQ on the MXFP4 grid, and runs the module's forward on the packed codes; beside
-it the same forward with dense, MXFP8 and int8 weights rounded to the nearest, and
-one fine-tuning step of the dense experts. Random weights and rows.
+GPTQ on the MXFP4 grid, and runs the module's forward on the packed codes, for a
+single token in two launches; beside it the same forward with dense, MXFP8, affine
+and int8 weights rounded to the nearest, and one fine-tuning step of the dense
+experts. The router's choice comes with its gradient. Random weights and rows.
 
     python examples/experts_forward.py [--tokens 512] [--device cuda:0]
 """
@@ -21,7 +22,7 @@ sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."
                                 "mlx-gptq-mxfp_amd"))
 
 from mlx_gptq import capture, gptq, grid  # noqa: E402
-from mlx_gptq.experts import ExpertMLP, route  # noqa: E402
+from mlx_gptq.experts import ExpertMLP, route, top_k_softmax  # noqa: E402
 
 
 def relative(y: torch.Tensor, ref: torch.Tensor) -> float:
@@ -47,7 +48,7 @@ def main(argv=None) -> dict[str, float]:
     gate_up, down = rand(E, 2 * I, H, scale=H**-0.5), rand(E, H, I, scale=I**-0.5)
     x = rand(T, H, scale=1.0)
     score = torch.randn(T, E, generator=g).to(dev)
-    weights, index = torch.softmax(score, dim=1).topk(k, dim=1)
+    index, weights = top_k_softmax(score, k, renormalize=False)
 
     dense = ExpertMLP(gate_up, down)
     y = dense(x, index, weights)
@@ -65,13 +66,13 @@ def main(argv=None) -> dict[str, float]:
         codes.append((q, s))
 
     errors = {"mxfp4 solved": relative(ExpertMLP.from_codes(*codes, "mxfp4")(x, index, weights), y)}
-    for mode in ("mxfp4", "mxfp8", "int8"):
+    for mode in ("mxfp4", "mxfp8", "int8", "affine"):
         errors[f"{mode} nearest"] = relative(
             ExpertMLP.from_weights(gate_up, down, mode)(x, index, weights), y)
-        if mode != "int8":  # of the weights themselves
+        if mode in ("mxfp4", "mxfp8"):  # of the weights themselves
             errors[f"{mode} weights"] = max(
                 relative(grid.rtn_quantize_mxfp(w, mode)[3], w) for w in (gate_up, down))
-    one = ExpertMLP.from_codes(*codes, "mxfp4")(x[:1], index[:1], weights[:1])  # a single token
+    one = ExpertMLP.from_codes(*codes, "mxfp4").decode(x[:1], index[:1], weights[:1])  # a single token
     errors["single token"] = relative(one, y[:1])
     for name, e in errors.items():
         print(f"{name:16s} relative error {e:.4f}")
