@@ -319,18 +319,25 @@ class ExpertMLP:
         return nat.Weight(t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr() if len(t) > 2 else None,
                           0, 0, group, code, params), t
 
-    def _decode_weights(self, cols: int, dtype: torch.dtype, dev: torch.device):
-        """Both weights as mgq_experts_decode takes them: described once, and again for
-        other rows or when a tensor is no longer the one described."""
+    def _tensors(self) -> tuple[torch.Tensor, ...]:
+        """Those of gate_up, then those of down."""
         gate_up, down = self.gate_up, self.down
-        given = (gate_up, down) if self.mode == "dense" else (*gate_up, *down)
+        return (gate_up, down) if self.mode == "dense" else (*gate_up, *down)
+
+    def _decode_weights(self, cols: int, dtype: torch.dtype, dev: torch.device, given=None):
+        """Both weights as mgq_experts_decode takes them: described once, and again for
+        other rows or when a tensor is no longer the one described. The caller holds
+        `given` (``_tensors``) until they are launched: the description does not."""
+        given = self._tensors() if given is None else given
         d = self._described
         if (d is not None and d.cols == cols and d.dtype is dtype and d.device == dev
                 and d.current(given)):
             return d
         # (before new copies are made, and if an error follows)
         self._described = None
-        inner = (gate_up if self.mode == "dense" else gate_up[0]).shape[1] // 2
+        half = len(given) // 2
+        gate_up, down = given if self.mode == "dense" else (given[:half], given[half:])
+        inner = given[0].shape[1] // 2
         up, up_tensors = self._decode_weight(gate_up, 2 * inner, cols, dtype, dev)
         dn, dn_tensors = self._decode_weight(down, cols, inner, dtype, dev)
         d = _DecodeWeights(cols, dtype, dev, inner, up, dn, given, up_tensors + dn_tensors)
@@ -353,8 +360,11 @@ class ExpertMLP:
         if self.mode == "int8":
             raise ValueError(f"{fn}: int8 experts are not supported, use forward")
         x = hidden_states
-        dense = (self.gate_up, self.down) if self.mode == "dense" else ()
-        floats = (*self.gate_up[1:], *self.down[1:]) if self.mode == "affine" else dense
+        given = self._tensors()
+        if self.mode == "dense":
+            floats = given
+        else:
+            floats = (*given[1:3], *given[4:]) if self.mode == "affine" else ()
         tracked = linear._tracked(fn, x, top_k_weights, *floats)
         if x.dtype not in linear._HALF or (self.mode[:2] == "mx" and x.dtype is not torch.bfloat16):
             raise TypeError(f"{fn}: expects bfloat16 rows, or float16 ones without MXFP weights "
@@ -371,8 +381,8 @@ class ExpertMLP:
         if T > 64 or not 1 <= k <= 16:
             raise ValueError(f"{fn}: up to 64 rows with 1 to 16 experts each (got {(T, k)}); "
                              "forward takes any number")
-        dev = linear._device(x, *(dense or self.gate_up[:1]))
-        d = self._decode_weights(H, x.dtype, dev)
+        dev = linear._device(x, *given)
+        d = self._decode_weights(H, x.dtype, dev, given)
         xd = linear._pitched(x, dev)
         index = top_k_index
         if index.dtype is not torch.int64:

@@ -129,3 +129,30 @@ def test_a_layer_that_has_decoded_can_be_copied(mode, how, launches):
     assert nat.Weight.from_address(launches[1][12]).data == own.data_ptr()
     decode(layer)
     assert launches[2][12] == launches[0][12]
+
+
+@pytest.mark.parametrize("mode", ["dense", "mxfp4", "affine"])
+def test_a_call_holds_its_weights_until_they_are_launched(mode, monkeypatch):
+    """Another thread replaces the layer's weights once they are described."""
+
+    class Replaced(ExpertMLP):
+        def __setattr__(self, name, value):
+            super().__setattr__(name, value)
+            if name == "_described" and value is not None:
+                self.gate_up, self.down = weight(64, 64, self.mode), weight(64, 32, self.mode)
+
+    layer = Replaced(weight(64, 64, mode), weight(64, 32, mode), mode)
+    given = [t for w in (layer.gate_up, layer.down) for t in ([w] if mode == "dense" else w)]
+    pointers, alive = [t.data_ptr() for t in given], [weakref.ref(t) for t in given]
+    del given
+    seen = []
+
+    def launch(dev, name, *args):
+        parts = [nat.Weight.from_address(a) for a in args[11:13]]
+        seen.extend(p for w in parts for p in (w.data, w.scales, w.biases) if p)
+        seen.append(all(ref() is not None for ref in alive))
+
+    monkeypatch.setattr(nat, "launch", launch)
+    decode(layer)
+    assert seen == [*pointers, True]
+    assert all(ref() is None for ref in alive)
